@@ -1,0 +1,475 @@
+"""The operators of a tree-drafting step over a KV cache, as cases that can be timed and compared.
+
+A draft/verify step whose drafts form a tree (several guesses per position) needs four things of its
+device library: attention of the tree's nodes over their request's cache, a cache that is quantised as
+it is written and read back, the walk that accepts one path of the tree, and the move of that path's
+keys and values to the front.  ``run`` computes them in elementary torch operations where ``own`` is
+false and by the framework's calls where it is true.
+
+Definitions that both forms share
+  block      T tree nodes of one request: cache row, ctx committed positions; node i sits at cache slot
+             ctx + i and at position ctx + depth(i).  parent[i] < i, node 0 is the root (parent -1).
+  attention  node i sees the slots below ctx and the slots of its ancestors and itself (tree), or the slots
+             up to ctx + i (causal: a chain, a prefill chunk); scale 1 / sqrt(head_dim); grouped heads.
+  8 bits     one power-of-two scale 2^e per (row, KV head, slot) for K and for V, e the smallest with
+             max|x| <= Q 2^e (Q = 448 for e4m3, 127 for int8), clamped to [-100, 120]; the stored value is
+             x 2^-e rounded to nearest even.  The exponent is kept as the byte e + 127.
+  RoPE       rotate-half on q and k as the framework defines it for bf16: tables, products and the sum
+             rounded to bf16.
+  accept     from the root: y[node] is the model's token after the node; go to the lowest-numbered child
+             that was drafted as that token, until there is none.  The last y is the next token.
+"""
+import math
+
+import numpy as np
+import torch
+
+own = False
+
+QMAX = {"e4m3": 448.0, "int8": 127.0}
+SHAPES = {
+    # query heads, KV heads, head dim of the framework's presets
+    "llama3-1b": (32, 8, 64),
+    "llama3-8b": (32, 8, 128),
+    "llama2-7b": (32, 32, 128),
+    "tiny": (4, 2, 64),
+    "d128": (4, 1, 128),
+}
+
+
+# ----------------------------------------------------------------------------- cases
+def listed():
+    return [
+        # one new token of one short request, 1B shape: latency alone
+        {"name": "attn_one_token", "op": "attn", "shape": "llama3-1b", "fmt": "bf16", "rows": 1, "nodes": 1, "lo": 300,
+         "hi": 300, "tree": False},
+        # a decode step of 64 requests over an int8 cache, contexts of the benchmark's prompts and outputs
+        {"name": "attn_decode_int8", "op": "attn", "shape": "llama3-8b", "fmt": "int8", "rows": 64, "nodes": 1, "lo": 129,
+         "hi": 1023, "tree": False},
+        # the benchmark's verify step with its five tokens as a small tree
+        {"name": "attn_verify_tree", "op": "attn", "shape": "llama3-8b", "fmt": "bf16", "rows": 64, "nodes": 5, "lo": 129,
+         "hi": 1023, "tree": True},
+        # a wider tree at a smaller batch, e4m3 cache, contexts off every tile edge
+        {"name": "attn_tree31_e4m3", "op": "attn", "shape": "llama3-8b", "fmt": "e4m3", "rows": 16, "nodes": 31,
+         "lo": 1001, "hi": 4001, "tree": True},
+        # no grouped heads (the 7B shape): every KV head read for 17 nodes
+        {"name": "attn_tree17_mha", "op": "attn", "shape": "llama2-7b", "fmt": "bf16", "rows": 8, "nodes": 17, "lo": 501,
+         "hi": 2013, "tree": True},
+        # one request with a very long context: the work is split along the keys
+        {"name": "attn_long_int8", "op": "attn", "shape": "llama3-8b", "fmt": "int8", "rows": 1, "nodes": 48,
+         "lo": 130999, "hi": 130999, "tree": True},
+        # a prefill round: 512-token chunks of four prompts over the e4m3 cache, arithmetic-bound
+        {"name": "attn_prefill_e4m3", "op": "attn", "shape": "llama3-8b", "fmt": "e4m3", "rows": 4, "nodes": 512, "lo": 0,
+         "hi": 3583, "tree": False},
+        # the benchmark's verify step writing 320 tokens, and reading them back
+        {"name": "write_verify_e4m3", "op": "write", "shape": "llama3-8b", "fmt": "e4m3", "rows": 64, "nodes": 5,
+         "lo": 129, "hi": 1023, "tree": True},
+        # a prefill call of 2048 tokens
+        {"name": "write_prefill_int8", "op": "write", "shape": "llama3-8b", "fmt": "int8", "rows": 4, "nodes": 512,
+         "lo": 0, "hi": 1536, "tree": False},
+        # whole contexts of 64 requests read back (a cache handed to another process, or kept on the host)
+        {"name": "read_contexts_int8", "op": "read", "shape": "llama3-8b", "fmt": "int8", "rows": 64, "nodes": 0,
+         "lo": 129, "hi": 1023, "tree": False},
+        # the end of a round: a few requests of the 1B shape, and the benchmark's depth with a wider tree
+        {"name": "accept_4", "op": "accept", "shape": "llama3-1b", "fmt": "bf16", "rows": 4, "nodes": 15, "lo": 33,
+         "hi": 97, "tree": True, "layers": 16},
+        {"name": "accept_32", "op": "accept", "shape": "llama3-8b", "fmt": "bf16", "rows": 32, "nodes": 31, "lo": 33,
+         "hi": 97, "tree": True, "layers": 32},
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    most = {c["op"]: {"bytes": 0, "flops": 0} for c in listed()}
+    for c in listed():
+        w = work(c)
+        for k in ("bytes", "flops"):
+            most[c["op"]][k] = max(most[c["op"]][k], w[k])
+    while True:
+        op = rng.choice(["attn", "attn", "attn", "write", "read", "accept"])
+        c = {"op": op, "shape": rng.choice(sorted(SHAPES)), "fmt": rng.choice(["bf16", "e4m3", "int8"])}
+        if op == "attn":
+            c["rows"], c["nodes"] = _log(rng, 1, 64), _log(rng, 1, 64)
+            c["tree"] = c["nodes"] > 1 and rng.random() < 0.7
+            if not c["tree"] and rng.random() < 0.4:
+                c["nodes"] = _log(rng, 64, 512)
+            c["hi"] = _log(rng, 1, 131000)
+        elif op == "accept":
+            c["rows"], c["nodes"], c["tree"], c["fmt"] = _log(rng, 1, 32), rng.randint(2, 64), True, "bf16"
+            c["hi"], c["layers"] = rng.randint(1, 97), rng.randint(2, 32)
+        else:
+            c["fmt"] = rng.choice(["e4m3", "int8"])
+            c["rows"], c["nodes"], c["tree"] = _log(rng, 1, 64), _log(rng, 1, 512) if op == "write" else 0, False
+            c["hi"] = _log(rng, 1, 4000)
+        c["lo"] = rng.randint(1 if op == "read" else 0, c["hi"])
+        w = work(c)
+        if all(w[k] <= most[op][k] for k in w):
+            return c
+
+
+def _contexts(case):
+    """Committed positions per row: evenly spread over [lo, hi], in an order that is not sorted."""
+    n = case["rows"]
+    v = [case["lo"] + (case["hi"] - case["lo"]) * i // max(n - 1, 1) for i in range(n)]
+    if n == 1:
+        v = [case["hi"]]
+    step = next((s for s in (7, 11, 13, 17, 19) if n % s), 1)
+    return [v[i * step % n] for i in range(n)]
+
+
+def _max_seq(case):
+    return (case["hi"] + max(case["nodes"], 1) + 63) // 64 * 64
+
+
+def work(case):
+    H, Hkv, D = SHAPES[case["shape"]]
+    eb = 2 if case["fmt"] == "bf16" else 1
+    slot = 2 * Hkv * (D * eb + (0 if eb == 2 else 1))            # K and V (and their exponents) of one slot
+    ctx, T = _contexts(case), case["nodes"]
+    n = T * len(ctx)
+    if case["op"] == "attn":
+        keys = sum(ctx) + n
+        seen = sum(T * c + (T * (T + 1) // 2 if not case["tree"] else 2 * T) for c in ctx)
+        mask = n * 8 if case["tree"] else 0
+        return {"bytes": keys * slot + 2 * n * H * D * 2 + mask, "flops": 4 * H * D * seen}
+    if case["op"] == "write":          # read q, k, v; write q and the 8-bit slots; read those back, write them as bf16
+        return {"bytes": n * (2 * H * D * 2 + 2 * Hkv * D * 2 + 2 * slot + 2 * Hkv * D * 2), "flops": n * 6 * (H + 2 * Hkv) * D}
+    if case["op"] == "read":
+        return {"bytes": sum(ctx) * (slot + 2 * Hkv * D * 2 + 8), "flops": sum(ctx) * 2 * Hkv * D}
+    moved = 3 * len(ctx)               # a path of a few nodes is accepted
+    return {"bytes": n * 12 + moved * 2 * slot * case["layers"], "flops": n}
+
+
+# ----------------------------------------------------------------------------- inputs
+def _parents(case, rng):
+    """Parents of every block's nodes: a random tree of some breadth (nodes in topological order)."""
+    T = case["nodes"]
+    out = []
+    for _ in range(case["rows"]):
+        if not case["tree"]:
+            out.append([-1] + list(range(T - 1)))
+        else:
+            out.append([-1] + [int(rng.integers(max(0, i - 1 - i // 2), i)) for i in range(1, T)])
+    return out
+
+
+def _depths(parents):
+    d = []
+    for p in parents:
+        d.append(0 if p < 0 else d[p] + 1)
+    return d
+
+
+def _mask_words(parents):
+    """Bit j of node i's row: i sees node j (its ancestors and itself)."""
+    W = (len(parents) + 63) // 64
+    vis = []
+    for i, p in enumerate(parents):
+        vis.append((vis[p] if p >= 0 else 0) | 1 << i)
+    words = [[v >> 64 * w & (1 << 64) - 1 for w in range(W)] for v in vis]
+    return np.array(words, dtype=np.uint64).view(np.int64).reshape(len(parents), W)
+
+
+def _quantise(x, fmt):
+    """(8-bit values, exponent bytes) of x [..., D]; exact for finite x."""
+    x = x.float()
+    m, e = torch.frexp(x.abs().amax(-1))                        # amax = m 2^e, m in [0.5, 1)
+    q = QMAX[fmt]
+    limit, shift = math.frexp(q)
+    e = e - shift + (m > limit).int()
+    e = torch.where(m == 0, torch.full_like(e, -100), e).clamp(-100, 120)
+    y = torch.ldexp(x, -e[..., None])
+    y = y.to(torch.float8_e4m3fn) if fmt == "e4m3" else y.round().to(torch.int8)
+    return y, (e + 127).to(torch.uint8)
+
+
+def _values(q, e):
+    return torch.ldexp(q.float(), (e.int() - 127)[..., None])
+
+
+def _rope_tables(max_pos, D):
+    inv = 1.0 / 500000.0 ** (torch.arange(0, D, 2, dtype=torch.float64) / D)
+    a = torch.outer(torch.arange(max_pos, dtype=torch.float64), inv)
+    a = torch.cat([a, a], -1)
+    return a.cos().float().cuda(), a.sin().float().cuda()
+
+
+def prepare(case, seed):
+    H, Hkv, D = SHAPES[case["shape"]]
+    dev = torch.device("cuda")
+    g = torch.Generator(device=dev).manual_seed(seed)
+    rng = np.random.default_rng(seed)
+    B, T, S, fmt, op = case["rows"], case["nodes"], _max_seq(case), case["fmt"], case["op"]
+    L = case.get("layers", 1)
+    ctx = _contexts(case)
+    st = {"case": case, "ctx": ctx, "H": H, "Hkv": Hkv, "D": D, "S": S}
+
+    def normal(*shape):
+        return torch.randn(*shape, device=dev, generator=g)
+
+    def kv(layers, scale):
+        """One cache half: keys with a few strong channels, slots of different size, a small first slot."""
+        x = torch.empty(layers, B, Hkv, S, D, device=dev, dtype=torch.bfloat16)
+        ch = 1 + 3 * (torch.rand(Hkv, 1, D, device=dev, generator=g) < 0.03)
+        size = torch.exp(0.4 * normal(B, Hkv, S, 1)) * scale
+        size[:, :, 0] *= 0.1
+        for i in range(layers):
+            x[i] = (normal(B, Hkv, S, D) * ch * size).bfloat16()
+        return x
+
+    K, V = kv(L, 1.0), kv(L, 0.7)
+    if fmt == "bf16":
+        st["k"], st["v"], st["ke"], st["ve"] = K, V, None, None
+    else:
+        (st["k"], st["ke"]), (st["v"], st["ve"]) = _quantise(K, fmt), _quantise(V, fmt)
+    del K, V
+    if op == "read":
+        st["tok_row"] = torch.tensor([b for b in range(B) for _ in range(ctx[b])], dtype=torch.int32, device=dev)
+        st["tok_slot"] = torch.tensor([s for b in range(B) for s in range(ctx[b])], dtype=torch.int32, device=dev)
+    else:
+        parents = _parents(case, rng)
+        st["parents"] = parents
+        pos = [ctx[b] + d for b in range(B) for d in _depths(parents[b])]
+        st["tok_pos"] = torch.tensor(pos, dtype=torch.int32, device=dev)
+        st["tok_row"] = torch.tensor([b for b in range(B) for _ in range(T)], dtype=torch.int32, device=dev)
+        st["tok_slot"] = torch.tensor([ctx[b] + i for b in range(B) for i in range(T)], dtype=torch.int32, device=dev)
+        st["mask"] = None
+        if case["tree"]:
+            st["mask"] = torch.from_numpy(np.concatenate([_mask_words(p) for p in parents])).to(dev)
+    n = B * T
+    if op == "attn":
+        st["q"] = (normal(n, H * D) * 0.8).bfloat16()
+    elif op == "write":
+        st["qkv"] = (normal(n, (H + 2 * Hkv) * D) * torch.exp(0.5 * normal(n, 1))).bfloat16()
+        st["cos"], st["sin"] = _rope_tables(S, D)
+    elif op == "accept":
+        # drafted tokens, and the model's: one of the node's children most of the time
+        ids = rng.integers(0, 32000, n).astype(np.int32)
+        y = rng.integers(0, 32000, n).astype(np.int32)
+        for b, p in enumerate(parents):
+            for i in range(T):
+                kids = [j for j in range(T) if p[j] == i]
+                if kids and rng.random() < 0.75:
+                    y[b * T + i] = ids[b * T + kids[rng.integers(0, len(kids))]]
+        st["ids"], st["y"] = torch.from_numpy(ids).to(dev), torch.from_numpy(y).to(dev)
+        st["parent"] = torch.tensor([v for p in parents for v in p], dtype=torch.int32, device=dev)
+        st["ctx_t"] = torch.tensor(ctx, dtype=torch.int32, device=dev)
+    if own:
+        _prepare_own(st)
+    return st
+
+
+def _prepare_own(st):
+    """The handles a user's program keeps: the cache, the round's tree metadata, outputs and workspace."""
+    from thesis_b200 import tree as tr
+
+    case, H, Hkv, D = st["case"], st["H"], st["Hkv"], st["D"]
+    dev = st["k"].device
+    n = case["rows"] * case["nodes"]
+    st["cache"] = tr.KVCache.wrap(st["k"], st["v"], st["ke"], st["ve"])
+    if case["op"] == "read":
+        m = st["tok_row"].numel()
+        st["k_out"] = torch.empty(m, Hkv, D, dtype=torch.bfloat16, device=dev)
+        st["v_out"] = torch.empty_like(st["k_out"])
+        return
+    blocks = [(b, st["ctx"][b], p if case["tree"] else case["nodes"]) for b, p in enumerate(st["parents"])]
+    st["tree"] = tr.TreeBatch(blocks, st["cache"])
+    if case["op"] == "attn":
+        st["out"] = torch.empty(n, H * D, dtype=torch.bfloat16, device=dev)
+        st["ws"] = tr.attention_workspace(st["tree"], st["cache"], H)
+    elif case["op"] == "write":
+        st["q_out"] = torch.empty(n, H * D, dtype=torch.bfloat16, device=dev)
+        st["k_out"] = torch.empty(n, Hkv, D, dtype=torch.bfloat16, device=dev)
+        st["v_out"] = torch.empty_like(st["k_out"])
+    else:
+        st["path"] = torch.empty(case["rows"], case["nodes"], dtype=torch.int32, device=dev)
+        st["n_acc"] = torch.empty(case["rows"], dtype=torch.int32, device=dev)
+        st["next"] = torch.empty(case["rows"], dtype=torch.int32, device=dev)
+
+
+# ----------------------------------------------------------------------------- one pass
+def run(st):
+    op = st["case"]["op"]
+    if own:
+        return _run_own(st, op)
+    return {"attn": _plain_attn, "write": _plain_write, "read": _plain_read, "accept": _plain_accept}[op](st)
+
+
+def _run_own(st, op):
+    from thesis_b200 import tree as tr
+
+    if op == "attn":
+        return tr.tree_attention(st["q"], st["cache"], st["tree"], st["out"], workspace=st["ws"])
+    if op == "write":
+        tr.kv_append(st["qkv"], st["cache"], st["tree"], st["cos"], st["sin"], q_out=st["q_out"])
+        tr.kv_read(st["cache"], st["tok_row"], st["tok_slot"], st["k_out"], st["v_out"])
+        return st["q_out"], st["k_out"], st["v_out"]
+    if op == "read":
+        tr.kv_read(st["cache"], st["tok_row"], st["tok_slot"], st["k_out"], st["v_out"])
+        return st["k_out"], st["v_out"]
+    tr.tree_accept(st["y"], st["ids"], st["tree"], st["path"], st["n_acc"], st["next"])
+    tr.kv_compact(st["cache"], st["tree"], st["path"], st["n_acc"])
+    return st["path"], st["n_acc"], st["next"], st["k"], st["v"]
+
+
+def _plain_attn(st):
+    case, H, Hkv, D, T = st["case"], st["H"], st["Hkv"], st["D"], st["case"]["nodes"]
+    G = H // Hkv
+    out = torch.empty_like(st["q"])
+    dev = out.device
+    i = torch.arange(T, device=dev)
+    for b, c in enumerate(st["ctx"]):
+        k, v = st["k"][0, b, :, :c + T], st["v"][0, b, :, :c + T]
+        if st["ke"] is None:
+            k, v = k.float(), v.float()
+        else:
+            k, v = _values(k, st["ke"][0, b, :, :c + T]), _values(v, st["ve"][0, b, :, :c + T])
+        q = st["q"][b * T:(b + 1) * T].float().view(T, Hkv, G, D).permute(1, 2, 0, 3).reshape(Hkv, G * T, D)
+        s = (q @ k.transpose(1, 2)).view(Hkv, G, T, c + T) / math.sqrt(D)
+        if st["mask"] is None:
+            see = i[None, :] <= i[:, None]
+        else:
+            m = st["mask"][b * T:(b + 1) * T]
+            see = (m[:, i // 64] >> (i % 64)[None, :] & 1).bool()
+        s[..., c:] = s[..., c:].masked_fill(~see, float("-inf"))
+        p = torch.exp(s - s.amax(-1, keepdim=True))
+        o = (p.view(Hkv, G * T, -1) @ v).view(Hkv, G, T, D) / p.sum(-1, keepdim=True)
+        out[b * T:(b + 1) * T] = o.permute(2, 0, 1, 3).reshape(T, H * D).bfloat16()
+    return out
+
+
+def _rotate(x, cos, sin):
+    """x [n, heads, D] bf16; cos, sin [n, 1, D] rounded to bf16; every product and the sum rounded to bf16."""
+    x1, x2 = x.float().chunk(2, -1)
+    turned = torch.cat([-x2, x1], -1)
+    a, b = (x.float() * cos).bfloat16().float(), (turned * sin).bfloat16().float()
+    return (a + b).bfloat16()
+
+
+def _plain_write(st):
+    H, Hkv, D, fmt = st["H"], st["Hkv"], st["D"], st["case"]["fmt"]
+    q, k, v = st["qkv"].split([H * D, Hkv * D, Hkv * D], -1)
+    pos, row, slot = st["tok_pos"].long(), st["tok_row"].long(), st["tok_slot"].long()
+    cos, sin = (t[pos].bfloat16().float()[:, None] for t in (st["cos"], st["sin"]))
+    q = _rotate(q.view(-1, H, D), cos, sin).view(-1, H * D)
+    k, v = _rotate(k.view(-1, Hkv, D), cos, sin), v.view(-1, Hkv, D)
+    for x, data, exps in ((k, st["k"], st["ke"]), (v, st["v"], st["ve"])):
+        y, e = _quantise(x, fmt)
+        data.view(torch.uint8)[0, row, :, slot] = y.view(torch.uint8)
+        exps[0, row, :, slot] = e
+    return (q, *_read(st, row, slot))
+
+
+def _read(st, row, slot):
+    return tuple(_values(data.view(torch.uint8)[0, row, :, slot].view(data.dtype), exps[0, row, :, slot]).bfloat16()
+                 for data, exps in ((st["k"], st["ke"]), (st["v"], st["ve"])))
+
+
+def _plain_read(st):
+    return _read(st, st["tok_row"].long(), st["tok_slot"].long())
+
+
+def _plain_accept(st):
+    B, T = st["case"]["rows"], st["case"]["nodes"]
+    y, ids, parent = (st[k].view(B, T) for k in ("y", "ids", "parent"))
+    dev = y.device
+    i = torch.arange(T, device=dev)
+    cur, going, n_acc = torch.zeros(B, 1, dtype=torch.long, device=dev), torch.ones(B, 1, dtype=torch.bool, device=dev), 0
+    path = [torch.zeros(B, 1, dtype=torch.long, device=dev)]
+    n_acc = torch.zeros(B, 1, dtype=torch.long, device=dev)
+    for _ in range(T - 1):
+        fits = (parent == cur) & (ids == y.gather(1, cur)) & (i > 0)
+        child = torch.where(fits, i, T).amin(1, keepdim=True)
+        going = going & (child < T)
+        cur = torch.where(going, child, cur)
+        n_acc = n_acc + going
+        path.append(torch.where(going, cur, -1))
+    path = torch.cat(path, 1)
+    b = torch.arange(B, device=dev)[:, None].expand(B, T)
+    src = st["ctx_t"].long()[:, None] + torch.where(path < 0, i, path)          # a slot past the path stays as it is
+    dst = st["ctx_t"].long()[:, None] + i
+    for t in (st["k"], st["v"]):
+        for layer in t:
+            layer.transpose(1, 2)[b, dst] = layer.transpose(1, 2)[b, src]
+    return path.int(), n_acc[:, 0].int(), y.gather(1, cur)[:, 0].int(), st["k"], st["v"]
+
+
+# ----------------------------------------------------------------------------- the definition in 64 bits
+def exact(case, seed):
+    global own
+    was, own = own, False
+    try:
+        st = prepare(case, seed)
+    finally:
+        own = was
+    H, Hkv, D, T = st["H"], st["Hkv"], st["D"], case["nodes"]
+
+    def double(q, e):
+        return q.double() if e is None else q.double() * torch.exp2(e.double() - 127)[..., None]
+
+    if case["op"] == "attn":
+        out = torch.zeros(case["rows"] * T, H * D, dtype=torch.float64, device="cuda")
+        for b, c in enumerate(st["ctx"]):
+            see = torch.zeros(T, T, dtype=torch.bool)
+            for i in range(T):
+                j = i
+                while j >= 0:
+                    see[i, j] = True
+                    j = st["parents"][b][j]
+            see = see.cuda()
+            for h in range(Hkv):
+                k = double(st["k"][0, b, h, :c + T], None if st["ke"] is None else st["ke"][0, b, h, :c + T])
+                v = double(st["v"][0, b, h, :c + T], None if st["ve"] is None else st["ve"][0, b, h, :c + T])
+                for j in range(h * (H // Hkv), (h + 1) * (H // Hkv)):
+                    s = st["q"][b * T:(b + 1) * T, j * D:(j + 1) * D].double() @ k.T * D ** -0.5
+                    s[:, c:][~see] = -math.inf
+                    out[b * T:(b + 1) * T, j * D:(j + 1) * D] = torch.exp(s - torch.logsumexp(s, -1)[:, None]) @ v
+        return out
+    if case["op"] == "accept":
+        y, ids = st["y"].tolist(), st["ids"].tolist()
+        path, n_acc, last = np.full((case["rows"], T), -1, np.int32), [], []
+        for b, p in enumerate(st["parents"]):
+            walk = [0]
+            while True:
+                want = y[b * T + walk[-1]]
+                kid = [j for j in range(1, T) if p[j] == walk[-1] and ids[b * T + j] == want]
+                if not kid:
+                    break
+                walk.append(kid[0])
+            path[b, :len(walk)] = walk
+            n_acc.append(len(walk) - 1)
+            last.append(y[b * T + walk[-1]])
+            for t in (st["k"], st["v"]):
+                c = st["ctx"][b]
+                t[:, b, :, c:c + len(walk)] = t[:, b, :, [c + w for w in walk]].clone()
+        return (torch.from_numpy(path), torch.tensor(n_acc, dtype=torch.int32), torch.tensor(last, dtype=torch.int32),
+                st["k"], st["v"])
+    row, slot = st["tok_row"].long(), st["tok_slot"].long()
+    if case["op"] == "read":
+        return tuple(double(d.view(torch.uint8)[0, row, :, slot].view(d.dtype), e[0, row, :, slot])
+                     for d, e in ((st["k"], st["ke"]), (st["v"], st["ve"])))
+    cos, sin = (t[st["tok_pos"].long()].bfloat16().double() for t in (st["cos"], st["sin"]))
+    x = st["qkv"].double().view(-1, H + 2 * Hkv, D)
+    turn, half = x[:, :H + Hkv], D // 2
+    even = (turn[..., :half] * cos[:, None, :half]).bfloat16().double() - (turn[..., half:] * sin[:, None, :half]).bfloat16().double()
+    odd = (turn[..., half:] * cos[:, None, half:]).bfloat16().double() + (turn[..., :half] * sin[:, None, half:]).bfloat16().double()
+    turned = torch.cat([even, odd], -1).bfloat16().double()
+
+    def eight(z):
+        z = z.cpu().numpy()
+        top = np.abs(z).max(-1)
+        e = np.full(top.shape, -100)
+        for k in range(-100, 120):                                   # the smallest exponent that holds the largest value
+            e += top > QMAX[case["fmt"]] * 2.0 ** k
+        u = z / 2.0 ** e[..., None]
+        if case["fmt"] == "int8":
+            u = np.rint(u)
+        else:                                                        # 4 significant bits, subnormals below 2^-6
+            step = 2.0 ** (np.floor(np.log2(np.maximum(np.abs(u), 2.0 ** -6))) - 3)
+            u = np.rint(u / step) * step
+        return torch.from_numpy(u * 2.0 ** e[..., None])
+
+    return turned[:, :H].reshape(-1, H * D), eight(turned[:, H:]), eight(x[:, H + Hkv:])
