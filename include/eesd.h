@@ -262,6 +262,106 @@ int eesd_head_argmax_static(const void* x, int x_rows, const int32_t* rows, int 
                             const void* norm_w, const void* lm_head, float eps, int32_t* out_ids,
                             int32_t* status_out, void* stream);
 
+/* ------------------------------------------------------------------------------------ */
+/* Tree drafts and 8-bit KV caches: primitives for a draft/verify step whose drafts form a tree, over a
+ * cache in the model dtype or in 8 bits.  The reference drafts chains over an unquantised cache
+ * (solutions/packed.py:142-196, solutions/engine.py:453-475); with chains and EESD_KV_MODEL these calls
+ * compute what eesd_rope_kv_append, eesd_attn_varlen_gqa and eesd_greedy_accept compute.
+ *
+ * One round: eesd_tree_meta once; per layer eesd_kv_append, then eesd_attn_tree; after the head
+ * eesd_tree_accept, then eesd_kv_compact over all layers (the accepted path's K/V move to the front, so
+ * that positions ctx .. ctx + n_acc of every row hold the path; rollback stays a length reset). */
+
+#define EESD_KV_MODEL 0        /* elements of the model dtype (EESD_BF16 or EESD_F32) */
+#define EESD_KV_E4M3 1         /* 8-bit floats (4 exponent, 3 mantissa bits, no infinities), max 448 */
+#define EESD_KV_INT8 2         /* 8-bit integers -127 .. 127 */
+
+/* 8-bit formats: K and V each have one power-of-two scale 2^e per (row, KV head, slot), stored as the
+ * byte e + 127.  e is the smallest integer with max|x| <= Q 2^e (Q = 448 or 127) and e >= -100; the
+ * stored element is x 2^-e rounded to nearest even, so every element is within half a step of x and
+ * reads back exactly into bf16.  A vector with an infinity or NaN stores byte 255 and zeros, and reads
+ * back as NaN. */
+typedef struct EesdKvCache {
+  int32_t format;                /* EESD_KV_* */
+  int32_t n_layers, max_batch, n_kv_heads, max_seq, head_dim;   /* head_dim 64 or 128 */
+  void* k;                       /* [n_layers, max_batch, Hkv, max_seq, D], 16-byte aligned */
+  void* v;
+  uint8_t* k_exp;                /* [n_layers, max_batch, Hkv, max_seq], 16-byte aligned; 8-bit formats only */
+  uint8_t* v_exp;
+} EesdKvCache;
+
+#define EESD_TREE_MAX_NODES 256  /* nodes per block with a visibility mask (or eesd_tree_accept) */
+
+/* Blocks of tree nodes.  Block b: T nodes of cache row `row` behind `ctx` committed positions; node i
+ * sits at cache slot ctx + i.  A tree's nodes are numbered so that parent[i] < i (indices within the
+ * block; -1 for a node whose parent is the committed context). */
+typedef struct EesdTree {
+  int32_t n_tokens, n_blocks;
+  int32_t max_nodes;             /* host: largest T, at least */
+  int32_t max_ctx;               /* host: largest ctx + T, at least (<= max_seq) */
+  int32_t words;                 /* 64-bit words per mask row: (max_nodes + 63) / 64, at most 4; 0 without a mask */
+  int32_t reserved;              /* 0 */
+  const int32_t* blk;            /* [n_blocks, 4] = (start, T, row, ctx); the blocks tile the tokens */
+  const int32_t* parent;         /* [n_tokens], NULL: every block is a chain */
+  int32_t* tok_pos;              /* [n_tokens] RoPE position: ctx + depth */
+  int32_t* tok_slot;             /* [n_tokens] cache slot: ctx + i */
+  int32_t* tok_row;              /* [n_tokens] cache row */
+  uint64_t* mask;                /* [n_tokens, words]: bit j of node i's row: i sees node j of its block.  NULL:
+                                    causal, i sees nodes 0 .. i.  Any mask works in eesd_attn_tree. */
+} EesdTree;
+
+/* tok_pos, tok_slot, tok_row and (unless NULL) mask from blk and parent, on the device: a node sees its
+ * ancestors and itself.  A block outside the tokens or the cache, or a parent that does not come before
+ * its node, sets a bit in *status (device int32, nullable); the tokens of a bad block get slot -1, which
+ * eesd_kv_append and eesd_kv_read skip, and a bad parent counts as -1. */
+int eesd_tree_meta(const EesdTree* tree, int max_batch, int max_seq, int32_t* status, void* stream);
+
+/* RoPE of q and k and the KV append of n_tok packed tokens into layer `layer`, quantising where the
+ * cache is 8-bit.  The rounding of q and k is that of eesd_rope_kv_append (in the model dtype); the 8-bit
+ * element is the quantised model-dtype element.  qkv [n_tok, (Hq + 2 Hkv) D], tokens ld_qkv elements apart
+ * (ld_qkv % 8 == 0); q_out [n_tok, Hq D] receives the rotated q (NULL: in place in qkv).  tok_pos indexes the
+ * RoPE tables [rope_len, D], tok_slot (NULL: tok_pos) the cache.  A token whose position, row or slot is
+ * out of range sets a bit in *status and is skipped.  Two tokens with the same row and slot: the slot
+ * holds neither reliably. */
+int eesd_kv_append(int dtype, const EesdKvCache* cache, int layer, void* qkv, int ld_qkv, int n_heads,
+                   const int32_t* tok_pos, const int32_t* tok_slot, const int32_t* tok_row, int n_tok,
+                   const float* rope_cos, const float* rope_sin, int rope_len, void* q_out, int32_t* status, void* stream);
+
+/* k_out / v_out [n_tok, Hkv, D] (each nullable, 16-byte aligned) = the values of layer `layer` at
+ * (tok_row[t], tok_slot[t]), in dtype.  A token out of range sets a bit in *status; its outputs are left. */
+int eesd_kv_read(int dtype, const EesdKvCache* cache, int layer, const int32_t* tok_slot, const int32_t* tok_row, int n_tok,
+                 void* k_out, void* v_out, int32_t* status, void* stream);
+
+/* Attention of tree nodes (or causal chains of any length, e.g. prefill chunks) over one layer of the
+ * cache, which already holds the nodes' K and V: node i of a block sees the slots below ctx and those
+ * nodes of its block that the mask (NULL: causality) shows; softmax scale 1 / sqrt(D).  A node that sees
+ * nothing (ctx 0, empty mask row) gets zeros.  K and V in slots that a node does not see, NaN and
+ * infinities among them, do not reach it.  q: rotated queries, tokens ld_q elements apart (ld_q % 8 == 0,
+ * 16-byte aligned), Hq D used; out [n_tokens, Hq D].  split_keys: 0 lets the library split long key ranges
+ * over CTAs as the launch needs; a multiple of 256 fixes the split, so that a block's result does not
+ * depend on the other blocks of the launch.  workspace: eesd_attn_tree_workspace_bytes() bytes, 256-byte aligned,
+ * not initialised, not shared by calls that may overlap.  A block that does not fit the tree's maxima or
+ * the cache sets a bit in *status and is skipped. */
+size_t eesd_attn_tree_workspace_bytes(int dtype, const EesdKvCache* cache, const EesdTree* tree, int n_heads, int split_keys);
+int eesd_attn_tree(int dtype, const EesdKvCache* cache, int layer, const EesdTree* tree, const void* q, int ld_q,
+                   int n_heads, void* out, int split_keys, void* workspace, size_t workspace_bytes, int32_t* status,
+                   void* stream);
+
+/* Greedy acceptance in a tree (for chains what eesd_greedy_accept computes).  ids[n_tokens]: the node's
+ * token; y [n_tokens]: the model's token after the node.  From node 0: go to the lowest-numbered child whose
+ * id is y of the current node, until there is none.  path [n_blocks, max_nodes]: the visited nodes, node 0
+ * first, then -1; n_acc [n_blocks]: visited nodes - 1; next [n_blocks]: y of the last one.  tree: blk, parent,
+ * max_nodes are used.  A bad block sets a bit in *status: path -1, n_acc -1, next -1. */
+int eesd_tree_accept(const int32_t* y, const int32_t* ids, const EesdTree* tree, int32_t* path, int32_t* n_acc,
+                     int32_t* next, int32_t* status, void* stream);
+
+/* In all layers: slot ctx + j of every block's row = slot ctx + path[b, j], j = 1 .. n_acc[b] (K, V and
+ * exponents).  path [n_blocks, max_nodes] must rise (eesd_tree_accept's does); a block whose path does not,
+ * or that does not fit, sets a bit in *status and is left as it is.  Blocks of one call are on different
+ * rows. */
+int eesd_kv_compact(int dtype, const EesdKvCache* cache, const EesdTree* tree, const int32_t* path, const int32_t* n_acc,
+                    int32_t* status, void* stream);
+
 /* Device status word helpers for the primitive kernels (a caller-owned int32). */
 int eesd_status_read(const int32_t* status, int* bits_out, void* stream);
 

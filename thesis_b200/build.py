@@ -13,13 +13,15 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "_lib" / "libeesd.so"
-SOURCES = ["gemm_tc.cu", "kernels.cu", "runtime.cu", "head_static.cu"]
+SOURCES = ["gemm_tc.cu", "kernels.cu", "runtime.cu", "head_static.cu", "cache_ops.cu", "attn_tree.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -43,12 +45,19 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         return LIB
     LIB.parent.mkdir(parents=True, exist_ok=True)
     tmp = LIB.with_suffix(".so.tmp")
-    cmd = [nvcc(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "-shared", "-Xcompiler", "-fPIC,-O2",
-           "-I", str(ROOT / "include"), "-o", str(tmp)] + [str(CSRC / s) for s in SOURCES]
+    flags = [*ARCH, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-O2", "-I", str(ROOT / "include")]
     if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-        print(" ".join(cmd), flush=True)
-    subprocess.run(cmd, check=True, cwd=str(CSRC))
+        flags.insert(0, "-Xptxas=-v")
+
+    def run(cmd):
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        subprocess.run(cmd, check=True, cwd=str(CSRC))
+
+    with tempfile.TemporaryDirectory() as d, ThreadPoolExecutor(len(SOURCES)) as pool:   # one nvcc per source
+        objs = [str(Path(d) / (s + ".o")) for s in SOURCES]
+        list(pool.map(lambda so: run([nvcc(), *flags, "-c", str(CSRC / so[0]), "-o", so[1]]), zip(SOURCES, objs)))
+        run([nvcc(), *flags, "-shared", "-o", str(tmp), *objs])
     os.replace(tmp, LIB)
     return LIB
 

@@ -1,0 +1,25 @@
+// Internal interface of the tree attention and its C entry points' helpers (not part of the C ABI).
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "../../include/eesd.h"
+
+namespace eesd {
+
+struct CacheGeom;
+
+// record a formatted message for eesd_last_error() and return `code`
+int fail_arg(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+// the stream must be one of the current device's (a launch on another device's stream would read foreign memory)
+int check_stream(const char* who, void* stream);
+int check_cache(const char* who, int dtype, const EesdKvCache* c, int layer);
+int check_tree(const char* who, const EesdTree* t);
+CacheGeom cache_layer(const EesdKvCache* c, int dtype, int layer);
+inline size_t cache_elem_bytes(const EesdKvCache* c, int dtype) {
+  return c->format != EESD_KV_MODEL ? 1 : dtype == EESD_BF16 ? 2 : 4;
+}
+
+}  // namespace eesd

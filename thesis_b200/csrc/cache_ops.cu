@@ -1,0 +1,536 @@
+// Tree metadata, quantising KV append and read-back, tree acceptance and cache compaction: the kernels
+// around the tree attention, and their C entry points.
+#include <stdarg.h>
+#include <stdio.h>
+
+#include "attn_tree.h"
+#include "cache.cuh"
+#include "kernels.h"
+
+namespace eesd {
+
+int fail_arg(int code, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof buf, fmt, ap);
+  va_end(ap);
+  set_last_error(buf);
+  return code;
+}
+
+int check_stream(const char* who, void* stream) {
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  cudaError_t e = cudaStreamIsCapturing(s, &cap);
+  if (e == cudaSuccess && cap != cudaStreamCaptureStatusNone) return EESD_OK;   // the device query below would end the capture
+  int dev = -1, sdev = -2;
+  if (e == cudaSuccess) e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaStreamGetDevice(s, &sdev);
+  if (e != cudaSuccess) return fail_arg(EESD_ERR_CUDA, "%s: stream: %s", who, cudaGetErrorString(e));
+  if (dev != sdev) return fail_arg(EESD_ERR_ARG, "%s: the stream belongs to device %d, the current device is %d", who, sdev, dev);
+  return EESD_OK;
+}
+
+int check_cache(const char* who, int dtype, const EesdKvCache* c, int layer) {
+  if (!c || !c->k || !c->v) return fail_arg(EESD_ERR_ARG, "%s: null cache", who);
+  if (dtype != EESD_BF16 && dtype != EESD_F32) return fail_arg(EESD_ERR_ARG, "%s: dtype %d", who, dtype);
+  if (c->format < EESD_KV_MODEL || c->format > EESD_KV_INT8) return fail_arg(EESD_ERR_ARG, "%s: cache format %d", who, c->format);
+  if (c->head_dim != 64 && c->head_dim != 128) return fail_arg(EESD_ERR_ARG, "%s: head_dim %d (64 or 128)", who, c->head_dim);
+  if (c->n_layers <= 0 || c->max_batch <= 0 || c->n_kv_heads <= 0 || c->max_seq <= 0 || c->max_seq % 16)
+    return fail_arg(EESD_ERR_ARG, "%s: cache sizes (max_seq must be a multiple of 16)", who);
+  if ((long long)c->max_batch * c->n_kv_heads * c->max_seq >= (1LL << 31))
+    return fail_arg(EESD_ERR_ARG, "%s: more than 2^31 slots in one layer of the cache", who);
+  if (layer < 0 || layer >= c->n_layers) return fail_arg(EESD_ERR_ARG, "%s: layer %d of %d", who, layer, c->n_layers);
+  uintptr_t a = reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v);
+  if (c->format != EESD_KV_MODEL) {
+    if (!c->k_exp || !c->v_exp) return fail_arg(EESD_ERR_ARG, "%s: an 8-bit cache needs k_exp and v_exp", who);
+    a |= reinterpret_cast<uintptr_t>(c->k_exp) | reinterpret_cast<uintptr_t>(c->v_exp);
+  }
+  if (a & 15) return fail_arg(EESD_ERR_ARG, "%s: cache pointers must be 16-byte aligned", who);
+  return EESD_OK;
+}
+
+int check_tree(const char* who, const EesdTree* t) {
+  if (!t) return fail_arg(EESD_ERR_ARG, "%s: null tree", who);
+  if (t->n_tokens < 0 || t->n_blocks < 0 || t->n_blocks > 65535)
+    return fail_arg(EESD_ERR_ARG, "%s: n_tokens %d, n_blocks %d (at most 65535)", who, t->n_tokens, t->n_blocks);
+  if (t->n_tokens == 0 || t->n_blocks == 0) return EESD_OK;
+  if (!t->blk || t->max_nodes <= 0 || t->max_ctx <= 0) return fail_arg(EESD_ERR_ARG, "%s: missing block metadata", who);
+  if (t->mask && (t->max_nodes > EESD_TREE_MAX_NODES || t->words != (t->max_nodes + 63) / 64))
+    return fail_arg(EESD_ERR_ARG, "%s: a mask needs max_nodes <= %d and words = (max_nodes + 63) / 64", who, EESD_TREE_MAX_NODES);
+  return EESD_OK;
+}
+
+CacheGeom cache_layer(const EesdKvCache* c, int dtype, int layer) {
+  const size_t slots = (size_t)c->max_batch * c->n_kv_heads * c->max_seq * layer;
+  const size_t eb = cache_elem_bytes(c, dtype);
+  CacheGeom g{c->n_kv_heads, c->max_batch, c->max_seq, nullptr, nullptr, nullptr, nullptr};
+  g.k = static_cast<const uint8_t*>(c->k) + slots * c->head_dim * eb;
+  g.v = static_cast<const uint8_t*>(c->v) + slots * c->head_dim * eb;
+  if (c->format != EESD_KV_MODEL) {
+    g.ke = c->k_exp + slots;
+    g.ve = c->v_exp + slots;
+  }
+  return g;
+}
+
+namespace {
+
+// ---------------------------------------------------------------- metadata
+// One CTA per block.  Each thread walks up from its nodes through the parents in shared memory (at most
+// depth steps), counting the depth and setting the ancestors' bits.  Latency-bound: a few us.
+__global__ void __launch_bounds__(128) tree_meta_kernel(EesdTree t, int max_batch, int max_seq, int* status) {
+  pdl_trigger();
+  pdl_wait();
+  __shared__ int16_t par[EESD_TREE_MAX_NODES];
+  const int b = blockIdx.x;
+  const int start = t.blk[4 * b], T = t.blk[4 * b + 1], row = t.blk[4 * b + 2], ctx = t.blk[4 * b + 3];
+  if (start < 0 || T <= 0 || start > t.n_tokens - T) {
+    if (threadIdx.x == 0) set_status(status, kStatusBadIndex);
+    return;
+  }
+  const bool ok = row >= 0 && row < max_batch && ctx >= 0 && T <= t.max_nodes && ctx <= max_seq - T;
+  if (!ok && threadIdx.x == 0) set_status(status, kStatusBadIndex);
+  const bool tree = t.parent && T <= EESD_TREE_MAX_NODES;   // the entry point refuses parents with larger max_nodes
+  if (tree)
+    for (int i = threadIdx.x; i < T; i += blockDim.x) {
+      int p = t.parent[start + i];
+      if (p < -1 || p >= i) {
+        set_status(status, kStatusBadIndex);
+        p = -1;
+      }
+      par[i] = (int16_t)p;
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < T; i += blockDim.x) {
+    uint64_t m0 = 0, m1 = 0, m2 = 0, m3 = 0;
+    int depth = -1;
+    if (tree) {
+      for (int j = i; j >= 0; j = par[j]) {
+        ++depth;
+        const uint64_t bit = 1ull << (j & 63);
+        m0 |= (j >> 6) == 0 ? bit : 0;
+        m1 |= (j >> 6) == 1 ? bit : 0;
+        m2 |= (j >> 6) == 2 ? bit : 0;
+        m3 |= (j >> 6) == 3 ? bit : 0;
+      }
+    } else {
+      depth = i;
+      auto upto = [&](int w) { return i >= 64 * w + 63 ? ~0ull : i < 64 * w ? 0ull : (2ull << (i - 64 * w)) - 1; };
+      m0 = upto(0);
+      m1 = upto(1);
+      m2 = upto(2);
+      m3 = upto(3);
+    }
+    const int tok = start + i;
+    t.tok_pos[tok] = ok ? ctx + depth : -1;
+    t.tok_slot[tok] = ok ? ctx + i : -1;
+    t.tok_row[tok] = ok ? row : -1;
+    if (t.mask) {
+      uint64_t* m = t.mask + (size_t)tok * t.words;
+      m[0] = m0;
+      if (t.words > 1) m[1] = m1;
+      if (t.words > 2) m[2] = m2;
+      if (t.words > 3) m[3] = m3;
+    }
+  }
+}
+
+// ---------------------------------------------------------------- append
+// 4 consecutive elements as floats, and back
+template <typename T> __device__ __forceinline__ void load4(const T* p, float (&x)[4]);
+template <> __device__ __forceinline__ void load4<float>(const float* p, float (&x)[4]) {
+  const float4 v = *reinterpret_cast<const float4*>(p);
+  x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+}
+template <> __device__ __forceinline__ void load4<bf16>(const bf16* p, float (&x)[4]) {
+  const uint2 v = *reinterpret_cast<const uint2*>(p);
+  x[0] = __uint_as_float(v.x << 16), x[1] = __uint_as_float(v.x & 0xffff0000u);
+  x[2] = __uint_as_float(v.y << 16), x[3] = __uint_as_float(v.y & 0xffff0000u);
+}
+template <typename T> __device__ __forceinline__ void store4(T* p, const float (&x)[4]);
+template <> __device__ __forceinline__ void store4<float>(float* p, const float (&x)[4]) {
+  *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+}
+template <> __device__ __forceinline__ void store4<bf16>(bf16* p, const float (&x)[4]) {
+  __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
+  *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
+}
+
+// A group of D / 8 lanes owns one head of one token: lane l holds elements 4 l .. 4 l + 3 of both halves,
+// that is four rotation pairs, so the rotation needs no exchange and the largest |x| of the vector is a
+// shuffle over the group.  Bound by the bytes of qkv, q_out and the cache.
+template <typename T, int FMT, int D>
+__global__ void __launch_bounds__(128) kv_append_kernel(const T* __restrict__ qkv, int ld_qkv, T* __restrict__ q_out, int ld_qo,
+                                                        int n_heads, const int32_t* __restrict__ tok_pos,
+                                                        const int32_t* __restrict__ tok_slot,
+                                                        const int32_t* __restrict__ tok_row, CacheGeom c,
+                                                        const float* __restrict__ cosb, const float* __restrict__ sinb,
+                                                        int rope_len, int* status) {
+  pdl_trigger();
+  pdl_wait();
+  constexpr int L = D / 8, GROUPS = 128 / L, H2 = D / 2;
+  const int t = blockIdx.x;
+  const int pos = tok_pos[t], row = tok_row[t], slot = tok_slot[t];
+  if (pos < 0 || pos >= rope_len || row < 0 || row >= c.max_batch || slot < 0 || slot >= c.max_seq) {
+    if (threadIdx.x == 0) set_status(status, kStatusBadIndex);
+    return;
+  }
+  const int l = threadIdx.x % L;
+  const T* base = qkv + (size_t)t * ld_qkv + 4 * l;
+  float c1[4], c2[4], s1[4], s2[4];
+  load4<float>(cosb + (size_t)pos * D + 4 * l, c1);
+  load4<float>(cosb + (size_t)pos * D + H2 + 4 * l, c2);
+  load4<float>(sinb + (size_t)pos * D + 4 * l, s1);
+  load4<float>(sinb + (size_t)pos * D + H2 + 4 * l, s2);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    c1[i] = rnd<T>(c1[i]);
+    c2[i] = rnd<T>(c2[i]);
+    s1[i] = rnd<T>(s1[i]);
+    s2[i] = rnd<T>(s2[i]);
+  }
+  const int heads = n_heads + 2 * c.n_kv_heads;
+  // every lane of a warp takes part in the shuffles: head numbers past the end repeat the last head, unstored
+  for (int h0 = 0; h0 < heads; h0 += GROUPS) {
+    const int hh = h0 + threadIdx.x / L;
+    const bool in = hh < heads;
+    const int h = in ? hh : heads - 1;
+    float x1[4], x2[4];
+    load4<T>(base + (size_t)h * D, x1);
+    load4<T>(base + (size_t)h * D + H2, x2);
+    if (h < n_heads + c.n_kv_heads) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // the roundings of the reference's apply_rope in the model dtype, no contraction to FMA
+        const float a = __fadd_rn(rnd<T>(__fmul_rn(x1[i], c1[i])), rnd<T>(__fmul_rn(-x2[i], s1[i])));
+        const float b = __fadd_rn(rnd<T>(__fmul_rn(x2[i], c2[i])), rnd<T>(__fmul_rn(x1[i], s2[i])));
+        x1[i] = rnd<T>(a);
+        x2[i] = rnd<T>(b);
+      }
+    }
+    if (h < n_heads) {
+      if (in) {
+        T* q = q_out + (size_t)t * ld_qo + (size_t)h * D + 4 * l;
+        store4<T>(q, x1);
+        store4<T>(q + H2, x2);
+      }
+      if constexpr (FMT == EESD_KV_MODEL) continue;
+    }
+    const bool isk = h < n_heads + c.n_kv_heads;
+    const size_t at = cache_slot(c, row, isk ? h - n_heads : h - n_heads - c.n_kv_heads, slot);
+    if constexpr (FMT == EESD_KV_MODEL) {
+      if (in) {
+        T* d = static_cast<T*>(const_cast<void*>(isk ? c.k : c.v)) + at * D + 4 * l;
+        store4<T>(d, x1);
+        store4<T>(d + H2, x2);
+      }
+    } else {
+      uint32_t amax = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) amax = max(amax, max(__float_as_uint(x1[i]) & 0x7fffffffu, __float_as_uint(x2[i]) & 0x7fffffffu));
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      if (!in || h < n_heads) continue;
+      const int eb = exp_byte<FMT>(amax);
+      const float inv = exp_inv_scale(eb);
+      uint32_t w1 = 0, w2 = 0;
+      if (eb != 255) {
+        w1 = quant2<FMT>(x1[0] * inv, x1[1] * inv) | quant2<FMT>(x1[2] * inv, x1[3] * inv) << 16;
+        w2 = quant2<FMT>(x2[0] * inv, x2[1] * inv) | quant2<FMT>(x2[2] * inv, x2[3] * inv) << 16;
+      }
+      uint8_t* d = static_cast<uint8_t*>(const_cast<void*>(isk ? c.k : c.v)) + at * D + 4 * l;
+      *reinterpret_cast<uint32_t*>(d) = w1;
+      *reinterpret_cast<uint32_t*>(d + H2) = w2;
+      if (l == 0) const_cast<uint8_t*>(isk ? c.ke : c.ve)[at] = (uint8_t)eb;
+    }
+  }
+}
+
+// ---------------------------------------------------------------- read-back
+// One thread per 8 elements: an 8-byte (8-bit formats) load and 16-byte stores, neighbouring threads on
+// neighbouring chunks of a head, then heads, then tokens.  Bound by the bytes of the output.
+template <typename T, int FMT, int D>
+__global__ void __launch_bounds__(256) kv_read_kernel(CacheGeom c, const int32_t* __restrict__ tok_slot,
+                                                      const int32_t* __restrict__ tok_row, int n_tok, T* __restrict__ k_out,
+                                                      T* __restrict__ v_out, int* status) {
+  pdl_trigger();
+  pdl_wait();
+  constexpr int C = D / 8;
+  const size_t per = (size_t)c.n_kv_heads * C;
+  const bool isk = blockIdx.y == 0 && k_out;
+  T* out = isk ? k_out : v_out;
+  const size_t n = (size_t)n_tok * per;
+  for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x) {
+    const int t = (int)(i / per), r = (int)(i - (size_t)t * per), h = r / C, ch = r % C;
+    const int row = tok_row[t], slot = tok_slot[t];
+    if (row < 0 || row >= c.max_batch || slot < 0 || slot >= c.max_seq) {
+      set_status(status, kStatusBadIndex);
+      continue;
+    }
+    const size_t at = cache_slot(c, row, h, slot);
+    T* o = out + ((size_t)t * c.n_kv_heads + h) * D + ch * 8;
+    const void* src = isk ? c.k : c.v;
+    float x[4], y[4];
+    if constexpr (FMT == EESD_KV_MODEL) {
+      load4<T>(static_cast<const T*>(src) + at * D + ch * 8, x);
+      load4<T>(static_cast<const T*>(src) + at * D + ch * 8 + 4, y);
+    } else {
+      const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(src) + at * D + ch * 8);
+      const float s = exp_scale((isk ? c.ke : c.ve)[at]) * kHalfUnit<FMT>;
+      uint32_t a, b, e, f;
+      unpack4<FMT>(w.x, a, b);
+      unpack4<FMT>(w.y, e, f);
+      const float2 fa = half2_to_float2(a), fb = half2_to_float2(b), fe = half2_to_float2(e), ff = half2_to_float2(f);
+      x[0] = fa.x * s, x[1] = fa.y * s, x[2] = fb.x * s, x[3] = fb.y * s;
+      y[0] = fe.x * s, y[1] = fe.y * s, y[2] = ff.x * s, y[3] = ff.y * s;
+    }
+    store4<T>(o, x);
+    store4<T>(o + 4, y);
+  }
+}
+
+// ---------------------------------------------------------------- acceptance
+// One warp per block: the walk is serial, each step one vote over the nodes behind the current one.
+__global__ void __launch_bounds__(32) tree_accept_kernel(EesdTree t, const int32_t* __restrict__ y,
+                                                         const int32_t* __restrict__ ids, int32_t* __restrict__ path,
+                                                         int32_t* __restrict__ n_acc, int32_t* __restrict__ next, int* status) {
+  pdl_trigger();
+  pdl_wait();
+  __shared__ int32_t par[EESD_TREE_MAX_NODES], id[EESD_TREE_MAX_NODES], ys[EESD_TREE_MAX_NODES];
+  const int b = blockIdx.x, lane = threadIdx.x;
+  const int start = t.blk[4 * b], T = t.blk[4 * b + 1];
+  int32_t* out = path + (size_t)b * t.max_nodes;
+  bool ok = start >= 0 && T > 0 && T <= t.max_nodes && T <= EESD_TREE_MAX_NODES && start <= t.n_tokens - T;
+  if (ok) {
+    for (int i = lane; i < T; i += 32) {
+      par[i] = t.parent ? t.parent[start + i] : i - 1;
+      id[i] = ids[start + i];
+      ys[i] = y[start + i];
+    }
+    __syncwarp();
+  } else if (lane == 0) {
+    set_status(status, kStatusBadIndex);
+  }
+  int cur = 0, len = 0;
+  if (ok) {
+    for (;;) {
+      if (lane == 0) out[len] = cur;
+      ++len;
+      const int want = ys[cur];
+      int child = -1;
+      // children come after their parent, so the walk ends after at most T nodes
+      for (int i0 = (cur + 1) & ~31; i0 < T && child < 0; i0 += 32) {
+        const int i = i0 + lane;
+        const unsigned hit = __ballot_sync(0xffffffffu, i > cur && i < T && par[i] == cur && id[i] == want);
+        if (hit) child = i0 + __ffs(hit) - 1;
+      }
+      if (child < 0) break;
+      cur = child;
+    }
+  }
+  for (int i = len + lane; i < t.max_nodes; i += 32) out[i] = -1;
+  if (lane == 0) {
+    n_acc[b] = len - 1;
+    next[b] = ok ? ys[cur] : -1;
+  }
+}
+
+// ---------------------------------------------------------------- compaction
+// grid (16-byte chunks of all layers, heads, K and V; blocks).  A thread owns one 16-byte column of one
+// (layer, head) and moves its path slots in rising order: path[j] >= j, so every source is read before the
+// move that overwrites it (four loads, then four stores).  Latency-bound: few bytes over many threads.
+__global__ void __launch_bounds__(256) kv_compact_kernel(uint8_t* __restrict__ k, uint8_t* __restrict__ v,
+                                                         uint8_t* __restrict__ ke, uint8_t* __restrict__ ve, int n_layers,
+                                                         int n_kv_heads, int max_batch, int max_seq, int slot_bytes, EesdTree t,
+                                                         const int32_t* __restrict__ path,
+                                                         const int32_t* __restrict__ n_acc, int* status) {
+  pdl_trigger();
+  pdl_wait();
+  __shared__ int16_t src[EESD_TREE_MAX_NODES];
+  __shared__ int first;
+  const int b = blockIdx.y;
+  const int T = t.blk[4 * b + 1], row = t.blk[4 * b + 2], ctx = t.blk[4 * b + 3], acc = n_acc[b];
+  bool ok = T > 0 && T <= t.max_nodes && T <= EESD_TREE_MAX_NODES && row >= 0 && row < max_batch && ctx >= 0 && ctx <= max_seq - T &&
+            acc >= 0 && acc < T;
+  if (threadIdx.x == 0) first = acc + 1;
+  __syncthreads();
+  if (ok)
+    for (int j = threadIdx.x; j <= acc; j += blockDim.x) {
+      const int p = path[(size_t)b * t.max_nodes + j], before = j ? path[(size_t)b * t.max_nodes + j - 1] : -1;
+      if (p <= before || p >= T) ok = false;
+      src[j] = (int16_t)p;
+      if (p != j) atomicMin(&first, j);   // the slots before the first gap stay where they are
+    }
+  ok = __syncthreads_and(ok);
+  if (!ok) {
+    if (threadIdx.x == 0) set_status(status, kStatusBadIndex);
+    return;
+  }
+  const int j0 = max(first, 1);
+  if (j0 > acc) return;
+  const int cols = slot_bytes / 16;
+  const long long n_vec = (long long)n_layers * n_kv_heads * cols * 2;
+  const long long n_exp = ke ? (long long)n_layers * n_kv_heads * 2 : 0;
+  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i < n_vec) {
+    const int col = (int)(i % cols), h = (int)(i / cols % n_kv_heads);
+    const long long lk = i / cols / n_kv_heads;
+    uint8_t* base = (lk & 1 ? v : k);
+    uint4* p = reinterpret_cast<uint4*>(base + ((((size_t)(lk >> 1) * max_batch + row) * n_kv_heads + h) * max_seq + ctx) * slot_bytes) + col;
+    for (int j = j0; j <= acc; j += 4) {
+      uint4 buf[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (j + u <= acc) buf[u] = p[(size_t)src[j + u] * cols];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (j + u <= acc) p[(size_t)(j + u) * cols] = buf[u];
+    }
+  } else if (i < n_vec + n_exp) {
+    const long long e = i - n_vec;
+    const int h = (int)(e % n_kv_heads);
+    const long long lk = e / n_kv_heads;
+    uint8_t* p = (lk & 1 ? ve : ke) + (((size_t)(lk >> 1) * max_batch + row) * n_kv_heads + h) * max_seq + ctx;
+    for (int j = j0; j <= acc; ++j) p[j] = p[src[j]];
+  }
+}
+
+template <typename T, int FMT>
+cudaError_t append_d(int D, int n_tok, cudaStream_t s, const T* qkv, int ld, T* q_out, int ldo, int H, const int32_t* pos,
+                     const int32_t* slot, const int32_t* row, const CacheGeom& g, const float* cs, const float* sn, int rl, int* st) {
+  if (D == 64)
+    return launch_pdl(kv_append_kernel<T, FMT, 64>, dim3(n_tok), dim3(128), 0, s, qkv, ld, q_out, ldo, H, pos, slot, row, g, cs, sn, rl, st);
+  return launch_pdl(kv_append_kernel<T, FMT, 128>, dim3(n_tok), dim3(128), 0, s, qkv, ld, q_out, ldo, H, pos, slot, row, g, cs, sn, rl, st);
+}
+template <typename T>
+cudaError_t append_t(int fmt, int D, int n_tok, cudaStream_t s, void* qkv, int ld, void* q_out, int ldo, int H, const int32_t* pos,
+                     const int32_t* slot, const int32_t* row, const CacheGeom& g, const float* cs, const float* sn, int rl, int* st) {
+  const T* x = static_cast<const T*>(qkv);
+  T* q = static_cast<T*>(q_out);
+  if (fmt == EESD_KV_E4M3) return append_d<T, EESD_KV_E4M3>(D, n_tok, s, x, ld, q, ldo, H, pos, slot, row, g, cs, sn, rl, st);
+  if (fmt == EESD_KV_INT8) return append_d<T, EESD_KV_INT8>(D, n_tok, s, x, ld, q, ldo, H, pos, slot, row, g, cs, sn, rl, st);
+  return append_d<T, EESD_KV_MODEL>(D, n_tok, s, x, ld, q, ldo, H, pos, slot, row, g, cs, sn, rl, st);
+}
+
+template <typename T, int FMT>
+cudaError_t read_d(int D, dim3 grid, cudaStream_t s, const CacheGeom& g, const int32_t* slot, const int32_t* row, int n, void* k,
+                   void* v, int* st) {
+  if (D == 64)
+    return launch_pdl(kv_read_kernel<T, FMT, 64>, grid, dim3(256), 0, s, g, slot, row, n, static_cast<T*>(k), static_cast<T*>(v), st);
+  return launch_pdl(kv_read_kernel<T, FMT, 128>, grid, dim3(256), 0, s, g, slot, row, n, static_cast<T*>(k), static_cast<T*>(v), st);
+}
+template <typename T>
+cudaError_t read_t(int fmt, int D, dim3 grid, cudaStream_t s, const CacheGeom& g, const int32_t* slot, const int32_t* row, int n,
+                   void* k, void* v, int* st) {
+  if (fmt == EESD_KV_E4M3) return read_d<T, EESD_KV_E4M3>(D, grid, s, g, slot, row, n, k, v, st);
+  if (fmt == EESD_KV_INT8) return read_d<T, EESD_KV_INT8>(D, grid, s, g, slot, row, n, k, v, st);
+  return read_d<T, EESD_KV_MODEL>(D, grid, s, g, slot, row, n, k, v, st);
+}
+
+int launched(const char* who, cudaError_t e) {
+  return e == cudaSuccess ? EESD_OK : fail_arg(EESD_ERR_CUDA, "%s: launch: %s", who, cudaGetErrorString(e));
+}
+
+}  // namespace
+}  // namespace eesd
+
+using namespace eesd;
+
+extern "C" {
+
+int eesd_tree_meta(const EesdTree* t, int max_batch, int max_seq, int32_t* status, void* stream) {
+  int rc = check_tree("tree_meta", t);
+  if (rc) return rc;
+  if (max_batch <= 0 || max_seq <= 0) return fail_arg(EESD_ERR_ARG, "tree_meta: cache sizes");
+  if (t->n_tokens == 0 || t->n_blocks == 0) return EESD_OK;
+  if (!t->tok_pos || !t->tok_slot || !t->tok_row) return fail_arg(EESD_ERR_ARG, "tree_meta: null output");
+  if (t->parent && t->max_nodes > EESD_TREE_MAX_NODES)
+    return fail_arg(EESD_ERR_ARG, "tree_meta: parents need max_nodes <= %d", EESD_TREE_MAX_NODES);
+  if ((rc = check_stream("tree_meta", stream))) return rc;
+  return launched("tree_meta", launch_pdl(tree_meta_kernel, dim3(t->n_blocks), dim3(128), 0, static_cast<cudaStream_t>(stream), *t,
+                                          max_batch, max_seq, status));
+}
+
+int eesd_kv_append(int dtype, const EesdKvCache* c, int layer, void* qkv, int ld_qkv, int n_heads, const int32_t* tok_pos,
+                   const int32_t* tok_slot, const int32_t* tok_row, int n_tok, const float* rope_cos, const float* rope_sin,
+                   int rope_len, void* q_out, int32_t* status, void* stream) {
+  int rc = check_cache("kv_append", dtype, c, layer);
+  if (rc) return rc;
+  if (n_tok < 0 || rope_len <= 0 || n_heads <= 0 || n_heads % c->n_kv_heads)
+    return fail_arg(EESD_ERR_ARG, "kv_append: n_tok %d, rope_len %d, heads %d / %d", n_tok, rope_len, n_heads, c->n_kv_heads);
+  if (n_tok == 0) return EESD_OK;
+  if (!qkv || !tok_pos || !tok_row || !rope_cos || !rope_sin) return fail_arg(EESD_ERR_ARG, "kv_append: null argument");
+  if (ld_qkv % 8 || ld_qkv < (n_heads + 2 * c->n_kv_heads) * c->head_dim)
+    return fail_arg(EESD_ERR_ARG, "kv_append: ld_qkv %d (a multiple of 8, at least the fused row)", ld_qkv);
+  if ((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(rope_cos) |
+       reinterpret_cast<uintptr_t>(rope_sin)) & 15)
+    return fail_arg(EESD_ERR_ARG, "kv_append: qkv, q_out and the RoPE tables must be 16-byte aligned");
+  if ((rc = check_stream("kv_append", stream))) return rc;
+  const CacheGeom g = cache_layer(c, dtype, layer);
+  const int ldo = q_out ? n_heads * c->head_dim : ld_qkv;
+  void* qo = q_out ? q_out : qkv;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int32_t* slot = tok_slot ? tok_slot : tok_pos;
+  const cudaError_t e =
+      dtype == EESD_BF16
+          ? append_t<bf16>(c->format, c->head_dim, n_tok, s, qkv, ld_qkv, qo, ldo, n_heads, tok_pos, slot, tok_row, g, rope_cos, rope_sin, rope_len, status)
+          : append_t<float>(c->format, c->head_dim, n_tok, s, qkv, ld_qkv, qo, ldo, n_heads, tok_pos, slot, tok_row, g, rope_cos, rope_sin, rope_len, status);
+  return launched("kv_append", e);
+}
+
+int eesd_kv_read(int dtype, const EesdKvCache* c, int layer, const int32_t* tok_slot, const int32_t* tok_row, int n_tok, void* k_out,
+                 void* v_out, int32_t* status, void* stream) {
+  int rc = check_cache("kv_read", dtype, c, layer);
+  if (rc) return rc;
+  if (n_tok < 0) return fail_arg(EESD_ERR_ARG, "kv_read: n_tok %d", n_tok);
+  if (n_tok == 0 || (!k_out && !v_out)) return EESD_OK;
+  if (!tok_slot || !tok_row) return fail_arg(EESD_ERR_ARG, "kv_read: null argument");
+  if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15)
+    return fail_arg(EESD_ERR_ARG, "kv_read: outputs must be 16-byte aligned");
+  if ((rc = check_stream("kv_read", stream))) return rc;
+  const CacheGeom g = cache_layer(c, dtype, layer);
+  const size_t n = (size_t)n_tok * c->n_kv_heads * (c->head_dim / 8);
+  const size_t ctas = (n + 255) / 256;
+  const dim3 grid((unsigned)(ctas < 148 * 16 ? ctas : 148 * 16), (k_out && v_out) ? 2 : 1);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = dtype == EESD_BF16 ? read_t<bf16>(c->format, c->head_dim, grid, s, g, tok_slot, tok_row, n_tok, k_out, v_out, status)
+                                           : read_t<float>(c->format, c->head_dim, grid, s, g, tok_slot, tok_row, n_tok, k_out, v_out, status);
+  return launched("kv_read", e);
+}
+
+int eesd_tree_accept(const int32_t* y, const int32_t* ids, const EesdTree* t, int32_t* path, int32_t* n_acc, int32_t* next,
+                     int32_t* status, void* stream) {
+  int rc = check_tree("tree_accept", t);
+  if (rc) return rc;
+  if (t->n_tokens == 0 || t->n_blocks == 0) return EESD_OK;
+  if (!y || !ids || !path || !n_acc || !next) return fail_arg(EESD_ERR_ARG, "tree_accept: null argument");
+  if (t->max_nodes > EESD_TREE_MAX_NODES)
+    return fail_arg(EESD_ERR_ARG, "tree_accept: max_nodes %d (at most %d)", t->max_nodes, EESD_TREE_MAX_NODES);
+  if ((rc = check_stream("tree_accept", stream))) return rc;
+  return launched("tree_accept", launch_pdl(tree_accept_kernel, dim3(t->n_blocks), dim3(32), 0, static_cast<cudaStream_t>(stream), *t,
+                                            y, ids, path, n_acc, next, status));
+}
+
+int eesd_kv_compact(int dtype, const EesdKvCache* c, const EesdTree* t, const int32_t* path, const int32_t* n_acc, int32_t* status,
+                    void* stream) {
+  int rc = check_cache("kv_compact", dtype, c, 0);
+  if (!rc) rc = check_tree("kv_compact", t);
+  if (rc) return rc;
+  if (t->n_tokens == 0 || t->n_blocks == 0) return EESD_OK;
+  if (!path || !n_acc) return fail_arg(EESD_ERR_ARG, "kv_compact: null argument");
+  if (t->max_nodes > EESD_TREE_MAX_NODES)
+    return fail_arg(EESD_ERR_ARG, "kv_compact: max_nodes %d (at most %d)", t->max_nodes, EESD_TREE_MAX_NODES);
+  if ((rc = check_stream("kv_compact", stream))) return rc;
+  const int slot_bytes = c->head_dim * (int)cache_elem_bytes(c, dtype);
+  const bool q8 = c->format != EESD_KV_MODEL;
+  const long long n = (long long)c->n_layers * c->n_kv_heads * 2 * (slot_bytes / 16 + (q8 ? 1 : 0));
+  return launched("kv_compact",
+                  launch_pdl(kv_compact_kernel, dim3((unsigned)((n + 255) / 256), t->n_blocks), dim3(256), 0,
+                             static_cast<cudaStream_t>(stream), static_cast<uint8_t*>(c->k), static_cast<uint8_t*>(c->v),
+                             q8 ? c->k_exp : nullptr, q8 ? c->v_exp : nullptr, c->n_layers, c->n_kv_heads, c->max_batch, c->max_seq,
+                             slot_bytes, *t, path, n_acc, status));
+}
+
+}  // extern "C"

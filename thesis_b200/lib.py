@@ -13,6 +13,8 @@ LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libeesd.so"
 OK, ERR_ARG, ERR_CUDA, ERR_DEVICE = 0, 1, 2, 3
 BF16, F32 = 0, 1
 EPI_STORE, EPI_RESIDUAL, EPI_SWIGLU = 0, 1, 2
+KV_MODEL, KV_E4M3, KV_INT8 = 0, 1, 2
+TREE_MAX_NODES = 256
 OPT_MMA_N, OPT_SPLITS, OPT_STAGES, OPT_PAIR, OPT_HEAD_TWO_TILES, OPT_SPIN_LIMIT, OPT_MMA_SPLIT = 1, 2, 3, 4, 5, 6, 7
 PROF_KINDS = 9
 PROF_NAMES = ["norm", "gemm_qkv", "rope_kv", "attn", "gemm_o", "gemm_w13", "gemm_w2", "head", "misc"]
@@ -35,6 +37,17 @@ class ModelDesc(C.Structure):
 class Batch(C.Structure):
     _fields_ = [("n_tokens", i32), ("n_blocks", i32), ("n_items", i32), ("max_ctx", i32), ("tok_pos", vp),
                 ("tok_row", vp), ("blk", vp), ("items", vp)]
+
+
+class KvCache(C.Structure):
+    _fields_ = [("format", i32), ("n_layers", i32), ("max_batch", i32), ("n_kv_heads", i32), ("max_seq", i32),
+                ("head_dim", i32), ("k", vp), ("v", vp), ("k_exp", vp), ("v_exp", vp)]
+
+
+class Tree(C.Structure):
+    _fields_ = [("n_tokens", i32), ("n_blocks", i32), ("max_nodes", i32), ("max_ctx", i32), ("words", i32),
+                ("reserved", i32), ("blk", vp), ("parent", vp), ("tok_pos", vp), ("tok_slot", vp), ("tok_row", vp),
+                ("mask", vp)]
 
 
 # name -> (restype, argtypes); every symbol declared in include/eesd.h
@@ -72,6 +85,15 @@ SIGNATURES = {
                                        C.POINTER(Batch), C.c_int, vp, vp, vp, vp, vp]),
     "eesd_rope_kv_append": (C.c_int, [C.c_int, vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp, vp, vp,
                                       C.c_int, C.c_int, vp, vp]),
+    "eesd_tree_meta": (C.c_int, [C.POINTER(Tree), C.c_int, C.c_int, vp, vp]),
+    "eesd_kv_append": (C.c_int, [C.c_int, C.POINTER(KvCache), C.c_int, vp, C.c_int, C.c_int, vp, vp, vp, C.c_int, vp, vp,
+                                 C.c_int, vp, vp, vp]),
+    "eesd_kv_read": (C.c_int, [C.c_int, C.POINTER(KvCache), C.c_int, vp, vp, C.c_int, vp, vp, vp, vp]),
+    "eesd_attn_tree_workspace_bytes": (sz, [C.c_int, C.POINTER(KvCache), C.POINTER(Tree), C.c_int, C.c_int]),
+    "eesd_attn_tree": (C.c_int, [C.c_int, C.POINTER(KvCache), C.c_int, C.POINTER(Tree), vp, C.c_int, C.c_int, vp, C.c_int,
+                                 vp, sz, vp, vp]),
+    "eesd_tree_accept": (C.c_int, [vp, vp, C.POINTER(Tree), vp, vp, vp, vp, vp]),
+    "eesd_kv_compact": (C.c_int, [C.c_int, C.POINTER(KvCache), C.POINTER(Tree), vp, vp, vp, vp]),
 }
 
 _lib = None
@@ -105,7 +127,8 @@ def check(rc: int, what: str = "") -> None:
 # entry points that launch exactly one kernel (counted for the bench's launch total)
 KERNEL_CALLS = {"eesd_pack_weight", "eesd_copy_rows", "eesd_gather_ids", "eesd_scatter_ids", "eesd_greedy_accept",
                 "eesd_round_meta", "eesd_round_advance", "eesd_rmsnorm",
-                "eesd_gemm", "eesd_attn_varlen_gqa", "eesd_rope_kv_append"}
+                "eesd_gemm", "eesd_attn_varlen_gqa", "eesd_rope_kv_append", "eesd_tree_meta", "eesd_kv_append",
+                "eesd_kv_read", "eesd_attn_tree", "eesd_tree_accept", "eesd_kv_compact"}
 direct_launches = 0
 
 
