@@ -5,8 +5,11 @@
 // read of a key serves all heads of its group and all nodes of the block.
 #include <math.h>
 
+#include <algorithm>
+
 #include "attn_tree.h"
 #include "cache.cuh"
+#include "gemm_tc.h"
 
 namespace eesd {
 namespace {
@@ -19,6 +22,10 @@ struct TreeGeom {
   int ld_q;
   float scale;
   int* status;
+  uint32_t spin;       // poll limit of the pipeline waits
+  int chunk, splits;   // keys per CTA; key ranges of the longest row
+  float* part_o;       // [n_tokens, Hq, splits, D] normalised partial outputs
+  float2* part_ml;     // [n_tokens, Hq, splits] (max in the log2 domain, sum)
 };
 
 struct BlockInfo {
@@ -144,6 +151,655 @@ __global__ void __launch_bounds__(128) attn_tree_simt_kernel(TreeGeom g, CacheGe
   }
 }
 
+// ---------------------------------------------------------------- small row tiles: mma.sync
+// One CTA per (row tile of 16 MT rows, KV head, key range of a block): a few query rows against a stream of
+// keys, bound by the bytes of K and V.  Its 4 warps are independent: warp w takes every fourth group of KG keys
+// (16 .. 64, 8 KB of K and V) through a TMA ring of its own, so nothing in the key loop waits for another warp;
+// the warps' running (max, sum, output) meet once at the end.
+//
+// S = Q K^T and O = P V run on m16n8k16.  Both products may order their contraction index as they like, which
+// the 8-bit formats use: thread (g, t) = (lane / 4, lane % 4) takes the dims [t D/4, (t + 1) D/4) of key g as K
+// fragments and the dims [g D/8, (g + 1) D/8) of keys 2t, 2t + 1, 2t + 8, 2t + 9 as V fragments, so K and V come
+// from shared memory as 16-byte words and turn into f16 pairs in registers, without a transpose.  The values'
+// powers of two never touch the operands: K's scale multiplies the score, V's the weight (relative to the
+// largest one so far of the row, eref, as the running maximum does), a power of two of each q row its f16 form.
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds_u16(uint32_t addr) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr));
+  return v;
+}
+template <int FMT> __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (FMT == EESD_KV_MODEL)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <int FMT> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (FMT == EESD_KV_MODEL) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+// bf16 pair with its non-finite elements replaced by zero
+__device__ __forceinline__ uint32_t drop_nonfinite(uint32_t v, bool& hit) {
+  const bool lo = (v & 0x7f80u) == 0x7f80u, hi = (v & 0x7f800000u) == 0x7f800000u;
+  hit = hit || lo || hi;
+  return (lo ? 0u : v & 0xffffu) | (hi ? 0u : v & 0xffff0000u);
+}
+
+// Which of the 32 nodes j0 .. j0 + 31 a node sees (bit i: node j0 + i); negative nodes are committed slots.
+// mask: the node's 4 words in shared memory, or null for causal blocks.
+__device__ __forceinline__ uint32_t sees32(const uint64_t* mask, int node, int j0) {
+  if (!mask) {
+    const int n = node - j0 + 1;
+    return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1;
+  }
+  if (j0 <= -32) return ~0u;
+  if (j0 < 0) return (uint32_t)(mask[0] << -j0) | ((1u << -j0) - 1);
+  const int w = j0 >> 6, sh = j0 & 63;
+  uint64_t v = w < 4 ? mask[w] >> sh : 0;
+  if (sh > 32 && w < 3) v |= mask[w + 1] << (64 - sh);
+  return (uint32_t)v;
+}
+
+template <int D, int FMT, int MT> struct MmaShape {
+  static constexpr int kEb = FMT == EESD_KV_MODEL ? 2 : 1;
+  static constexpr int KG = 4096 / (D * kEb);          // keys per group: 4 KB of K, 4 KB of V
+  static constexpr int NS = MT == 1 ? 2 : 3;           // ring stages per warp
+  static constexpr int CTAS = MT == 1 ? 3 : 2;         // resident CTAs per SM
+  static constexpr int ROWS = 16 * MT;
+  static constexpr int STAGE = 8192;
+  static constexpr int LDQ = D + 8;                    // bf16: padded q row (elements), conflict-free ldmatrix
+  static constexpr int Q_BYTES = FMT == EESD_KV_MODEL ? ROWS * LDQ * 2 : MT * (D / 16) * 512;
+  static constexpr int OLD = D + 4;
+  static constexpr size_t smem = 1024 + 4 * NS * STAGE + Q_BYTES + 4 * NS * 128 + ROWS * 32 + ROWS * 4 + 4 * NS * 8 + 16;
+  static_assert((4 * ROWS * OLD + 12 * ROWS) * 4 <= 4 * NS * STAGE, "the merge does not fit the stage memory");
+};
+
+template <int D, int FMT, int MT>
+__global__ void __launch_bounds__(128, MmaShape<D, FMT, MT>::CTAS)
+    attn_tree_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, TreeGeom g, CacheGeom c,
+                         const bf16* __restrict__ q, bf16* __restrict__ out) {
+  using P = MmaShape<D, FMT, MT>;
+  constexpr bool Q8 = FMT != EESD_KV_MODEL;
+  constexpr int KG = P::KG, NS = P::NS, ROWS = P::ROWS, LDQ = P::LDQ, OLD = P::OLD, ND = D / 8, KK = D / 16;
+  constexpr int HALF = 4096;                           // K bytes (then V bytes) of a stage
+  pdl_trigger();
+  pdl_wait();
+  extern __shared__ uint8_t smem8[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem8) + 1023) & ~uintptr_t(1023));
+  uint8_t* stages = sm;                                                 // [4 warps][NS][K | V]
+  uint8_t* qs = sm + 4 * NS * P::STAGE;
+  uint8_t* exps = qs + P::Q_BYTES;                                      // [4][NS][K bytes 64 | V bytes 64]
+  uint64_t* masks = reinterpret_cast<uint64_t*>(exps + 4 * NS * 128);   // [ROWS][4], a row's node
+  float* qscale = reinterpret_cast<float*>(masks + ROWS * 4);           // [ROWS] power of two taken out of the q row
+  uint64_t* full = reinterpret_cast<uint64_t*>(qscale + ROWS);          // [4][NS]
+  volatile int* flags = reinterpret_cast<volatile int*>(full + 4 * NS);   // [0] a wait gave up, [1] a non-finite V was dropped
+
+  BlockInfo bi;
+  if (!load_block(g, c, blockIdx.z, bi)) return;
+  const int kvh = blockIdx.y % c.n_kv_heads, r0 = blockIdx.y / c.n_kv_heads * ROWS;
+  const int nrows = min(ROWS, bi.T * g.G - r0);
+  if (nrows <= 0) return;
+  const int first = r0 / g.G, last = (r0 + nrows - 1) / g.G;            // the tile's nodes
+  const int n_keys = bi.ctx + (g.mask ? bi.T : last + 1);
+  const int k_lo = blockIdx.x * g.chunk, k_hi = min(n_keys, k_lo + g.chunk);
+  if (k_lo >= n_keys) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, tq = lane & 3;
+  const int all_see = bi.ctx + (g.mask ? 0 : first + 1);                // slots below this are seen by every row
+  const int n_groups = (k_hi - k_lo + KG - 1) / KG;
+  const int my_groups = warp < n_groups ? (n_groups - warp + 3) / 4 : 0;
+  const int slot0 = (int)cache_slot(c, bi.row, kvh, 0);                 // fits: the entry point bounds the layer's slots
+
+  const uint32_t st0 = smem_u32(stages) + warp * NS * P::STAGE;
+  const uint32_t ex0 = smem_u32(exps) + warp * NS * 128;
+  const uint32_t fb0 = smem_u32(full + warp * NS);
+  auto issue = [&](int i) {                                             // lane 0: this warp's i-th group
+    const int s = i % NS, key = k_lo + (warp + 4 * i) * KG;
+    const uint32_t fb = fb0 + s * 8, dst = st0 + s * P::STAGE;
+    if constexpr (Q8) {
+      const uint32_t eb = min(KG, c.max_seq - key);                     // max_seq % 16 == 0 and key % 16 == 0
+      mbar_arrive_expect_tx(fb, P::STAGE + 2 * eb);
+      tma_load_2d(dst, &kmap, 0, slot0 + key, fb);
+      tma_load_2d(dst + HALF, &vmap, 0, slot0 + key, fb);
+      bulk_g2s(ex0 + s * 128, c.ke + slot0 + key, eb, fb);
+      bulk_g2s(ex0 + s * 128 + 64, c.ve + slot0 + key, eb, fb);
+    } else {
+      mbar_arrive_expect_tx(fb, P::STAGE);
+#pragma unroll
+      for (int h = 0; h < D / 64; ++h) {
+        tma_load_2d(dst + h * KG * 128, &kmap, h * 64, slot0 + key, fb);
+        tma_load_2d(dst + HALF + h * KG * 128, &vmap, h * 64, slot0 + key, fb);
+      }
+    }
+  };
+  if (lane == 0) {
+    for (int s = 0; s < NS; ++s) mbar_init(fb0 + s * 8, 1);
+    fence_mbar_init();
+    for (int i = 0; i < NS && i < my_groups; ++i) issue(i);
+  }
+  if (threadIdx.x == 0) flags[0] = flags[1] = 0;
+  // q rows of the tile (zeros behind nrows) and their nodes' masks
+  for (int r = warp; r < ROWS; r += 4) {
+    const int R = r0 + r;
+    const bool in = r < nrows;
+    const bf16* src = q + (size_t)(bi.start + (in ? R / g.G : 0)) * g.ld_q + (kvh * g.G + (in ? R % g.G : 0)) * D;
+    if constexpr (!Q8) {
+      for (int e = lane * 2; e < D; e += 64)
+        *reinterpret_cast<uint32_t*>(qs + (r * LDQ + e) * 2) = in ? *reinterpret_cast<const uint32_t*>(src + e) : 0u;
+    } else {
+      uint32_t v[D / 64], amax = 0;
+#pragma unroll
+      for (int j = 0; j < D / 64; ++j) {
+        v[j] = in ? *reinterpret_cast<const uint32_t*>(src + lane * 2 + 64 * j) : 0u;
+        amax = max(amax, max(v[j] << 16 & 0x7fff0000u, v[j] & 0x7fff0000u));
+      }
+      amax = __reduce_max_sync(0xffffffffu, amax);
+      // take the largest element's power of two out (|q'| < 2): f16 keeps every bit of a bf16 down to 2^-14 of
+      // the row's largest, and below that an absolute 2^-25 of it
+      const int e = min(max((int)(amax >> 23), 27), 227);
+      const float inv = __int_as_float((254 - e) << 23);
+      if (lane == 0) qscale[r] = __int_as_float(e << 23);
+#pragma unroll
+      for (int j = 0; j < D / 64; ++j) {
+        const int d = lane * 2 + 64 * j;                                // dims d, d + 1 of the row, in fragment order
+        const int t = d / (D / 4), kk = d % (D / 4) / 4, pair = d % 4 / 2;
+        const uint32_t h = pack2<FMT>(__uint_as_float(v[j] << 16) * inv, __uint_as_float(v[j] & 0xffff0000u) * inv);
+        const int m = r >> 4, rr = r & 15;                              // a0: row g, pair 0; a1: row g + 8; a2, a3: pair 1
+        reinterpret_cast<uint32_t*>(qs)[((m * KK + kk) * 32 + (rr & 7) * 4 + t) * 4 + (rr >> 3) + 2 * pair] = h;
+      }
+    }
+    if (lane < 4) masks[r * 4 + lane] = (g.mask && in && lane < g.words) ? g.mask[(size_t)(bi.start + R / g.G) * g.words + lane] : 0ull;
+  }
+  __syncthreads();
+
+  float o[MT][ND][4], m[MT][2], l[MT][2], rf[MT][2];
+  int er[MT][2];                                                        // 8-bit: exponent byte of the largest V scale so far
+#pragma unroll
+  for (int a = 0; a < MT; ++a)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      m[a][h] = -INFINITY;
+      l[a][h] = 0.f;
+      er[a][h] = 0;
+      rf[a][h] = g.scale * 1.4426950408889634f * (Q8 ? qscale[a * 16 + h * 8 + gq] * kHalfUnit<FMT> : 1.f);
+#pragma unroll
+      for (int n = 0; n < ND; ++n) o[a][n][2 * h] = o[a][n][2 * h + 1] = 0.f;
+    }
+  int done = 0;                                                         // groups waited for
+  bool ok = true;
+  for (int i = 0; i < my_groups; ++i) {
+    const int s = i % NS;
+    ok = mbar_wait(fb0 + s * 8, (i / NS) & 1, flags, g.spin);
+    if (!__all_sync(0xffffffffu, ok)) {
+      ok = false;
+      break;
+    }
+    done = i + 1;
+    const uint32_t kt = st0 + s * P::STAGE, vt = kt + HALF, ex = ex0 + s * 128;
+    const int key0 = k_lo + (warp + 4 * i) * KG;
+    const bool partial = key0 + KG > min(all_see, k_hi);                // some row does not see some key of the group
+    float sc[MT][KG / 8][4];
+#pragma unroll
+    for (int a = 0; a < MT; ++a)
+#pragma unroll
+      for (int n = 0; n < KG / 8; ++n) sc[a][n][0] = sc[a][n][1] = sc[a][n][2] = sc[a][n][3] = 0.f;
+    if constexpr (!Q8) {
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        uint32_t a[MT][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+          ldsm_x4(smem_u32(qs) + ((mt * 16 + (lane & 15)) * LDQ + kk * 16 + (lane >> 4) * 8) * 2, a[mt]);
+        const int dim = kk * 16 + ((lane >> 3) & 1) * 8;
+#pragma unroll
+        for (int n2 = 0; n2 < KG / 16; ++n2) {
+          const int key = n2 * 16 + (lane & 7) + ((lane >> 4) << 3);
+          uint32_t b[4];
+          ldsm_x4(kt + (dim >> 6) * KG * 128 + key * 128 + ((((dim & 63) >> 3) ^ (key & 7)) << 4), b);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            mma16816<FMT>(sc[mt][2 * n2], a[mt], b[0], b[1]);
+            mma16816<FMT>(sc[mt][2 * n2 + 1], a[mt], b[2], b[3]);
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < KG / 8; ++n) {
+        const int key = n * 8 + gq;
+#pragma unroll
+        for (int u = 0; u < D / 64; ++u) {                              // 16 bytes: four k-steps
+          const int ch = tq * (D / 64) + u;
+          const uint32_t sw = D == 128 ? (ch ^ (key & 7)) << 4 : (ch ^ ((key >> 1) & 3)) << 4;
+          const uint4 w = lds128(kt + key * D + sw);
+          const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            uint32_t b0, b1;
+            unpack4<FMT>(ww[x], b0, b1);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              const uint4 av = lds128(smem_u32(qs) + ((mt * KK + u * 4 + x) * 32 + lane) * 16);
+              const uint32_t a[4] = {av.x, av.y, av.z, av.w};
+              mma16816<FMT>(sc[mt][n], a, b0, b1);
+            }
+          }
+        }
+      }
+    }
+    // per-key factors of the 8-bit formats: this thread's columns are keys 8 n + 2 tq, + 1
+    float fk[Q8 ? KG / 8 : 1][2], fv[Q8 ? KG / 8 : 1][2];
+    int evb[Q8 ? KG / 8 : 1][2];
+    if constexpr (Q8) {
+#pragma unroll
+      for (int n = 0; n < KG / 8; ++n) {
+        const uint32_t kb = lds_u16(ex + n * 8 + 2 * tq), vb = lds_u16(ex + 64 + n * 8 + 2 * tq);
+        fk[n][0] = exp_scale(kb & 255);
+        fk[n][1] = exp_scale(kb >> 8);
+        evb[n][0] = vb & 255;
+        evb[n][1] = vb >> 8;
+        fv[n][0] = exp_scale(evb[n][0]);
+        fv[n][1] = exp_scale(evb[n][1]);
+      }
+    }
+    int emax = 0;
+    if constexpr (Q8) {
+      if (!partial) {
+#pragma unroll
+        for (int n = 0; n < KG / 8; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) emax = max(emax, evb[n][e] == 255 ? 0 : evb[n][e]);
+        emax = __reduce_max_sync(0xffffffffu, emax);
+      }
+    }
+#pragma unroll
+    for (int a = 0; a < MT; ++a) {
+      float corr[2];
+      bool moved = false;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = a * 16 + h * 8 + gq;
+        uint32_t see[KG > 32 ? 2 : 1] = {};
+        int em = emax;
+        if (partial) {
+          em = 0;
+          const int node = (r0 + min(r, nrows - 1)) / g.G;
+#pragma unroll
+          for (int w = 0; w < (KG > 32 ? 2 : 1); ++w) {
+            const int kb = key0 + 32 * w;
+            see[w] = sees32(g.mask ? masks + r * 4 : nullptr, node, kb - bi.ctx);
+            const int left = k_hi - kb;
+            if (left < 32) see[w] &= left <= 0 ? 0u : (1u << left) - 1;
+          }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < KG / 8; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float& x = sc[a][n][2 * h + e];
+            x *= Q8 ? rf[a][h] * fk[Q8 ? n : 0][e] : rf[a][h];
+            if (partial) {
+              const int bit = n * 8 + 2 * tq + e;
+              const bool sees = see[bit >> 5] >> (bit & 31) & 1;
+              if (!sees) x = -INFINITY;
+              if constexpr (Q8) em = max(em, sees && evb[n][e] != 255 ? evb[n][e] : 0);
+            }
+            mx = fmaxf(mx, x);
+          }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        if (Q8 && partial) {
+          em = max(em, __shfl_xor_sync(0xffffffffu, em, 1));
+          em = max(em, __shfl_xor_sync(0xffffffffu, em, 2));
+        }
+        const float mn = fmaxf(m[a][h], mx);
+        const float ms = mn == -INFINITY ? 0.f : mn;
+        corr[h] = fast_exp2(m[a][h] - ms);
+        moved = moved || mn != m[a][h];
+        m[a][h] = mn;
+        float rv = 0.f;
+        if constexpr (Q8) {
+          const int en = max(er[a][h], em);
+          rv = __int_as_float((254 - max(en, 1)) << 23);                // 2^-(en - 127)
+        }
+        float sum = 0.f;
+#pragma unroll
+        for (int n = 0; n < KG / 8; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float& x = sc[a][n][2 * h + e];
+            const float p = fast_exp2(x - ms);
+            sum += p;
+            if constexpr (Q8) x = p == 0.f ? 0.f : p * (fv[n][e] * rv);
+            else x = p;
+          }
+        l[a][h] = l[a][h] * corr[h] + sum;
+        if constexpr (Q8) {
+          const int en = max(er[a][h], em);
+          if (en != er[a][h]) {
+            corr[h] *= er[a][h] == 0 ? 0.f : fast_exp2((float)(er[a][h] - en));
+            moved = true;
+          }
+          er[a][h] = en;
+        }
+      }
+      if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int n = 0; n < ND; ++n) {
+          o[a][n][0] *= corr[0];
+          o[a][n][1] *= corr[0];
+          o[a][n][2] *= corr[1];
+          o[a][n][3] *= corr[1];
+        }
+      }
+    }
+    bool hit = false;
+#pragma unroll
+    for (int st = 0; st < KG / 16; ++st) {
+      uint32_t p[MT][4];
+#pragma unroll
+      for (int a = 0; a < MT; ++a) {
+        p[a][0] = pack2<FMT>(sc[a][2 * st][0], sc[a][2 * st][1]);
+        p[a][1] = pack2<FMT>(sc[a][2 * st][2], sc[a][2 * st][3]);
+        p[a][2] = pack2<FMT>(sc[a][2 * st + 1][0], sc[a][2 * st + 1][1]);
+        p[a][3] = pack2<FMT>(sc[a][2 * st + 1][2], sc[a][2 * st + 1][3]);
+      }
+      if constexpr (!Q8) {
+#pragma unroll
+        for (int n2 = 0; n2 < ND; n2 += 2) {
+          const int key = st * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
+          const int dim = n2 * 8 + (lane >> 4) * 8;
+          uint32_t b[4];
+          ldsm_x4_t(vt + (dim >> 6) * KG * 128 + key * 128 + ((((dim & 63) >> 3) ^ (key & 7)) << 4), b);
+          if (partial) {                 // 0 x NaN would reach every row: drop it here, put it back at the end
+#pragma unroll
+            for (int x = 0; x < 4; ++x) b[x] = drop_nonfinite(b[x], hit);
+          }
+#pragma unroll
+          for (int a = 0; a < MT; ++a) {
+            mma16816<FMT>(o[a][n2], p[a], b[0], b[1]);
+            mma16816<FMT>(o[a][n2 + 1], p[a], b[2], b[3]);
+          }
+        }
+      } else {
+        // keys 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9 of this step, D / 8 bytes each
+        uint32_t w[4][D / 32];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int key = st * 16 + 2 * tq + (x & 1) + (x >> 1) * 8;
+          if constexpr (D == 128) {
+            const uint4 v = lds128(vt + key * D + ((gq ^ (key & 7)) << 4));
+            w[x][0] = v.x, w[x][1] = v.y, w[x][2] = v.z, w[x][3] = v.w;
+          } else {
+            const uint2 v = lds64(vt + key * D + ((((gq >> 1) ^ ((key >> 1) & 3)) << 4) | (gq & 1) << 3));
+            w[x][0] = v.x, w[x][1] = v.y;
+          }
+          if constexpr (FMT == EESD_KV_INT8)
+#pragma unroll
+            for (int y = 0; y < D / 32; ++y) w[x][y] ^= 0x80808080u;
+        }
+#pragma unroll
+        for (int n = 0; n < ND; ++n) {
+          const int y = n >> 2, z = n & 3;
+          uint32_t b0, b1;
+          if constexpr (FMT == EESD_KV_E4M3) {                          // bytes into the high halves of each lane
+            const uint32_t sel = (4 + z) << 12 | (z << 4);              // [., z of x, ., z of y]: low bytes are masked off
+            b0 = bytes_to_half2<FMT>(__byte_perm(w[0][y], w[1][y], sel));
+            b1 = bytes_to_half2<FMT>(__byte_perm(w[2][y], w[3][y], sel));
+          } else {
+            const uint32_t sel = (4 + z) << 4 | z;                      // [z of x, z of y, ., .], then 0x64 in between
+            b0 = bytes_to_half2<FMT>(__byte_perm(__byte_perm(w[0][y], w[1][y], sel), 0x64646464u, 0x4140));
+            b1 = bytes_to_half2<FMT>(__byte_perm(__byte_perm(w[2][y], w[3][y], sel), 0x64646464u, 0x4140));
+          }
+#pragma unroll
+          for (int a = 0; a < MT; ++a) mma16816<FMT>(o[a][n], p[a], b0, b1);
+        }
+      }
+    }
+    if (!Q8 && hit) flags[1] = 1;
+    __syncwarp();                                                       // every lane is done with the stage
+    if (lane == 0 && i + NS < my_groups) issue(i + NS);
+  }
+  if (!ok) {
+    if (lane == 0) {
+      set_status(g.status, kStatusTimeoutMma);
+      flags[0] = 1;
+      // groups issued and not waited for: one per stage at most
+      const int issued = min(my_groups, done + NS);
+      for (int i = done; i < issued; ++i) mbar_drain(fb0 + (i % NS) * 8, (i / NS) & 1);
+    }
+  }
+  __syncthreads();
+  if (flags[0]) return;
+
+  // ---- the four warps' states, through the stage memory (every copy has landed)
+  float* Ow = reinterpret_cast<float*>(stages);                         // [4][ROWS][OLD]
+  float* Mw = Ow + 4 * ROWS * OLD;                                      // [4][ROWS] each: max, sum, eref
+  float* Lw = Mw + 4 * ROWS;
+  float* Ew = Lw + 4 * ROWS;
+#pragma unroll
+  for (int a = 0; a < MT; ++a)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = a * 16 + h * 8 + gq;
+      float s = l[a][h];
+      s += __shfl_xor_sync(0xffffffffu, s, 1);
+      s += __shfl_xor_sync(0xffffffffu, s, 2);
+      if (tq == 0) {
+        Mw[warp * ROWS + r] = m[a][h];
+        Lw[warp * ROWS + r] = s;
+        Ew[warp * ROWS + r] = (float)er[a][h];
+      }
+      float* dst = Ow + (warp * ROWS + r) * OLD;
+#pragma unroll
+      for (int n = 0; n < ND; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) dst[Q8 ? (2 * tq + e) * ND + n : n * 8 + 2 * tq + e] = o[a][n][2 * h + e];
+    }
+  __syncthreads();
+  const bool whole = n_keys <= g.chunk;
+  constexpr int LPR = D / 4;                                            // threads per row, 4 dims each
+  for (int r = threadIdx.x / LPR; r < nrows; r += 128 / LPR) {
+    const int d = threadIdx.x % LPR * 4;
+    float M = -INFINITY, E = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      M = fmaxf(M, Mw[w * ROWS + r]);
+      E = fmaxf(E, Ew[w * ROWS + r]);
+    }
+    const float ms = M == -INFINITY ? 0.f : M;
+    float L = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = fast_exp2(Mw[w * ROWS + r] - ms);
+      const float fo = Q8 ? f * fast_exp2(Ew[w * ROWS + r] - E) : f;
+      L += f * Lw[w * ROWS + r];
+      const float4 v = *reinterpret_cast<const float4*>(Ow + (w * ROWS + r) * OLD + d);
+      acc[0] += fo * v.x, acc[1] += fo * v.y, acc[2] += fo * v.z, acc[3] += fo * v.w;
+    }
+    float inv = L == 0.f ? 0.f : 1.f / L;                               // a row that sees nothing: zeros
+    if constexpr (Q8) inv *= kHalfUnit<FMT> * __int_as_float((int)fmaxf(E, 1.f) << 23);
+    const int R = r0 + r, node = R / g.G;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] *= inv;
+    if (!Q8 && flags[1]) {                                              // the dropped elements of keys this row sees
+      const uint64_t* mk = g.mask ? masks + r * 4 : nullptr;
+      for (int key = max(k_lo, min(all_see, k_hi)); key < k_hi; ++key)
+        if (sees32(mk, node, key - bi.ctx) & 1) {
+          const bf16* v = static_cast<const bf16*>(c.v) + ((size_t)slot0 + key) * D + d;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = __bfloat162float(v[e]);
+            if (!(fabsf(x) < INFINITY)) acc[e] += x;
+          }
+        }
+    }
+    const size_t at = (size_t)(bi.start + node) * g.n_heads + kvh * g.G + R % g.G;
+    if (whole) {
+      *reinterpret_cast<uint2*>(out + at * D + d) = make_uint2(pack2<EESD_KV_MODEL>(acc[0], acc[1]), pack2<EESD_KV_MODEL>(acc[2], acc[3]));
+    } else {
+      const size_t p = at * g.splits + blockIdx.x;
+      *reinterpret_cast<float4*>(g.part_o + p * D + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      if (d == 0) g.part_ml[p] = make_float2(M, L);
+    }
+  }
+}
+
+// Joins the key ranges of a row in range order (no atomics: the same bits every time): partial outputs are
+// normalised, range c weighs L_c 2^(M_c - M).  One warp per row.
+template <int D>
+__global__ void __launch_bounds__(128) attn_tree_join_kernel(TreeGeom g, CacheGeom c, int rows_per_tile, bf16* __restrict__ out) {
+  pdl_trigger();
+  pdl_wait();
+  BlockInfo bi;
+  if (!load_block(g, c, blockIdx.z, bi)) return;
+  const int R = blockIdx.x * 4 + (threadIdx.x >> 5), kvh = blockIdx.y, lane = threadIdx.x & 31;
+  if (R >= bi.T * g.G) return;
+  const int node = R / g.G;
+  // the key count of the row tile that R was in
+  const int last = (min((R / rows_per_tile + 1) * rows_per_tile, bi.T * g.G) - 1) / g.G;
+  const int n_keys = bi.ctx + (g.mask ? bi.T : last + 1);
+  if (n_keys <= g.chunk) return;                                        // written whole
+  const int n = (n_keys + g.chunk - 1) / g.chunk;
+  const size_t at = (size_t)(bi.start + node) * g.n_heads + kvh * g.G + R % g.G;
+  const float2* ml = g.part_ml + at * g.splits;
+  const float* po = g.part_o + at * g.splits * D;
+  float M = -INFINITY;
+  for (int s = lane; s < n; s += 32) M = fmaxf(M, ml[s].x);
+  M = warp_max(M);
+  const float ms = M == -INFINITY ? 0.f : M;
+  float L = 0.f;
+  constexpr int E = D / 32;
+  float acc[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  for (int s0 = 0; s0 < n; s0 += 32) {
+    float w = 0.f;
+    if (s0 + lane < n) {
+      const float2 v = ml[s0 + lane];
+      w = v.y * fast_exp2(v.x - ms);
+    }
+    const int cnt = min(32, n - s0);
+#pragma unroll 4
+    for (int s = 0; s < cnt; ++s) {
+      const float ws = __shfl_sync(0xffffffffu, w, s);
+      L += ws;
+      const float* src = po + (size_t)(s0 + s) * D + lane * E;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = ws == 0.f ? acc[e] : fmaf(ws, src[e], acc[e]);
+    }
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  bf16* dst = out + at * D + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack2<EESD_KV_MODEL>(acc[e] * inv, acc[e + 1] * inv);
+}
+
+// ---------------------------------------------------------------- plan and launch
+// One layer of the cache as a 2-D map of slots; box: `keys` slots of 64 bf16 (a 128-byte swizzled half row) or of
+// the whole 8-bit row.
+int encode_cache_map(CUtensorMap* map, const void* base, const EesdKvCache* c, int keys) {
+  PFN_encodeTiled_t enc = tensor_map_encoder();
+  if (!enc) return fail_arg(EESD_ERR_CUDA, "attn_tree: no tensor map encoder");
+  const bool q8 = c->format != EESD_KV_MODEL;
+  const int D = c->head_dim, eb = q8 ? 1 : 2;
+  cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)c->max_batch * c->n_kv_heads * c->max_seq};
+  cuuint64_t strides[1] = {(cuuint64_t)D * eb};
+  cuuint32_t box[2] = {(cuuint32_t)(q8 ? D : 64), (cuuint32_t)keys};
+  cuuint32_t estr[2] = {1, 1};
+  const CUresult r = enc(map, q8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims,
+                         strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         q8 && D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? EESD_OK : fail_arg(EESD_ERR_CUDA, "attn_tree: cache tensor map (%d)", (int)r);
+}
+
+struct Plan {
+  int mt;               // bf16: 16-row m-tiles per CTA
+  int tiles;            // row tiles of the largest block
+  int chunk, splits;    // keys per CTA, key ranges of the longest row
+  size_t ml_off, bytes;
+};
+
+Plan plan_for(const EesdKvCache* c, const EesdTree* t, int n_heads, int split_keys) {
+  Plan p{};
+  const int G = n_heads / c->n_kv_heads, rows = t->max_nodes * G;
+  p.mt = rows <= 16 ? 1 : 2;
+  p.tiles = (rows + 16 * p.mt - 1) / (16 * p.mt);
+  const int slots = 148 * (p.mt == 1 ? 3 : 2);
+  p.chunk = split_keys;
+  if (!p.chunk) {
+    const long long ctas = (long long)t->n_blocks * c->n_kv_heads * p.tiles;
+    const int want = (int)std::max(1LL, slots / std::max(1LL, ctas));
+    const int per = (t->max_ctx + want - 1) / want;
+    p.chunk = (per + 255) / 256 * 256;
+  }
+  p.splits = (t->max_ctx + p.chunk - 1) / p.chunk;
+  if (p.splits > 1) {
+    const size_t n = (size_t)t->n_tokens * n_heads * p.splits;
+    p.ml_off = n * c->head_dim * 4;
+    p.bytes = p.ml_off + n * 8;
+  }
+  p.bytes = std::max<size_t>((p.bytes + 255) / 256 * 256, 256);
+  return p;
+}
+
+template <int D, int FMT, int MT>
+cudaError_t launch_mma(const Plan& p, const TreeGeom& g, const CacheGeom& c, const CUtensorMap& km, const CUtensorMap& vm, int n_blocks,
+                       const void* q, void* out, cudaStream_t s) {
+  using S = MmaShape<D, FMT, MT>;
+  auto kernel = attn_tree_mma_kernel<D, FMT, MT>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::smem);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(kernel, dim3(p.splits, p.tiles * c.n_kv_heads, n_blocks), dim3(128), S::smem, s, km, vm, g, c,
+                    static_cast<const bf16*>(q), static_cast<bf16*>(out));
+}
+template <int D, int FMT>
+cudaError_t launch_mt(const Plan& p, const TreeGeom& g, const CacheGeom& c, const CUtensorMap& km, const CUtensorMap& vm, int nb,
+                      const void* q, void* out, cudaStream_t s) {
+  cudaError_t e = p.mt == 1 ? launch_mma<D, FMT, 1>(p, g, c, km, vm, nb, q, out, s) : launch_mma<D, FMT, 2>(p, g, c, km, vm, nb, q, out, s);
+  if (e == cudaSuccess && p.splits > 1)
+    e = launch_pdl(attn_tree_join_kernel<D>, dim3((g.max_nodes * g.G + 3) / 4, c.n_kv_heads, nb), dim3(128), 0, s, g, c, 16 * p.mt,
+                   static_cast<bf16*>(out));
+  return e;
+}
+
 template <typename T, int FMT, int D>
 cudaError_t launch_simt(const TreeGeom& g, const CacheGeom& c, int n_blocks, const void* q, void* out, cudaStream_t s) {
   const dim3 grid((g.max_nodes * g.G + 31) / 32, c.n_kv_heads, n_blocks);
@@ -152,15 +808,25 @@ cudaError_t launch_simt(const TreeGeom& g, const CacheGeom& c, int n_blocks, con
   if (e != cudaSuccess) return e;
   return launch_pdl(attn_tree_simt_kernel<T, FMT, D>, grid, dim3(128), smem, s, g, c, static_cast<const T*>(q), static_cast<T*>(out));
 }
-template <typename T>
-cudaError_t launch_simt_fmt(int fmt, int D, const TreeGeom& g, const CacheGeom& c, int nb, const void* q, void* out, cudaStream_t s) {
+cudaError_t launch_f32(int fmt, int D, const TreeGeom& g, const CacheGeom& c, int nb, const void* q, void* out, cudaStream_t s) {
   switch (fmt * 2 + (D == 128)) {
-    case 0: return launch_simt<T, EESD_KV_MODEL, 64>(g, c, nb, q, out, s);
-    case 1: return launch_simt<T, EESD_KV_MODEL, 128>(g, c, nb, q, out, s);
-    case 2: return launch_simt<T, EESD_KV_E4M3, 64>(g, c, nb, q, out, s);
-    case 3: return launch_simt<T, EESD_KV_E4M3, 128>(g, c, nb, q, out, s);
-    case 4: return launch_simt<T, EESD_KV_INT8, 64>(g, c, nb, q, out, s);
-    default: return launch_simt<T, EESD_KV_INT8, 128>(g, c, nb, q, out, s);
+    case 0: return launch_simt<float, EESD_KV_MODEL, 64>(g, c, nb, q, out, s);
+    case 1: return launch_simt<float, EESD_KV_MODEL, 128>(g, c, nb, q, out, s);
+    case 2: return launch_simt<float, EESD_KV_E4M3, 64>(g, c, nb, q, out, s);
+    case 3: return launch_simt<float, EESD_KV_E4M3, 128>(g, c, nb, q, out, s);
+    case 4: return launch_simt<float, EESD_KV_INT8, 64>(g, c, nb, q, out, s);
+    default: return launch_simt<float, EESD_KV_INT8, 128>(g, c, nb, q, out, s);
+  }
+}
+cudaError_t launch_bf16(int fmt, int D, const Plan& p, const TreeGeom& g, const CacheGeom& c, const CUtensorMap& km, const CUtensorMap& vm,
+                        int nb, const void* q, void* out, cudaStream_t s) {
+  switch (fmt * 2 + (D == 128)) {
+    case 0: return launch_mt<64, EESD_KV_MODEL>(p, g, c, km, vm, nb, q, out, s);
+    case 1: return launch_mt<128, EESD_KV_MODEL>(p, g, c, km, vm, nb, q, out, s);
+    case 2: return launch_mt<64, EESD_KV_E4M3>(p, g, c, km, vm, nb, q, out, s);
+    case 3: return launch_mt<128, EESD_KV_E4M3>(p, g, c, km, vm, nb, q, out, s);
+    case 4: return launch_mt<64, EESD_KV_INT8>(p, g, c, km, vm, nb, q, out, s);
+    default: return launch_mt<128, EESD_KV_INT8>(p, g, c, km, vm, nb, q, out, s);
   }
 }
 
@@ -184,7 +850,8 @@ extern "C" {
 
 size_t eesd_attn_tree_workspace_bytes(int dtype, const EesdKvCache* c, const EesdTree* t, int n_heads, int split_keys) {
   if (check_attn(dtype, c, 0, t, n_heads, split_keys)) return 0;
-  return 256;
+  if (dtype == EESD_F32 || t->n_tokens == 0 || t->n_blocks == 0) return 256;
+  return plan_for(c, t, n_heads, split_keys).bytes;
 }
 
 int eesd_attn_tree(int dtype, const EesdKvCache* c, int layer, const EesdTree* t, const void* q, int ld_q, int n_heads, void* out,
@@ -202,11 +869,23 @@ int eesd_attn_tree(int dtype, const EesdKvCache* c, int layer, const EesdTree* t
     return fail_arg(EESD_ERR_ARG, "attn_tree: workspace %zu < %zu bytes, or not 256-byte aligned", workspace_bytes, need);
   if ((rc = check_stream("attn_tree", stream))) return rc;
   const CacheGeom cg = cache_layer(c, dtype, layer);
-  const TreeGeom g{n_heads, n_heads / c->n_kv_heads, t->n_tokens, t->max_nodes, t->max_ctx, t->words, t->blk, t->mask, ld_q,
-                   1.f / sqrtf((float)c->head_dim), status};
+  TreeGeom g{n_heads, n_heads / c->n_kv_heads, t->n_tokens, t->max_nodes, t->max_ctx, t->words, t->blk, t->mask, ld_q,
+             1.f / sqrtf((float)c->head_dim), status, spin_limit(), 0, 0, nullptr, nullptr};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = dtype == EESD_BF16 ? launch_simt_fmt<bf16>(c->format, c->head_dim, g, cg, t->n_blocks, q, out, s)
-                                           : launch_simt_fmt<float>(c->format, c->head_dim, g, cg, t->n_blocks, q, out, s);
+  cudaError_t e;
+  if (dtype == EESD_F32) {
+    e = launch_f32(c->format, c->head_dim, g, cg, t->n_blocks, q, out, s);
+  } else {
+    const Plan p = plan_for(c, t, n_heads, split_keys);
+    g.chunk = p.chunk;
+    g.splits = p.splits;
+    g.part_o = static_cast<float*>(workspace);
+    g.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + p.ml_off);
+    const int keys = 4096 / (c->head_dim * (c->format == EESD_KV_MODEL ? 2 : 1));
+    CUtensorMap km, vm;
+    if ((rc = encode_cache_map(&km, cg.k, c, keys)) || (rc = encode_cache_map(&vm, cg.v, c, keys))) return rc;
+    e = launch_bf16(c->format, c->head_dim, p, g, cg, km, vm, t->n_blocks, q, out, s);
+  }
   return e == cudaSuccess ? EESD_OK : fail_arg(EESD_ERR_CUDA, "attn_tree: launch: %s", cudaGetErrorString(e));
 }
 
