@@ -339,7 +339,7 @@ int eesd_kv_read(int dtype, const EesdKvCache* cache, int layer, const int32_t* 
  * infinities among them, do not reach it.  q: rotated queries, tokens ld_q elements apart (ld_q % 8 == 0,
  * 16-byte aligned), Hq D used; out [n_tokens, Hq D].  split_keys: 0 lets the library split long key ranges
  * over CTAs as the launch needs; a multiple of 256 fixes the split, so that a block's result does not
- * depend on the other blocks of the launch.  workspace: eesd_attn_tree_workspace_bytes() bytes, 256-byte aligned,
+ * depend on the other blocks of the launch (at the same max_nodes, which decides the kernel).  workspace: eesd_attn_tree_workspace_bytes() bytes, 256-byte aligned,
  * not initialised, not shared by calls that may overlap.  A block that does not fit the tree's maxima or
  * the cache sets a bit in *status and is skipped. */
 size_t eesd_attn_tree_workspace_bytes(int dtype, const EesdKvCache* cache, const EesdTree* tree, int n_heads, int split_keys);

@@ -21,7 +21,8 @@ PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "_lib" / "libeesd.so"
-SOURCES = ["gemm_tc.cu", "kernels.cu", "runtime.cu", "head_static.cu", "cache_ops.cu", "attn_tree.cu"]
+SOURCES = ["gemm_tc.cu", "kernels.cu", "runtime.cu", "head_static.cu", "cache_ops.cu", "attn_tree.cu",
+           "attn_tree_tc.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

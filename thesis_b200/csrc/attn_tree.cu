@@ -8,38 +8,13 @@
 #include <algorithm>
 
 #include "attn_tree.h"
-#include "cache.cuh"
+#include "attn_tree_dev.cuh"
+#include "attn_tree_tc.h"
 #include "gemm_tc.h"
 
 namespace eesd {
 namespace {
 
-struct TreeGeom {
-  int n_heads, G;
-  int n_tokens, max_nodes, max_ctx, words;
-  const int32_t* blk;
-  const uint64_t* mask;
-  int ld_q;
-  float scale;
-  int* status;
-  uint32_t spin;       // poll limit of the pipeline waits
-  int chunk, splits;   // keys per CTA; key ranges of the longest row
-  float* part_o;       // [n_tokens, Hq, splits, D] normalised partial outputs
-  float2* part_ml;     // [n_tokens, Hq, splits] (max in the log2 domain, sum)
-};
-
-struct BlockInfo {
-  int start, T, row, ctx;
-};
-// Reads block b; false (and a status bit, from one thread) where it does not fit the tokens, the maxima or the cache.
-__device__ __forceinline__ bool load_block(const TreeGeom& g, const CacheGeom& c, int b, BlockInfo& i) {
-  const int4 v = *reinterpret_cast<const int4*>(g.blk + 4 * b);
-  i.start = v.x, i.T = v.y, i.row = v.z, i.ctx = v.w;
-  const bool ok = i.start >= 0 && i.T > 0 && i.T <= g.max_nodes && i.start <= g.n_tokens - i.T && i.row >= 0 &&
-                  i.row < c.max_batch && i.ctx >= 0 && i.ctx <= min(g.max_ctx, c.max_seq) - i.T;
-  if (!ok && threadIdx.x == 0) set_status(g.status, kStatusBadIndex);
-  return ok;
-}
 __device__ __forceinline__ bool node_sees(const TreeGeom& g, const BlockInfo& i, int node, int j) {
   if (!g.mask) return j <= node;
   return j < 64 * g.words && (g.mask[(size_t)(i.start + node) * g.words + (j >> 6)] >> (j & 63) & 1);
@@ -163,11 +138,6 @@ __global__ void __launch_bounds__(128) attn_tree_simt_kernel(TreeGeom g, CacheGe
 // from shared memory as 16-byte words and turn into f16 pairs in registers, without a transpose.  The values'
 // powers of two never touch the operands: K's scale multiplies the score, V's the weight (relative to the
 // largest one so far of the row, eref, as the running maximum does), a power of two of each q row its f16 form.
-__device__ __forceinline__ float fast_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -178,19 +148,9 @@ __device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t (&r)[4]) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr));
 }
-__device__ __forceinline__ uint4 lds128(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-  return v;
-}
 __device__ __forceinline__ uint2 lds64(uint32_t addr) {
   uint2 v;
   asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
-  return v;
-}
-__device__ __forceinline__ uint32_t lds_u16(uint32_t addr) {
-  uint16_t v;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr));
   return v;
 }
 template <int FMT> __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -205,37 +165,6 @@ template <int FMT> __device__ __forceinline__ void mma16816(float (&c)[4], const
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-template <int FMT> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  if constexpr (FMT == EESD_KV_MODEL) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  } else {
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
-}
-// bf16 pair with its non-finite elements replaced by zero
-__device__ __forceinline__ uint32_t drop_nonfinite(uint32_t v, bool& hit) {
-  const bool lo = (v & 0x7f80u) == 0x7f80u, hi = (v & 0x7f800000u) == 0x7f800000u;
-  hit = hit || lo || hi;
-  return (lo ? 0u : v & 0xffffu) | (hi ? 0u : v & 0xffff0000u);
-}
-
-// Which of the 32 nodes j0 .. j0 + 31 a node sees (bit i: node j0 + i); negative nodes are committed slots.
-// mask: the node's 4 words in shared memory, or null for causal blocks.
-__device__ __forceinline__ uint32_t sees32(const uint64_t* mask, int node, int j0) {
-  if (!mask) {
-    const int n = node - j0 + 1;
-    return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1;
-  }
-  if (j0 <= -32) return ~0u;
-  if (j0 < 0) return (uint32_t)(mask[0] << -j0) | ((1u << -j0) - 1);
-  const int w = j0 >> 6, sh = j0 & 63;
-  uint64_t v = w < 4 ? mask[w] >> sh : 0;
-  if (sh > 32 && w < 3) v |= mask[w + 1] << (64 - sh);
-  return (uint32_t)v;
-}
-
 template <int D, int FMT, int MT> struct MmaShape {
   static constexpr int kEb = FMT == EESD_KV_MODEL ? 2 : 1;
   static constexpr int KG = 4096 / (D * kEb);          // keys per group: 4 KB of K, 4 KB of V
@@ -462,7 +391,7 @@ __global__ void __launch_bounds__(128, MmaShape<D, FMT, MT>::CTAS)
 #pragma unroll
           for (int w = 0; w < (KG > 32 ? 2 : 1); ++w) {
             const int kb = key0 + 32 * w;
-            see[w] = sees32(g.mask ? masks + r * 4 : nullptr, node, kb - bi.ctx);
+            see[w] = sees32(g.mask ? masks + r * 4 : nullptr, 4, node, kb - bi.ctx);
             const int left = k_hi - kb;
             if (left < 32) see[w] &= left <= 0 ? 0u : (1u << left) - 1;
           }
@@ -661,7 +590,7 @@ __global__ void __launch_bounds__(128, MmaShape<D, FMT, MT>::CTAS)
     if (!Q8 && flags[1]) {                                              // the dropped elements of keys this row sees
       const uint64_t* mk = g.mask ? masks + r * 4 : nullptr;
       for (int key = max(k_lo, min(all_see, k_hi)); key < k_hi; ++key)
-        if (sees32(mk, node, key - bi.ctx) & 1) {
+        if (sees32(mk, 4, node, key - bi.ctx) & 1) {
           const bf16* v = static_cast<const bf16*>(c.v) + ((size_t)slot0 + key) * D + d;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -751,32 +680,50 @@ int encode_cache_map(CUtensorMap* map, const void* base, const EesdKvCache* c, i
 }
 
 struct Plan {
-  int mt;               // bf16: 16-row m-tiles per CTA
-  int tiles;            // row tiles of the largest block
+  bool tc;              // tcgen05 kernel (attn_tree_tc.cu), else mma.sync
+  int mt;               // mma.sync: 16-row m-tiles per CTA
+  int rows, tiles;      // rows per tile, row tiles of the largest block
   int chunk, splits;    // keys per CTA, key ranges of the longest row
-  size_t ml_off, bytes;
+  int ctas;             // tcgen05: persistent CTAs
+  size_t ml_off, table_off, bytes;
 };
+
+int sm_count() {
+  static const int n = [] {
+    int dev = 0, v = 148;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) v = 148;
+    return v;
+  }();
+  return n;
+}
 
 Plan plan_for(const EesdKvCache* c, const EesdTree* t, int n_heads, int split_keys) {
   Plan p{};
   const int G = n_heads / c->n_kv_heads, rows = t->max_nodes * G;
+  p.tc = rows > 32;
   p.mt = rows <= 16 ? 1 : 2;
-  p.tiles = (rows + 16 * p.mt - 1) / (16 * p.mt);
-  const int slots = 148 * (p.mt == 1 ? 3 : 2);
+  p.rows = p.tc ? (rows <= 128 ? 128 : 256) : 16 * p.mt;
+  p.tiles = (rows + p.rows - 1) / p.rows;
+  const long long units = (long long)t->n_blocks * c->n_kv_heads * p.tiles;
   p.chunk = split_keys;
-  if (!p.chunk) {
-    const long long ctas = (long long)t->n_blocks * c->n_kv_heads * p.tiles;
-    const int want = (int)std::max(1LL, slots / std::max(1LL, ctas));
+  size_t parts = 0;     // partial rows
+  if (p.tc) {
+    // a run of less than 8 tiles is not worth a CTA of its own
+    const long long most = units * ((t->max_ctx + 63) / 64);
+    p.ctas = (int)std::max(1LL, std::min<long long>(sm_count(), (most + 7) / 8));
+    if (!p.chunk) parts = (size_t)p.ctas * 2 * p.rows;
+  } else if (!p.chunk) {
+    const int slots = sm_count() * (p.mt == 1 ? 3 : 2);
+    const int want = (int)std::max(1LL, slots / std::max(1LL, units));
     const int per = (t->max_ctx + want - 1) / want;
     p.chunk = (per + 255) / 256 * 256;
   }
-  p.splits = (t->max_ctx + p.chunk - 1) / p.chunk;
-  if (p.splits > 1) {
-    const size_t n = (size_t)t->n_tokens * n_heads * p.splits;
-    p.ml_off = n * c->head_dim * 4;
-    p.bytes = p.ml_off + n * 8;
-  }
-  p.bytes = std::max<size_t>((p.bytes + 255) / 256 * 256, 256);
+  p.splits = p.chunk ? (t->max_ctx + p.chunk - 1) / p.chunk : 1;
+  if (p.splits > 1) parts = (size_t)t->n_tokens * n_heads * p.splits;
+  const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
+  p.ml_off = up(parts * c->head_dim * 4);
+  p.table_off = p.ml_off + up(parts * 8);
+  p.bytes = std::max<size_t>(p.table_off + (p.tc ? up(((size_t)t->n_blocks * p.tiles + 1) * 8) : 0), 256);
   return p;
 }
 
@@ -793,11 +740,7 @@ cudaError_t launch_mma(const Plan& p, const TreeGeom& g, const CacheGeom& c, con
 template <int D, int FMT>
 cudaError_t launch_mt(const Plan& p, const TreeGeom& g, const CacheGeom& c, const CUtensorMap& km, const CUtensorMap& vm, int nb,
                       const void* q, void* out, cudaStream_t s) {
-  cudaError_t e = p.mt == 1 ? launch_mma<D, FMT, 1>(p, g, c, km, vm, nb, q, out, s) : launch_mma<D, FMT, 2>(p, g, c, km, vm, nb, q, out, s);
-  if (e == cudaSuccess && p.splits > 1)
-    e = launch_pdl(attn_tree_join_kernel<D>, dim3((g.max_nodes * g.G + 3) / 4, c.n_kv_heads, nb), dim3(128), 0, s, g, c, 16 * p.mt,
-                   static_cast<bf16*>(out));
-  return e;
+  return p.mt == 1 ? launch_mma<D, FMT, 1>(p, g, c, km, vm, nb, q, out, s) : launch_mma<D, FMT, 2>(p, g, c, km, vm, nb, q, out, s);
 }
 
 template <typename T, int FMT, int D>
@@ -881,10 +824,21 @@ int eesd_attn_tree(int dtype, const EesdKvCache* c, int layer, const EesdTree* t
     g.splits = p.splits;
     g.part_o = static_cast<float*>(workspace);
     g.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + p.ml_off);
-    const int keys = 4096 / (c->head_dim * (c->format == EESD_KV_MODEL ? 2 : 1));
+    const int keys = p.tc ? 64 : 4096 / (c->head_dim * (c->format == EESD_KV_MODEL ? 2 : 1));
     CUtensorMap km, vm;
     if ((rc = encode_cache_map(&km, cg.k, c, keys)) || (rc = encode_cache_map(&vm, cg.v, c, keys))) return rc;
-    e = launch_bf16(c->format, c->head_dim, p, g, cg, km, vm, t->n_blocks, q, out, s);
+    if (p.tc) {
+      const TcSchedule sc{p.ctas, p.rows, p.tiles, t->n_blocks * p.tiles, split_keys / 64,
+                          reinterpret_cast<long long*>(static_cast<uint8_t*>(workspace) + p.table_off)};
+      e = launch_attn_tree_tc(c->format, c->head_dim, sc, g, cg, km, vm, t->n_blocks, q, out, s);
+    } else {
+      e = launch_bf16(c->format, c->head_dim, p, g, cg, km, vm, t->n_blocks, q, out, s);
+    }
+    if (e == cudaSuccess && p.splits > 1) {
+      const dim3 grid((t->max_nodes * g.G + 3) / 4, c->n_kv_heads, t->n_blocks);
+      e = c->head_dim == 64 ? launch_pdl(attn_tree_join_kernel<64>, grid, dim3(128), 0, s, g, cg, p.rows, static_cast<bf16*>(out))
+                            : launch_pdl(attn_tree_join_kernel<128>, grid, dim3(128), 0, s, g, cg, p.rows, static_cast<bf16*>(out));
+    }
   }
   return e == cudaSuccess ? EESD_OK : fail_arg(EESD_ERR_CUDA, "attn_tree: launch: %s", cudaGetErrorString(e));
 }

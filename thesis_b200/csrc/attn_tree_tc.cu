@@ -1,0 +1,844 @@
+// Tree attention for many query rows per KV head (wide trees, prefill chunks): tcgen05.
+//
+// A persistent CTA per SM works on row tiles of up to 256 rows (two M = 128 accumulators).  All (block, row tile,
+// KV head) units are laid end to end in 64-key tiles and cut into equal runs, one per CTA, so ragged contexts and
+// causal tiles balance whatever their number; a unit that a cut goes through leaves normalised partial outputs,
+// which a second kernel joins in order.
+//
+// Per 64-key tile: S = Q K^T (Q in TMEM, K in shared memory), softmax weights P from S in registers back into S's
+// columns, O += P V (P in TMEM, V in shared memory, both from the tile's own layout: V is the MN-major operand).
+// With Q and P in TMEM the tensor cores read shared memory for K and V only.  Two streams alternate so that one's
+// softmax runs under the other's products: with more than 128 rows each stream is one half of the rows over all
+// key tiles; with fewer, both share the rows and take every other key tile, and meet at the end.
+//
+// 8-bit caches: a warpgroup turns the TMA-loaded bytes into the f16 tiles that the products read (exactly; the
+// powers of two stay out of the operands and multiply scores and weights instead).
+//
+// Roles of the 16 warps: 0 TMA, 1 MMA issue, 4-7 and 8-11 softmax of stream 0 and 1 (a thread is a row), 12-15
+// conversion (8-bit) or the check of V tiles that some row does not wholly see (bf16).
+#include <algorithm>
+
+#include "attn_tree.h"
+#include "attn_tree_dev.cuh"
+#include "attn_tree_tc.h"
+#include "gemm_tc.h"
+#include "kernels.h"
+
+namespace eesd {
+namespace {
+
+constexpr int KT = 64;                     // keys per tile
+constexpr int kThreads = 512;
+constexpr uint32_t kColO = 0, kColQ = 256, kColS = 384;   // TMEM columns; stream x adds 128, 64, 64
+
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// D[tmem] (+)= A[tmem] * B[smem]
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+#define EESD_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
+#define EESD_W8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
+// 32 lanes x 32 columns; lane i of the warp holds TMEM lane (quadrant base + i)
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,"
+      "%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : EESD_R8(r, 0), EESD_R8(r, 8), EESD_R8(r, 16), EESD_R8(r, 24)
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,"
+      "%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::EESD_W8(r, 0),
+      EESD_W8(r, 8), EESD_W8(r, 16), EESD_W8(r, 24), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// The whole warp waits and goes on together (what follows are warp-wide instructions).
+__device__ __forceinline__ bool warp_wait(const void* bar, uint32_t parity, volatile int* abort_flag, uint32_t limit) {
+  return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, abort_flag, limit));
+}
+template <int N> __device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// two fp32 operations at once
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack_f2(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack_f2(f32x2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// MN-major operand tile (64-element, 128-byte rows of the MN index per K index, 128-byte swizzle): 8 K indices
+// are 1024 bytes (stride), the next 64 MN elements lie `lbo` bytes on.
+__device__ __forceinline__ uint64_t sw128_mnmajor_desc(uint32_t smem_addr, uint32_t lbo) {
+  return sw128_kmajor_desc(smem_addr) & ~((uint64_t)0x3FFF << 16) | (uint64_t)((lbo >> 4) & 0x3FFF) << 16;
+}
+// M = 128 x N, fp32 accumulate; f16 or bf16 operands, B K-major or MN-major
+template <int FMT> __device__ __forceinline__ uint32_t idesc_f32(int n, bool b_mn) {
+  const uint32_t ab = FMT == EESD_KV_MODEL ? (1u << 7 | 1u << 10) : 0u;
+  return (1u << 4) | ab | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+}
+
+// ------------------------------------------------------------------ the flat schedule
+// Entry e = (block, row tile); its unit of each KV head takes tiles() key tiles.  Flat position = tiles of the
+// entries before, all heads, then head by head.
+struct Entry {
+  BlockInfo bi;
+  int r0, nrows, n_keys, all_see, tiles;   // slots below all_see are seen by every row of the tile
+};
+__device__ __forceinline__ Entry entry_of(const TreeGeom& g, const CacheGeom& c, const TcSchedule& sc, int e, bool& bad) {
+  Entry x;
+  const int b = e / sc.tiles_max, tile = e - b * sc.tiles_max;
+  x.tiles = 0;
+  bad = !block_fits(g, c, b, x.bi);
+  if (bad) return x;
+  x.r0 = tile * sc.rows;
+  x.nrows = min(sc.rows, x.bi.T * g.G - x.r0);
+  if (x.nrows <= 0) return x;
+  x.n_keys = x.bi.ctx + (g.mask ? x.bi.T : (x.r0 + x.nrows - 1) / g.G + 1);
+  x.all_see = x.bi.ctx + (g.mask ? 0 : x.r0 / g.G + 1);
+  x.tiles = (x.n_keys + KT - 1) / KT;
+  return x;
+}
+struct Piece : Entry {
+  int h, t0, t1, index;     // KV head, key tiles [t0, t1), number of the piece in its CTA
+  bool whole;               // the unit in one piece
+};
+// The pieces of one CTA's run [pos, end).  With a fixed split (sc.chunk_tiles) a unit is cut at multiples of it and
+// a piece belongs to the CTA whose run holds its first tile; otherwise a piece is what the run holds of a unit.
+struct PieceIter {
+  long long pos, end, base;
+  int e, index;
+  __device__ bool next(const TreeGeom& g, const CacheGeom& c, const TcSchedule& sc, Piece& p) {
+    while (pos < end) {
+      bool bad;
+      static_cast<Entry&>(p) = entry_of(g, c, sc, e, bad);
+      const long long span = (long long)p.tiles * c.n_kv_heads;
+      if (pos >= base + span) {
+        base += span;
+        ++e;
+        continue;
+      }
+      const int off = (int)(pos - base);
+      p.h = off / p.tiles;
+      p.t0 = off - p.h * p.tiles;
+      if (sc.chunk_tiles) {
+        const int up = (p.t0 + sc.chunk_tiles - 1) / sc.chunk_tiles * sc.chunk_tiles;
+        if (up != p.t0) {                                  // inside a piece of the CTA before
+          pos += min(up, p.tiles) - p.t0;
+          continue;
+        }
+        p.t1 = min(p.tiles, p.t0 + sc.chunk_tiles);
+      } else {
+        p.t1 = (int)min((long long)p.tiles, p.t0 + (end - pos));
+      }
+      p.whole = p.t0 == 0 && p.t1 == p.tiles;
+      p.index = index++;
+      pos += p.t1 - p.t0;
+      return true;
+    }
+    return false;
+  }
+};
+
+template <int D, int FMT> struct TcShape {
+  static constexpr bool Q8 = FMT != EESD_KV_MODEL;
+  static constexpr int TILE = KT * D * 2;              // bytes of one 16-bit K (or V) tile
+  static constexpr int RAW = KT * D * 2;               // 8-bit: K and V bytes of one tile
+  static constexpr int NS = Q8 ? 2 : 6;                // 16-bit K / V stages
+  static constexpr int RS = Q8 ? 8 : 0;                // raw stages
+  static constexpr int FR = 4;                         // factor ring
+  static constexpr size_t ctl = 12288;
+  static constexpr size_t smem = 1024 + (size_t)2 * NS * TILE + (size_t)RS * RAW + ctl;
+};
+struct TcControl {
+  uint64_t kfull[6], kempty[6], vfull[6], vempty[6], vclean[6], raw_full[8], raw_empty[8], ffull[4];
+  uint64_t s_full[2], p_ready[2], q_ready, o_done, ml_ready, drain;
+  alignas(16) float fk[4][KT];             // 8-bit: 2^ek of a tile's keys
+  alignas(16) float fv[4][KT];             // 2^(ev - emax)
+  alignas(16) uint8_t ev[4][KT];
+  alignas(16) uint8_t exps[8][2 * KT];     // raw exponent bytes, K then V
+  int emax[4];
+  float ml[2][2][3][128];                  // one row tile: max, sum and eref of the streams (by piece parity)
+  long long lo, hi, base;
+  long long wsum[16];
+  uint32_t tmem;
+  int e0;
+  int abort, dropped;
+};
+static_assert(sizeof(TcControl) <= 12288 && alignof(TcControl) <= 16, "control block");
+
+template <int D, int FMT>
+__global__ void __launch_bounds__(kThreads, 1)
+    attn_tree_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, TreeGeom g, CacheGeom c,
+                        TcSchedule sc, const bf16* __restrict__ q, bf16* __restrict__ out) {
+  using S = TcShape<D, FMT>;
+  constexpr bool Q8 = S::Q8;
+  constexpr int NS = S::NS, RS = Q8 ? S::RS : 1, FR = S::FR, HALVES = D / 64;
+  pdl_trigger();
+  pdl_wait();
+  extern __shared__ uint8_t smem8[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem8) + 1023) & ~uintptr_t(1023));
+  const uint32_t kbuf = smem_u32(sm), vbuf = kbuf + NS * S::TILE, raw = vbuf + NS * S::TILE;
+  TcControl& ct = *reinterpret_cast<TcControl*>(sm + 2 * NS * S::TILE + S::RS * S::RAW);
+  volatile int* abort_flag = &ct.abort;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  // ---- this CTA's run of the flat schedule: block-wide prefix of the entries' tiles
+  {
+    const int E = sc.entries, seg = (E + kThreads - 1) / kThreads;
+    const int a = min(E, tid * seg), b = min(E, a + seg);
+    long long sum = 0;
+    for (int e = a; e < b; ++e) {
+      bool bad;
+      sum += entry_of(g, c, sc, e, bad).tiles;
+      if (bad && blockIdx.x == 0) set_status(g.status, kStatusBadIndex);
+    }
+    long long inc = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    if (lane == 31) ct.wsum[warp] = inc;
+    if (tid == 0) {
+      ct.abort = ct.dropped = 0;
+      ct.e0 = E;
+      for (int i = 0; i < NS; ++i) {
+        mbar_init(smem_u32(&ct.kfull[i]), Q8 ? 128 : 1);
+        mbar_init(smem_u32(&ct.vfull[i]), Q8 ? 128 : 1);
+        mbar_init(smem_u32(&ct.kempty[i]), 1);
+        mbar_init(smem_u32(&ct.vempty[i]), 1);
+        mbar_init(smem_u32(&ct.vclean[i]), 128);
+      }
+      for (int i = 0; i < RS; ++i) {
+        mbar_init(smem_u32(&ct.raw_full[i]), 1);
+        mbar_init(smem_u32(&ct.raw_empty[i]), 128);
+      }
+      for (int i = 0; i < FR; ++i) mbar_init(smem_u32(&ct.ffull[i]), 128);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(smem_u32(&ct.s_full[i]), 1);
+        mbar_init(smem_u32(&ct.p_ready[i]), 128);
+      }
+      mbar_init(smem_u32(&ct.q_ready), 256);
+      mbar_init(smem_u32(&ct.ml_ready), 256);
+      mbar_init(smem_u32(&ct.o_done), 1);
+      mbar_init(smem_u32(&ct.drain), 1);
+      fence_mbar_init();
+    }
+    if (warp == 1) {
+      tmem_alloc(smem_u32(&ct.tmem), 512);
+      tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    long long before = inc - sum, total = 0;
+    for (int w = 0; w < 16; ++w) {
+      if (w < warp) before += ct.wsum[w];
+      total += ct.wsum[w];
+    }
+    const int Hkv = c.n_kv_heads;
+    const long long W = total * Hkv, n = gridDim.x;
+    const long long lo = blockIdx.x * W / n, hi = (blockIdx.x + 1) * W / n;
+    if (tid == 0) {
+      ct.lo = lo;
+      ct.hi = hi;
+      if (blockIdx.x == 0) sc.table[E] = W;
+    }
+    if (blockIdx.x == 0 || (lo >= before * Hkv && lo < (before + sum) * Hkv)) {
+      long long base = before * Hkv;
+      for (int e = a; e < b; ++e) {
+        bool bad;
+        const long long span = (long long)entry_of(g, c, sc, e, bad).tiles * Hkv;
+        if (blockIdx.x == 0) sc.table[e] = base;
+        if (lo >= base && lo < base + span) {
+          ct.e0 = e;
+          ct.base = base;
+        }
+        base += span;
+      }
+    }
+    __syncthreads();
+  }
+  PieceIter it{ct.lo, ct.hi, ct.base, ct.e0, 0};
+  if (ct.e0 >= sc.entries) it.pos = it.end;
+  Piece p;
+  const uint32_t tmem = ct.tmem;
+
+  if (warp < 4) reg_dec<64>();
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA
+    if (lane == 0) {
+      int cnt = 0, k_issued = 0, v_issued = 0;
+      bool ok = true;
+      tma_prefetch_desc(&kmap);
+      tma_prefetch_desc(&vmap);
+      while (ok && it.next(g, c, sc, p)) {
+        const int slot0 = (int)cache_slot(c, p.bi.row, p.h, 0);
+        for (int t = p.t0; t < p.t1; ++t, ++cnt) {
+          if constexpr (Q8) {
+            const int s = cnt % RS;
+            if (!(ok = mbar_wait(smem_u32(&ct.raw_empty[s]), (cnt / RS & 1) ^ 1, abort_flag, g.spin))) break;
+            const uint32_t fb = smem_u32(&ct.raw_full[s]), dst = raw + s * S::RAW, ex = smem_u32(ct.exps[s]);
+            const uint32_t eb = min(KT, c.max_seq - t * KT);          // max_seq % 16 == 0
+            mbar_arrive_expect_tx(fb, S::RAW + 2 * eb);
+            tma_load_2d(dst, &kmap, 0, slot0 + t * KT, fb);
+            tma_load_2d(dst + S::RAW / 2, &vmap, 0, slot0 + t * KT, fb);
+            bulk_g2s(ex, c.ke + slot0 + t * KT, eb, fb);
+            bulk_g2s(ex + KT, c.ve + slot0 + t * KT, eb, fb);
+            k_issued = cnt + 1;
+          } else {
+            const int s = cnt % NS;
+            const uint32_t ph = (cnt / NS & 1) ^ 1;
+            if (!(ok = mbar_wait(smem_u32(&ct.kempty[s]), ph, abort_flag, g.spin))) break;
+            const uint32_t kb = smem_u32(&ct.kfull[s]), vb = smem_u32(&ct.vfull[s]);
+            mbar_arrive_expect_tx(kb, S::TILE);
+            for (int h = 0; h < HALVES; ++h) tma_load_2d(kbuf + s * S::TILE + h * KT * 128, &kmap, h * 64, slot0 + t * KT, kb);
+            k_issued = cnt + 1;
+            if (!(ok = mbar_wait(smem_u32(&ct.vempty[s]), ph, abort_flag, g.spin))) break;
+            mbar_arrive_expect_tx(vb, S::TILE);
+            for (int h = 0; h < HALVES; ++h) tma_load_2d(vbuf + s * S::TILE + h * KT * 128, &vmap, h * 64, slot0 + t * KT, vb);
+            v_issued = cnt + 1;
+          }
+        }
+      }
+      if (!ok) {
+        set_status(g.status, kStatusTimeoutProducer);
+        *abort_flag = 1;
+      }
+      // Nothing may be in flight when the CTA exits.  After a clean run every load has been waited for; after an
+      // abort the last load of every stage is waited for here.
+      if (*abort_flag) {
+        for (int i = max(0, k_issued - (Q8 ? RS : NS)); i < k_issued; ++i)
+          mbar_drain(Q8 ? smem_u32(&ct.raw_full[i % RS]) : smem_u32(&ct.kfull[i % NS]), (i / (Q8 ? RS : NS)) & 1);
+        for (int i = max(0, v_issued - NS); i < v_issued; ++i) mbar_drain(smem_u32(&ct.vfull[i % NS]), (i / NS) & 1);
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issue
+    if (lane == 0) {
+      const uint32_t id_qk = idesc_f32<FMT>(KT, false), id_pv = idesc_f32<FMT>(D, true);
+      int cnt0 = 0, piece = 0, n_p[2] = {0, 0};
+      bool ok = true, issued = false;
+      while (ok && it.next(g, c, sc, p)) {
+        const int nt = p.t1 - p.t0;
+        const bool two = p.nrows > 128;
+        const int steps = two ? 2 * nt : nt;
+        if (!(ok = mbar_wait(smem_u32(&ct.q_ready), piece & 1, abort_flag, g.spin))) break;
+        for (int s = 0; s <= steps; ++s) {
+          if (s < steps) {                                              // S of step s
+            const int x = s & 1, cnt = cnt0 + (two ? s >> 1 : s), st = cnt % NS;
+            if ((!two || x == 0) && !(ok = mbar_wait(smem_u32(&ct.kfull[st]), cnt / NS & 1, abort_flag, g.spin))) break;
+            tc_fence_after();
+            issued = true;
+            const uint64_t kd = sw128_kmajor_desc(kbuf + st * S::TILE);
+            const uint32_t qa = tmem + kColQ + (two ? x * 64 : 0);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk)
+              tc_mma_ts(tmem + kColS + x * 64, qa + kk * 8, kd + (kk >> 2) * (KT * 128 >> 4) + (kk & 3) * 2, id_qk, kk > 0);
+            if (!two || x == 1) tc_commit(smem_u32(&ct.kempty[st]));
+            tc_commit(smem_u32(&ct.s_full[x]));
+          }
+          if (s > 0) {                                                  // O of step s - 1
+            const int u = s - 1, x = u & 1, i = two ? u >> 1 : u, cnt = cnt0 + i, st = cnt % NS;
+            if (!(ok = mbar_wait(smem_u32(&ct.p_ready[x]), n_p[x]++ & 1, abort_flag, g.spin))) break;
+            if ((!two || x == 0) &&
+                !(ok = mbar_wait(smem_u32(Q8 ? &ct.vfull[st] : &ct.vclean[st]), cnt / NS & 1, abort_flag, g.spin)))
+              break;
+            tc_fence_after();
+            const uint64_t vd = sw128_mnmajor_desc(vbuf + st * S::TILE, KT * 128);
+            const bool first = two ? i == 0 : u < 2;
+#pragma unroll
+            for (int kk = 0; kk < KT / 16; ++kk)
+              tc_mma_ts(tmem + kColO + x * 128, tmem + kColS + x * 64 + kk * 8, vd + kk * (16 * 128 >> 4), id_pv, !(first && kk == 0));
+            if (!two || x == 1) tc_commit(smem_u32(&ct.vempty[st]));
+          }
+        }
+        if (!ok) break;
+        tc_commit(smem_u32(&ct.o_done));
+        cnt0 += nt;
+        ++piece;
+      }
+      if (!ok) {
+        set_status(g.status, kStatusTimeoutMma);
+        *abort_flag = 1;
+      }
+      if (issued) {                                                     // no product may be in flight at the end
+        tc_commit(smem_u32(&ct.drain));
+        mbar_drain(smem_u32(&ct.drain), 0);
+      }
+    }
+  } else if (warp >= 12) {
+    reg_dec<72>();
+    // ------------------------------------------------------------ conversion, or the check of V tiles
+    const int ti = tid - 384;
+    int cnt = 0;
+    bool ok = true;
+    while (ok && it.next(g, c, sc, p)) {
+      for (int t = p.t0; t < p.t1; ++t, ++cnt) {
+        const int st = cnt % NS;
+        if constexpr (Q8) {
+          const int rs = cnt % RS, f = cnt % FR;
+          if (!(ok = warp_wait(&ct.raw_full[rs], cnt / RS & 1, abort_flag, g.spin))) break;
+          {
+            // factors of the tile's keys (the ring slot's last reader is behind the product that freed this K stage)
+            const uint32_t vpair = lds_u16(smem_u32(&ct.exps[rs][KT + 2 * lane]));
+            const int left = p.n_keys - t * KT - 2 * lane;
+            const int e0 = left > 0 && (vpair & 255) != 255 ? vpair & 255 : 0, e1 = left > 1 && (vpair >> 8) != 255 ? vpair >> 8 : 0;
+            const int em = __reduce_max_sync(0xffffffffu, max(e0, e1));
+            if (!(ok = warp_wait(&ct.kempty[st], (cnt / NS & 1) ^ 1, abort_flag, g.spin))) break;
+            if (ti < KT) {
+              ct.fk[f][ti] = exp_scale(ct.exps[rs][ti]);
+              if (ti == 0) ct.emax[f] = em;
+            } else {
+              const int ev = ct.exps[rs][ti];
+              ct.ev[f][ti - KT] = (uint8_t)ev;
+              const int d = min(ev - em, 0) + 127;
+              ct.fv[f][ti - KT] = ev == 255 ? __int_as_float(0x7fffffff) : d <= 0 ? 0.f : __int_as_float(d << 23);
+            }
+            mbar_arrive(smem_u32(&ct.ffull[f]));
+          }
+          auto convert = [&](uint32_t src, uint32_t dst) {
+            constexpr int C = D / 16;                                   // 16-byte chunks of a raw row
+#pragma unroll
+            for (int i = 0; i < KT * C / 128; ++i) {
+              // 8 lanes of a phase on 8 rows and one chunk: conflict-free in both swizzles
+              const int idx = i * 128 + ti, j = idx >> 3, ch = j % C, row = j / C * 8 + (idx & 7);
+              const uint4 w = lds128(src + row * D + ((D == 128 ? ch ^ (row & 7) : ch ^ ((row >> 1) & 3)) << 4));
+              uint4 a, b;
+              unpack4<FMT>(w.x, a.x, a.y);
+              unpack4<FMT>(w.y, a.z, a.w);
+              unpack4<FMT>(w.z, b.x, b.y);
+              unpack4<FMT>(w.w, b.z, b.w);
+              const uint32_t to = dst + (ch >> 2) * (KT * 128) + row * 128;
+              const int c0 = 2 * ch & 7;
+              sts128(to + ((c0 ^ (row & 7)) << 4), a);
+              sts128(to + (((c0 + 1) ^ (row & 7)) << 4), b);
+            }
+            fence_proxy_async_smem();
+          };
+          convert(raw + rs * S::RAW, kbuf + st * S::TILE);
+          mbar_arrive(smem_u32(&ct.kfull[st]));
+          if (!(ok = warp_wait(&ct.vempty[st], (cnt / NS & 1) ^ 1, abort_flag, g.spin))) break;
+          convert(raw + rs * S::RAW + S::RAW / 2, vbuf + st * S::TILE);
+          mbar_arrive(smem_u32(&ct.vfull[st]));
+          mbar_arrive(smem_u32(&ct.raw_empty[rs]));
+        } else {
+          if (!(ok = warp_wait(&ct.vfull[st], cnt / NS & 1, abort_flag, g.spin))) break;
+          if ((t + 1) * KT > min(p.all_see, p.n_keys)) {
+            // some row does not see some key: 0 x NaN would reach it, so non-finite elements are dropped here and put
+            // back at the end for the rows that do see them
+            bool hit = false;
+            for (int i = ti; i < S::TILE / 16; i += 128) {
+              const uint32_t a = vbuf + st * S::TILE + i * 16;
+              uint4 v = lds128(a);
+              bool h = false;
+              v.x = drop_nonfinite(v.x, h);
+              v.y = drop_nonfinite(v.y, h);
+              v.z = drop_nonfinite(v.z, h);
+              v.w = drop_nonfinite(v.w, h);
+              if (h) sts128(a, v);
+              hit = hit || h;
+            }
+            if (hit) *reinterpret_cast<volatile int*>(&ct.dropped) = 1;
+            fence_proxy_async_smem();
+          }
+          mbar_arrive(smem_u32(&ct.vclean[st]));
+        }
+      }
+    }
+    if (!ok) {
+      set_status(g.status, kStatusTimeoutProducer);
+      *abort_flag = 1;
+    }
+  } else if (warp >= 4) {
+    reg_inc<184>();
+    // ------------------------------------------------------------ softmax: thread = row of stream x
+    const int x = (warp >> 2) - 1, r = tid & 127;
+    const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);         // TMEM lane quadrant of the warp
+    const uint32_t tS = lanes + kColS + x * 64, tO = lanes + kColO + x * 128;
+    int cnt0 = 0, n_s = 0, piece = 0, n_ml = 0;
+    bool ok = true;
+    while (ok && it.next(g, c, sc, p)) {
+      const int nt = p.t1 - p.t0;
+      const bool two = p.nrows > 128;
+      const int row = (two ? x * 128 : 0) + r;                          // of the row tile
+      const bool in = row < p.nrows;
+      const int R = p.r0 + min(row, p.nrows - 1), node = R / g.G;
+      const int head = p.h * g.G + R % g.G;
+      float rf = g.scale * 1.4426950408889634f;
+      {
+        // the q row: bf16 as it is, or f16 with the largest element's power of two taken out
+        const bf16* src = q + (size_t)(p.bi.start + node) * g.ld_q + (size_t)head * D;
+        uint32_t w[D / 2], amax = 0;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          const uint4 v = in ? *reinterpret_cast<const uint4*>(src + i * 8) : make_uint4(0, 0, 0, 0);
+          w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+        }
+        if constexpr (Q8) {
+#pragma unroll
+          for (int i = 0; i < D / 2; ++i) amax = max(amax, max(w[i] << 16 & 0x7fff0000u, w[i] & 0x7fff0000u));
+          const int e = min(max((int)(amax >> 23), 27), 227);
+          const float inv = __int_as_float((254 - e) << 23);
+          rf *= __int_as_float(e << 23) * kHalfUnit<FMT>;
+#pragma unroll
+          for (int i = 0; i < D / 2; ++i) w[i] = pack2<FMT>(__uint_as_float(w[i] << 16) * inv, __uint_as_float(w[i] & 0xffff0000u) * inv);
+        }
+        if (two || x == 0) {
+          const uint32_t tQ = lanes + kColQ + (two ? x * 64 : 0);
+#pragma unroll
+          for (int i = 0; i < D / 64; ++i) tmem_st32(tQ + 32 * i, w + 32 * i);
+          tmem_wait_st();
+        }
+      }
+      tc_fence_before();
+      mbar_arrive(smem_u32(&ct.q_ready));
+      float m = -INFINITY, l = 0.f;
+      int er = 0;                                                       // 8-bit: exponent byte that O and l are relative to
+      bool begun = false;
+      for (int i = two ? 0 : x; i < nt; i += two ? 1 : 2) {
+        const int t = p.t0 + i, cnt = cnt0 + i, f = cnt % FR;
+        if (!(ok = warp_wait(&ct.s_full[x], n_s++ & 1, abort_flag, g.spin))) break;
+        tc_fence_after();
+        if (Q8 && !(ok = warp_wait(&ct.ffull[f], cnt / FR & 1, abort_flag, g.spin))) break;
+        uint32_t a[KT];
+        tmem_ld32(tS, a);
+        tmem_ld32(tS + 32, a + 32);
+        tmem_wait_ld();
+        const bool partial = (t + 1) * KT > min(p.all_see, p.n_keys);
+        uint32_t see[2] = {~0u, ~0u};
+        int em = 0;
+        if constexpr (Q8) em = ct.emax[f];
+        float mx = -INFINITY;
+        if constexpr (Q8) {
+          const uint32_t fk = smem_u32(ct.fk[f]);
+          const f32x2 rf2 = pack_f2(rf, rf);
+#pragma unroll
+          for (int j = 0; j < KT; j += 4) {
+            const uint4 v = lds128(fk + j * 4);
+            const float2 y0 = unpack_f2(mul2(pack_f2(__uint_as_float(a[j]), __uint_as_float(a[j + 1])),
+                                             mul2(rf2, pack_f2(__uint_as_float(v.x), __uint_as_float(v.y)))));
+            const float2 y1 = unpack_f2(mul2(pack_f2(__uint_as_float(a[j + 2]), __uint_as_float(a[j + 3])),
+                                             mul2(rf2, pack_f2(__uint_as_float(v.z), __uint_as_float(v.w)))));
+            a[j] = __float_as_uint(y0.x), a[j + 1] = __float_as_uint(y0.y);
+            a[j + 2] = __float_as_uint(y1.x), a[j + 3] = __float_as_uint(y1.y);
+          }
+        }
+        if (partial) {
+          em = 0;
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const int kb = t * KT + 32 * w, left = p.n_keys - kb;
+            see[w] = sees32(g.mask ? g.mask + (size_t)(p.bi.start + node) * g.words : nullptr, g.words, node, kb - p.bi.ctx);
+            if (left < 32) see[w] &= left <= 0 ? 0u : (1u << left) - 1;
+          }
+#pragma unroll
+          for (int j = 0; j < KT; ++j) {
+            const bool s = see[j >> 5] >> (j & 31) & 1;
+            if (!s) a[j] = 0xff800000u;
+            if constexpr (Q8) em = max(em, s && ct.ev[f][j] != 255 ? (int)ct.ev[f][j] : 0);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < KT; j += 2) mx = fmaxf(mx, fmaxf(__uint_as_float(a[j]), __uint_as_float(a[j + 1])));
+        if constexpr (!Q8) mx *= rf;                                    // rf > 0
+        // O, l and m move to a new reference only when the old one is too small by 2^8 (2^4 for V's scale): the
+        // weights stay below 2^12, in range of f16
+        const float mn = fmaxf(m, mx);
+        const int en = max(er, em);
+        const bool need = !begun || mn > m + 8.f || (Q8 && em > er + 4);
+        float cf = 1.f;
+        if (need) {
+          cf = m == -INFINITY ? 0.f : fast_exp2(m - mn);
+          l *= cf;
+          if (Q8) cf *= er == 0 ? 0.f : fast_exp2((float)(er - en));
+          m = mn;
+          er = en;
+        }
+        if (begun && __any_sync(0xffffffffu, need)) {
+          // every product issued before this step's S is complete, the stream's last O among them
+#pragma unroll
+          for (int b = 0; b < D; b += 32) {
+            uint32_t o[32];
+            tmem_ld32(tO + b, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * cf);
+            tmem_st32(tO + b, o);
+          }
+        }
+        begun = true;
+        const float ms = m == -INFINITY ? 0.f : m;
+        uint32_t pk[KT / 2];
+        if constexpr (!Q8) {
+          // one FMA per weight leaves the rounding error of the score, 2^-24 |ms|, in the exponent: nothing at ordinary
+          // sizes, but at very large ones the largest score itself has to come out as exactly 0
+          if (__any_sync(0xffffffffu, fabsf(ms) > 65536.f)) {
+#pragma unroll
+            for (int j = 0; j < KT; ++j) a[j] = __float_as_uint(__fadd_rn(__fmul_rn(__uint_as_float(a[j]), rf), -ms));
+          } else {
+            const f32x2 nb = pack_f2(-ms, -ms), rf2 = pack_f2(rf, rf);
+#pragma unroll
+            for (int j = 0; j < KT; j += 2) {
+              const float2 y = unpack_f2(fma2(pack_f2(__uint_as_float(a[j]), __uint_as_float(a[j + 1])), rf2, nb));
+              a[j] = __float_as_uint(y.x), a[j + 1] = __float_as_uint(y.y);
+            }
+          }
+          f32x2 s2 = pack_f2(0.f, 0.f);
+#pragma unroll
+          for (int j = 0; j < KT; j += 2) {
+            const float p0 = fast_exp2(__uint_as_float(a[j])), p1 = fast_exp2(__uint_as_float(a[j + 1]));
+            s2 = add2(s2, pack_f2(p0, p1));
+            pk[j / 2] = pack2<FMT>(p0, p1);
+          }
+          const float2 sv = unpack_f2(s2);
+          l += sv.x + sv.y;
+        } else if (!partial) {
+          // the tile's V scale relative to er goes into the exponent, so l collects the same units and is brought
+          // back by the exact power of two; further below than 2^-64 no weight of the tile is left in f16
+          const int dd = max(em - er, -64);
+          const float nbs = (float)dd - ms, back = __int_as_float((127 - dd) << 23);
+          const float drop = em - er < -64 ? 0.f : 1.f;
+          const f32x2 nb = pack_f2(nbs, nbs);
+          const uint32_t fv = smem_u32(ct.fv[f]);
+          f32x2 s2 = pack_f2(0.f, 0.f);
+#pragma unroll
+          for (int j = 0; j < KT; j += 4) {
+            const uint4 v = lds128(fv + j * 4);
+            const float2 y0 = unpack_f2(add2(pack_f2(__uint_as_float(a[j]), __uint_as_float(a[j + 1])), nb));
+            const float2 y1 = unpack_f2(add2(pack_f2(__uint_as_float(a[j + 2]), __uint_as_float(a[j + 3])), nb));
+            const f32x2 e0 = pack_f2(fast_exp2(y0.x), fast_exp2(y0.y)), e1 = pack_f2(fast_exp2(y1.x), fast_exp2(y1.y));
+            s2 = add2(s2, add2(e0, e1));
+            const float2 w0 = unpack_f2(mul2(e0, pack_f2(__uint_as_float(v.x), __uint_as_float(v.y))));
+            const float2 w1 = unpack_f2(mul2(e1, pack_f2(__uint_as_float(v.z), __uint_as_float(v.w))));
+            pk[j / 2] = pack2<FMT>(w0.x, w0.y);
+            pk[j / 2 + 1] = pack2<FMT>(w1.x, w1.y);
+          }
+          if (drop == 0.f) {
+#pragma unroll
+            for (int j = 0; j < KT / 2; ++j) pk[j] = 0u;
+          }
+          const float2 sv = unpack_f2(s2);
+          l = fmaf(sv.x + sv.y, back, l);
+        } else {
+          float sum = 0.f;
+#pragma unroll
+          for (int j = 0; j < KT; j += 2) {
+            float w[2];
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              const float e = fast_exp2(__uint_as_float(a[j + b]) - ms);
+              sum += e;
+              const int ev = ct.ev[f][j + b], d = ev - er + 127;
+              const float s = ev == 255 ? __int_as_float(0x7fffffff) : d <= 0 ? 0.f : __int_as_float(min(d, 254) << 23);
+              w[b] = see[(j + b) >> 5] >> ((j + b) & 31) & 1 ? e * s : 0.f;
+            }
+            pk[j / 2] = pack2<FMT>(w[0], w[1]);
+          }
+          l += sum;
+        }
+        tmem_st32(tS, pk);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(smem_u32(&ct.p_ready[x]));
+      }
+      if (!ok) break;
+      // ---- the piece's output
+      float(&ml)[2][3][128] = ct.ml[piece & 1];
+      if (!two) {
+        ml[x][0][r] = m;
+        ml[x][1][r] = l;
+        ml[x][2][r] = begun ? (float)er : -1.f;                      // -1: the stream had no tile, its O is not there
+        mbar_arrive(smem_u32(&ct.ml_ready));
+        if (!(ok = warp_wait(&ct.ml_ready, n_ml++ & 1, abort_flag, g.spin))) break;
+      }
+      if (!(ok = warp_wait(&ct.o_done, piece & 1, abort_flag, g.spin))) break;
+      tc_fence_after();
+      float f0 = 1.f, f1 = 0.f, M = m, L = l, E = (float)er;
+      if (!two) {
+        const float m0 = ml[0][0][r], m1 = ml[1][0][r], e0 = ml[0][2][r], e1 = ml[1][2][r];
+        M = fmaxf(m0, m1);
+        const float ms = M == -INFINITY ? 0.f : M;
+        E = fmaxf(fmaxf(e0, e1), 0.f);
+        const float w0 = fast_exp2(m0 - ms), w1 = e1 < 0.f ? 0.f : fast_exp2(m1 - ms);
+        L = w0 * ml[0][1][r] + (e1 < 0.f ? 0.f : w1 * ml[1][1][r]);
+        f0 = Q8 ? w0 * fast_exp2(e0 - E) : w0;
+        f1 = e1 < 0.f ? 0.f : Q8 ? w1 * fast_exp2(e1 - E) : w1;
+      }
+      float inv = L == 0.f ? 0.f : 1.f / L;                             // a row that sees nothing: zeros
+      if constexpr (Q8) inv *= kHalfUnit<FMT> * __int_as_float((int)fmaxf(E, 1.f) << 23);
+      const bool join = !two && ml[1][2][r] >= 0.f;
+      const size_t at = (size_t)(p.bi.start + node) * g.n_heads + head;
+      const bool to_out = sc.chunk_tiles ? p.tiles <= sc.chunk_tiles : p.whole;
+      const size_t part = sc.chunk_tiles ? at * g.splits + p.t0 / sc.chunk_tiles
+                                         : ((size_t)blockIdx.x * 2 + (p.index ? 1 : 0)) * sc.rows + row;
+      // one row tile: each stream's threads write half of the columns
+      const int d0 = two ? 0 : x * (D / 2), d1 = two ? D : d0 + D / 2;
+      for (int d = d0; d < d1; d += 32) {
+        uint32_t o[32];
+        tmem_ld32(two ? tO + d : lanes + kColO + d, o);
+        tmem_wait_ld();
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(o[j]) * (f0 * inv);
+        if (!two && __any_sync(0xffffffffu, join)) {                    // the same for all rows: the tile count decides
+          tmem_ld32(lanes + kColO + 128 + d, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = fmaf(__uint_as_float(o[j]), f1 * inv, v[j]);
+        }
+        if (!Q8 && in && *reinterpret_cast<volatile int*>(&ct.dropped)) {     // the dropped elements of keys this row sees
+          const uint64_t* mk = g.mask ? g.mask + (size_t)(p.bi.start + node) * g.words : nullptr;
+          for (int key = max(p.t0 * KT, p.all_see); key < min(p.t1 * KT, p.n_keys); ++key)
+            if (sees32(mk, g.words, node, key - p.bi.ctx) & 1) {
+              const bf16* vp = static_cast<const bf16*>(c.v) + (cache_slot(c, p.bi.row, p.h, key)) * D + d;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                const float y = __bfloat162float(vp[j]);
+                if (!(fabsf(y) < INFINITY)) v[j] += y;
+              }
+            }
+        }
+        if (in && to_out) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 8)
+            *reinterpret_cast<uint4*>(out + at * D + d + j) =
+                make_uint4(pack2<EESD_KV_MODEL>(v[j], v[j + 1]), pack2<EESD_KV_MODEL>(v[j + 2], v[j + 3]),
+                           pack2<EESD_KV_MODEL>(v[j + 4], v[j + 5]), pack2<EESD_KV_MODEL>(v[j + 6], v[j + 7]));
+        } else if (in) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 4)
+            *reinterpret_cast<float4*>(g.part_o + part * D + d + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+        }
+        __syncwarp();
+      }
+      if (in && !to_out && (two || x == 0)) g.part_ml[part] = make_float2(M, L);
+      cnt0 += nt;
+      ++piece;
+    }
+    if (!ok) {
+      set_status(g.status, kStatusTimeoutEpilogue);
+      *abort_flag = 1;
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, 512);
+}
+
+// Joins the pieces of the units that a cut of the equal runs went through, in run order.  One warp per row.
+template <int D>
+__global__ void __launch_bounds__(128) attn_tree_tc_join_kernel(TreeGeom g, CacheGeom c, TcSchedule sc, bf16* __restrict__ out) {
+  pdl_trigger();
+  pdl_wait();
+  const int b = blockIdx.z, h = blockIdx.y, R = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  BlockInfo bi;
+  if (!block_fits(g, c, b, bi) || R >= bi.T * g.G) return;
+  const int tile = R / sc.rows;
+  bool bad;
+  const Entry x = entry_of(g, c, sc, b * sc.tiles_max + tile, bad);
+  const long long W = sc.table[sc.entries], n = sc.ctas;
+  const long long u0 = sc.table[b * sc.tiles_max + tile] + (long long)h * x.tiles, u1 = u0 + x.tiles;
+  // run k is [k W / n, (k + 1) W / n): the run that holds u is the last one that starts at or before u
+  const int c0 = (int)(((u0 + 1) * n - 1) / W), c1 = (int)((u1 * n - 1) / W);
+  if (c0 == c1) return;                                                 // in one piece: written whole
+  const int at0 = c0 * W / n == u0 ? 0 : 1;                             // the unit is the first or a later piece of run c0
+  const int node = R / g.G, row = R - tile * sc.rows;
+  auto slot = [&](int k) { return ((size_t)k * 2 + (k == c0 ? at0 : 0)) * sc.rows + row; };
+  auto empty = [&](int k) { return k * W / n == (k + 1) * W / n; };     // runs of no tile write nothing
+  float M = -INFINITY;
+  for (int k = c0 + lane; k <= c1; k += 32)
+    if (!empty(k)) M = fmaxf(M, g.part_ml[slot(k)].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  const float ms = M == -INFINITY ? 0.f : M;
+  constexpr int E = D / 32;
+  float L = 0.f, acc[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  for (int k0 = c0; k0 <= c1; k0 += 32) {
+    float w = 0.f;
+    if (k0 + lane <= c1 && !empty(k0 + lane)) {
+      const float2 v = g.part_ml[slot(k0 + lane)];
+      w = v.y * fast_exp2(v.x - ms);
+    }
+    const int cnt = min(32, c1 - k0 + 1);
+    for (int k = 0; k < cnt; ++k) {
+      const float wk = __shfl_sync(0xffffffffu, w, k);
+      if (wk == 0.f) continue;
+      L += wk;
+      const float* src = g.part_o + slot(k0 + k) * D + lane * E;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = fmaf(wk, src[e], acc[e]);
+    }
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  bf16* dst = out + ((size_t)(bi.start + node) * g.n_heads + h * g.G + R % g.G) * D + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack2<EESD_KV_MODEL>(acc[e] * inv, acc[e + 1] * inv);
+}
+
+template <int D, int FMT>
+cudaError_t launch(const TcSchedule& sc, const TreeGeom& g, const CacheGeom& c, const CUtensorMap& km, const CUtensorMap& vm, int n_blocks,
+                   const void* q, void* out, cudaStream_t s) {
+  using S = TcShape<D, FMT>;
+  auto kernel = attn_tree_tc_kernel<D, FMT>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::smem);
+  if (e != cudaSuccess) return e;
+  e = launch_pdl(kernel, dim3(sc.ctas), dim3(kThreads), S::smem, s, km, vm, g, c, sc, static_cast<const bf16*>(q), static_cast<bf16*>(out));
+  if (e == cudaSuccess && !sc.chunk_tiles)
+    e = launch_pdl(attn_tree_tc_join_kernel<D>, dim3((g.max_nodes * g.G + 3) / 4, c.n_kv_heads, n_blocks), dim3(128), 0, s, g, c, sc,
+                   static_cast<bf16*>(out));
+  return e;
+}
+
+}  // namespace
+
+cudaError_t launch_attn_tree_tc(int fmt, int D, const TcSchedule& sc, const TreeGeom& g, const CacheGeom& c, const CUtensorMap& km,
+                                const CUtensorMap& vm, int nb, const void* q, void* out, cudaStream_t s) {
+  switch (fmt * 2 + (D == 128)) {
+    case 0: return launch<64, EESD_KV_MODEL>(sc, g, c, km, vm, nb, q, out, s);
+    case 1: return launch<128, EESD_KV_MODEL>(sc, g, c, km, vm, nb, q, out, s);
+    case 2: return launch<64, EESD_KV_E4M3>(sc, g, c, km, vm, nb, q, out, s);
+    case 3: return launch<128, EESD_KV_E4M3>(sc, g, c, km, vm, nb, q, out, s);
+    case 4: return launch<64, EESD_KV_INT8>(sc, g, c, km, vm, nb, q, out, s);
+    default: return launch<128, EESD_KV_INT8>(sc, g, c, km, vm, nb, q, out, s);
+  }
+}
+
+}  // namespace eesd

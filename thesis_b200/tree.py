@@ -115,9 +115,10 @@ class TreeBatch:
 
     ``blk`` [n_blocks, 4] = (start, T, row, ctx), ``parent``, ``tok_pos``, ``tok_slot``, ``tok_row`` [n_tokens]
     int32 and ``mask`` [n_tokens, words] int64 are device tensors.  A program that advances ``ctx`` on the device
-    edits ``blk`` and calls ``update`` (``max_ctx`` must still bound ``ctx + T``)."""
+    edits ``blk`` and calls ``update``; ``max_ctx`` (default: the largest ``ctx + T`` given) has to bound ``ctx + T``
+    from then on too, as ``max_nodes`` does T."""
 
-    def __init__(self, blocks: Sequence[tuple], cache: KVCache, max_ctx: Optional[int] = None):
+    def __init__(self, blocks: Sequence[tuple], cache: KVCache, max_ctx: Optional[int] = None, max_nodes: Optional[int] = None):
         blk, par, chains, start = [], [], True, 0
         for row, ctx, parents in blocks:
             T = parents if isinstance(parents, (int, np.integer)) else len(parents)
@@ -137,8 +138,8 @@ class TreeBatch:
         self.n_blocks, self.n_tokens = len(blk), start
         if not blk:
             raise ValueError("a tree batch needs at least one block")
-        self.max_nodes = max(b[1] for b in blk)
-        self.max_ctx = max(b[1] + b[3] for b in blk) if max_ctx is None else int(max_ctx)
+        self.max_nodes = max(max(b[1] for b in blk), max_nodes or 1)
+        self.max_ctx = max(max(b[1] + b[3] for b in blk), max_ctx or 1)
         if not chains and self.max_nodes > lib.TREE_MAX_NODES:
             raise ValueError(f"a tree has at most {lib.TREE_MAX_NODES} nodes per block, got {self.max_nodes}")
         self.device, self._cache = cache.device, cache
