@@ -685,7 +685,7 @@ struct Plan {
   int rows, tiles;      // rows per tile, row tiles of the largest block
   int chunk, splits;    // keys per CTA, key ranges of the longest row
   int ctas;             // tcgen05: persistent CTAs
-  size_t ml_off, table_off, bytes;
+  size_t ml_off, cuts_off, bytes;
 };
 
 int sm_count() {
@@ -722,8 +722,8 @@ Plan plan_for(const EesdKvCache* c, const EesdTree* t, int n_heads, int split_ke
   if (p.splits > 1) parts = (size_t)t->n_tokens * n_heads * p.splits;
   const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
   p.ml_off = up(parts * c->head_dim * 4);
-  p.table_off = p.ml_off + up(parts * 8);
-  p.bytes = std::max<size_t>(p.table_off + (p.tc ? up(((size_t)t->n_blocks * p.tiles + 1) * 8) : 0), 256);
+  p.cuts_off = p.ml_off + up(parts * 8);
+  p.bytes = std::max<size_t>(p.cuts_off + (p.tc ? up(((size_t)p.ctas + 1) * sizeof(TcCut)) : 0), 256);
   return p;
 }
 
@@ -829,8 +829,8 @@ int eesd_attn_tree(int dtype, const EesdKvCache* c, int layer, const EesdTree* t
     if ((rc = encode_cache_map(&km, cg.k, c, keys)) || (rc = encode_cache_map(&vm, cg.v, c, keys))) return rc;
     if (p.tc) {
       const TcSchedule sc{p.ctas, p.rows, p.tiles, t->n_blocks * p.tiles, split_keys / 64,
-                          reinterpret_cast<long long*>(static_cast<uint8_t*>(workspace) + p.table_off)};
-      e = launch_attn_tree_tc(c->format, c->head_dim, sc, g, cg, km, vm, t->n_blocks, q, out, s);
+                          reinterpret_cast<TcCut*>(static_cast<uint8_t*>(workspace) + p.cuts_off)};
+      e = launch_attn_tree_tc(c->format, c->head_dim, sc, g, cg, km, vm, q, out, s);
     } else {
       e = launch_bf16(c->format, c->head_dim, p, g, cg, km, vm, t->n_blocks, q, out, s);
     }

@@ -35,6 +35,13 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// One lane of a converged warp.  The branch on it keeps the warp's scalar registers usable, which a branch on the
+// lane number does not: a product then issues every 42 clocks (N = 64) instead of every 118.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.b32 %0, 1, 0, P;\n\t}" : "=r"(p));
+  return p != 0;
+}
 // D[tmem] (+)= A[tmem] * B[smem]
 __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -112,11 +119,13 @@ template <int FMT> __device__ __forceinline__ uint32_t idesc_f32(int n, bool b_m
 }
 
 // ------------------------------------------------------------------ the flat schedule
-// Entry e = (block, row tile); its unit of each KV head takes tiles() key tiles.  Flat position = tiles of the
-// entries before, all heads, then head by head.
+// Entry e = (block, row tile); its unit of each KV head takes `tiles` key tiles.  On the flat axis a unit is kUnitCost
+// positions (what starting a unit costs, in tiles) and then its tiles; entries follow one another, their heads inside.
+constexpr int kUnitCost = 6;
 struct Entry {
   BlockInfo bi;
   int r0, nrows, n_keys, all_see, tiles;   // slots below all_see are seen by every row of the tile
+  __device__ int length() const { return tiles ? tiles + kUnitCost : 0; }
 };
 __device__ __forceinline__ Entry entry_of(const TreeGeom& g, const CacheGeom& c, const TcSchedule& sc, int e, bool& bad) {
   Entry x;
@@ -134,39 +143,47 @@ __device__ __forceinline__ Entry entry_of(const TreeGeom& g, const CacheGeom& c,
 }
 struct Piece : Entry {
   int h, t0, t1, index;     // KV head, key tiles [t0, t1), number of the piece in its CTA
-  bool whole;               // the unit in one piece
+  long long u0;             // flat position of the unit
+  __device__ bool whole() const { return t0 == 0 && t1 == tiles; }
 };
 // The pieces of one CTA's run [pos, end).  With a fixed split (sc.chunk_tiles) a unit is cut at multiples of it and
-// a piece belongs to the CTA whose run holds its first tile; otherwise a piece is what the run holds of a unit.
+// a piece belongs to the CTA whose run holds its first position; otherwise a piece is what the run holds of a unit.
 struct PieceIter {
   long long pos, end, base;
-  int e, index;
+  int e, index, loaded;
   __device__ bool next(const TreeGeom& g, const CacheGeom& c, const TcSchedule& sc, Piece& p) {
     while (pos < end) {
-      bool bad;
-      static_cast<Entry&>(p) = entry_of(g, c, sc, e, bad);
-      const long long span = (long long)p.tiles * c.n_kv_heads;
+      if (loaded != e) {
+        bool bad;
+        static_cast<Entry&>(p) = entry_of(g, c, sc, e, bad);
+        loaded = e;
+      }
+      const int len = p.length();
+      const long long span = (long long)len * c.n_kv_heads;
       if (pos >= base + span) {
         base += span;
         ++e;
         continue;
       }
-      const int off = (int)(pos - base);
-      p.h = off / p.tiles;
-      p.t0 = off - p.h * p.tiles;
+      const int in = (int)(pos - base);
+      p.h = in / len;
+      p.u0 = base + (long long)p.h * len;
+      const int off = (int)(pos - p.u0);
       if (sc.chunk_tiles) {
-        const int up = (p.t0 + sc.chunk_tiles - 1) / sc.chunk_tiles * sc.chunk_tiles;
-        if (up != p.t0) {                                  // inside a piece of the CTA before
-          pos += min(up, p.tiles) - p.t0;
-          continue;
-        }
+        p.t0 = off == 0 ? 0 : (max(off - kUnitCost, 1) + sc.chunk_tiles - 1) / sc.chunk_tiles * sc.chunk_tiles;
         p.t1 = min(p.tiles, p.t0 + sc.chunk_tiles);
+        if (p.t0 < p.tiles && p.u0 + (p.t0 ? kUnitCost + p.t0 : 0) >= end) return false;
       } else {
-        p.t1 = (int)min((long long)p.tiles, p.t0 + (end - pos));
+        p.t0 = max(off - kUnitCost, 0);
+        p.t1 = (int)max(0LL, min((long long)p.tiles, end - p.u0 - kUnitCost));
       }
-      p.whole = p.t0 == 0 && p.t1 == p.tiles;
+      pos = p.u0 + kUnitCost + min(p.t1, p.tiles);
+      if (p.t0 >= p.t1) {                                  // a run that ends before the unit's first tile
+        if (!sc.chunk_tiles) return false;
+        pos = p.u0 + len;
+        continue;
+      }
       p.index = index++;
-      pos += p.t1 - p.t0;
       return true;
     }
     return false;
@@ -190,7 +207,7 @@ struct TcControl {
   alignas(16) float fv[4][KT];             // 2^(ev - emax)
   alignas(16) uint8_t ev[4][KT];
   alignas(16) uint8_t exps[8][2 * KT];     // raw exponent bytes, K then V
-  int emax[4];
+  int emax[4], even[4];                    // largest V exponent; the others within 2^4 of it and no NaN
   float ml[2][2][3][128];                  // one row tile: max, sum and eref of the streams (by piece parity)
   long long lo, hi, base;
   long long wsum[16];
@@ -223,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     long long sum = 0;
     for (int e = a; e < b; ++e) {
       bool bad;
-      sum += entry_of(g, c, sc, e, bad).tiles;
+      sum += entry_of(g, c, sc, e, bad).length();
       if (bad && blockIdx.x == 0) set_status(g.status, kStatusBadIndex);
     }
     long long inc = sum;
@@ -276,14 +293,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (tid == 0) {
       ct.lo = lo;
       ct.hi = hi;
-      if (blockIdx.x == 0) sc.table[E] = W;
+      sc.cuts[blockIdx.x].e = -1;                                       // no unit of this run goes on in the next one
+      if (blockIdx.x == 0) sc.cuts[gridDim.x].u0 = W;
     }
-    if (blockIdx.x == 0 || (lo >= before * Hkv && lo < (before + sum) * Hkv)) {
+    if (lo >= before * Hkv && lo < (before + sum) * Hkv) {
       long long base = before * Hkv;
       for (int e = a; e < b; ++e) {
         bool bad;
-        const long long span = (long long)entry_of(g, c, sc, e, bad).tiles * Hkv;
-        if (blockIdx.x == 0) sc.table[e] = base;
+        const long long span = (long long)entry_of(g, c, sc, e, bad).length() * Hkv;
         if (lo >= base && lo < base + span) {
           ct.e0 = e;
           ct.base = base;
@@ -293,15 +310,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncthreads();
   }
-  PieceIter it{ct.lo, ct.hi, ct.base, ct.e0, 0};
+  PieceIter it{ct.lo, ct.hi, ct.base, ct.e0, 0, -1};
   if (ct.e0 >= sc.entries) it.pos = it.end;
   Piece p;
   const uint32_t tmem = ct.tmem;
 
-  if (warp < 4) reg_dec<64>();
+  if (warp < 4) reg_dec<88>();
   if (warp == 0) {
     // ------------------------------------------------------------ TMA
-    if (lane == 0) {
+    if (elect_one()) {
       int cnt = 0, k_issued = 0, v_issued = 0;
       bool ok = true;
       tma_prefetch_desc(&kmap);
@@ -349,7 +366,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issue
-    if (lane == 0) {
+    if (elect_one()) {
       const uint32_t id_qk = idesc_f32<FMT>(KT, false), id_pv = idesc_f32<FMT>(D, true);
       int cnt0 = 0, piece = 0, n_p[2] = {0, 0};
       bool ok = true, issued = false;
@@ -402,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else if (warp >= 12) {
-    reg_dec<72>();
+    reg_dec<80>();
     // ------------------------------------------------------------ conversion, or the check of V tiles
     const int ti = tid - 384;
     int cnt = 0;
@@ -416,18 +433,23 @@ __global__ void __launch_bounds__(kThreads, 1)
           {
             // factors of the tile's keys (the ring slot's last reader is behind the product that freed this K stage)
             const uint32_t vpair = lds_u16(smem_u32(&ct.exps[rs][KT + 2 * lane]));
-            const int left = p.n_keys - t * KT - 2 * lane;
-            const int e0 = left > 0 && (vpair & 255) != 255 ? vpair & 255 : 0, e1 = left > 1 && (vpair >> 8) != 255 ? vpair >> 8 : 0;
-            const int em = __reduce_max_sync(0xffffffffu, max(e0, e1));
+            const int left = p.n_keys - t * KT, a0 = vpair & 255, a1 = vpair >> 8;
+            const bool in0 = 2 * lane < left && a0 != 255, in1 = 2 * lane + 1 < left && a1 != 255;
+            const int em = __reduce_max_sync(0xffffffffu, max(in0 ? a0 : 0, in1 ? a1 : 0));
+            const int en = __reduce_min_sync(0xffffffffu, min(in0 ? a0 : em, in1 ? a1 : em));
+            const bool nan = __any_sync(0xffffffffu, (2 * lane < left && a0 == 255) || (2 * lane + 1 < left && a1 == 255));
             if (!(ok = warp_wait(&ct.kempty[st], (cnt / NS & 1) ^ 1, abort_flag, g.spin))) break;
             if (ti < KT) {
               ct.fk[f][ti] = exp_scale(ct.exps[rs][ti]);
-              if (ti == 0) ct.emax[f] = em;
+              if (ti == 0) {
+                ct.emax[f] = em;
+                ct.even[f] = em - en <= 4 && !nan;
+              }
             } else {
               const int ev = ct.exps[rs][ti];
               ct.ev[f][ti - KT] = (uint8_t)ev;
-              const int d = min(ev - em, 0) + 127;
-              ct.fv[f][ti - KT] = ev == 255 ? __int_as_float(0x7fffffff) : d <= 0 ? 0.f : __int_as_float(d << 23);
+              const int d = ev - em + 127;
+              ct.fv[f][ti - KT] = ti - KT >= left ? 0.f : ev == 255 ? __int_as_float(0x7fffffff) : d <= 0 ? 0.f : __int_as_float(d << 23);
             }
             mbar_arrive(smem_u32(&ct.ffull[f]));
           }
@@ -485,7 +507,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       *abort_flag = 1;
     }
   } else if (warp >= 4) {
-    reg_inc<184>();
+    reg_inc<168>();
     // ------------------------------------------------------------ softmax: thread = row of stream x
     const int x = (warp >> 2) - 1, r = tid & 127;
     const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);         // TMEM lane quadrant of the warp
@@ -558,8 +580,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             a[j + 2] = __float_as_uint(y1.x), a[j + 3] = __float_as_uint(y1.y);
           }
         }
+        // V's scales of a tile that some row does not wholly see: row by row only where they differ much
+        const bool by_row = Q8 && partial && !ct.even[f];
         if (partial) {
-          em = 0;
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
             const int kb = t * KT + 32 * w, left = p.n_keys - kb;
@@ -567,10 +590,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (left < 32) see[w] &= left <= 0 ? 0u : (1u << left) - 1;
           }
 #pragma unroll
-          for (int j = 0; j < KT; ++j) {
-            const bool s = see[j >> 5] >> (j & 31) & 1;
-            if (!s) a[j] = 0xff800000u;
-            if constexpr (Q8) em = max(em, s && ct.ev[f][j] != 255 ? (int)ct.ev[f][j] : 0);
+          for (int j = 0; j < KT; ++j)
+            if (!(see[j >> 5] >> (j & 31) & 1)) a[j] = 0xff800000u;
+          if (by_row) {
+            em = 0;
+#pragma unroll 8
+            for (int j = 0; j < KT; ++j)
+              if (see[j >> 5] >> (j & 31) & 1) em = max(em, ct.ev[f][j] == 255 ? 0 : (int)ct.ev[f][j]);
           }
         }
 #pragma unroll
@@ -627,7 +653,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           const float2 sv = unpack_f2(s2);
           l += sv.x + sv.y;
-        } else if (!partial) {
+        } else if (!by_row) {
           // the tile's V scale relative to er goes into the exponent, so l collects the same units and is brought
           // back by the exact power of two; further below than 2^-64 no weight of the tile is left in f16
           const int dd = max(em - er, -64);
@@ -703,7 +729,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if constexpr (Q8) inv *= kHalfUnit<FMT> * __int_as_float((int)fmaxf(E, 1.f) << 23);
       const bool join = !two && ml[1][2][r] >= 0.f;
       const size_t at = (size_t)(p.bi.start + node) * g.n_heads + head;
-      const bool to_out = sc.chunk_tiles ? p.tiles <= sc.chunk_tiles : p.whole;
+      const bool to_out = sc.chunk_tiles ? p.tiles <= sc.chunk_tiles : p.whole();
       const size_t part = sc.chunk_tiles ? at * g.splits + p.t0 / sc.chunk_tiles
                                          : ((size_t)blockIdx.x * 2 + (p.index ? 1 : 0)) * sc.rows + row;
       // one row tile: each stream's threads write half of the columns
@@ -747,6 +773,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
       }
       if (in && !to_out && (two || x == 0)) g.part_ml[part] = make_float2(M, L);
+      if (tid == 128 && !sc.chunk_tiles && p.t0 == 0 && p.t1 < p.tiles) sc.cuts[blockIdx.x] = TcCut{p.u0, it.e, p.h, p.index ? 1 : 0, p.tiles};
       cnt0 += nt;
       ++piece;
     }
@@ -761,68 +788,69 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 1) tmem_dealloc(tmem, 512);
 }
 
-// Joins the pieces of the units that a cut of the equal runs went through, in run order.  One warp per row.
+// Joins the pieces of the unit that goes from run blockIdx.x on into the next ones, in run order.  A warp takes
+// every 8th row of its group of 32.
 template <int D>
-__global__ void __launch_bounds__(128) attn_tree_tc_join_kernel(TreeGeom g, CacheGeom c, TcSchedule sc, bf16* __restrict__ out) {
+__global__ void __launch_bounds__(256) attn_tree_tc_join_kernel(TreeGeom g, CacheGeom c, TcSchedule sc, bf16* __restrict__ out) {
   pdl_trigger();
   pdl_wait();
-  const int b = blockIdx.z, h = blockIdx.y, R = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  BlockInfo bi;
-  if (!block_fits(g, c, b, bi) || R >= bi.T * g.G) return;
-  const int tile = R / sc.rows;
+  const int c0 = blockIdx.x, lane = threadIdx.x & 31;
+  const TcCut cut = sc.cuts[c0];
+  if (cut.e < 0) return;
+  const long long W = sc.cuts[sc.ctas].u0, n = sc.ctas;
   bool bad;
-  const Entry x = entry_of(g, c, sc, b * sc.tiles_max + tile, bad);
-  const long long W = sc.table[sc.entries], n = sc.ctas;
-  const long long u0 = sc.table[b * sc.tiles_max + tile] + (long long)h * x.tiles, u1 = u0 + x.tiles;
-  // run k is [k W / n, (k + 1) W / n): the run that holds u is the last one that starts at or before u
-  const int c0 = (int)(((u0 + 1) * n - 1) / W), c1 = (int)((u1 * n - 1) / W);
-  if (c0 == c1) return;                                                 // in one piece: written whole
-  const int at0 = c0 * W / n == u0 ? 0 : 1;                             // the unit is the first or a later piece of run c0
-  const int node = R / g.G, row = R - tile * sc.rows;
-  auto slot = [&](int k) { return ((size_t)k * 2 + (k == c0 ? at0 : 0)) * sc.rows + row; };
-  auto empty = [&](int k) { return k * W / n == (k + 1) * W / n; };     // runs of no tile write nothing
-  float M = -INFINITY;
-  for (int k = c0 + lane; k <= c1; k += 32)
-    if (!empty(k)) M = fmaxf(M, g.part_ml[slot(k)].x);
+  const Entry x = entry_of(g, c, sc, cut.e, bad);
+  // run k is [k W / n, (k + 1) W / n): the run that holds position u is the last one that starts at or before it
+  const int c1 = (int)(((cut.u0 + kUnitCost + cut.tiles) * n - 1) / W);
+  auto slot = [&](int k, int row) { return ((size_t)k * 2 + (k == c0 ? cut.second : 0)) * sc.rows + row; };
+  auto empty = [&](int k) { return k * W / n == (k + 1) * W / n; };     // a run of no position writes nothing
+  for (int row = blockIdx.y * 32 + (threadIdx.x >> 5); row < min(x.nrows, (int)blockIdx.y * 32 + 32); row += 8) {
+    const int R = x.r0 + row, node = R / g.G;
+    float M = -INFINITY;
+    for (int k = c0 + lane; k <= c1; k += 32)
+      if (!empty(k)) M = fmaxf(M, g.part_ml[slot(k, row)].x);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  const float ms = M == -INFINITY ? 0.f : M;
-  constexpr int E = D / 32;
-  float L = 0.f, acc[E];
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    const float ms = M == -INFINITY ? 0.f : M;
+    constexpr int E = D / 32;
+    float L = 0.f, acc[E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  for (int k0 = c0; k0 <= c1; k0 += 32) {
-    float w = 0.f;
-    if (k0 + lane <= c1 && !empty(k0 + lane)) {
-      const float2 v = g.part_ml[slot(k0 + lane)];
-      w = v.y * fast_exp2(v.x - ms);
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    for (int k0 = c0; k0 <= c1; k0 += 32) {
+      float w = 0.f;
+      if (k0 + lane <= c1 && !empty(k0 + lane)) {
+        const float2 v = g.part_ml[slot(k0 + lane, row)];
+        w = v.y * fast_exp2(v.x - ms);
+      }
+      const int cnt = min(32, c1 - k0 + 1);
+#pragma unroll 4
+      for (int k = 0; k < cnt; ++k) {
+        const float wk = __shfl_sync(0xffffffffu, w, k);
+        if (wk != 0.f) {
+          L += wk;
+          const float* src = g.part_o + slot(k0 + k, row) * D + lane * E;
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[e] = fmaf(wk, src[e], acc[e]);
+        }
+      }
     }
-    const int cnt = min(32, c1 - k0 + 1);
-    for (int k = 0; k < cnt; ++k) {
-      const float wk = __shfl_sync(0xffffffffu, w, k);
-      if (wk == 0.f) continue;
-      L += wk;
-      const float* src = g.part_o + slot(k0 + k) * D + lane * E;
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    bf16* dst = out + ((size_t)(x.bi.start + node) * g.n_heads + cut.h * g.G + R % g.G) * D + lane * E;
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = fmaf(wk, src[e], acc[e]);
-    }
+    for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack2<EESD_KV_MODEL>(acc[e] * inv, acc[e + 1] * inv);
   }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-  bf16* dst = out + ((size_t)(bi.start + node) * g.n_heads + h * g.G + R % g.G) * D + lane * E;
-#pragma unroll
-  for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack2<EESD_KV_MODEL>(acc[e] * inv, acc[e + 1] * inv);
 }
 
 template <int D, int FMT>
-cudaError_t launch(const TcSchedule& sc, const TreeGeom& g, const CacheGeom& c, const CUtensorMap& km, const CUtensorMap& vm, int n_blocks,
+cudaError_t launch(const TcSchedule& sc, const TreeGeom& g, const CacheGeom& c, const CUtensorMap& km, const CUtensorMap& vm,
                    const void* q, void* out, cudaStream_t s) {
   using S = TcShape<D, FMT>;
   auto kernel = attn_tree_tc_kernel<D, FMT>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::smem);
   if (e != cudaSuccess) return e;
   e = launch_pdl(kernel, dim3(sc.ctas), dim3(kThreads), S::smem, s, km, vm, g, c, sc, static_cast<const bf16*>(q), static_cast<bf16*>(out));
-  if (e == cudaSuccess && !sc.chunk_tiles)
-    e = launch_pdl(attn_tree_tc_join_kernel<D>, dim3((g.max_nodes * g.G + 3) / 4, c.n_kv_heads, n_blocks), dim3(128), 0, s, g, c, sc,
+  if (e == cudaSuccess && !sc.chunk_tiles && sc.ctas > 1)
+    e = launch_pdl(attn_tree_tc_join_kernel<D>, dim3(sc.ctas, (std::min(sc.rows, g.max_nodes * g.G) + 31) / 32), dim3(256), 0, s, g, c, sc,
                    static_cast<bf16*>(out));
   return e;
 }
@@ -830,14 +858,14 @@ cudaError_t launch(const TcSchedule& sc, const TreeGeom& g, const CacheGeom& c, 
 }  // namespace
 
 cudaError_t launch_attn_tree_tc(int fmt, int D, const TcSchedule& sc, const TreeGeom& g, const CacheGeom& c, const CUtensorMap& km,
-                                const CUtensorMap& vm, int nb, const void* q, void* out, cudaStream_t s) {
+                                const CUtensorMap& vm, const void* q, void* out, cudaStream_t s) {
   switch (fmt * 2 + (D == 128)) {
-    case 0: return launch<64, EESD_KV_MODEL>(sc, g, c, km, vm, nb, q, out, s);
-    case 1: return launch<128, EESD_KV_MODEL>(sc, g, c, km, vm, nb, q, out, s);
-    case 2: return launch<64, EESD_KV_E4M3>(sc, g, c, km, vm, nb, q, out, s);
-    case 3: return launch<128, EESD_KV_E4M3>(sc, g, c, km, vm, nb, q, out, s);
-    case 4: return launch<64, EESD_KV_INT8>(sc, g, c, km, vm, nb, q, out, s);
-    default: return launch<128, EESD_KV_INT8>(sc, g, c, km, vm, nb, q, out, s);
+    case 0: return launch<64, EESD_KV_MODEL>(sc, g, c, km, vm, q, out, s);
+    case 1: return launch<128, EESD_KV_MODEL>(sc, g, c, km, vm, q, out, s);
+    case 2: return launch<64, EESD_KV_E4M3>(sc, g, c, km, vm, q, out, s);
+    case 3: return launch<128, EESD_KV_E4M3>(sc, g, c, km, vm, q, out, s);
+    case 4: return launch<64, EESD_KV_INT8>(sc, g, c, km, vm, q, out, s);
+    default: return launch<128, EESD_KV_INT8>(sc, g, c, km, vm, q, out, s);
   }
 }
 
