@@ -5,11 +5,12 @@
 // causal tiles balance whatever their number; a unit that a cut goes through leaves normalised partial outputs,
 // which a second kernel joins in order.
 //
-// Per 64-key tile: S = Q K^T (Q in TMEM, K in shared memory), softmax weights P from S in registers back into S's
-// columns, O += P V (P in TMEM, V in shared memory, both from the tile's own layout: V is the MN-major operand).
-// With Q and P in TMEM the tensor cores read shared memory for K and V only.  Two streams alternate so that one's
-// softmax runs under the other's products: with more than 128 rows each stream is one half of the rows over all
-// key tiles; with fewer, both share the rows and take every other key tile, and meet at the end.
+// Per 64-key tile: S = Q K^T, softmax weights P from S in registers into TMEM, O += P V, K and V in shared memory in the
+// layout they arrive in (V is the MN-major operand).  Operands in TMEM issue faster than from shared memory (42
+// against 75 clocks for N = 64), so P and the first 128 rows of Q are there; the other 128 rows of Q have no room
+// left beside two fp32 O (256 columns) and two S and P (192).  Two streams alternate, and S of a stream's next tile is
+// computed while its softmax still works on this one: with more than 128 rows each stream is one half of the rows
+// over all key tiles; with fewer, both share the rows and take every other key tile, and meet at the end.
 //
 // 8-bit caches: a warpgroup turns the TMA-loaded bytes into the f16 tiles that the products read (exactly; the
 // powers of two stay out of the operands and multiply scores and weights instead).
@@ -29,7 +30,8 @@ namespace {
 
 constexpr int KT = 64;                     // keys per tile
 constexpr int kThreads = 512;
-constexpr uint32_t kColO = 0, kColQ = 256, kColS = 384;   // TMEM columns; stream x adds 128, 64, 64
+constexpr uint32_t kColO = 0, kColQ = 256;                // TMEM columns; O of stream x at 128 x
+constexpr uint32_t kColS = 320, kColP = 384, kSP = 96;    // S and P of stream x add kSP x
 
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -101,10 +103,11 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
   return r;
 }
 
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-  f32x2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
+// (x, y) *= f, floats held as bits
+__device__ __forceinline__ void scale2(uint32_t& x, uint32_t& y, f32x2 f) {
+  const float2 r = unpack_f2(mul2(pack_f2(__uint_as_float(x), __uint_as_float(y)), f));
+  x = __float_as_uint(r.x);
+  y = __float_as_uint(r.y);
 }
 
 // MN-major operand tile (64-element, 128-byte rows of the MN index per K index, 128-byte swizzle): 8 K indices
@@ -142,7 +145,7 @@ __device__ __forceinline__ Entry entry_of(const TreeGeom& g, const CacheGeom& c,
   return x;
 }
 struct Piece : Entry {
-  int h, t0, t1, index;     // KV head, key tiles [t0, t1), number of the piece in its CTA
+  int e, h, t0, t1, index;  // entry, KV head, key tiles [t0, t1), number of the piece in its CTA
   long long u0;             // flat position of the unit
   __device__ bool whole() const { return t0 == 0 && t1 == tiles; }
 };
@@ -156,7 +159,7 @@ struct PieceIter {
       if (loaded != e) {
         bool bad;
         static_cast<Entry&>(p) = entry_of(g, c, sc, e, bad);
-        loaded = e;
+        p.e = loaded = e;
       }
       const int len = p.length();
       const long long span = (long long)len * c.n_kv_heads;
@@ -194,20 +197,27 @@ template <int D, int FMT> struct TcShape {
   static constexpr bool Q8 = FMT != EESD_KV_MODEL;
   static constexpr int TILE = KT * D * 2;              // bytes of one 16-bit K (or V) tile
   static constexpr int RAW = KT * D * 2;               // 8-bit: K and V bytes of one tile
-  static constexpr int NS = Q8 ? 2 : 6;                // 16-bit K / V stages
-  static constexpr int RS = Q8 ? 8 : 0;                // raw stages
-  static constexpr int FR = 4;                         // factor ring
-  static constexpr size_t ctl = 12288;
-  static constexpr size_t smem = 1024 + (size_t)2 * NS * TILE + (size_t)RS * RAW + ctl;
+  static constexpr int NS = Q8 ? 2 : 5;                // 16-bit K / V stages
+  static constexpr int RS = Q8 ? 6 : 0;                // raw stages
+  static constexpr int FR = 8;                         // factor ring: six tiles can be between conversion and softmax
+  static constexpr int QB = 128 * D * 2;               // Q of stream 1 (more than 128 rows)
+  static constexpr size_t ctl = 16384;
+  static constexpr size_t smem = 1024 + (size_t)2 * NS * TILE + (size_t)RS * RAW + QB + ctl;
 };
+constexpr int kPieces = 4;                 // pieces between the schedule warp and the slowest role
+constexpr int kReaders = 14;               // warps that read them: TMA, MMA, 8 softmax, 4 conversion
 struct TcControl {
-  uint64_t kfull[6], kempty[6], vfull[6], vempty[6], vclean[6], raw_full[8], raw_empty[8], ffull[4];
-  uint64_t s_full[2], p_ready[2], q_ready, o_done, ml_ready, drain;
-  alignas(16) float fk[4][KT];             // 8-bit: 2^ek of a tile's keys
-  alignas(16) float fv[4][KT];             // 2^(ev - emax)
-  alignas(16) uint8_t ev[4][KT];
-  alignas(16) uint8_t exps[8][2 * KT];     // raw exponent bytes, K then V
-  int emax[4], even[4];                    // largest V exponent; the others within 2^4 of it and no NaN
+  uint64_t kfull[5], kempty[5], vfull[5], vempty[5], vclean[5], raw_full[6], raw_empty[6], ffull[8];
+  uint64_t piece_full[kPieces], piece_empty[kPieces];
+  Piece piece[kPieces];                    // tiles == 0: there are no more
+  uint64_t s_full[2], s_free[2], p_ready[2], pv_done[2], q_ready, o_done, ml_ready, epi_done, drain;
+  alignas(16) float fk[8][KT];             // 8-bit: 2^ek of a tile's keys
+  alignas(16) float fv[8][KT];             // 2^(ev - ref), 0 for NaN and slots past the end
+  alignas(16) uint8_t ev[8][KT];           // V's exponent bytes, 0 likewise
+  alignas(16) uint8_t exps[6][2 * KT];     // raw exponent bytes, K then V
+  alignas(16) float zeros[KT];
+  int ref[8];                              // the exponent byte that fv is relative to
+  uint32_t nan[8][2];                      // keys whose V is NaN
   float ml[2][2][3][128];                  // one row tile: max, sum and eref of the streams (by piece parity)
   long long lo, hi, base;
   long long wsum[16];
@@ -215,7 +225,7 @@ struct TcControl {
   int e0;
   int abort, dropped;
 };
-static_assert(sizeof(TcControl) <= 12288 && alignof(TcControl) <= 16, "control block");
+static_assert(sizeof(TcControl) <= 16384 && alignof(TcControl) <= 16, "control block");
 
 template <int D, int FMT>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -227,9 +237,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_trigger();
   pdl_wait();
   extern __shared__ uint8_t smem8[];
-  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem8) + 1023) & ~uintptr_t(1023));
-  const uint32_t kbuf = smem_u32(sm), vbuf = kbuf + NS * S::TILE, raw = vbuf + NS * S::TILE;
-  TcControl& ct = *reinterpret_cast<TcControl*>(sm + 2 * NS * S::TILE + S::RS * S::RAW);
+  uint8_t* sm = smem8 + (-smem_u32(smem8) & 1023);     // an offset, so that the compiler still knows it as shared memory
+  const uint32_t kbuf = smem_u32(sm), vbuf = kbuf + NS * S::TILE, raw = vbuf + NS * S::TILE, qbuf = raw + S::RS * S::RAW;
+  TcControl& ct = *reinterpret_cast<TcControl*>(sm + 2 * NS * S::TILE + S::RS * S::RAW + S::QB);
   volatile int* abort_flag = &ct.abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -267,14 +277,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = 0; i < FR; ++i) mbar_init(smem_u32(&ct.ffull[i]), 128);
       for (int i = 0; i < 2; ++i) {
         mbar_init(smem_u32(&ct.s_full[i]), 1);
+        mbar_init(smem_u32(&ct.s_free[i]), 128);
         mbar_init(smem_u32(&ct.p_ready[i]), 128);
+        mbar_init(smem_u32(&ct.pv_done[i]), 1);
+      }
+      for (int i = 0; i < kPieces; ++i) {
+        mbar_init(smem_u32(&ct.piece_full[i]), 1);
+        mbar_init(smem_u32(&ct.piece_empty[i]), kReaders);
       }
       mbar_init(smem_u32(&ct.q_ready), 256);
       mbar_init(smem_u32(&ct.ml_ready), 256);
+      mbar_init(smem_u32(&ct.epi_done), 256);
       mbar_init(smem_u32(&ct.o_done), 1);
       mbar_init(smem_u32(&ct.drain), 1);
       fence_mbar_init();
     }
+    if (tid < KT) ct.zeros[tid] = 0.f;
     if (warp == 1) {
       tmem_alloc(smem_u32(&ct.tmem), 512);
       tmem_relinquish();
@@ -310,12 +328,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncthreads();
   }
-  PieceIter it{ct.lo, ct.hi, ct.base, ct.e0, 0, -1};
-  if (ct.e0 >= sc.entries) it.pos = it.end;
-  Piece p;
+  // Every role reads its pieces, in order, from the ring that warp 2 fills.
+  auto piece_wait = [&](int k) { return mbar_wait(smem_u32(&ct.piece_full[k % kPieces]), k / kPieces & 1, abort_flag, g.spin); };
+  auto piece_free = [&](int k) { mbar_arrive(smem_u32(&ct.piece_empty[k % kPieces])); };
   const uint32_t tmem = ct.tmem;
 
-  if (warp < 4) reg_dec<88>();
+  if (warp < 4) reg_dec<56>();
   if (warp == 0) {
     // ------------------------------------------------------------ TMA
     if (elect_one()) {
@@ -323,7 +341,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       tma_prefetch_desc(&kmap);
       tma_prefetch_desc(&vmap);
-      while (ok && it.next(g, c, sc, p)) {
+      for (int k = 0; (ok = piece_wait(k)); ++k) {
+        const Piece& p = ct.piece[k % kPieces];
+        if (p.tiles == 0) break;
         const int slot0 = (int)cache_slot(c, p.bi.row, p.h, 0);
         for (int t = p.t0; t < p.t1; ++t, ++cnt) {
           if constexpr (Q8) {
@@ -351,6 +371,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             v_issued = cnt + 1;
           }
         }
+        if (!ok) break;
+        piece_free(k);
       }
       if (!ok) {
         set_status(g.status, kStatusTimeoutProducer);
@@ -368,29 +390,42 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------ MMA issue
     if (elect_one()) {
       const uint32_t id_qk = idesc_f32<FMT>(KT, false), id_pv = idesc_f32<FMT>(D, true);
-      int cnt0 = 0, piece = 0, n_p[2] = {0, 0};
+      int cnt0 = 0, piece = 0, n_q[2] = {0, 0}, n_p[2] = {0, 0};
       bool ok = true, issued = false;
-      while (ok && it.next(g, c, sc, p)) {
+      for (; (ok = piece_wait(piece)); ++piece) {
+        const Piece& p = ct.piece[piece % kPieces];
+        if (p.tiles == 0) break;
         const int nt = p.t1 - p.t0;
         const bool two = p.nrows > 128;
         const int steps = two ? 2 * nt : nt;
         if (!(ok = mbar_wait(smem_u32(&ct.q_ready), piece & 1, abort_flag, g.spin))) break;
-        for (int s = 0; s <= steps; ++s) {
-          if (s < steps) {                                              // S of step s
+        // S of step s as soon as its stream has taken S of step s - 2 into registers, then O of that step when its
+        // softmax ends.  (A longer lead would need a third converted V tile: conversion goes K, V, K, V.)
+        for (int s = 0; s < steps + 2; ++s) {
+          if (s < steps) {
             const int x = s & 1, cnt = cnt0 + (two ? s >> 1 : s), st = cnt % NS;
+            if (n_q[x] && !(ok = mbar_wait(smem_u32(&ct.s_free[x]), (n_q[x] - 1) & 1, abort_flag, g.spin))) break;
+            ++n_q[x];
             if ((!two || x == 0) && !(ok = mbar_wait(smem_u32(&ct.kfull[st]), cnt / NS & 1, abort_flag, g.spin))) break;
             tc_fence_after();
             issued = true;
             const uint64_t kd = sw128_kmajor_desc(kbuf + st * S::TILE);
-            const uint32_t qa = tmem + kColQ + (two ? x * 64 : 0);
+            const uint32_t d = tmem + kColS + x * kSP;
+            if (two && x == 1) {
+              const uint64_t qd = sw128_kmajor_desc(qbuf);
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk)
-              tc_mma_ts(tmem + kColS + x * 64, qa + kk * 8, kd + (kk >> 2) * (KT * 128 >> 4) + (kk & 3) * 2, id_qk, kk > 0);
+              for (int kk = 0; kk < D / 16; ++kk)
+                tc_mma_f16(d, qd + (kk >> 2) * (128 * 128 >> 4) + (kk & 3) * 2, kd + (kk >> 2) * (KT * 128 >> 4) + (kk & 3) * 2, id_qk, kk > 0);
+            } else {
+#pragma unroll
+              for (int kk = 0; kk < D / 16; ++kk)
+                tc_mma_ts(d, tmem + kColQ + kk * 8, kd + (kk >> 2) * (KT * 128 >> 4) + (kk & 3) * 2, id_qk, kk > 0);
+            }
             if (!two || x == 1) tc_commit(smem_u32(&ct.kempty[st]));
             tc_commit(smem_u32(&ct.s_full[x]));
           }
-          if (s > 0) {                                                  // O of step s - 1
-            const int u = s - 1, x = u & 1, i = two ? u >> 1 : u, cnt = cnt0 + i, st = cnt % NS;
+          if (s >= 2) {
+            const int u = s - 2, x = u & 1, i = two ? u >> 1 : u, cnt = cnt0 + i, st = cnt % NS;
             if (!(ok = mbar_wait(smem_u32(&ct.p_ready[x]), n_p[x]++ & 1, abort_flag, g.spin))) break;
             if ((!two || x == 0) &&
                 !(ok = mbar_wait(smem_u32(Q8 ? &ct.vfull[st] : &ct.vclean[st]), cnt / NS & 1, abort_flag, g.spin)))
@@ -400,14 +435,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool first = two ? i == 0 : u < 2;
 #pragma unroll
             for (int kk = 0; kk < KT / 16; ++kk)
-              tc_mma_ts(tmem + kColO + x * 128, tmem + kColS + x * 64 + kk * 8, vd + kk * (16 * 128 >> 4), id_pv, !(first && kk == 0));
+              tc_mma_ts(tmem + kColO + x * 128, tmem + kColP + x * kSP + kk * 8, vd + kk * (16 * 128 >> 4), id_pv, !(first && kk == 0));
             if (!two || x == 1) tc_commit(smem_u32(&ct.vempty[st]));
+            tc_commit(smem_u32(&ct.pv_done[x]));
           }
         }
         if (!ok) break;
         tc_commit(smem_u32(&ct.o_done));
         cnt0 += nt;
-        ++piece;
+        piece_free(piece);
       }
       if (!ok) {
         set_status(g.status, kStatusTimeoutMma);
@@ -418,66 +454,91 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_drain(smem_u32(&ct.drain), 0);
       }
     }
+  } else if (warp == 2) {
+    // ------------------------------------------------------------ the schedule
+    if (elect_one()) {
+      PieceIter it{ct.lo, ct.hi, ct.base, ct.e0, 0, -1};
+      if (ct.e0 >= sc.entries) it.pos = it.end;
+      bool ok = true;
+      Piece p;
+      for (int k = 0;; ++k) {
+        if (!(ok = mbar_wait(smem_u32(&ct.piece_empty[k % kPieces]), (k / kPieces & 1) ^ 1, abort_flag, g.spin))) break;
+        const bool more = it.next(g, c, sc, p);
+        if (!more) p.tiles = 0;
+        ct.piece[k % kPieces] = p;
+        mbar_arrive(smem_u32(&ct.piece_full[k % kPieces]));
+        if (!more) break;
+      }
+      if (!ok) {
+        set_status(g.status, kStatusTimeoutProducer);
+        *abort_flag = 1;
+      }
+    }
   } else if (warp >= 12) {
-    reg_dec<80>();
+    reg_dec<56>();
     // ------------------------------------------------------------ conversion, or the check of V tiles
     const int ti = tid - 384;
+    [[maybe_unused]] auto convert = [&](const uint8_t* src, uint8_t* dst) {
+      constexpr int C = D / 16;                                         // 16-byte chunks of a raw row
+#pragma unroll
+      for (int i = 0; i < KT * C / 128; ++i) {
+        // 8 lanes of a phase on 8 rows and one chunk: conflict-free in both swizzles
+        const int idx = i * 128 + ti, j = idx >> 3, ch = j % C, row = j / C * 8 + (idx & 7);
+        const uint4 w = *reinterpret_cast<const uint4*>(src + row * D + ((D == 128 ? ch ^ (row & 7) : ch ^ ((row >> 1) & 3)) << 4));
+        uint4 a, b;
+        unpack4<FMT>(w.x, a.x, a.y);
+        unpack4<FMT>(w.y, a.z, a.w);
+        unpack4<FMT>(w.z, b.x, b.y);
+        unpack4<FMT>(w.w, b.z, b.w);
+        uint8_t* to = dst + (ch >> 2) * (KT * 128) + row * 128;
+        const int c0 = 2 * ch & 7;
+        *reinterpret_cast<uint4*>(to + ((c0 ^ (row & 7)) << 4)) = a;
+        *reinterpret_cast<uint4*>(to + (((c0 + 1) ^ (row & 7)) << 4)) = b;
+      }
+      fence_proxy_async_smem();
+    };
+    // V of a tile waits for the product two tiles before it, K does not: K goes one tile ahead
+    [[maybe_unused]] auto convert_v = [&](int cnt) {
+      const int st = cnt % NS, rs = cnt % RS;
+      if (!warp_wait(&ct.vempty[st], (cnt / NS & 1) ^ 1, abort_flag, g.spin)) return false;
+      convert(sm + 2 * NS * S::TILE + rs * S::RAW + S::RAW / 2, sm + (NS + st) * S::TILE);
+      mbar_arrive(smem_u32(&ct.vfull[st]));
+      mbar_arrive(smem_u32(&ct.raw_empty[rs]));
+      return true;
+    };
     int cnt = 0;
     bool ok = true;
-    while (ok && it.next(g, c, sc, p)) {
+    for (int k = 0; (ok = __all_sync(0xffffffffu, piece_wait(k))); ++k) {
+      const Piece& p = ct.piece[k % kPieces];
+      if (p.tiles == 0) break;
       for (int t = p.t0; t < p.t1; ++t, ++cnt) {
         const int st = cnt % NS;
         if constexpr (Q8) {
           const int rs = cnt % RS, f = cnt % FR;
           if (!(ok = warp_wait(&ct.raw_full[rs], cnt / RS & 1, abort_flag, g.spin))) break;
-          {
-            // factors of the tile's keys (the ring slot's last reader is behind the product that freed this K stage)
-            const uint32_t vpair = lds_u16(smem_u32(&ct.exps[rs][KT + 2 * lane]));
-            const int left = p.n_keys - t * KT, a0 = vpair & 255, a1 = vpair >> 8;
-            const bool in0 = 2 * lane < left && a0 != 255, in1 = 2 * lane + 1 < left && a1 != 255;
-            const int em = __reduce_max_sync(0xffffffffu, max(in0 ? a0 : 0, in1 ? a1 : 0));
-            const int en = __reduce_min_sync(0xffffffffu, min(in0 ? a0 : em, in1 ? a1 : em));
-            const bool nan = __any_sync(0xffffffffu, (2 * lane < left && a0 == 255) || (2 * lane + 1 < left && a1 == 255));
-            if (!(ok = warp_wait(&ct.kempty[st], (cnt / NS & 1) ^ 1, abort_flag, g.spin))) break;
-            if (ti < KT) {
-              ct.fk[f][ti] = exp_scale(ct.exps[rs][ti]);
-              if (ti == 0) {
-                ct.emax[f] = em;
-                ct.even[f] = em - en <= 4 && !nan;
-              }
-            } else {
-              const int ev = ct.exps[rs][ti];
-              ct.ev[f][ti - KT] = (uint8_t)ev;
-              const int d = ev - em + 127;
-              ct.fv[f][ti - KT] = ti - KT >= left ? 0.f : ev == 255 ? __int_as_float(0x7fffffff) : d <= 0 ? 0.f : __int_as_float(d << 23);
-            }
-            mbar_arrive(smem_u32(&ct.ffull[f]));
+          // factors of the tile's keys (the ring slot's last reader is behind the product that freed this K stage).
+          // V's are relative to the largest exponent; in a tile that some row does not wholly see to 2^60 below it,
+          // so that they last for rows whose own largest is far smaller
+          const uint32_t vpair = *reinterpret_cast<const uint16_t*>(&ct.exps[rs][KT + 2 * lane]);
+          const int left = p.n_keys - t * KT, a0 = vpair & 255, a1 = vpair >> 8;
+          const int em = __reduce_max_sync(0xffffffffu, max(2 * lane < left && a0 != 255 ? a0 : 0, 2 * lane + 1 < left && a1 != 255 ? a1 : 0));
+          const int ref = em - ((t + 1) * KT > min(p.all_see, p.n_keys) ? 60 : 0);
+          if (!(ok = warp_wait(&ct.kempty[st], (cnt / NS & 1) ^ 1, abort_flag, g.spin))) break;
+          if (ti < KT) {
+            ct.fk[f][ti] = exp_scale(ct.exps[rs][ti]);
+            if (ti == 0) ct.ref[f] = ref;
+          } else {
+            const int ev = ct.exps[rs][ti], d = ev - ref + 127;
+            const bool nan = ev == 255, in = ti - KT < left;
+            ct.ev[f][ti - KT] = nan || !in ? 0 : (uint8_t)ev;
+            ct.fv[f][ti - KT] = nan || !in || d <= 0 ? 0.f : __int_as_float(d << 23);
+            const uint32_t nans = __ballot_sync(0xffffffffu, nan && in);
+            if (lane == 0) ct.nan[f][(ti - KT) >> 5] = nans;
           }
-          auto convert = [&](uint32_t src, uint32_t dst) {
-            constexpr int C = D / 16;                                   // 16-byte chunks of a raw row
-#pragma unroll
-            for (int i = 0; i < KT * C / 128; ++i) {
-              // 8 lanes of a phase on 8 rows and one chunk: conflict-free in both swizzles
-              const int idx = i * 128 + ti, j = idx >> 3, ch = j % C, row = j / C * 8 + (idx & 7);
-              const uint4 w = lds128(src + row * D + ((D == 128 ? ch ^ (row & 7) : ch ^ ((row >> 1) & 3)) << 4));
-              uint4 a, b;
-              unpack4<FMT>(w.x, a.x, a.y);
-              unpack4<FMT>(w.y, a.z, a.w);
-              unpack4<FMT>(w.z, b.x, b.y);
-              unpack4<FMT>(w.w, b.z, b.w);
-              const uint32_t to = dst + (ch >> 2) * (KT * 128) + row * 128;
-              const int c0 = 2 * ch & 7;
-              sts128(to + ((c0 ^ (row & 7)) << 4), a);
-              sts128(to + (((c0 + 1) ^ (row & 7)) << 4), b);
-            }
-            fence_proxy_async_smem();
-          };
-          convert(raw + rs * S::RAW, kbuf + st * S::TILE);
+          mbar_arrive(smem_u32(&ct.ffull[f]));
+          convert(sm + 2 * NS * S::TILE + rs * S::RAW, sm + st * S::TILE);
           mbar_arrive(smem_u32(&ct.kfull[st]));
-          if (!(ok = warp_wait(&ct.vempty[st], (cnt / NS & 1) ^ 1, abort_flag, g.spin))) break;
-          convert(raw + rs * S::RAW + S::RAW / 2, vbuf + st * S::TILE);
-          mbar_arrive(smem_u32(&ct.vfull[st]));
-          mbar_arrive(smem_u32(&ct.raw_empty[rs]));
+          if (cnt && !(ok = convert_v(cnt - 1))) break;
         } else {
           if (!(ok = warp_wait(&ct.vfull[st], cnt / NS & 1, abort_flag, g.spin))) break;
           if ((t + 1) * KT > min(p.all_see, p.n_keys)) {
@@ -501,122 +562,203 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_arrive(smem_u32(&ct.vclean[st]));
         }
       }
+      if (!ok) break;
+      if (lane == 0) piece_free(k);
     }
+    if (Q8 && ok && cnt) ok = convert_v(cnt - 1);
     if (!ok) {
       set_status(g.status, kStatusTimeoutProducer);
       *abort_flag = 1;
     }
   } else if (warp >= 4) {
-    reg_inc<168>();
+    reg_inc<200>();
     // ------------------------------------------------------------ softmax: thread = row of stream x
     const int x = (warp >> 2) - 1, r = tid & 127;
     const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);         // TMEM lane quadrant of the warp
-    const uint32_t tS = lanes + kColS + x * 64, tO = lanes + kColO + x * 128;
+    const uint32_t tS = lanes + kColS + x * kSP, tP = lanes + kColP + x * kSP, tO = lanes + kColO + x * 128;
     int cnt0 = 0, n_s = 0, piece = 0, n_ml = 0;
     bool ok = true;
-    while (ok && it.next(g, c, sc, p)) {
-      const int nt = p.t1 - p.t0;
-      const bool two = p.nrows > 128;
-      const int row = (two ? x * 128 : 0) + r;                          // of the row tile
-      const bool in = row < p.nrows;
-      const int R = p.r0 + min(row, p.nrows - 1), node = R / g.G;
-      const int head = p.h * g.G + R % g.G;
-      float rf = g.scale * 1.4426950408889634f;
-      {
-        // the q row: bf16 as it is, or f16 with the largest element's power of two taken out
-        const bf16* src = q + (size_t)(p.bi.start + node) * g.ld_q + (size_t)head * D;
-        uint32_t w[D / 2], amax = 0;
+    struct Row {
+      bool two, in;
+      int row, node, head;   // of the row tile; the row's node; its query head
+    };
+    auto row_of = [&](const Piece& p) {
+      Row w;
+      w.two = p.nrows > 128;
+      w.row = (w.two ? x * 128 : 0) + r;
+      w.in = w.row < p.nrows;
+      const int R = p.r0 + min(w.row, p.nrows - 1);
+      w.node = R / g.G;
+      w.head = p.h * g.G + R - w.node * g.G;
+      return w;
+    };
+    const float scale_l2 = g.scale * 1.4426950408889634f;
+    auto load_q = [&](const Piece& p, const Row& w, uint32_t (&v)[D / 2]) {
+      const bf16* src = q + (size_t)(p.bi.start + w.node) * g.ld_q + (size_t)w.head * D;
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          const uint4 v = in ? *reinterpret_cast<const uint4*>(src + i * 8) : make_uint4(0, 0, 0, 0);
-          w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
-        }
-        if constexpr (Q8) {
+      for (int i = 0; i < D / 8; ++i) {
+        const uint4 u = w.in ? *reinterpret_cast<const uint4*>(src + i * 8) : make_uint4(0, 0, 0, 0);
+        v[4 * i] = u.x, v[4 * i + 1] = u.y, v[4 * i + 2] = u.z, v[4 * i + 3] = u.w;
+      }
+    };
+    // the q row where the products read it: bf16 as it is, or f16 with the largest element's power of two taken out
+    // (returned with the softmax scale)
+    auto put_q = [&](const Row& w, uint32_t (&v)[D / 2]) {
+      float rf = scale_l2;
+      if constexpr (Q8) {
+        uint32_t amax = 0;
 #pragma unroll
-          for (int i = 0; i < D / 2; ++i) amax = max(amax, max(w[i] << 16 & 0x7fff0000u, w[i] & 0x7fff0000u));
-          const int e = min(max((int)(amax >> 23), 27), 227);
-          const float inv = __int_as_float((254 - e) << 23);
-          rf *= __int_as_float(e << 23) * kHalfUnit<FMT>;
+        for (int i = 0; i < D / 2; ++i) amax = max(amax, max(v[i] << 16 & 0x7fff0000u, v[i] & 0x7fff0000u));
+        const int e = min(max((int)(amax >> 23), 27), 227);
+        const float inv = __int_as_float((254 - e) << 23);
+        rf *= __int_as_float(e << 23) * kHalfUnit<FMT>;
 #pragma unroll
-          for (int i = 0; i < D / 2; ++i) w[i] = pack2<FMT>(__uint_as_float(w[i] << 16) * inv, __uint_as_float(w[i] & 0xffff0000u) * inv);
-        }
-        if (two || x == 0) {
-          const uint32_t tQ = lanes + kColQ + (two ? x * 64 : 0);
+        for (int i = 0; i < D / 2; ++i) v[i] = pack2<FMT>(__uint_as_float(v[i] << 16) * inv, __uint_as_float(v[i] & 0xffff0000u) * inv);
+      }
+      if (x == 0) {
 #pragma unroll
-          for (int i = 0; i < D / 64; ++i) tmem_st32(tQ + 32 * i, w + 32 * i);
-          tmem_wait_st();
-        }
+        for (int i = 0; i < D / 64; ++i) tmem_st32(lanes + kColQ + 32 * i, v + 32 * i);
+        tmem_wait_st();
+      } else if (w.two) {
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i)
+          sts128(qbuf + (i >> 3) * (128 * 128) + r * 128 + (((i & 7) ^ (r & 7)) << 4),
+                 make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]));
+        fence_proxy_async_smem();
       }
       tc_fence_before();
       mbar_arrive(smem_u32(&ct.q_ready));
+      return rf;
+    };
+    float rf = 0.f;
+    bool more = false;
+    if ((ok = __all_sync(0xffffffffu, piece_wait(0))) && ct.piece[0].tiles) {
+      uint32_t v[D / 2];
+      const Row w = row_of(ct.piece[0]);
+      load_q(ct.piece[0], w, v);
+      rf = put_q(w, v);
+      more = true;
+    }
+    while (more) {
+      const Piece& cur = ct.piece[piece % kPieces];
+      const int nt = cur.t1 - cur.t0;
+      const bool two = cur.nrows > 128;
       float m = -INFINITY, l = 0.f;
       int er = 0;                                                       // 8-bit: exponent byte that O and l are relative to
       bool begun = false;
       for (int i = two ? 0 : x; i < nt; i += two ? 1 : 2) {
-        const int t = p.t0 + i, cnt = cnt0 + i, f = cnt % FR;
-        if (!(ok = warp_wait(&ct.s_full[x], n_s++ & 1, abort_flag, g.spin))) break;
+        const int t = cur.t0 + i, cnt = cnt0 + i, f = cnt % FR;
+        if (!(ok = warp_wait(&ct.s_full[x], n_s & 1, abort_flag, g.spin))) break;
         tc_fence_after();
         if (Q8 && !(ok = warp_wait(&ct.ffull[f], cnt / FR & 1, abort_flag, g.spin))) break;
         uint32_t a[KT];
         tmem_ld32(tS, a);
         tmem_ld32(tS + 32, a + 32);
         tmem_wait_ld();
-        const bool partial = (t + 1) * KT > min(p.all_see, p.n_keys);
-        uint32_t see[2] = {~0u, ~0u};
-        int em = 0;
-        if constexpr (Q8) em = ct.emax[f];
-        float mx = -INFINITY;
+        tc_fence_before();
+        mbar_arrive(smem_u32(&ct.s_free[x]));
+        // ---- scores in the log2 domain and their maximum
         if constexpr (Q8) {
-          const uint32_t fk = smem_u32(ct.fk[f]);
+          const float4* fk = reinterpret_cast<const float4*>(ct.fk[f]);
           const f32x2 rf2 = pack_f2(rf, rf);
 #pragma unroll
           for (int j = 0; j < KT; j += 4) {
-            const uint4 v = lds128(fk + j * 4);
-            const float2 y0 = unpack_f2(mul2(pack_f2(__uint_as_float(a[j]), __uint_as_float(a[j + 1])),
-                                             mul2(rf2, pack_f2(__uint_as_float(v.x), __uint_as_float(v.y)))));
-            const float2 y1 = unpack_f2(mul2(pack_f2(__uint_as_float(a[j + 2]), __uint_as_float(a[j + 3])),
-                                             mul2(rf2, pack_f2(__uint_as_float(v.z), __uint_as_float(v.w)))));
-            a[j] = __float_as_uint(y0.x), a[j + 1] = __float_as_uint(y0.y);
-            a[j + 2] = __float_as_uint(y1.x), a[j + 3] = __float_as_uint(y1.y);
+            const float4 v = fk[j / 4];
+            scale2(a[j], a[j + 1], mul2(rf2, pack_f2(v.x, v.y)));
+            scale2(a[j + 2], a[j + 3], mul2(rf2, pack_f2(v.z, v.w)));
           }
-        }
-        // V's scales of a tile that some row does not wholly see: row by row only where they differ much
-        const bool by_row = Q8 && partial && !ct.even[f];
-        if (partial) {
+        } else {
+          const f32x2 rf2 = pack_f2(rf, rf);
 #pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            const int kb = t * KT + 32 * w, left = p.n_keys - kb;
-            see[w] = sees32(g.mask ? g.mask + (size_t)(p.bi.start + node) * g.words : nullptr, g.words, node, kb - p.bi.ctx);
-            if (left < 32) see[w] &= left <= 0 ? 0u : (1u << left) - 1;
-          }
+          for (int j = 0; j < KT; j += 2) scale2(a[j], a[j + 1], rf2);
+        }
+        int ref = 0, em = 0;
+        uint32_t nan = 0;
+        if constexpr (Q8) {
+          em = ref = ct.ref[f];
+          nan = ct.nan[f][0] | ct.nan[f][1];
+        }
+        if ((t + 1) * KT > min(cur.all_see, cur.n_keys)) {              // some row does not see some key of the tile
+          const int node = row_of(cur).node, left = cur.n_keys - t * KT;
+          const uint64_t* mk = g.mask ? g.mask + (size_t)(cur.bi.start + node) * g.words : nullptr;
+          uint32_t s0 = sees32(mk, g.words, node, t * KT - cur.bi.ctx), s1 = sees32(mk, g.words, node, t * KT + 32 - cur.bi.ctx);
+          if (left < 32) s0 &= (1u << left) - 1;
+          if (left < 64) s1 &= left <= 32 ? 0u : (1u << (left - 32)) - 1;
 #pragma unroll
           for (int j = 0; j < KT; ++j)
-            if (!(see[j >> 5] >> (j & 31) & 1)) a[j] = 0xff800000u;
-          if (by_row) {
-            em = 0;
-#pragma unroll 8
-            for (int j = 0; j < KT; ++j)
-              if (see[j >> 5] >> (j & 31) & 1) em = max(em, ct.ev[f][j] == 255 ? 0 : (int)ct.ev[f][j]);
+            if (!((j < 32 ? s0 : s1) >> (j & 31) & 1)) a[j] = 0xff800000u;
+          if constexpr (Q8) {                                           // V's largest exponent among the keys this row sees
+            uint32_t top = 0;
+#pragma unroll 2
+            for (int j = 0; j < KT / 4; ++j) {
+              const uint32_t bits = (j < 8 ? s0 >> 4 * j : s1 >> (4 * j - 32)) & 15;
+              top = __vmaxu4(top, reinterpret_cast<const uint32_t*>(ct.ev[f])[j] & ((bits * 0x204081u & 0x1010101u) * 255u));
+            }
+            em = max(max(top & 255, top >> 8 & 255), max(top >> 16 & 255, top >> 24));
+            nan = (ct.nan[f][0] & s0) | (ct.nan[f][1] & s1);
           }
         }
+        if (Q8 && nan) l = __int_as_float(0x7fffffff);                  // the row sees a V that is NaN
+        float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < KT; j += 2) mx = fmaxf(mx, fmaxf(__uint_as_float(a[j]), __uint_as_float(a[j + 1])));
-        if constexpr (!Q8) mx *= rf;                                    // rf > 0
+        for (int j = 0; j < KT; j += 4) {
+          mx0 = fmaxf(mx0, fmaxf(__uint_as_float(a[j]), __uint_as_float(a[j + 1])));
+          mx1 = fmaxf(mx1, fmaxf(__uint_as_float(a[j + 2]), __uint_as_float(a[j + 3])));
+        }
         // O, l and m move to a new reference only when the old one is too small by 2^8 (2^4 for V's scale): the
         // weights stay below 2^12, in range of f16
-        const float mn = fmaxf(m, mx);
-        const int en = max(er, em);
+        const float mn = fmaxf(m, fmaxf(mx0, mx1));
         const bool need = !begun || mn > m + 8.f || (Q8 && em > er + 4);
         float cf = 1.f;
         if (need) {
+          const int en = max(er, em);
           cf = m == -INFINITY ? 0.f : fast_exp2(m - mn);
           l *= cf;
           if (Q8) cf *= er == 0 ? 0.f : fast_exp2((float)(er - en));
           m = mn;
           er = en;
         }
-        if (begun && __any_sync(0xffffffffu, need)) {
-          // every product issued before this step's S is complete, the stream's last O among them
+        const bool rescale = begun && __any_sync(0xffffffffu, need);
+        const float ms = m == -INFINITY ? 0.f : m;
+        // ---- weights.  V's scale relative to er: its common part goes into the exponent, so l collects the same units
+        // and is brought back by the exact power of two, the rest multiplies.  Below 2^-40 no weight of the tile is left
+        // in f16.
+        const bool gone = Q8 && em - er < -40;
+        const int dd = Q8 && !gone ? min(ref - er, 100) : 0;
+        const float4* fv = reinterpret_cast<const float4*>(gone ? ct.zeros : ct.fv[f]);
+        // The packed product and sum may be contracted to one FMA, which leaves 2^-24 |m| of the score in the exponent:
+        // nothing at ordinary sizes, but at very large ones the largest score has to come out as exactly 0.
+        float nbs = (float)dd - ms;
+        if (__any_sync(0xffffffffu, fabsf(ms) > 65536.f)) {
+#pragma unroll
+          for (int j = 0; j < KT; ++j) a[j] = __float_as_uint(__fadd_rn(__uint_as_float(a[j]), -ms));
+          nbs = (float)dd;
+        }
+        const f32x2 nb = pack_f2(nbs, nbs);
+        f32x2 sum0 = pack_f2(0.f, 0.f), sum1 = pack_f2(0.f, 0.f);
+#pragma unroll
+        for (int j = 0; j < KT; j += 4) {
+          const float2 y0 = unpack_f2(add2(pack_f2(__uint_as_float(a[j]), __uint_as_float(a[j + 1])), nb));
+          const float2 y1 = unpack_f2(add2(pack_f2(__uint_as_float(a[j + 2]), __uint_as_float(a[j + 3])), nb));
+          f32x2 e0 = pack_f2(fast_exp2(y0.x), fast_exp2(y0.y)), e1 = pack_f2(fast_exp2(y1.x), fast_exp2(y1.y));
+          sum0 = add2(sum0, e0);
+          sum1 = add2(sum1, e1);
+          if constexpr (Q8) {
+            const float4 v = fv[j / 4];
+            e0 = mul2(e0, pack_f2(v.x, v.y));
+            e1 = mul2(e1, pack_f2(v.z, v.w));
+          }
+          const float2 w0 = unpack_f2(e0), w1 = unpack_f2(e1);
+          a[j / 2] = pack2<FMT>(w0.x, w0.y);
+          a[j / 2 + 1] = pack2<FMT>(w1.x, w1.y);
+        }
+        const float2 sv = unpack_f2(add2(sum0, sum1));
+        l = Q8 ? fmaf(sv.x + sv.y, __int_as_float((127 - dd) << 23), l) : l + sv.x + sv.y;
+        // ---- P, once the product that read the last one is done (O is at rest then)
+        if (n_s && !(ok = warp_wait(&ct.pv_done[x], (n_s - 1) & 1, abort_flag, g.spin))) break;
+        ++n_s;
+        tc_fence_after();
+        if (rescale) {
 #pragma unroll
           for (int b = 0; b < D; b += 32) {
             uint32_t o[32];
@@ -627,91 +769,30 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_st32(tO + b, o);
           }
         }
+        // the other stream's threads may still read this stream's O of the piece before
+        if (!begun && piece && !(ok = warp_wait(&ct.epi_done, (piece - 1) & 1, abort_flag, g.spin))) break;
         begun = true;
-        const float ms = m == -INFINITY ? 0.f : m;
-        uint32_t pk[KT / 2];
-        if constexpr (!Q8) {
-          // one FMA per weight leaves the rounding error of the score, 2^-24 |ms|, in the exponent: nothing at ordinary
-          // sizes, but at very large ones the largest score itself has to come out as exactly 0
-          if (__any_sync(0xffffffffu, fabsf(ms) > 65536.f)) {
-#pragma unroll
-            for (int j = 0; j < KT; ++j) a[j] = __float_as_uint(__fadd_rn(__fmul_rn(__uint_as_float(a[j]), rf), -ms));
-          } else {
-            const f32x2 nb = pack_f2(-ms, -ms), rf2 = pack_f2(rf, rf);
-#pragma unroll
-            for (int j = 0; j < KT; j += 2) {
-              const float2 y = unpack_f2(fma2(pack_f2(__uint_as_float(a[j]), __uint_as_float(a[j + 1])), rf2, nb));
-              a[j] = __float_as_uint(y.x), a[j + 1] = __float_as_uint(y.y);
-            }
-          }
-          f32x2 s2 = pack_f2(0.f, 0.f);
-#pragma unroll
-          for (int j = 0; j < KT; j += 2) {
-            const float p0 = fast_exp2(__uint_as_float(a[j])), p1 = fast_exp2(__uint_as_float(a[j + 1]));
-            s2 = add2(s2, pack_f2(p0, p1));
-            pk[j / 2] = pack2<FMT>(p0, p1);
-          }
-          const float2 sv = unpack_f2(s2);
-          l += sv.x + sv.y;
-        } else if (!by_row) {
-          // the tile's V scale relative to er goes into the exponent, so l collects the same units and is brought
-          // back by the exact power of two; further below than 2^-64 no weight of the tile is left in f16
-          const int dd = max(em - er, -64);
-          const float nbs = (float)dd - ms, back = __int_as_float((127 - dd) << 23);
-          const float drop = em - er < -64 ? 0.f : 1.f;
-          const f32x2 nb = pack_f2(nbs, nbs);
-          const uint32_t fv = smem_u32(ct.fv[f]);
-          f32x2 s2 = pack_f2(0.f, 0.f);
-#pragma unroll
-          for (int j = 0; j < KT; j += 4) {
-            const uint4 v = lds128(fv + j * 4);
-            const float2 y0 = unpack_f2(add2(pack_f2(__uint_as_float(a[j]), __uint_as_float(a[j + 1])), nb));
-            const float2 y1 = unpack_f2(add2(pack_f2(__uint_as_float(a[j + 2]), __uint_as_float(a[j + 3])), nb));
-            const f32x2 e0 = pack_f2(fast_exp2(y0.x), fast_exp2(y0.y)), e1 = pack_f2(fast_exp2(y1.x), fast_exp2(y1.y));
-            s2 = add2(s2, add2(e0, e1));
-            const float2 w0 = unpack_f2(mul2(e0, pack_f2(__uint_as_float(v.x), __uint_as_float(v.y))));
-            const float2 w1 = unpack_f2(mul2(e1, pack_f2(__uint_as_float(v.z), __uint_as_float(v.w))));
-            pk[j / 2] = pack2<FMT>(w0.x, w0.y);
-            pk[j / 2 + 1] = pack2<FMT>(w1.x, w1.y);
-          }
-          if (drop == 0.f) {
-#pragma unroll
-            for (int j = 0; j < KT / 2; ++j) pk[j] = 0u;
-          }
-          const float2 sv = unpack_f2(s2);
-          l = fmaf(sv.x + sv.y, back, l);
-        } else {
-          float sum = 0.f;
-#pragma unroll
-          for (int j = 0; j < KT; j += 2) {
-            float w[2];
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-              const float e = fast_exp2(__uint_as_float(a[j + b]) - ms);
-              sum += e;
-              const int ev = ct.ev[f][j + b], d = ev - er + 127;
-              const float s = ev == 255 ? __int_as_float(0x7fffffff) : d <= 0 ? 0.f : __int_as_float(min(d, 254) << 23);
-              w[b] = see[(j + b) >> 5] >> ((j + b) & 31) & 1 ? e * s : 0.f;
-            }
-            pk[j / 2] = pack2<FMT>(w[0], w[1]);
-          }
-          l += sum;
-        }
-        tmem_st32(tS, pk);
+        tmem_st32(tP, a);
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(smem_u32(&ct.p_ready[x]));
       }
       if (!ok) break;
-      // ---- the piece's output
+      // ---- the next piece's Q goes out before this one's output: its first S runs under it
+      uint32_t v[D / 2];
+      if (!(ok = __all_sync(0xffffffffu, piece_wait(piece + 1)))) break;
+      const Piece& nxt = ct.piece[(piece + 1) % kPieces];
+      more = nxt.tiles != 0;
+      if (more) load_q(nxt, row_of(nxt), v);
       float(&ml)[2][3][128] = ct.ml[piece & 1];
       if (!two) {
         ml[x][0][r] = m;
         ml[x][1][r] = l;
-        ml[x][2][r] = begun ? (float)er : -1.f;                      // -1: the stream had no tile, its O is not there
+        ml[x][2][r] = begun ? (float)er : -1.f;                         // -1: the stream had no tile, its O is not there
         mbar_arrive(smem_u32(&ct.ml_ready));
         if (!(ok = warp_wait(&ct.ml_ready, n_ml++ & 1, abort_flag, g.spin))) break;
       }
+      if (more) rf = put_q(row_of(nxt), v);
       if (!(ok = warp_wait(&ct.o_done, piece & 1, abort_flag, g.spin))) break;
       tc_fence_after();
       float f0 = 1.f, f1 = 0.f, M = m, L = l, E = (float)er;
@@ -727,54 +808,59 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       float inv = L == 0.f ? 0.f : 1.f / L;                             // a row that sees nothing: zeros
       if constexpr (Q8) inv *= kHalfUnit<FMT> * __int_as_float((int)fmaxf(E, 1.f) << 23);
-      const bool join = !two && ml[1][2][r] >= 0.f;
-      const size_t at = (size_t)(p.bi.start + node) * g.n_heads + head;
-      const bool to_out = sc.chunk_tiles ? p.tiles <= sc.chunk_tiles : p.whole();
-      const size_t part = sc.chunk_tiles ? at * g.splits + p.t0 / sc.chunk_tiles
-                                         : ((size_t)blockIdx.x * 2 + (p.index ? 1 : 0)) * sc.rows + row;
+      const Row cw = row_of(cur);
+      const bool join = !two && nt > 1;
+      const size_t at = (size_t)(cur.bi.start + cw.node) * g.n_heads + cw.head;
+      const bool to_out = sc.chunk_tiles ? cur.tiles <= sc.chunk_tiles : cur.whole();
+      const size_t part = sc.chunk_tiles ? at * g.splits + cur.t0 / sc.chunk_tiles
+                                         : ((size_t)blockIdx.x * 2 + (cur.index ? 1 : 0)) * sc.rows + cw.row;
       // one row tile: each stream's threads write half of the columns
       const int d0 = two ? 0 : x * (D / 2), d1 = two ? D : d0 + D / 2;
       for (int d = d0; d < d1; d += 32) {
-        uint32_t o[32];
+        uint32_t o[32], o1[32];
         tmem_ld32(two ? tO + d : lanes + kColO + d, o);
+        if (join) tmem_ld32(lanes + kColO + 128 + d, o1);
         tmem_wait_ld();
-        float v[32];
+        float z[32];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(o[j]) * (f0 * inv);
-        if (!two && __any_sync(0xffffffffu, join)) {                    // the same for all rows: the tile count decides
-          tmem_ld32(lanes + kColO + 128 + d, o);
-          tmem_wait_ld();
+        for (int j = 0; j < 32; ++j) z[j] = __uint_as_float(o[j]) * (f0 * inv);
+        if (join) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = fmaf(__uint_as_float(o[j]), f1 * inv, v[j]);
+          for (int j = 0; j < 32; ++j) z[j] = fmaf(__uint_as_float(o1[j]), f1 * inv, z[j]);
         }
-        if (!Q8 && in && *reinterpret_cast<volatile int*>(&ct.dropped)) {     // the dropped elements of keys this row sees
-          const uint64_t* mk = g.mask ? g.mask + (size_t)(p.bi.start + node) * g.words : nullptr;
-          for (int key = max(p.t0 * KT, p.all_see); key < min(p.t1 * KT, p.n_keys); ++key)
-            if (sees32(mk, g.words, node, key - p.bi.ctx) & 1) {
-              const bf16* vp = static_cast<const bf16*>(c.v) + (cache_slot(c, p.bi.row, p.h, key)) * D + d;
+        if (!Q8 && cw.in && *reinterpret_cast<volatile int*>(&ct.dropped)) {   // the dropped elements of keys this row sees
+          const uint64_t* mk = g.mask ? g.mask + (size_t)(cur.bi.start + cw.node) * g.words : nullptr;
+          for (int key = max(cur.t0 * KT, cur.all_see); key < min(cur.t1 * KT, cur.n_keys); ++key)
+            if (sees32(mk, g.words, cw.node, key - cur.bi.ctx) & 1) {
+              const bf16* vp = static_cast<const bf16*>(c.v) + (cache_slot(c, cur.bi.row, cur.h, key)) * D + d;
 #pragma unroll
               for (int j = 0; j < 32; ++j) {
                 const float y = __bfloat162float(vp[j]);
-                if (!(fabsf(y) < INFINITY)) v[j] += y;
+                if (!(fabsf(y) < INFINITY)) z[j] += y;
               }
             }
         }
-        if (in && to_out) {
+        if (cw.in && to_out) {
 #pragma unroll
           for (int j = 0; j < 32; j += 8)
             *reinterpret_cast<uint4*>(out + at * D + d + j) =
-                make_uint4(pack2<EESD_KV_MODEL>(v[j], v[j + 1]), pack2<EESD_KV_MODEL>(v[j + 2], v[j + 3]),
-                           pack2<EESD_KV_MODEL>(v[j + 4], v[j + 5]), pack2<EESD_KV_MODEL>(v[j + 6], v[j + 7]));
-        } else if (in) {
+                make_uint4(pack2<EESD_KV_MODEL>(z[j], z[j + 1]), pack2<EESD_KV_MODEL>(z[j + 2], z[j + 3]),
+                           pack2<EESD_KV_MODEL>(z[j + 4], z[j + 5]), pack2<EESD_KV_MODEL>(z[j + 6], z[j + 7]));
+        } else if (cw.in) {
 #pragma unroll
           for (int j = 0; j < 32; j += 4)
-            *reinterpret_cast<float4*>(g.part_o + part * D + d + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+            *reinterpret_cast<float4*>(g.part_o + part * D + d + j) = make_float4(z[j], z[j + 1], z[j + 2], z[j + 3]);
         }
         __syncwarp();
       }
-      if (in && !to_out && (two || x == 0)) g.part_ml[part] = make_float2(M, L);
-      if (tid == 128 && !sc.chunk_tiles && p.t0 == 0 && p.t1 < p.tiles) sc.cuts[blockIdx.x] = TcCut{p.u0, it.e, p.h, p.index ? 1 : 0, p.tiles};
+      tc_fence_before();
+      mbar_arrive(smem_u32(&ct.epi_done));
+      if (cw.in && !to_out && (two || x == 0)) g.part_ml[part] = make_float2(M, L);
+      if (tid == 128 && !sc.chunk_tiles && cur.t0 == 0 && cur.t1 < cur.tiles)
+        sc.cuts[blockIdx.x] = TcCut{cur.u0, cur.e, cur.h, cur.index ? 1 : 0, cur.tiles};
       cnt0 += nt;
+      __syncwarp();
+      if (lane == 0) piece_free(piece);
       ++piece;
     }
     if (!ok) {
@@ -788,8 +874,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 1) tmem_dealloc(tmem, 512);
 }
 
-// Joins the pieces of the unit that goes from run blockIdx.x on into the next ones, in run order.  A warp takes
-// every 8th row of its group of 32.
+// Joins the pieces of the unit that goes from run blockIdx.x on into the next ones, in run order.  One warp per row.
 template <int D>
 __global__ void __launch_bounds__(256) attn_tree_tc_join_kernel(TreeGeom g, CacheGeom c, TcSchedule sc, bf16* __restrict__ out) {
   pdl_trigger();
@@ -804,41 +889,49 @@ __global__ void __launch_bounds__(256) attn_tree_tc_join_kernel(TreeGeom g, Cach
   const int c1 = (int)(((cut.u0 + kUnitCost + cut.tiles) * n - 1) / W);
   auto slot = [&](int k, int row) { return ((size_t)k * 2 + (k == c0 ? cut.second : 0)) * sc.rows + row; };
   auto empty = [&](int k) { return k * W / n == (k + 1) * W / n; };     // a run of no position writes nothing
-  for (int row = blockIdx.y * 32 + (threadIdx.x >> 5); row < min(x.nrows, (int)blockIdx.y * 32 + 32); row += 8) {
-    const int R = x.r0 + row, node = R / g.G;
-    float M = -INFINITY;
-    for (int k = c0 + lane; k <= c1; k += 32)
-      if (!empty(k)) M = fmaxf(M, g.part_ml[slot(k, row)].x);
+  const int row = blockIdx.y * 8 + (threadIdx.x >> 5);
+  if (row >= x.nrows) return;
+  const int R = x.r0 + row, node = R / g.G;
+  float M = -INFINITY;
+  for (int k = c0 + lane; k <= c1; k += 32)
+    if (!empty(k)) M = fmaxf(M, g.part_ml[slot(k, row)].x);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    const float ms = M == -INFINITY ? 0.f : M;
-    constexpr int E = D / 32;
-    float L = 0.f, acc[E];
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  const float ms = M == -INFINITY ? 0.f : M;
+  constexpr int E = D / 32;
+  float L = 0.f, acc[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    for (int k0 = c0; k0 <= c1; k0 += 32) {
-      float w = 0.f;
-      if (k0 + lane <= c1 && !empty(k0 + lane)) {
-        const float2 v = g.part_ml[slot(k0 + lane, row)];
-        w = v.y * fast_exp2(v.x - ms);
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  for (int k0 = c0; k0 <= c1; k0 += 32) {
+    float w = 0.f;
+    if (k0 + lane <= c1 && !empty(k0 + lane)) {
+      const float2 v = g.part_ml[slot(k0 + lane, row)];
+      w = v.y * fast_exp2(v.x - ms);
+    }
+    const int cnt = min(32, c1 - k0 + 1);
+    for (int kb = 0; kb < cnt; kb += 8) {                               // eight loads in flight
+      float v[8][E];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float* src = g.part_o + slot(min(k0 + kb + u, c1), row) * D + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[u][e] = src[e];
       }
-      const int cnt = min(32, c1 - k0 + 1);
-#pragma unroll 4
-      for (int k = 0; k < cnt; ++k) {
-        const float wk = __shfl_sync(0xffffffffu, w, k);
-        if (wk != 0.f) {
-          L += wk;
-          const float* src = g.part_o + slot(k0 + k, row) * D + lane * E;
 #pragma unroll
-          for (int e = 0; e < E; ++e) acc[e] = fmaf(wk, src[e], acc[e]);
+      for (int u = 0; u < 8; ++u) {
+        const float wk = kb + u < 32 ? __shfl_sync(0xffffffffu, w, (kb + u) & 31) : 0.f;
+        if (kb + u < cnt && wk != 0.f) {                                // what an empty run left there is not read
+          L += wk;
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[e] = fmaf(wk, v[u][e], acc[e]);
         }
       }
     }
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    bf16* dst = out + ((size_t)(x.bi.start + node) * g.n_heads + cut.h * g.G + R % g.G) * D + lane * E;
-#pragma unroll
-    for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack2<EESD_KV_MODEL>(acc[e] * inv, acc[e + 1] * inv);
   }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  bf16* dst = out + ((size_t)(x.bi.start + node) * g.n_heads + cut.h * g.G + R % g.G) * D + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack2<EESD_KV_MODEL>(acc[e] * inv, acc[e + 1] * inv);
 }
 
 template <int D, int FMT>
@@ -850,7 +943,7 @@ cudaError_t launch(const TcSchedule& sc, const TreeGeom& g, const CacheGeom& c, 
   if (e != cudaSuccess) return e;
   e = launch_pdl(kernel, dim3(sc.ctas), dim3(kThreads), S::smem, s, km, vm, g, c, sc, static_cast<const bf16*>(q), static_cast<bf16*>(out));
   if (e == cudaSuccess && !sc.chunk_tiles && sc.ctas > 1)
-    e = launch_pdl(attn_tree_tc_join_kernel<D>, dim3(sc.ctas, (std::min(sc.rows, g.max_nodes * g.G) + 31) / 32), dim3(256), 0, s, g, c, sc,
+    e = launch_pdl(attn_tree_tc_join_kernel<D>, dim3(sc.ctas, (std::min(sc.rows, g.max_nodes * g.G) + 7) / 8), dim3(256), 0, s, g, c, sc,
                    static_cast<bf16*>(out));
   return e;
 }
