@@ -12,11 +12,15 @@
 // computed while its softmax still works on this one: with more than 128 rows each stream is one half of the rows
 // over all key tiles; with fewer, both share the rows and take every other key tile, and meet at the end.
 //
-// 8-bit caches: a warpgroup turns the TMA-loaded bytes into the f16 tiles that the products read (exactly; the
-// powers of two stay out of the operands and multiply scores and weights instead).
+// 8-bit caches: a warpgroup turns the TMA-loaded bytes into the f16 tiles that the products read, each key's power of
+// two relative to the tile's largest multiplied in (exact, as f16 goes, while they are within 2^21, e4m3, or 2^22, int8;
+// keys further below than 2^28 or 2^22 count as zeros), so the softmax sees one scale per tile.  In tiles that some row
+// does not wholly see a key's scale stays out of the operands and multiplies scores and weights instead: what
+// a row does not see must not decide its precision.
 //
-// Roles of the 16 warps: 0 TMA, 1 MMA issue, 4-7 and 8-11 softmax of stream 0 and 1 (a thread is a row), 12-15
-// conversion (8-bit) or the check of V tiles that some row does not wholly see (bf16).
+// Roles of the 16 warps: 0 TMA, 1 and 3 MMA issue of stream 0 and 1 (a satisfied barrier wait costs some 150 clocks,
+// and each tile takes four of them), 2 the schedule, 4-7 and 8-11 softmax of stream 0 and 1 (a thread is a row),
+// 12-15 conversion (8-bit) or the check of V tiles that some row does not wholly see (bf16).
 #include <algorithm>
 
 #include "attn_tree.h"
@@ -63,6 +67,18 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
       : EESD_R8(r, 0), EESD_R8(r, 8), EESD_R8(r, 16), EESD_R8(r, 24)
       : "r"(taddr));
 }
+__device__ __forceinline__ void tmem_ld_16(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : EESD_R8(r, 0), EESD_R8(r, 8)
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st_16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::EESD_W8(r, 0), EESD_W8(r, 8),
+      "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,"
@@ -73,9 +89,26 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// mbar_wait that suspends the thread for up to 2 us per poll: most of the 16 warps wait most of the time, and polling
+// would take the issue slots of those that do not.
+__device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t limit) {
+  for (uint32_t i = 0; i < limit; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred P;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2, %3;\n\t"
+        "selp.b32 %0, 1, 0, P;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(2000u)
+        : "memory");
+    if (ok) return true;
+    if ((i & 255u) == 255u && *abort_flag) return false;
+  }
+  return false;
+}
 // The whole warp waits and goes on together (what follows are warp-wide instructions).
 __device__ __forceinline__ bool warp_wait(const void* bar, uint32_t parity, volatile int* abort_flag, uint32_t limit) {
-  return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, abort_flag, limit));
+  return __all_sync(0xffffffffu, wait_on(smem_u32(bar), parity, abort_flag, limit));
 }
 template <int N> __device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -200,23 +233,26 @@ template <int D, int FMT> struct TcShape {
   static constexpr int NS = Q8 ? 2 : 5;                // 16-bit K / V stages
   static constexpr int RS = Q8 ? 6 : 0;                // raw stages
   static constexpr int FR = 8;                         // factor ring: six tiles can be between conversion and softmax
+  static constexpr int kUp = FMT == EESD_KV_E4M3 ? 14 : 8;   // a tile's largest 8-bit elements go up to 2^15 in f16
   static constexpr int QB = 128 * D * 2;               // Q of stream 1 (more than 128 rows)
   static constexpr size_t ctl = 16384;
   static constexpr size_t smem = 1024 + (size_t)2 * NS * TILE + (size_t)RS * RAW + QB + ctl;
 };
 constexpr int kPieces = 4;                 // pieces between the schedule warp and the slowest role
-constexpr int kReaders = 14;               // warps that read them: TMA, MMA, 8 softmax, 4 conversion
+constexpr int kReaders = 15;               // warps that read them: TMA, 2 MMA, 8 softmax, 4 conversion
 struct TcControl {
   uint64_t kfull[5], kempty[5], vfull[5], vempty[5], vclean[5], raw_full[6], raw_empty[6], ffull[8];
   uint64_t piece_full[kPieces], piece_empty[kPieces];
   Piece piece[kPieces];                    // tiles == 0: there are no more
-  uint64_t s_full[2], s_free[2], p_ready[2], pv_done[2], q_ready, o_done, ml_ready, epi_done, drain;
-  alignas(16) float fk[8][KT];             // 8-bit: 2^ek of a tile's keys
-  alignas(16) float fv[8][KT];             // 2^(ev - ref), 0 for NaN and slots past the end
+  uint64_t s_full[2], s_free[2], p_ready[2], pv_done[2], q_ready, o_done, ml_ready, epi_done, drain[2];
+  // 8-bit, per tile: 2^ek and 2^(ev - ref) of its keys where some row does not wholly see it (0 for NaN and slots past
+  // the end), else one factor for K, kt; ref is the exponent byte that V is relative to
+  alignas(16) float fk[8][KT];
+  alignas(16) float fv[8][KT];
+  float kt[8];
   alignas(16) uint8_t ev[8][KT];           // V's exponent bytes, 0 likewise
   alignas(16) uint8_t exps[6][2 * KT];     // raw exponent bytes, K then V
-  alignas(16) float zeros[KT];
-  int ref[8];                              // the exponent byte that fv is relative to
+  int ref[8];
   uint32_t nan[8][2];                      // keys whose V is NaN
   float ml[2][2][3][128];                  // one row tile: max, sum and eref of the streams (by piece parity)
   long long lo, hi, base;
@@ -266,8 +302,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = 0; i < NS; ++i) {
         mbar_init(smem_u32(&ct.kfull[i]), Q8 ? 128 : 1);
         mbar_init(smem_u32(&ct.vfull[i]), Q8 ? 128 : 1);
-        mbar_init(smem_u32(&ct.kempty[i]), 1);
-        mbar_init(smem_u32(&ct.vempty[i]), 1);
+        mbar_init(smem_u32(&ct.kempty[i]), 2);
+        mbar_init(smem_u32(&ct.vempty[i]), 2);
         mbar_init(smem_u32(&ct.vclean[i]), 128);
       }
       for (int i = 0; i < RS; ++i) {
@@ -288,11 +324,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(smem_u32(&ct.q_ready), 256);
       mbar_init(smem_u32(&ct.ml_ready), 256);
       mbar_init(smem_u32(&ct.epi_done), 256);
-      mbar_init(smem_u32(&ct.o_done), 1);
-      mbar_init(smem_u32(&ct.drain), 1);
+      mbar_init(smem_u32(&ct.o_done), 2);
+      mbar_init(smem_u32(&ct.drain[0]), 1);
+      mbar_init(smem_u32(&ct.drain[1]), 1);
       fence_mbar_init();
     }
-    if (tid < KT) ct.zeros[tid] = 0.f;
     if (warp == 1) {
       tmem_alloc(smem_u32(&ct.tmem), 512);
       tmem_relinquish();
@@ -329,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
   }
   // Every role reads its pieces, in order, from the ring that warp 2 fills.
-  auto piece_wait = [&](int k) { return mbar_wait(smem_u32(&ct.piece_full[k % kPieces]), k / kPieces & 1, abort_flag, g.spin); };
+  auto piece_wait = [&](int k) { return wait_on(smem_u32(&ct.piece_full[k % kPieces]), k / kPieces & 1, abort_flag, g.spin); };
   auto piece_free = [&](int k) { mbar_arrive(smem_u32(&ct.piece_empty[k % kPieces])); };
   const uint32_t tmem = ct.tmem;
 
@@ -348,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int t = p.t0; t < p.t1; ++t, ++cnt) {
           if constexpr (Q8) {
             const int s = cnt % RS;
-            if (!(ok = mbar_wait(smem_u32(&ct.raw_empty[s]), (cnt / RS & 1) ^ 1, abort_flag, g.spin))) break;
+            if (!(ok = wait_on(smem_u32(&ct.raw_empty[s]), (cnt / RS & 1) ^ 1, abort_flag, g.spin))) break;
             const uint32_t fb = smem_u32(&ct.raw_full[s]), dst = raw + s * S::RAW, ex = smem_u32(ct.exps[s]);
             const uint32_t eb = min(KT, c.max_seq - t * KT);          // max_seq % 16 == 0
             mbar_arrive_expect_tx(fb, S::RAW + 2 * eb);
@@ -360,12 +396,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           } else {
             const int s = cnt % NS;
             const uint32_t ph = (cnt / NS & 1) ^ 1;
-            if (!(ok = mbar_wait(smem_u32(&ct.kempty[s]), ph, abort_flag, g.spin))) break;
+            if (!(ok = wait_on(smem_u32(&ct.kempty[s]), ph, abort_flag, g.spin))) break;
             const uint32_t kb = smem_u32(&ct.kfull[s]), vb = smem_u32(&ct.vfull[s]);
             mbar_arrive_expect_tx(kb, S::TILE);
             for (int h = 0; h < HALVES; ++h) tma_load_2d(kbuf + s * S::TILE + h * KT * 128, &kmap, h * 64, slot0 + t * KT, kb);
             k_issued = cnt + 1;
-            if (!(ok = mbar_wait(smem_u32(&ct.vempty[s]), ph, abort_flag, g.spin))) break;
+            if (!(ok = wait_on(smem_u32(&ct.vempty[s]), ph, abort_flag, g.spin))) break;
             mbar_arrive_expect_tx(vb, S::TILE);
             for (int h = 0; h < HALVES; ++h) tma_load_2d(vbuf + s * S::TILE + h * KT * 128, &vmap, h * 64, slot0 + t * KT, vb);
             v_issued = cnt + 1;
@@ -386,58 +422,60 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = max(0, v_issued - NS); i < v_issued; ++i) mbar_drain(smem_u32(&ct.vfull[i % NS]), (i / NS) & 1);
       }
     }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issue
+  } else if (warp == 1 || warp == 3) {
+    // ------------------------------------------------------------ MMA issue of stream x
     if (elect_one()) {
+      const int x = warp >> 1;
       const uint32_t id_qk = idesc_f32<FMT>(KT, false), id_pv = idesc_f32<FMT>(D, true);
-      int cnt0 = 0, piece = 0, n_q[2] = {0, 0}, n_p[2] = {0, 0};
+      const uint32_t dS = tmem + kColS + x * kSP, dO = tmem + kColO + x * 128, aP = tmem + kColP + x * kSP;
+      int cnt0 = 0, piece = 0, n_q = 0, n_p = 0;
       bool ok = true, issued = false;
       for (; (ok = piece_wait(piece)); ++piece) {
         const Piece& p = ct.piece[piece % kPieces];
         if (p.tiles == 0) break;
         const int nt = p.t1 - p.t0;
         const bool two = p.nrows > 128;
-        const int steps = two ? 2 * nt : nt;
-        if (!(ok = mbar_wait(smem_u32(&ct.q_ready), piece & 1, abort_flag, g.spin))) break;
-        // S of step s as soon as its stream has taken S of step s - 2 into registers, then O of that step when its
-        // softmax ends.  (A longer lead would need a third converted V tile: conversion goes K, V, K, V.)
-        for (int s = 0; s < steps + 2; ++s) {
-          if (s < steps) {
-            const int x = s & 1, cnt = cnt0 + (two ? s >> 1 : s), st = cnt % NS;
-            if (n_q[x] && !(ok = mbar_wait(smem_u32(&ct.s_free[x]), (n_q[x] - 1) & 1, abort_flag, g.spin))) break;
-            ++n_q[x];
-            if ((!two || x == 0) && !(ok = mbar_wait(smem_u32(&ct.kfull[st]), cnt / NS & 1, abort_flag, g.spin))) break;
+        const int step = two ? 1 : 2, t0 = two ? 0 : x;
+        // with one row tile a key tile has this stream only: it frees the stage for both
+        auto free_stage = [&](uint64_t* bar) {
+          tc_commit(smem_u32(bar));
+          if (!two) tc_commit(smem_u32(bar));
+        };
+        if (!(ok = wait_on(smem_u32(&ct.q_ready), piece & 1, abort_flag, g.spin))) break;
+        // S of the stream's next tile as soon as the last one is in registers, then O of the last one when its softmax ends
+        for (int i = t0 - step; i < nt; i += step) {
+          const int j = i + step;
+          if (j < nt) {
+            const int cnt = cnt0 + j, st = cnt % NS;
+            if (n_q && !(ok = wait_on(smem_u32(&ct.s_free[x]), (n_q - 1) & 1, abort_flag, g.spin))) break;
+            ++n_q;
+            if (!(ok = wait_on(smem_u32(&ct.kfull[st]), cnt / NS & 1, abort_flag, g.spin))) break;
             tc_fence_after();
             issued = true;
             const uint64_t kd = sw128_kmajor_desc(kbuf + st * S::TILE);
-            const uint32_t d = tmem + kColS + x * kSP;
             if (two && x == 1) {
               const uint64_t qd = sw128_kmajor_desc(qbuf);
 #pragma unroll
               for (int kk = 0; kk < D / 16; ++kk)
-                tc_mma_f16(d, qd + (kk >> 2) * (128 * 128 >> 4) + (kk & 3) * 2, kd + (kk >> 2) * (KT * 128 >> 4) + (kk & 3) * 2, id_qk, kk > 0);
+                tc_mma_f16(dS, qd + (kk >> 2) * (128 * 128 >> 4) + (kk & 3) * 2, kd + (kk >> 2) * (KT * 128 >> 4) + (kk & 3) * 2, id_qk, kk > 0);
             } else {
 #pragma unroll
               for (int kk = 0; kk < D / 16; ++kk)
-                tc_mma_ts(d, tmem + kColQ + kk * 8, kd + (kk >> 2) * (KT * 128 >> 4) + (kk & 3) * 2, id_qk, kk > 0);
+                tc_mma_ts(dS, tmem + kColQ + kk * 8, kd + (kk >> 2) * (KT * 128 >> 4) + (kk & 3) * 2, id_qk, kk > 0);
             }
-            if (!two || x == 1) tc_commit(smem_u32(&ct.kempty[st]));
             tc_commit(smem_u32(&ct.s_full[x]));
+            free_stage(&ct.kempty[st]);
           }
-          if (s >= 2) {
-            const int u = s - 2, x = u & 1, i = two ? u >> 1 : u, cnt = cnt0 + i, st = cnt % NS;
-            if (!(ok = mbar_wait(smem_u32(&ct.p_ready[x]), n_p[x]++ & 1, abort_flag, g.spin))) break;
-            if ((!two || x == 0) &&
-                !(ok = mbar_wait(smem_u32(Q8 ? &ct.vfull[st] : &ct.vclean[st]), cnt / NS & 1, abort_flag, g.spin)))
-              break;
+          if (i >= 0) {
+            const int cnt = cnt0 + i, st = cnt % NS;
+            if (!(ok = wait_on(smem_u32(Q8 ? &ct.vfull[st] : &ct.vclean[st]), cnt / NS & 1, abort_flag, g.spin))) break;
+            if (!(ok = wait_on(smem_u32(&ct.p_ready[x]), n_p++ & 1, abort_flag, g.spin))) break;
             tc_fence_after();
             const uint64_t vd = sw128_mnmajor_desc(vbuf + st * S::TILE, KT * 128);
-            const bool first = two ? i == 0 : u < 2;
 #pragma unroll
-            for (int kk = 0; kk < KT / 16; ++kk)
-              tc_mma_ts(tmem + kColO + x * 128, tmem + kColP + x * kSP + kk * 8, vd + kk * (16 * 128 >> 4), id_pv, !(first && kk == 0));
-            if (!two || x == 1) tc_commit(smem_u32(&ct.vempty[st]));
+            for (int kk = 0; kk < KT / 16; ++kk) tc_mma_ts(dO, aP + kk * 8, vd + kk * (16 * 128 >> 4), id_pv, i != t0 || kk > 0);
             tc_commit(smem_u32(&ct.pv_done[x]));
+            free_stage(&ct.vempty[st]);
           }
         }
         if (!ok) break;
@@ -450,8 +488,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         *abort_flag = 1;
       }
       if (issued) {                                                     // no product may be in flight at the end
-        tc_commit(smem_u32(&ct.drain));
-        mbar_drain(smem_u32(&ct.drain), 0);
+        tc_commit(smem_u32(&ct.drain[x]));
+        mbar_drain(smem_u32(&ct.drain[x]), 0);
       }
     }
   } else if (warp == 2) {
@@ -462,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       Piece p;
       for (int k = 0;; ++k) {
-        if (!(ok = mbar_wait(smem_u32(&ct.piece_empty[k % kPieces]), (k / kPieces & 1) ^ 1, abort_flag, g.spin))) break;
+        if (!(ok = wait_on(smem_u32(&ct.piece_empty[k % kPieces]), (k / kPieces & 1) ^ 1, abort_flag, g.spin))) break;
         const bool more = it.next(g, c, sc, p);
         if (!more) p.tiles = 0;
         ct.piece[k % kPieces] = p;
@@ -478,30 +516,44 @@ __global__ void __launch_bounds__(kThreads, 1)
     reg_dec<56>();
     // ------------------------------------------------------------ conversion, or the check of V tiles
     const int ti = tid - 384;
-    [[maybe_unused]] auto convert = [&](const uint8_t* src, uint8_t* dst) {
-      constexpr int C = D / 16;                                         // 16-byte chunks of a raw row
+    // The raw tile's bytes as f16, row r times 2^(e_r - top) (none below 2^-14; byte 255, a NaN, comes out as one);
+    // top = 0: all rows times 2^flat.  A thread has one 16-byte chunk of every 16th (D = 64: 32nd) row; the 8 lanes of a
+    // phase are on 8 rows and one chunk, conflict-free in both swizzles.
+    constexpr int kChunks = D / 16, kRowStep = 128 / kChunks;
+    const uint32_t ch = (uint32_t)ti / 8 % kChunks, row0 = (uint32_t)ti / (8 * kChunks) * 8 + (ti & 7);
+    const uint32_t from = row0 * D + ((D == 128 ? ch ^ (row0 & 7) : ch ^ (row0 >> 1 & 3)) << 4);
+    const uint32_t to0 = (ch >> 2) * (KT * 128) + row0 * 128 + ((2 * ch & 7 ^ (row0 & 7)) << 4), to1 = to0 ^ 16;
+    [[maybe_unused]] auto convert = [&](const uint8_t* src, uint8_t* dst, const uint8_t* e, int top, int flat) {
 #pragma unroll
-      for (int i = 0; i < KT * C / 128; ++i) {
-        // 8 lanes of a phase on 8 rows and one chunk: conflict-free in both swizzles
-        const int idx = i * 128 + ti, j = idx >> 3, ch = j % C, row = j / C * 8 + (idx & 7);
-        const uint4 w = *reinterpret_cast<const uint4*>(src + row * D + ((D == 128 ? ch ^ (row & 7) : ch ^ ((row >> 1) & 3)) << 4));
+      for (int i = 0; i < KT / kRowStep; ++i) {
+        const uint4 w = *reinterpret_cast<const uint4*>(src + from + i * (kRowStep * D));
         uint4 a, b;
         unpack4<FMT>(w.x, a.x, a.y);
         unpack4<FMT>(w.y, a.z, a.w);
         unpack4<FMT>(w.z, b.x, b.y);
         unpack4<FMT>(w.w, b.z, b.w);
-        uint8_t* to = dst + (ch >> 2) * (KT * 128) + row * 128;
-        const int c0 = 2 * ch & 7;
-        *reinterpret_cast<uint4*>(to + ((c0 ^ (row & 7)) << 4)) = a;
-        *reinterpret_cast<uint4*>(to + (((c0 + 1) ^ (row & 7)) << 4)) = b;
+        const int er = e[row0 + i * kRowStep];
+        const uint32_t h = top == 0 ? (uint32_t)(flat + 15) << 10 : er == 255 ? 0x7fffu : (uint32_t)max(er - top + 15, 0) << 10;
+        const uint32_t hh = __byte_perm(h, 0, 0x1010);
+        const __half2 m = *reinterpret_cast<const __half2*>(&hh);
+        __half2* v = reinterpret_cast<__half2*>(&a);
+        __half2* u = reinterpret_cast<__half2*>(&b);
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          v[y] = __hmul2(v[y], m);
+          u[y] = __hmul2(u[y], m);
+        }
+        *reinterpret_cast<uint4*>(dst + to0 + i * (kRowStep * 128)) = a;
+        *reinterpret_cast<uint4*>(dst + to1 + i * (kRowStep * 128)) = b;
       }
       fence_proxy_async_smem();
     };
     // V of a tile waits for the product two tiles before it, K does not: K goes one tile ahead
+    int v_top = 0;                                                      // of the tile whose V is still to be converted
     [[maybe_unused]] auto convert_v = [&](int cnt) {
       const int st = cnt % NS, rs = cnt % RS;
       if (!warp_wait(&ct.vempty[st], (cnt / NS & 1) ^ 1, abort_flag, g.spin)) return false;
-      convert(sm + 2 * NS * S::TILE + rs * S::RAW + S::RAW / 2, sm + (NS + st) * S::TILE);
+      convert(sm + 2 * NS * S::TILE + rs * S::RAW + S::RAW / 2, sm + (NS + st) * S::TILE, ct.exps[rs] + KT, v_top, TcShape<D, FMT>::kUp);
       mbar_arrive(smem_u32(&ct.vfull[st]));
       mbar_arrive(smem_u32(&ct.raw_empty[rs]));
       return true;
@@ -516,29 +568,41 @@ __global__ void __launch_bounds__(kThreads, 1)
         if constexpr (Q8) {
           const int rs = cnt % RS, f = cnt % FR;
           if (!(ok = warp_wait(&ct.raw_full[rs], cnt / RS & 1, abort_flag, g.spin))) break;
-          // factors of the tile's keys (the ring slot's last reader is behind the product that freed this K stage).
-          // V's are relative to the largest exponent; in a tile that some row does not wholly see to 2^60 below it,
-          // so that they last for rows whose own largest is far smaller
-          const uint32_t vpair = *reinterpret_cast<const uint16_t*>(&ct.exps[rs][KT + 2 * lane]);
-          const int left = p.n_keys - t * KT, a0 = vpair & 255, a1 = vpair >> 8;
-          const int em = __reduce_max_sync(0xffffffffu, max(2 * lane < left && a0 != 255 ? a0 : 0, 2 * lane + 1 < left && a1 != 255 ? a1 : 0));
-          const int ref = em - ((t + 1) * KT > min(p.all_see, p.n_keys) ? 60 : 0);
+          const bool partial = (t + 1) * KT > min(p.all_see, p.n_keys);
+          const int left = p.n_keys - t * KT;
+          // the tile's largest exponents (of slots before its end, NaN apart)
+          auto top_of = [&](const uint8_t* e) {
+            const uint32_t v = *reinterpret_cast<const uint16_t*>(e + 2 * lane);
+            const int a0 = v & 255, a1 = v >> 8;
+            return __reduce_max_sync(0xffffffffu, max(2 * lane < left && a0 != 255 ? a0 : 0, 2 * lane + 1 < left && a1 != 255 ? a1 : 0));
+          };
+          const int ek = top_of(ct.exps[rs]), ev = top_of(ct.exps[rs] + KT);
+          // V's factors in a tile that some row does not wholly see are relative to 2^60 below the largest, so that they
+          // last for rows whose own largest is far smaller
+          const int k_top = partial ? 0 : max(ek, 27) - S::kUp, next_v_top = partial ? 0 : max(ev, 27) - S::kUp, ref = partial ? ev - 60 : ev;
           if (!(ok = warp_wait(&ct.kempty[st], (cnt / NS & 1) ^ 1, abort_flag, g.spin))) break;
-          if (ti < KT) {
-            ct.fk[f][ti] = exp_scale(ct.exps[rs][ti]);
-            if (ti == 0) ct.ref[f] = ref;
-          } else {
-            const int ev = ct.exps[rs][ti], d = ev - ref + 127;
-            const bool nan = ev == 255, in = ti - KT < left;
-            ct.ev[f][ti - KT] = nan || !in ? 0 : (uint8_t)ev;
-            ct.fv[f][ti - KT] = nan || !in || d <= 0 ? 0.f : __int_as_float(d << 23);
-            const uint32_t nans = __ballot_sync(0xffffffffu, nan && in);
-            if (lane == 0) ct.nan[f][(ti - KT) >> 5] = nans;
+          if (ti == 0) {
+            ct.ref[f] = ref;
+            ct.kt[f] = __int_as_float(max(k_top, 1) << 23);
+          }
+          if (partial) {
+            // (the ring slot's last reader is behind the product that freed this K stage)
+            if (ti < KT) {
+              ct.fk[f][ti] = exp_scale(ct.exps[rs][ti]);
+            } else {
+              const int e = ct.exps[rs][ti], d = e - ref + 127;
+              const bool nan = e == 255, in = ti - KT < left;
+              ct.ev[f][ti - KT] = nan || !in ? 0 : (uint8_t)e;
+              ct.fv[f][ti - KT] = nan || !in || d <= 0 ? 0.f : __int_as_float(d << 23);
+              const uint32_t nans = __ballot_sync(0xffffffffu, nan && in);
+              if (lane == 0) ct.nan[f][(ti - KT) >> 5] = nans;
+            }
           }
           mbar_arrive(smem_u32(&ct.ffull[f]));
-          convert(sm + 2 * NS * S::TILE + rs * S::RAW, sm + st * S::TILE);
+          convert(sm + 2 * NS * S::TILE + rs * S::RAW, sm + st * S::TILE, ct.exps[rs], k_top, 0);
           mbar_arrive(smem_u32(&ct.kfull[st]));
           if (cnt && !(ok = convert_v(cnt - 1))) break;
+          v_top = next_v_top;
         } else {
           if (!(ok = warp_wait(&ct.vfull[st], cnt / NS & 1, abort_flag, g.spin))) break;
           if ((t + 1) * KT > min(p.all_see, p.n_keys)) {
@@ -658,27 +722,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
         mbar_arrive(smem_u32(&ct.s_free[x]));
         // ---- scores in the log2 domain and their maximum
-        if constexpr (Q8) {
+        const bool partial = (t + 1) * KT > min(cur.all_see, cur.n_keys);   // some row does not see some key of the tile
+        int ref = 0, em = 0;
+        if constexpr (Q8) em = ref = ct.ref[f];
+        if (!Q8 || !partial) {
+          const float rt = Q8 ? rf * ct.kt[f] : rf;
+          const f32x2 rt2 = pack_f2(rt, rt);
+#pragma unroll
+          for (int j = 0; j < KT; j += 2) scale2(a[j], a[j + 1], rt2);
+        } else {
           const float4* fk = reinterpret_cast<const float4*>(ct.fk[f]);
-          const f32x2 rf2 = pack_f2(rf, rf);
 #pragma unroll
           for (int j = 0; j < KT; j += 4) {
             const float4 v = fk[j / 4];
-            scale2(a[j], a[j + 1], mul2(rf2, pack_f2(v.x, v.y)));
-            scale2(a[j + 2], a[j + 3], mul2(rf2, pack_f2(v.z, v.w)));
+            scale2(a[j], a[j + 1], pack_f2(rf * v.x, rf * v.y));
+            scale2(a[j + 2], a[j + 3], pack_f2(rf * v.z, rf * v.w));
           }
-        } else {
-          const f32x2 rf2 = pack_f2(rf, rf);
-#pragma unroll
-          for (int j = 0; j < KT; j += 2) scale2(a[j], a[j + 1], rf2);
         }
-        int ref = 0, em = 0;
-        uint32_t nan = 0;
-        if constexpr (Q8) {
-          em = ref = ct.ref[f];
-          nan = ct.nan[f][0] | ct.nan[f][1];
-        }
-        if ((t + 1) * KT > min(cur.all_see, cur.n_keys)) {              // some row does not see some key of the tile
+        if (partial) {
           const int node = row_of(cur).node, left = cur.n_keys - t * KT;
           const uint64_t* mk = g.mask ? g.mask + (size_t)(cur.bi.start + node) * g.words : nullptr;
           uint32_t s0 = sees32(mk, g.words, node, t * KT - cur.bi.ctx), s1 = sees32(mk, g.words, node, t * KT + 32 - cur.bi.ctx);
@@ -695,10 +756,9 @@ __global__ void __launch_bounds__(kThreads, 1)
               top = __vmaxu4(top, reinterpret_cast<const uint32_t*>(ct.ev[f])[j] & ((bits * 0x204081u & 0x1010101u) * 255u));
             }
             em = max(max(top & 255, top >> 8 & 255), max(top >> 16 & 255, top >> 24));
-            nan = (ct.nan[f][0] & s0) | (ct.nan[f][1] & s1);
+            if ((ct.nan[f][0] & s0) | (ct.nan[f][1] & s1)) l = __int_as_float(0x7fffffff);   // the row sees a V that is NaN
           }
         }
-        if (Q8 && nan) l = __int_as_float(0x7fffffff);                  // the row sees a V that is NaN
         float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
         for (int j = 0; j < KT; j += 4) {
@@ -725,7 +785,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         // in f16.
         const bool gone = Q8 && em - er < -40;
         const int dd = Q8 && !gone ? min(ref - er, 100) : 0;
-        const float4* fv = reinterpret_cast<const float4*>(gone ? ct.zeros : ct.fv[f]);
         // The packed product and sum may be contracted to one FMA, which leaves 2^-24 |m| of the score in the exponent:
         // nothing at ordinary sizes, but at very large ones the largest score has to come out as exactly 0.
         float nbs = (float)dd - ms;
@@ -743,14 +802,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           f32x2 e0 = pack_f2(fast_exp2(y0.x), fast_exp2(y0.y)), e1 = pack_f2(fast_exp2(y1.x), fast_exp2(y1.y));
           sum0 = add2(sum0, e0);
           sum1 = add2(sum1, e1);
-          if constexpr (Q8) {
-            const float4 v = fv[j / 4];
+          if (Q8 && partial) {
+            const float4 v = reinterpret_cast<const float4*>(ct.fv[f])[j / 4];
             e0 = mul2(e0, pack_f2(v.x, v.y));
             e1 = mul2(e1, pack_f2(v.z, v.w));
           }
           const float2 w0 = unpack_f2(e0), w1 = unpack_f2(e1);
           a[j / 2] = pack2<FMT>(w0.x, w0.y);
           a[j / 2 + 1] = pack2<FMT>(w1.x, w1.y);
+        }
+        if (Q8 && __any_sync(0xffffffffu, gone)) {
+#pragma unroll
+          for (int j = 0; j < KT / 2; ++j) a[j] = gone ? 0u : a[j];
         }
         const float2 sv = unpack_f2(add2(sum0, sum1));
         l = Q8 ? fmaf(sv.x + sv.y, __int_as_float((127 - dd) << 23), l) : l + sv.x + sv.y;
@@ -759,14 +822,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++n_s;
         tc_fence_after();
         if (rescale) {
-#pragma unroll
-          for (int b = 0; b < D; b += 32) {
-            uint32_t o[32];
-            tmem_ld32(tO + b, o);
+#pragma unroll 1
+          for (int b = 0; b < D; b += 16) {
+            uint32_t o[16];
+            tmem_ld_16(tO + b, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * cf);
-            tmem_st32(tO + b, o);
+            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * cf);
+            tmem_st_16(tO + b, o);
           }
         }
         // the other stream's threads may still read this stream's O of the piece before
@@ -807,7 +870,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         f1 = e1 < 0.f ? 0.f : Q8 ? w1 * fast_exp2(e1 - E) : w1;
       }
       float inv = L == 0.f ? 0.f : 1.f / L;                             // a row that sees nothing: zeros
-      if constexpr (Q8) inv *= kHalfUnit<FMT> * __int_as_float((int)fmaxf(E, 1.f) << 23);
+      if constexpr (Q8) inv *= kHalfUnit<FMT> / (1 << S::kUp) * __int_as_float((int)fmaxf(E, 1.f) << 23);
       const Row cw = row_of(cur);
       const bool join = !two && nt > 1;
       const size_t at = (size_t)(cur.bi.start + cw.node) * g.n_heads + cw.head;
@@ -816,17 +879,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                                          : ((size_t)blockIdx.x * 2 + (cur.index ? 1 : 0)) * sc.rows + cw.row;
       // one row tile: each stream's threads write half of the columns
       const int d0 = two ? 0 : x * (D / 2), d1 = two ? D : d0 + D / 2;
-      for (int d = d0; d < d1; d += 32) {
-        uint32_t o[32], o1[32];
-        tmem_ld32(two ? tO + d : lanes + kColO + d, o);
-        if (join) tmem_ld32(lanes + kColO + 128 + d, o1);
+#pragma unroll 1
+      for (int d = d0; d < d1; d += 16) {
+        uint32_t o[16], o1[16];
+        tmem_ld_16(two ? tO + d : lanes + kColO + d, o);
+        if (join) tmem_ld_16(lanes + kColO + 128 + d, o1);
         tmem_wait_ld();
-        float z[32];
+        float z[16];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) z[j] = __uint_as_float(o[j]) * (f0 * inv);
+        for (int j = 0; j < 16; ++j) z[j] = __uint_as_float(o[j]) * (f0 * inv);
         if (join) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) z[j] = fmaf(__uint_as_float(o1[j]), f1 * inv, z[j]);
+          for (int j = 0; j < 16; ++j) z[j] = fmaf(__uint_as_float(o1[j]), f1 * inv, z[j]);
         }
         if (!Q8 && cw.in && *reinterpret_cast<volatile int*>(&ct.dropped)) {   // the dropped elements of keys this row sees
           const uint64_t* mk = g.mask ? g.mask + (size_t)(cur.bi.start + cw.node) * g.words : nullptr;
@@ -834,7 +898,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (sees32(mk, g.words, cw.node, key - cur.bi.ctx) & 1) {
               const bf16* vp = static_cast<const bf16*>(c.v) + (cache_slot(c, cur.bi.row, cur.h, key)) * D + d;
 #pragma unroll
-              for (int j = 0; j < 32; ++j) {
+              for (int j = 0; j < 16; ++j) {
                 const float y = __bfloat162float(vp[j]);
                 if (!(fabsf(y) < INFINITY)) z[j] += y;
               }
@@ -842,13 +906,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (cw.in && to_out) {
 #pragma unroll
-          for (int j = 0; j < 32; j += 8)
+          for (int j = 0; j < 16; j += 8)
             *reinterpret_cast<uint4*>(out + at * D + d + j) =
                 make_uint4(pack2<EESD_KV_MODEL>(z[j], z[j + 1]), pack2<EESD_KV_MODEL>(z[j + 2], z[j + 3]),
                            pack2<EESD_KV_MODEL>(z[j + 4], z[j + 5]), pack2<EESD_KV_MODEL>(z[j + 6], z[j + 7]));
         } else if (cw.in) {
 #pragma unroll
-          for (int j = 0; j < 32; j += 4)
+          for (int j = 0; j < 16; j += 4)
             *reinterpret_cast<float4*>(g.part_o + part * D + d + j) = make_float4(z[j], z[j + 1], z[j + 2], z[j + 3]);
         }
         __syncwarp();
