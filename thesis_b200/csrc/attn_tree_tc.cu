@@ -136,11 +136,10 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
   return r;
 }
 
-// (x, y) *= f, floats held as bits
-__device__ __forceinline__ void scale2(uint32_t& x, uint32_t& y, f32x2 f) {
-  const float2 r = unpack_f2(mul2(pack_f2(__uint_as_float(x), __uint_as_float(y)), f));
-  x = __float_as_uint(r.x);
-  y = __float_as_uint(r.y);
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
 }
 
 // MN-major operand tile (64-element, 128-byte rows of the MN index per K index, 128-byte swizzle): 8 K indices
@@ -721,25 +720,112 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_wait_ld();
         tc_fence_before();
         mbar_arrive(smem_u32(&ct.s_free[x]));
-        // ---- scores in the log2 domain and their maximum
         const bool partial = (t + 1) * KT > min(cur.all_see, cur.n_keys);   // some row does not see some key of the tile
-        int ref = 0, em = 0;
-        if constexpr (Q8) em = ref = ct.ref[f];
-        if (!Q8 || !partial) {
-          const float rt = Q8 ? rf * ct.kt[f] : rf;
-          const f32x2 rt2 = pack_f2(rt, rt);
+        const int ref = Q8 ? ct.ref[f] : 0;
+        int em = ref;
+        // O, l and m move to a new reference only when the old one is too small by 2^8 (2^4 for V's scale): the weights
+        // stay below 2^12, in range of f16.  Returns the factor that O is to be scaled by.
+        float cf = 1.f;
+        auto move_to = [&](float mx) {
+          const float mn = fmaxf(m, mx);
+          const bool need = !begun || mn > m + 8.f || (Q8 && em > er + 4);
+          if (need) {
+            const int en = max(er, em);
+            cf = m == -INFINITY ? 0.f : fast_exp2(m - mn);
+            l *= cf;
+            if (Q8) cf *= er == 0 ? 0.f : fast_exp2((float)(er - en));
+            m = mn;
+            er = en;
+          }
+          return begun && __any_sync(0xffffffffu, need);
+        };
+        // P goes out once the product that read the last one is done (O is at rest then)
+        auto put_p = [&](const uint32_t* w, bool rescale) {
+          if (n_s && !warp_wait(&ct.pv_done[x], (n_s - 1) & 1, abort_flag, g.spin)) return false;
+          ++n_s;
+          tc_fence_after();
+          if (rescale) {
+#pragma unroll 1
+            for (int b = 0; b < D; b += 16) {
+              uint32_t o[16];
+              tmem_ld_16(tO + b, o);
+              tmem_wait_ld();
 #pragma unroll
-          for (int j = 0; j < KT; j += 2) scale2(a[j], a[j + 1], rt2);
-        } else {
-          const float4* fk = reinterpret_cast<const float4*>(ct.fk[f]);
+              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * cf);
+              tmem_st_16(tO + b, o);
+            }
+          }
+          // the other stream's threads may still read this stream's O of the piece before
+          if (!begun && piece && !warp_wait(&ct.epi_done, (piece - 1) & 1, abort_flag, g.spin)) return false;
+          begun = true;
+          tmem_st32(tP, w);
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(smem_u32(&ct.p_ready[x]));
+          return true;
+        };
+        // weights of scores a (masked ones -inf), the tile's V factors apart.  V's scale relative to er: its common part
+        // goes into the exponent, so l collects the same units and is brought back by the exact power of two, the rest
+        // multiplies.  Below 2^-40 no weight of the tile is left in f16.
+        auto general = [&](uint32_t* a, const float4* fv, bool rescale) {
+          const bool gone = Q8 && em - er < -40;
+          const int dd = Q8 && !gone ? min(ref - er, 100) : 0;
+          const float ms = m == -INFINITY ? 0.f : m, keep = gone ? 0.f : 1.f;
+          float sum = 0.f;
 #pragma unroll
           for (int j = 0; j < KT; j += 4) {
-            const float4 v = fk[j / 4];
-            scale2(a[j], a[j + 1], pack_f2(rf * v.x, rf * v.y));
-            scale2(a[j + 2], a[j + 3], pack_f2(rf * v.z, rf * v.w));
+            float w[4];
+            const float4 v = fv ? fv[j / 4] : make_float4(1.f, 1.f, 1.f, 1.f);
+            const float vv[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+              w[b] = fast_exp2(__fadd_rn(__fadd_rn(__uint_as_float(a[j + b]), -ms), (float)dd));
+              sum += w[b];
+              if (Q8) w[b] *= vv[b] * keep;
+            }
+            a[j / 2] = pack2<FMT>(w[0], w[1]);
+            a[j / 2 + 1] = pack2<FMT>(w[2], w[3]);
           }
-        }
-        if (partial) {
+          l = Q8 ? fmaf(sum, __int_as_float((127 - dd) << 23), l) : l + sum;
+          return put_p(a, rescale);
+        };
+        if (!partial) {
+          const float rt = Q8 ? rf * ct.kt[f] : rf;
+          float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < KT; j += 4) {
+            mx0 = fmaxf(mx0, fmaxf(__uint_as_float(a[j]), __uint_as_float(a[j + 1])));
+            mx1 = fmaxf(mx1, fmaxf(__uint_as_float(a[j + 2]), __uint_as_float(a[j + 3])));
+          }
+          const bool rescale = move_to(fmaxf(mx0, mx1) * rt);
+          // One FMA per score leaves 2^-24 |m| of it in the exponent: nothing at ordinary sizes, but at very large ones
+          // the largest score has to come out as exactly 0.
+          if (__any_sync(0xffffffffu, !(fabsf(m) <= 65536.f) || (Q8 && em - er < -40))) {
+#pragma unroll
+            for (int j = 0; j < KT; ++j) a[j] = __float_as_uint(__fmul_rn(__uint_as_float(a[j]), rt));
+            if (!(ok = general(a, nullptr, rescale))) break;
+          } else {
+            const float nbs = (Q8 ? (float)(ref - er) : 0.f) - m;
+            const f32x2 nb = pack_f2(nbs, nbs), rt2 = pack_f2(rt, rt);
+            f32x2 sum0 = pack_f2(0.f, 0.f), sum1 = pack_f2(0.f, 0.f);
+            uint32_t w[KT / 2];
+#pragma unroll
+            for (int j = 0; j < KT; j += 4) {
+              const float2 y0 = unpack_f2(fma2(pack_f2(__uint_as_float(a[j]), __uint_as_float(a[j + 1])), rt2, nb));
+              const float2 y1 = unpack_f2(fma2(pack_f2(__uint_as_float(a[j + 2]), __uint_as_float(a[j + 3])), rt2, nb));
+              const float e0 = fast_exp2(y0.x), e1 = fast_exp2(y0.y), e2 = fast_exp2(y1.x), e3 = fast_exp2(y1.y);
+              sum0 = add2(sum0, pack_f2(e0, e1));
+              sum1 = add2(sum1, pack_f2(e2, e3));
+              w[j / 2] = pack2<FMT>(e0, e1);
+              w[j / 2 + 1] = pack2<FMT>(e2, e3);
+            }
+            const float2 sv = unpack_f2(add2(sum0, sum1));
+            l = Q8 ? fmaf(sv.x + sv.y, __int_as_float((127 - (ref - er)) << 23), l) : l + sv.x + sv.y;
+            if (!(ok = put_p(w, rescale))) break;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < KT; ++j) a[j] = __float_as_uint(__fmul_rn(__uint_as_float(a[j]), Q8 ? __fmul_rn(rf, ct.fk[f][j]) : rf));
           const int node = row_of(cur).node, left = cur.n_keys - t * KT;
           const uint64_t* mk = g.mask ? g.mask + (size_t)(cur.bi.start + node) * g.words : nullptr;
           uint32_t s0 = sees32(mk, g.words, node, t * KT - cur.bi.ctx), s1 = sees32(mk, g.words, node, t * KT + 32 - cur.bi.ctx);
@@ -758,87 +844,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             em = max(max(top & 255, top >> 8 & 255), max(top >> 16 & 255, top >> 24));
             if ((ct.nan[f][0] & s0) | (ct.nan[f][1] & s1)) l = __int_as_float(0x7fffffff);   // the row sees a V that is NaN
           }
-        }
-        float mx0 = -INFINITY, mx1 = -INFINITY;
+          float mx = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < KT; j += 4) {
-          mx0 = fmaxf(mx0, fmaxf(__uint_as_float(a[j]), __uint_as_float(a[j + 1])));
-          mx1 = fmaxf(mx1, fmaxf(__uint_as_float(a[j + 2]), __uint_as_float(a[j + 3])));
+          for (int j = 0; j < KT; ++j) mx = fmaxf(mx, __uint_as_float(a[j]));
+          const bool rescale = move_to(mx);
+          if (!(ok = general(a, Q8 ? reinterpret_cast<const float4*>(ct.fv[f]) : nullptr, rescale))) break;
         }
-        // O, l and m move to a new reference only when the old one is too small by 2^8 (2^4 for V's scale): the
-        // weights stay below 2^12, in range of f16
-        const float mn = fmaxf(m, fmaxf(mx0, mx1));
-        const bool need = !begun || mn > m + 8.f || (Q8 && em > er + 4);
-        float cf = 1.f;
-        if (need) {
-          const int en = max(er, em);
-          cf = m == -INFINITY ? 0.f : fast_exp2(m - mn);
-          l *= cf;
-          if (Q8) cf *= er == 0 ? 0.f : fast_exp2((float)(er - en));
-          m = mn;
-          er = en;
-        }
-        const bool rescale = begun && __any_sync(0xffffffffu, need);
-        const float ms = m == -INFINITY ? 0.f : m;
-        // ---- weights.  V's scale relative to er: its common part goes into the exponent, so l collects the same units
-        // and is brought back by the exact power of two, the rest multiplies.  Below 2^-40 no weight of the tile is left
-        // in f16.
-        const bool gone = Q8 && em - er < -40;
-        const int dd = Q8 && !gone ? min(ref - er, 100) : 0;
-        // The packed product and sum may be contracted to one FMA, which leaves 2^-24 |m| of the score in the exponent:
-        // nothing at ordinary sizes, but at very large ones the largest score has to come out as exactly 0.
-        float nbs = (float)dd - ms;
-        if (__any_sync(0xffffffffu, fabsf(ms) > 65536.f)) {
-#pragma unroll
-          for (int j = 0; j < KT; ++j) a[j] = __float_as_uint(__fadd_rn(__uint_as_float(a[j]), -ms));
-          nbs = (float)dd;
-        }
-        const f32x2 nb = pack_f2(nbs, nbs);
-        f32x2 sum0 = pack_f2(0.f, 0.f), sum1 = pack_f2(0.f, 0.f);
-#pragma unroll
-        for (int j = 0; j < KT; j += 4) {
-          const float2 y0 = unpack_f2(add2(pack_f2(__uint_as_float(a[j]), __uint_as_float(a[j + 1])), nb));
-          const float2 y1 = unpack_f2(add2(pack_f2(__uint_as_float(a[j + 2]), __uint_as_float(a[j + 3])), nb));
-          f32x2 e0 = pack_f2(fast_exp2(y0.x), fast_exp2(y0.y)), e1 = pack_f2(fast_exp2(y1.x), fast_exp2(y1.y));
-          sum0 = add2(sum0, e0);
-          sum1 = add2(sum1, e1);
-          if (Q8 && partial) {
-            const float4 v = reinterpret_cast<const float4*>(ct.fv[f])[j / 4];
-            e0 = mul2(e0, pack_f2(v.x, v.y));
-            e1 = mul2(e1, pack_f2(v.z, v.w));
-          }
-          const float2 w0 = unpack_f2(e0), w1 = unpack_f2(e1);
-          a[j / 2] = pack2<FMT>(w0.x, w0.y);
-          a[j / 2 + 1] = pack2<FMT>(w1.x, w1.y);
-        }
-        if (Q8 && __any_sync(0xffffffffu, gone)) {
-#pragma unroll
-          for (int j = 0; j < KT / 2; ++j) a[j] = gone ? 0u : a[j];
-        }
-        const float2 sv = unpack_f2(add2(sum0, sum1));
-        l = Q8 ? fmaf(sv.x + sv.y, __int_as_float((127 - dd) << 23), l) : l + sv.x + sv.y;
-        // ---- P, once the product that read the last one is done (O is at rest then)
-        if (n_s && !(ok = warp_wait(&ct.pv_done[x], (n_s - 1) & 1, abort_flag, g.spin))) break;
-        ++n_s;
-        tc_fence_after();
-        if (rescale) {
-#pragma unroll 1
-          for (int b = 0; b < D; b += 16) {
-            uint32_t o[16];
-            tmem_ld_16(tO + b, o);
-            tmem_wait_ld();
-#pragma unroll
-            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * cf);
-            tmem_st_16(tO + b, o);
-          }
-        }
-        // the other stream's threads may still read this stream's O of the piece before
-        if (!begun && piece && !(ok = warp_wait(&ct.epi_done, (piece - 1) & 1, abort_flag, g.spin))) break;
-        begun = true;
-        tmem_st32(tP, a);
-        tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(smem_u32(&ct.p_ready[x]));
       }
       if (!ok) break;
       // ---- the next piece's Q goes out before this one's output: its first S runs under it
