@@ -13,14 +13,14 @@
 // over all key tiles; with fewer, both share the rows and take every other key tile, and meet at the end.
 //
 // 8-bit caches: a warpgroup turns the TMA-loaded bytes into the f16 tiles that the products read, each key's power of
-// two relative to the tile's largest multiplied in (exact, as f16 goes, while they are within 2^21, e4m3, or 2^22, int8;
-// keys further below than 2^28 or 2^22 count as zeros), so the softmax sees one scale per tile.  In tiles that some row
+// two relative to the tile's largest multiplied in (exact, as f16 goes, while they are within 2^21, e4m3, or 2^29, int8,
+// and zero from 2^38 or 2^29 on), so the softmax sees one scale per tile.  In tiles that some row
 // does not wholly see a key's scale stays out of the operands and multiplies scores and weights instead: what
 // a row does not see must not decide its precision.
 //
-// Roles of the 16 warps: 0 TMA, 1 and 3 MMA issue of stream 0 and 1 (a satisfied barrier wait costs some 150 clocks,
+// Roles of the 20 warps: 0 TMA, 1 and 3 MMA issue of stream 0 and 1 (a satisfied barrier wait costs some 150 clocks,
 // and each tile takes four of them), 2 the schedule, 4-7 and 8-11 softmax of stream 0 and 1 (a thread is a row),
-// 12-15 conversion (8-bit) or the check of V tiles that some row does not wholly see (bf16).
+// 12-15 and 16-19 conversion of K and of V (8-bit), or 12-15 the check of V tiles that some row does not wholly see (bf16).
 #include <algorithm>
 
 #include "attn_tree.h"
@@ -33,10 +33,17 @@ namespace eesd {
 namespace {
 
 constexpr int KT = 64;                     // keys per tile
-constexpr int kThreads = 512;
+constexpr int kThreads = 640;
 constexpr uint32_t kColO = 0, kColQ = 256;                // TMEM columns; O of stream x at 128 x
 constexpr uint32_t kColS = 320, kColP = 384, kSP = 96;    // S and P of stream x add kSP x
 
+// One arrival per warp, after all of its lanes: an arrival is an atomic on shared memory, and 32 of them on one
+// barrier serialise.
+__device__ __forceinline__ void mbar_arrive(uint32_t bar);
+__device__ __forceinline__ void warp_arrive(void* bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(bar));
+}
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -89,9 +96,10 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// mbar_wait that suspends the thread for up to 2 us per poll: most of the 16 warps wait most of the time, and polling
+// mbar_wait that suspends the thread for up to 2 us per poll: most of the 20 warps wait most of the time, and polling
 // would take the issue slots of those that do not.
 __device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t limit) {
+#pragma unroll 1
   for (uint32_t i = 0; i < limit; ++i) {
     uint32_t ok;
     asm volatile(
@@ -123,11 +131,6 @@ __device__ __forceinline__ f32x2 pack_f2(float a, float b) {
 __device__ __forceinline__ float2 unpack_f2(f32x2 v) {
   float2 r;
   asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
 __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
@@ -187,6 +190,7 @@ struct PieceIter {
   long long pos, end, base;
   int e, index, loaded;
   __device__ bool next(const TreeGeom& g, const CacheGeom& c, const TcSchedule& sc, Piece& p) {
+#pragma unroll 1
     while (pos < end) {
       if (loaded != e) {
         bool bad;
@@ -225,6 +229,30 @@ struct PieceIter {
   }
 };
 
+// Four stored bytes as f16 pairs times the half pair m: exact unpacking, then one product (e4m3) or, with the offset of
+// the integer trick folded in, one FMA: (1024 + u) m - 1152 m, u = element + 128 (int8; m at most 2^5 keeps 1152 m finite).
+template <int FMT> struct Scaler {
+  __half2 m, off;
+  __device__ explicit Scaler(uint32_t bits) {
+    m = *reinterpret_cast<const __half2*>(&bits);
+    off = FMT == EESD_KV_INT8 ? __hmul2(m, __halves2half2(__ushort_as_half(0xe480), __ushort_as_half(0xe480))) : m;   // -1152 m
+  }
+  __device__ void operator()(uint32_t w, uint32_t& lo, uint32_t& hi) const {
+    if constexpr (FMT == EESD_KV_INT8) {
+      w ^= 0x80808080u;
+      const uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+      const __half2 x = __hfma2(*reinterpret_cast<const __half2*>(&a), m, off), y = __hfma2(*reinterpret_cast<const __half2*>(&b), m, off);
+      lo = *reinterpret_cast<const uint32_t*>(&x);
+      hi = *reinterpret_cast<const uint32_t*>(&y);
+    } else {
+      unpack4<FMT>(w, lo, hi);
+      const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&lo), m), y = __hmul2(*reinterpret_cast<const __half2*>(&hi), m);
+      lo = *reinterpret_cast<const uint32_t*>(&x);
+      hi = *reinterpret_cast<const uint32_t*>(&y);
+    }
+  }
+};
+
 template <int D, int FMT> struct TcShape {
   static constexpr bool Q8 = FMT != EESD_KV_MODEL;
   static constexpr int TILE = KT * D * 2;              // bytes of one 16-bit K (or V) tile
@@ -232,13 +260,13 @@ template <int D, int FMT> struct TcShape {
   static constexpr int NS = Q8 ? 2 : 5;                // 16-bit K / V stages
   static constexpr int RS = Q8 ? 6 : 0;                // raw stages
   static constexpr int FR = 8;                         // factor ring: six tiles can be between conversion and softmax
-  static constexpr int kUp = FMT == EESD_KV_E4M3 ? 14 : 8;   // a tile's largest 8-bit elements go up to 2^15 in f16
+  [[maybe_unused]] static constexpr int kUp = FMT == EESD_KV_E4M3 ? 14 : 5;   // a tile's largest 8-bit elements in f16: 28672, 4064
   static constexpr int QB = 128 * D * 2;               // Q of stream 1 (more than 128 rows)
   static constexpr size_t ctl = 16384;
   static constexpr size_t smem = 1024 + (size_t)2 * NS * TILE + (size_t)RS * RAW + QB + ctl;
 };
 constexpr int kPieces = 4;                 // pieces between the schedule warp and the slowest role
-constexpr int kReaders = 15;               // warps that read them: TMA, 2 MMA, 8 softmax, 4 conversion
+constexpr int kReaders = 19;               // warps that read them: TMA, 2 MMA, 8 softmax, 8 conversion
 struct TcControl {
   uint64_t kfull[5], kempty[5], vfull[5], vempty[5], vclean[5], raw_full[6], raw_empty[6], ffull[8];
   uint64_t piece_full[kPieces], piece_empty[kPieces];
@@ -255,7 +283,7 @@ struct TcControl {
   uint32_t nan[8][2];                      // keys whose V is NaN
   float ml[2][2][3][128];                  // one row tile: max, sum and eref of the streams (by piece parity)
   long long lo, hi, base;
-  long long wsum[16];
+  long long wsum[20];
   uint32_t tmem;
   int e0;
   int abort, dropped;
@@ -283,6 +311,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int E = sc.entries, seg = (E + kThreads - 1) / kThreads;
     const int a = min(E, tid * seg), b = min(E, a + seg);
     long long sum = 0;
+#pragma unroll 1
     for (int e = a; e < b; ++e) {
       bool bad;
       sum += entry_of(g, c, sc, e, bad).length();
@@ -299,30 +328,30 @@ __global__ void __launch_bounds__(kThreads, 1)
       ct.abort = ct.dropped = 0;
       ct.e0 = E;
       for (int i = 0; i < NS; ++i) {
-        mbar_init(smem_u32(&ct.kfull[i]), Q8 ? 128 : 1);
-        mbar_init(smem_u32(&ct.vfull[i]), Q8 ? 128 : 1);
+        mbar_init(smem_u32(&ct.kfull[i]), Q8 ? 4 : 1);
+        mbar_init(smem_u32(&ct.vfull[i]), Q8 ? 4 : 1);
         mbar_init(smem_u32(&ct.kempty[i]), 2);
         mbar_init(smem_u32(&ct.vempty[i]), 2);
-        mbar_init(smem_u32(&ct.vclean[i]), 128);
+        mbar_init(smem_u32(&ct.vclean[i]), 4);
       }
       for (int i = 0; i < RS; ++i) {
         mbar_init(smem_u32(&ct.raw_full[i]), 1);
-        mbar_init(smem_u32(&ct.raw_empty[i]), 128);
+        mbar_init(smem_u32(&ct.raw_empty[i]), 8);
       }
-      for (int i = 0; i < FR; ++i) mbar_init(smem_u32(&ct.ffull[i]), 128);
+      for (int i = 0; i < FR; ++i) mbar_init(smem_u32(&ct.ffull[i]), 8);
       for (int i = 0; i < 2; ++i) {
         mbar_init(smem_u32(&ct.s_full[i]), 1);
-        mbar_init(smem_u32(&ct.s_free[i]), 128);
-        mbar_init(smem_u32(&ct.p_ready[i]), 128);
+        mbar_init(smem_u32(&ct.s_free[i]), 4);
+        mbar_init(smem_u32(&ct.p_ready[i]), 4);
         mbar_init(smem_u32(&ct.pv_done[i]), 1);
       }
       for (int i = 0; i < kPieces; ++i) {
         mbar_init(smem_u32(&ct.piece_full[i]), 1);
         mbar_init(smem_u32(&ct.piece_empty[i]), kReaders);
       }
-      mbar_init(smem_u32(&ct.q_ready), 256);
-      mbar_init(smem_u32(&ct.ml_ready), 256);
-      mbar_init(smem_u32(&ct.epi_done), 256);
+      mbar_init(smem_u32(&ct.q_ready), 8);
+      mbar_init(smem_u32(&ct.ml_ready), 8);
+      mbar_init(smem_u32(&ct.epi_done), 8);
       mbar_init(smem_u32(&ct.o_done), 2);
       mbar_init(smem_u32(&ct.drain[0]), 1);
       mbar_init(smem_u32(&ct.drain[1]), 1);
@@ -336,7 +365,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc_fence_after();
     long long before = inc - sum, total = 0;
-    for (int w = 0; w < 16; ++w) {
+#pragma unroll 1
+    for (int w = 0; w < kThreads / 32; ++w) {
       if (w < warp) before += ct.wsum[w];
       total += ct.wsum[w];
     }
@@ -351,6 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (lo >= before * Hkv && lo < (before + sum) * Hkv) {
       long long base = before * Hkv;
+#pragma unroll 1
       for (int e = a; e < b; ++e) {
         bool bad;
         const long long span = (long long)entry_of(g, c, sc, e, bad).length() * Hkv;
@@ -376,10 +407,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       tma_prefetch_desc(&kmap);
       tma_prefetch_desc(&vmap);
+#pragma unroll 1
       for (int k = 0; (ok = piece_wait(k)); ++k) {
         const Piece& p = ct.piece[k % kPieces];
         if (p.tiles == 0) break;
         const int slot0 = (int)cache_slot(c, p.bi.row, p.h, 0);
+#pragma unroll 1
         for (int t = p.t0; t < p.t1; ++t, ++cnt) {
           if constexpr (Q8) {
             const int s = cnt % RS;
@@ -429,6 +462,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t dS = tmem + kColS + x * kSP, dO = tmem + kColO + x * 128, aP = tmem + kColP + x * kSP;
       int cnt0 = 0, piece = 0, n_q = 0, n_p = 0;
       bool ok = true, issued = false;
+#pragma unroll 1
       for (; (ok = piece_wait(piece)); ++piece) {
         const Piece& p = ct.piece[piece % kPieces];
         if (p.tiles == 0) break;
@@ -442,6 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         if (!(ok = wait_on(smem_u32(&ct.q_ready), piece & 1, abort_flag, g.spin))) break;
         // S of the stream's next tile as soon as the last one is in registers, then O of the last one when its softmax ends
+#pragma unroll 1
         for (int i = t0 - step; i < nt; i += step) {
           const int j = i + step;
           if (j < nt) {
@@ -498,6 +533,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ct.e0 >= sc.entries) it.pos = it.end;
       bool ok = true;
       Piece p;
+#pragma unroll 1
       for (int k = 0;; ++k) {
         if (!(ok = wait_on(smem_u32(&ct.piece_empty[k % kPieces]), (k / kPieces & 1) ^ 1, abort_flag, g.spin))) break;
         const bool more = it.next(g, c, sc, p);
@@ -512,10 +548,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else if (warp >= 12) {
-    reg_dec<56>();
+    reg_dec<48>();
     // ------------------------------------------------------------ conversion, or the check of V tiles
-    const int ti = tid - 384;
-    // The raw tile's bytes as f16, row r times 2^(e_r - top) (none below 2^-14; byte 255, a NaN, comes out as one);
+    const int ti = tid & 127;
+    const bool is_v = warp >= 16;
+    // The raw tile's bytes as f16, row r times 2^(e_r - top) (none below 2^-24; byte 255, a NaN, comes out as one);
     // top = 0: all rows times 2^flat.  A thread has one 16-byte chunk of every 16th (D = 64: 32nd) row; the 8 lanes of a
     // phase are on 8 rows and one chunk, conflict-free in both swizzles.
     constexpr int kChunks = D / 16, kRowStep = 128 / kChunks;
@@ -526,88 +563,72 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int i = 0; i < KT / kRowStep; ++i) {
         const uint4 w = *reinterpret_cast<const uint4*>(src + from + i * (kRowStep * D));
+        const int er = e[row0 + i * kRowStep], x = top ? er - top : flat;
+        const uint32_t h = top && er == 255 ? 0x7fffu : x >= -14 ? (uint32_t)(x + 15) << 10 : x >= -24 ? 1u << (x + 24) : 0u;
+        const uint32_t m = __byte_perm(h, 0, 0x1010);
+        const Scaler<FMT> sc8(m);
         uint4 a, b;
-        unpack4<FMT>(w.x, a.x, a.y);
-        unpack4<FMT>(w.y, a.z, a.w);
-        unpack4<FMT>(w.z, b.x, b.y);
-        unpack4<FMT>(w.w, b.z, b.w);
-        const int er = e[row0 + i * kRowStep];
-        const uint32_t h = top == 0 ? (uint32_t)(flat + 15) << 10 : er == 255 ? 0x7fffu : (uint32_t)max(er - top + 15, 0) << 10;
-        const uint32_t hh = __byte_perm(h, 0, 0x1010);
-        const __half2 m = *reinterpret_cast<const __half2*>(&hh);
-        __half2* v = reinterpret_cast<__half2*>(&a);
-        __half2* u = reinterpret_cast<__half2*>(&b);
-#pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          v[y] = __hmul2(v[y], m);
-          u[y] = __hmul2(u[y], m);
-        }
+        sc8(w.x, a.x, a.y);
+        sc8(w.y, a.z, a.w);
+        sc8(w.z, b.x, b.y);
+        sc8(w.w, b.z, b.w);
         *reinterpret_cast<uint4*>(dst + to0 + i * (kRowStep * 128)) = a;
         *reinterpret_cast<uint4*>(dst + to1 + i * (kRowStep * 128)) = b;
       }
       fence_proxy_async_smem();
     };
-    // V of a tile waits for the product two tiles before it, K does not: K goes one tile ahead
-    int v_top = 0;                                                      // of the tile whose V is still to be converted
-    [[maybe_unused]] auto convert_v = [&](int cnt) {
-      const int st = cnt % NS, rs = cnt % RS;
-      if (!warp_wait(&ct.vempty[st], (cnt / NS & 1) ^ 1, abort_flag, g.spin)) return false;
-      convert(sm + 2 * NS * S::TILE + rs * S::RAW + S::RAW / 2, sm + (NS + st) * S::TILE, ct.exps[rs] + KT, v_top, TcShape<D, FMT>::kUp);
-      mbar_arrive(smem_u32(&ct.vfull[st]));
-      mbar_arrive(smem_u32(&ct.raw_empty[rs]));
-      return true;
-    };
     int cnt = 0;
     bool ok = true;
+#pragma unroll 1
     for (int k = 0; (ok = __all_sync(0xffffffffu, piece_wait(k))); ++k) {
       const Piece& p = ct.piece[k % kPieces];
       if (p.tiles == 0) break;
-      for (int t = p.t0; t < p.t1; ++t, ++cnt) {
+#pragma unroll 1
+      for (int t = p.t0; (Q8 || !is_v) && t < p.t1; ++t, ++cnt) {
         const int st = cnt % NS;
         if constexpr (Q8) {
           const int rs = cnt % RS, f = cnt % FR;
           if (!(ok = warp_wait(&ct.raw_full[rs], cnt / RS & 1, abort_flag, g.spin))) break;
           const bool partial = (t + 1) * KT > min(p.all_see, p.n_keys);
           const int left = p.n_keys - t * KT;
-          // the tile's largest exponents (of slots before its end, NaN apart)
-          auto top_of = [&](const uint8_t* e) {
-            const uint32_t v = *reinterpret_cast<const uint16_t*>(e + 2 * lane);
-            const int a0 = v & 255, a1 = v >> 8;
-            return __reduce_max_sync(0xffffffffu, max(2 * lane < left && a0 != 255 ? a0 : 0, 2 * lane + 1 < left && a1 != 255 ? a1 : 0));
-          };
-          const int ek = top_of(ct.exps[rs]), ev = top_of(ct.exps[rs] + KT);
+          // the tile's largest exponent (of slots before its end, NaN apart)
+          const uint8_t* ex = ct.exps[rs] + (is_v ? KT : 0);
+          const uint32_t v = *reinterpret_cast<const uint16_t*>(ex + 2 * lane);
+          const int a0 = v & 255, a1 = v >> 8;
+          const int em = __reduce_max_sync(0xffffffffu, max(2 * lane < left && a0 != 255 ? a0 : 0, 2 * lane + 1 < left && a1 != 255 ? a1 : 0));
+          const int top = partial ? 0 : max(em, 27) - S::kUp;
           // V's factors in a tile that some row does not wholly see are relative to 2^60 below the largest, so that they
           // last for rows whose own largest is far smaller
-          const int k_top = partial ? 0 : max(ek, 27) - S::kUp, next_v_top = partial ? 0 : max(ev, 27) - S::kUp, ref = partial ? ev - 60 : ev;
-          if (!(ok = warp_wait(&ct.kempty[st], (cnt / NS & 1) ^ 1, abort_flag, g.spin))) break;
+          const int ref = partial ? em - 60 : em;
+          if (!(ok = warp_wait(is_v ? &ct.vempty[st] : &ct.kempty[st], (cnt / NS & 1) ^ 1, abort_flag, g.spin))) break;
+          // (the factor ring's last reader is behind the products that freed this stage)
           if (ti == 0) {
-            ct.ref[f] = ref;
-            ct.kt[f] = __int_as_float(max(k_top, 1) << 23);
+            if (is_v) ct.ref[f] = ref;
+            else ct.kt[f] = __int_as_float(max(top, 1) << 23);
           }
-          if (partial) {
-            // (the ring slot's last reader is behind the product that freed this K stage)
-            if (ti < KT) {
-              ct.fk[f][ti] = exp_scale(ct.exps[rs][ti]);
+          if (partial && ti < KT) {
+            const int e = ex[ti], d = e - ref + 127;
+            if (!is_v) {
+              ct.fk[f][ti] = exp_scale(e);
             } else {
-              const int e = ct.exps[rs][ti], d = e - ref + 127;
-              const bool nan = e == 255, in = ti - KT < left;
-              ct.ev[f][ti - KT] = nan || !in ? 0 : (uint8_t)e;
-              ct.fv[f][ti - KT] = nan || !in || d <= 0 ? 0.f : __int_as_float(d << 23);
+              const bool nan = e == 255, in = ti < left;
+              ct.ev[f][ti] = nan || !in ? 0 : (uint8_t)e;
+              ct.fv[f][ti] = nan || !in || d <= 0 ? 0.f : __int_as_float(d << 23);
               const uint32_t nans = __ballot_sync(0xffffffffu, nan && in);
-              if (lane == 0) ct.nan[f][(ti - KT) >> 5] = nans;
+              if (lane == 0) ct.nan[f][ti >> 5] = nans;
             }
           }
-          mbar_arrive(smem_u32(&ct.ffull[f]));
-          convert(sm + 2 * NS * S::TILE + rs * S::RAW, sm + st * S::TILE, ct.exps[rs], k_top, 0);
-          mbar_arrive(smem_u32(&ct.kfull[st]));
-          if (cnt && !(ok = convert_v(cnt - 1))) break;
-          v_top = next_v_top;
+          warp_arrive(&ct.ffull[f]);
+          convert(sm + 2 * NS * S::TILE + rs * S::RAW + (is_v ? S::RAW / 2 : 0), sm + ((is_v ? NS : 0) + st) * S::TILE, ex, top, is_v ? S::kUp : 0);
+          warp_arrive(is_v ? &ct.vfull[st] : &ct.kfull[st]);
+          warp_arrive(&ct.raw_empty[rs]);
         } else {
           if (!(ok = warp_wait(&ct.vfull[st], cnt / NS & 1, abort_flag, g.spin))) break;
           if ((t + 1) * KT > min(p.all_see, p.n_keys)) {
             // some row does not see some key: 0 x NaN would reach it, so non-finite elements are dropped here and put
             // back at the end for the rows that do see them
             bool hit = false;
+#pragma unroll 2
             for (int i = ti; i < S::TILE / 16; i += 128) {
               const uint32_t a = vbuf + st * S::TILE + i * 16;
               uint4 v = lds128(a);
@@ -622,19 +643,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (hit) *reinterpret_cast<volatile int*>(&ct.dropped) = 1;
             fence_proxy_async_smem();
           }
-          mbar_arrive(smem_u32(&ct.vclean[st]));
+          warp_arrive(&ct.vclean[st]);
         }
       }
       if (!ok) break;
       if (lane == 0) piece_free(k);
     }
-    if (Q8 && ok && cnt) ok = convert_v(cnt - 1);
     if (!ok) {
       set_status(g.status, kStatusTimeoutProducer);
       *abort_flag = 1;
     }
   } else if (warp >= 4) {
-    reg_inc<200>();
+    reg_inc<160>();
     // ------------------------------------------------------------ softmax: thread = row of stream x
     const int x = (warp >> 2) - 1, r = tid & 127;
     const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);         // TMEM lane quadrant of the warp
@@ -656,52 +676,58 @@ __global__ void __launch_bounds__(kThreads, 1)
       return w;
     };
     const float scale_l2 = g.scale * 1.4426950408889634f;
-    auto load_q = [&](const Piece& p, const Row& w, uint32_t (&v)[D / 2]) {
-      const bf16* src = q + (size_t)(p.bi.start + w.node) * g.ld_q + (size_t)w.head * D;
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        const uint4 u = w.in ? *reinterpret_cast<const uint4*>(src + i * 8) : make_uint4(0, 0, 0, 0);
-        v[4 * i] = u.x, v[4 * i + 1] = u.y, v[4 * i + 2] = u.z, v[4 * i + 3] = u.w;
-      }
-    };
-    // the q row where the products read it: bf16 as it is, or f16 with the largest element's power of two taken out
-    // (returned with the softmax scale)
-    auto put_q = [&](const Row& w, uint32_t (&v)[D / 2]) {
-      float rf = scale_l2;
+    // The q row of a piece to where the products read it: bf16 as it is, or f16 with the largest element's power of two
+    // taken out (returned with the softmax scale).  32 words at a time: the whole row in registers would spill the softmax.
+    auto put_q = [&](const Piece& p) {
+      const Row w = row_of(p);
+      const uint4* src = reinterpret_cast<const uint4*>(q + (size_t)(p.bi.start + w.node) * g.ld_q + (size_t)w.head * D);
+      float rf = scale_l2, inv = 1.f;
       if constexpr (Q8) {
         uint32_t amax = 0;
 #pragma unroll
-        for (int i = 0; i < D / 2; ++i) amax = max(amax, max(v[i] << 16 & 0x7fff0000u, v[i] & 0x7fff0000u));
+        for (int i = 0; i < D / 8; ++i) {
+          const uint4 u = w.in ? src[i] : make_uint4(0, 0, 0, 0);
+          const uint32_t hi = max(max(u.x & 0x7fff0000u, u.y & 0x7fff0000u), max(u.z & 0x7fff0000u, u.w & 0x7fff0000u));
+          const uint32_t lo = max(max(u.x << 16 & 0x7fff0000u, u.y << 16 & 0x7fff0000u), max(u.z << 16 & 0x7fff0000u, u.w << 16 & 0x7fff0000u));
+          amax = max(amax, max(hi, lo));
+        }
         const int e = min(max((int)(amax >> 23), 27), 227);
-        const float inv = __int_as_float((254 - e) << 23);
+        inv = __int_as_float((254 - e) << 23);
         rf *= __int_as_float(e << 23) * kHalfUnit<FMT>;
-#pragma unroll
-        for (int i = 0; i < D / 2; ++i) v[i] = pack2<FMT>(__uint_as_float(v[i] << 16) * inv, __uint_as_float(v[i] & 0xffff0000u) * inv);
       }
-      if (x == 0) {
+#pragma unroll 1
+      for (int b = 0; b < D / 64; ++b) {
+        uint32_t v[32];
 #pragma unroll
-        for (int i = 0; i < D / 64; ++i) tmem_st32(lanes + kColQ + 32 * i, v + 32 * i);
-        tmem_wait_st();
-      } else if (w.two) {
+        for (int i = 0; i < 8; ++i) {
+          const uint4 u = w.in ? src[8 * b + i] : make_uint4(0, 0, 0, 0);
+          v[4 * i] = u.x, v[4 * i + 1] = u.y, v[4 * i + 2] = u.z, v[4 * i + 3] = u.w;
+        }
+        if constexpr (Q8) {
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i)
-          sts128(qbuf + (i >> 3) * (128 * 128) + r * 128 + (((i & 7) ^ (r & 7)) << 4),
-                 make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]));
-        fence_proxy_async_smem();
+          for (int i = 0; i < 32; ++i) v[i] = pack2<FMT>(__uint_as_float(v[i] << 16) * inv, __uint_as_float(v[i] & 0xffff0000u) * inv);
+        }
+        if (x == 0) {
+          tmem_st32(lanes + kColQ + 32 * b, v);
+        } else if (w.two) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            sts128(qbuf + b * (128 * 128) + r * 128 + ((i ^ (r & 7)) << 4), make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]));
+        }
       }
+      if (x == 0) tmem_wait_st();
+      else fence_proxy_async_smem();
       tc_fence_before();
-      mbar_arrive(smem_u32(&ct.q_ready));
+      warp_arrive(&ct.q_ready);
       return rf;
     };
     float rf = 0.f;
     bool more = false;
     if ((ok = __all_sync(0xffffffffu, piece_wait(0))) && ct.piece[0].tiles) {
-      uint32_t v[D / 2];
-      const Row w = row_of(ct.piece[0]);
-      load_q(ct.piece[0], w, v);
-      rf = put_q(w, v);
+      rf = put_q(ct.piece[0]);
       more = true;
     }
+#pragma unroll 1
     while (more) {
       const Piece& cur = ct.piece[piece % kPieces];
       const int nt = cur.t1 - cur.t0;
@@ -709,6 +735,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       float m = -INFINITY, l = 0.f;
       int er = 0;                                                       // 8-bit: exponent byte that O and l are relative to
       bool begun = false;
+#pragma unroll 1
       for (int i = two ? 0 : x; i < nt; i += two ? 1 : 2) {
         const int t = cur.t0 + i, cnt = cnt0 + i, f = cnt % FR;
         if (!(ok = warp_wait(&ct.s_full[x], n_s & 1, abort_flag, g.spin))) break;
@@ -719,12 +746,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_ld32(tS + 32, a + 32);
         tmem_wait_ld();
         tc_fence_before();
-        mbar_arrive(smem_u32(&ct.s_free[x]));
+        warp_arrive(&ct.s_free[x]);
         const bool partial = (t + 1) * KT > min(cur.all_see, cur.n_keys);   // some row does not see some key of the tile
         const int ref = Q8 ? ct.ref[f] : 0;
         int em = ref;
         // O, l and m move to a new reference only when the old one is too small by 2^8 (2^4 for V's scale): the weights
-        // stay below 2^12, in range of f16.  Returns the factor that O is to be scaled by.
+        // stay below 2^12, in range of f16.  O is then to be scaled by cf.
         float cf = 1.f;
         auto move_to = [&](float mx) {
           const float mn = fmaxf(m, mx);
@@ -739,134 +766,122 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           return begun && __any_sync(0xffffffffu, need);
         };
-        // P goes out once the product that read the last one is done (O is at rest then)
-        auto put_p = [&](const uint32_t* w, bool rescale) {
-          if (n_s && !warp_wait(&ct.pv_done[x], (n_s - 1) & 1, abort_flag, g.spin)) return false;
-          ++n_s;
-          tc_fence_after();
-          if (rescale) {
-#pragma unroll 1
-            for (int b = 0; b < D; b += 16) {
-              uint32_t o[16];
-              tmem_ld_16(tO + b, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * cf);
-              tmem_st_16(tO + b, o);
-            }
-          }
-          // the other stream's threads may still read this stream's O of the piece before
-          if (!begun && piece && !warp_wait(&ct.epi_done, (piece - 1) & 1, abort_flag, g.spin)) return false;
-          begun = true;
-          tmem_st32(tP, w);
-          tmem_wait_st();
-          tc_fence_before();
-          mbar_arrive(smem_u32(&ct.p_ready[x]));
-          return true;
-        };
-        // weights of scores a (masked ones -inf), the tile's V factors apart.  V's scale relative to er: its common part
-        // goes into the exponent, so l collects the same units and is brought back by the exact power of two, the rest
-        // multiplies.  Below 2^-40 no weight of the tile is left in f16.
-        auto general = [&](uint32_t* a, const float4* fv, bool rescale) {
-          const bool gone = Q8 && em - er < -40;
-          const int dd = Q8 && !gone ? min(ref - er, 100) : 0;
-          const float ms = m == -INFINITY ? 0.f : m, keep = gone ? 0.f : 1.f;
-          float sum = 0.f;
-#pragma unroll
-          for (int j = 0; j < KT; j += 4) {
-            float w[4];
-            const float4 v = fv ? fv[j / 4] : make_float4(1.f, 1.f, 1.f, 1.f);
-            const float vv[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-              w[b] = fast_exp2(__fadd_rn(__fadd_rn(__uint_as_float(a[j + b]), -ms), (float)dd));
-              sum += w[b];
-              if (Q8) w[b] *= vv[b] * keep;
-            }
-            a[j / 2] = pack2<FMT>(w[0], w[1]);
-            a[j / 2 + 1] = pack2<FMT>(w[2], w[3]);
-          }
-          l = Q8 ? fmaf(sum, __int_as_float((127 - dd) << 23), l) : l + sum;
-          return put_p(a, rescale);
-        };
-        if (!partial) {
-          const float rt = Q8 ? rf * ct.kt[f] : rf;
+        const float rt = Q8 && !partial ? rf * ct.kt[f] : rf;
+        bool rescale = false, slow = partial;
+        if (__builtin_expect(!partial, 1)) {
           float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
           for (int j = 0; j < KT; j += 4) {
             mx0 = fmaxf(mx0, fmaxf(__uint_as_float(a[j]), __uint_as_float(a[j + 1])));
             mx1 = fmaxf(mx1, fmaxf(__uint_as_float(a[j + 2]), __uint_as_float(a[j + 3])));
           }
-          const bool rescale = move_to(fmaxf(mx0, mx1) * rt);
+          rescale = move_to(fmaxf(mx0, mx1) * rt);
           // One FMA per score leaves 2^-24 |m| of it in the exponent: nothing at ordinary sizes, but at very large ones
-          // the largest score has to come out as exactly 0.
-          if (__any_sync(0xffffffffu, !(fabsf(m) <= 65536.f) || (Q8 && em - er < -40))) {
+          // the largest score has to come out as exactly 0.  V's scale relative to er goes into the exponent, so l
+          // collects the same units and is brought back by the exact power of two; below 2^-40 that is not f16 any more.
+          slow = __any_sync(0xffffffffu, !(fabsf(m) <= 65536.f) || (Q8 && em - er < -40));
+        }
+        uint32_t w[KT / 2];
+        if (__builtin_expect(!slow, 1)) {
+          const float nbs = (Q8 ? (float)(ref - er) : 0.f) - m;
+          const f32x2 nb = pack_f2(nbs, nbs), rt2 = pack_f2(rt, rt);
+          f32x2 sum0 = pack_f2(0.f, 0.f), sum1 = pack_f2(0.f, 0.f);
 #pragma unroll
-            for (int j = 0; j < KT; ++j) a[j] = __float_as_uint(__fmul_rn(__uint_as_float(a[j]), rt));
-            if (!(ok = general(a, nullptr, rescale))) break;
-          } else {
-            const float nbs = (Q8 ? (float)(ref - er) : 0.f) - m;
-            const f32x2 nb = pack_f2(nbs, nbs), rt2 = pack_f2(rt, rt);
-            f32x2 sum0 = pack_f2(0.f, 0.f), sum1 = pack_f2(0.f, 0.f);
-            uint32_t w[KT / 2];
-#pragma unroll
-            for (int j = 0; j < KT; j += 4) {
-              const float2 y0 = unpack_f2(fma2(pack_f2(__uint_as_float(a[j]), __uint_as_float(a[j + 1])), rt2, nb));
-              const float2 y1 = unpack_f2(fma2(pack_f2(__uint_as_float(a[j + 2]), __uint_as_float(a[j + 3])), rt2, nb));
-              const float e0 = fast_exp2(y0.x), e1 = fast_exp2(y0.y), e2 = fast_exp2(y1.x), e3 = fast_exp2(y1.y);
-              sum0 = add2(sum0, pack_f2(e0, e1));
-              sum1 = add2(sum1, pack_f2(e2, e3));
-              w[j / 2] = pack2<FMT>(e0, e1);
-              w[j / 2 + 1] = pack2<FMT>(e2, e3);
-            }
-            const float2 sv = unpack_f2(add2(sum0, sum1));
-            l = Q8 ? fmaf(sv.x + sv.y, __int_as_float((127 - (ref - er)) << 23), l) : l + sv.x + sv.y;
-            if (!(ok = put_p(w, rescale))) break;
+          for (int j = 0; j < KT; j += 4) {
+            const float2 y0 = unpack_f2(fma2(pack_f2(__uint_as_float(a[j]), __uint_as_float(a[j + 1])), rt2, nb));
+            const float2 y1 = unpack_f2(fma2(pack_f2(__uint_as_float(a[j + 2]), __uint_as_float(a[j + 3])), rt2, nb));
+            const float e0 = fast_exp2(y0.x), e1 = fast_exp2(y0.y), e2 = fast_exp2(y1.x), e3 = fast_exp2(y1.y);
+            sum0 = add2(sum0, pack_f2(e0, e1));
+            sum1 = add2(sum1, pack_f2(e2, e3));
+            w[j / 2] = pack2<FMT>(e0, e1);
+            w[j / 2 + 1] = pack2<FMT>(e2, e3);
           }
+          const float2 sv = unpack_f2(add2(sum0, sum1));
+          l = Q8 ? fmaf(sv.x + sv.y, __int_as_float((127 - (ref - er)) << 23), l) : l + sv.x + sv.y;
         } else {
-#pragma unroll
-          for (int j = 0; j < KT; ++j) a[j] = __float_as_uint(__fmul_rn(__uint_as_float(a[j]), Q8 ? __fmul_rn(rf, ct.fk[f][j]) : rf));
-          const int node = row_of(cur).node, left = cur.n_keys - t * KT;
-          const uint64_t* mk = g.mask ? g.mask + (size_t)(cur.bi.start + node) * g.words : nullptr;
-          uint32_t s0 = sees32(mk, g.words, node, t * KT - cur.bi.ctx), s1 = sees32(mk, g.words, node, t * KT + 32 - cur.bi.ctx);
-          if (left < 32) s0 &= (1u << left) - 1;
-          if (left < 64) s1 &= left <= 32 ? 0u : (1u << (left - 32)) - 1;
-#pragma unroll
-          for (int j = 0; j < KT; ++j)
-            if (!((j < 32 ? s0 : s1) >> (j & 31) & 1)) a[j] = 0xff800000u;
-          if constexpr (Q8) {                                           // V's largest exponent among the keys this row sees
-            uint32_t top = 0;
+          // scores, one by one with what is particular to a key: its scale and whether the row sees it
+          uint32_t s0 = ~0u, s1 = ~0u;
+          const bool keyed = Q8 && partial;
+          if (partial) {
+            const int node = row_of(cur).node, left = cur.n_keys - t * KT;
+            const uint64_t* mk = g.mask ? g.mask + (size_t)(cur.bi.start + node) * g.words : nullptr;
+            s0 = sees32(mk, g.words, node, t * KT - cur.bi.ctx);
+            s1 = sees32(mk, g.words, node, t * KT + 32 - cur.bi.ctx);
+            if (left < 32) s0 &= (1u << left) - 1;
+            if (left < 64) s1 &= left <= 32 ? 0u : (1u << (left - 32)) - 1;
+            if constexpr (Q8) {                                         // V's largest exponent among the keys this row sees
+              uint32_t top = 0;
 #pragma unroll 2
-            for (int j = 0; j < KT / 4; ++j) {
-              const uint32_t bits = (j < 8 ? s0 >> 4 * j : s1 >> (4 * j - 32)) & 15;
-              top = __vmaxu4(top, reinterpret_cast<const uint32_t*>(ct.ev[f])[j] & ((bits * 0x204081u & 0x1010101u) * 255u));
+              for (int j = 0; j < KT / 4; ++j) {
+                const uint32_t bits = (j < 8 ? s0 >> 4 * j : s1 >> (4 * j - 32)) & 15;
+                top = __vmaxu4(top, reinterpret_cast<const uint32_t*>(ct.ev[f])[j] & ((bits * 0x204081u & 0x1010101u) * 255u));
+              }
+              em = max(max(top & 255, top >> 8 & 255), max(top >> 16 & 255, top >> 24));
+              if ((ct.nan[f][0] & s0) | (ct.nan[f][1] & s1)) l = __int_as_float(0x7fffffff);   // the row sees a V that is NaN
             }
-            em = max(max(top & 255, top >> 8 & 255), max(top >> 16 & 255, top >> 24));
-            if ((ct.nan[f][0] & s0) | (ct.nan[f][1] & s1)) l = __int_as_float(0x7fffffff);   // the row sees a V that is NaN
           }
           float mx = -INFINITY;
 #pragma unroll
-          for (int j = 0; j < KT; ++j) mx = fmaxf(mx, __uint_as_float(a[j]));
-          const bool rescale = move_to(mx);
-          if (!(ok = general(a, Q8 ? reinterpret_cast<const float4*>(ct.fv[f]) : nullptr, rescale))) break;
+          for (int j = 0; j < KT; ++j) {
+            const float y = __fmul_rn(__uint_as_float(a[j]), keyed ? __fmul_rn(rt, ct.fk[f][j]) : rt);
+            a[j] = (j < 32 ? s0 : s1) >> (j & 31) & 1 ? __float_as_uint(y) : 0xff800000u;
+            mx = fmaxf(mx, __uint_as_float(a[j]));
+          }
+          if (partial) rescale = move_to(mx);
+          const bool gone = Q8 && em - er < -40;
+          const int dd = Q8 && !gone ? min(ref - er, 100) : 0;
+          const float ms = m == -INFINITY ? 0.f : m;
+          float sum = 0.f;
+#pragma unroll
+          for (int j = 0; j < KT; j += 2) {
+            float e[2];
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              e[b] = fast_exp2(__fadd_rn(__fadd_rn(__uint_as_float(a[j + b]), -ms), (float)dd));
+              sum += e[b];
+              if (Q8) e[b] = gone ? 0.f : keyed ? e[b] * ct.fv[f][j + b] : e[b];
+            }
+            w[j / 2] = pack2<FMT>(e[0], e[1]);
+          }
+          l = Q8 ? fmaf(sum, __int_as_float((127 - dd) << 23), l) : l + sum;
         }
+        // ---- P, once the product that read the last one is done (O is at rest then)
+        if (n_s && !(ok = warp_wait(&ct.pv_done[x], (n_s - 1) & 1, abort_flag, g.spin))) break;
+        ++n_s;
+        tc_fence_after();
+        if (__builtin_expect(rescale, 0)) {
+#pragma unroll 1
+          for (int b = 0; b < D; b += 16) {
+            uint32_t o[16];
+            tmem_ld_16(tO + b, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * cf);
+            tmem_st_16(tO + b, o);
+          }
+        }
+        // the other stream's threads may still read this stream's O of the piece before
+        if (__builtin_expect(!begun, 0) && piece && !(ok = warp_wait(&ct.epi_done, (piece - 1) & 1, abort_flag, g.spin))) break;
+        begun = true;
+        tmem_st32(tP, w);
+        tmem_wait_st();
+        tc_fence_before();
+        warp_arrive(&ct.p_ready[x]);
       }
       if (!ok) break;
       // ---- the next piece's Q goes out before this one's output: its first S runs under it
-      uint32_t v[D / 2];
       if (!(ok = __all_sync(0xffffffffu, piece_wait(piece + 1)))) break;
       const Piece& nxt = ct.piece[(piece + 1) % kPieces];
       more = nxt.tiles != 0;
-      if (more) load_q(nxt, row_of(nxt), v);
       float(&ml)[2][3][128] = ct.ml[piece & 1];
       if (!two) {
         ml[x][0][r] = m;
         ml[x][1][r] = l;
         ml[x][2][r] = begun ? (float)er : -1.f;                         // -1: the stream had no tile, its O is not there
-        mbar_arrive(smem_u32(&ct.ml_ready));
+        warp_arrive(&ct.ml_ready);
         if (!(ok = warp_wait(&ct.ml_ready, n_ml++ & 1, abort_flag, g.spin))) break;
       }
-      if (more) rf = put_q(row_of(nxt), v);
+      if (more) rf = put_q(nxt);
       if (!(ok = warp_wait(&ct.o_done, piece & 1, abort_flag, g.spin))) break;
       tc_fence_after();
       float f0 = 1.f, f1 = 0.f, M = m, L = l, E = (float)er;
@@ -905,6 +920,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (!Q8 && cw.in && *reinterpret_cast<volatile int*>(&ct.dropped)) {   // the dropped elements of keys this row sees
           const uint64_t* mk = g.mask ? g.mask + (size_t)(cur.bi.start + cw.node) * g.words : nullptr;
+#pragma unroll 1
           for (int key = max(cur.t0 * KT, cur.all_see); key < min(cur.t1 * KT, cur.n_keys); ++key)
             if (sees32(mk, g.words, cw.node, key - cur.bi.ctx) & 1) {
               const bf16* vp = static_cast<const bf16*>(c.v) + (cache_slot(c, cur.bi.row, cur.h, key)) * D + d;
@@ -929,7 +945,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
       }
       tc_fence_before();
-      mbar_arrive(smem_u32(&ct.epi_done));
+      warp_arrive(&ct.epi_done);
       if (cw.in && !to_out && (two || x == 0)) g.part_ml[part] = make_float2(M, L);
       if (tid == 128 && !sc.chunk_tiles && cur.t0 == 0 && cur.t1 < cur.tiles)
         sc.cuts[blockIdx.x] = TcCut{cur.u0, cur.e, cur.h, cur.index ? 1 : 0, cur.tiles};
