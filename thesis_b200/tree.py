@@ -35,20 +35,33 @@ FORMATS = {"bf16": (lib.KV_MODEL, torch.bfloat16), "f32": (lib.KV_MODEL, torch.f
 _FORMAT_OF = {dt: name for name, (_, dt) in FORMATS.items()}
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream     # current_stream() builds a Stream object first
+_current_device = torch._C._cuda_getDevice
+_fn = {}
+
+
 def _call(dev: torch.device, name: str, *args) -> None:
     """``lib.call`` with ``dev`` current and its current stream as the last argument."""
-    if torch.cuda.current_device() == dev.index:
-        lib.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+    fn = _fn.get(name)
+    if fn is None:
+        fn = _fn[name] = getattr(lib.load(), name)
+    i = dev.index
+    if _current_device() == i:
+        rc = fn(*args, _raw_stream(i))
     else:
         with torch.cuda.device(dev):
-            lib.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+            rc = fn(*args, _raw_stream(i))
+    if rc:
+        lib.check(rc, name)
+    lib.direct_launches += 1
 
 
-def _need(t: torch.Tensor, what: str, dev: torch.device, dtype, shape=None) -> torch.Tensor:
-    if t.dtype != dtype or t.device != dev or not t.is_contiguous() or (shape is not None and tuple(t.shape) != shape):
+def _need(t: torch.Tensor, what: str, dev: torch.device, dtype, shape=None) -> int:
+    """Address of ``t``, checked."""
+    if t.dtype is not dtype or t.device != dev or not t.is_contiguous() or (shape is not None and t.shape != shape):
         raise ValueError(f"{what}: need a contiguous {dtype} tensor {list(shape) if shape else ''} on {dev}, "
                          f"got {t.dtype} {list(t.shape)} on {t.device}")
-    return t
+    return t.data_ptr()
 
 
 class KVCache:
@@ -85,6 +98,8 @@ class KVCache:
         self.format = _FORMAT_OF[k.dtype]
         self.k, self.v, self.k_exp, self.v_exp = k, v, ke, ve
         self.device = k.device
+        self.quantised = k.dtype.itemsize == 1
+        self._dtypes = DTYPES if self.quantised else {k.dtype: DTYPES[k.dtype]}
         if self.quantised:
             for t, what in ((ke, "k_exp"), (ve, "v_exp")):
                 if t is None:
@@ -96,15 +111,12 @@ class KVCache:
                                   lib.ptr(ke if self.quantised else None), lib.ptr(ve if self.quantised else None))
         self.ref = C.byref(self.struct)
 
-    @property
-    def quantised(self) -> bool:
-        return self.k.dtype.itemsize == 1
-
     def model_dtype(self, t: torch.Tensor, what: str) -> int:
         """The library's dtype of an activation tensor that goes with this cache."""
-        if t.dtype not in DTYPES or t.device != self.device or (not self.quantised and t.dtype != self.k.dtype):
+        dt = self._dtypes.get(t.dtype)
+        if dt is None or t.device != self.device:
             raise ValueError(f"{what}: {t.dtype} on {t.device} does not go with a {self.format} cache on {self.device}")
-        return DTYPES[t.dtype]
+        return dt
 
 
 class TreeBatch:
@@ -155,11 +167,13 @@ class TreeBatch:
                                None if chains else self.parent.data_ptr(), self.tok_pos.data_ptr(), self.tok_slot.data_ptr(),
                                self.tok_row.data_ptr(), lib.ptr(self.mask))
         self.ref = C.byref(self.struct)
+        self.ptr_pos, self.ptr_slot, self.ptr_row = self.tok_pos.data_ptr(), self.tok_slot.data_ptr(), self.tok_row.data_ptr()
+        self.ptr_status = self.status.data_ptr()
         self.update()
 
     def update(self) -> None:
         """Positions, slots, rows and the mask from ``blk`` and ``parent`` (one launch)."""
-        _call(self.device, "eesd_tree_meta", self.ref, self._cache.max_batch, self._cache.max_seq, self.status.data_ptr())
+        _call(self.device, "eesd_tree_meta", self.ref, self._cache.max_batch, self._cache.max_seq, self.ptr_status)
 
     def check(self) -> None:
         """Raise if a call on this batch met a bad block, row, slot or path, or a wait that gave up; synchronises."""
@@ -176,19 +190,22 @@ def kv_append(qkv: torch.Tensor, cache: KVCache, tree: TreeBatch, rope_cos: torc
     """RoPE of q and k of ``qkv`` [n_tokens, (Hq + 2 Hkv) D] (rows may be strided) and the (quantising) append of k
     and v.  The rotated q goes to ``q_out`` [n_tokens, Hq D], or back into ``qkv``."""
     dt = cache.model_dtype(qkv, "qkv")
-    D, Hkv = cache.head_dim, cache.n_kv_heads
-    if qkv.dim() != 2 or qkv.shape[0] != tree.n_tokens or qkv.stride(1) != 1 or qkv.shape[1] % D:
-        raise ValueError(f"qkv: need [{tree.n_tokens}, (Hq + 2 Hkv) D] rows with unit stride, got {list(qkv.shape)}")
-    n_heads = qkv.shape[1] // D - 2 * Hkv
-    for t, what in ((rope_cos, "rope_cos"), (rope_sin, "rope_sin")):
-        _need(t, what, cache.device, torch.float32)
-    if rope_cos.shape != rope_sin.shape or rope_cos.dim() != 2 or rope_cos.shape[1] != D:
+    D, dev, n = cache.head_dim, cache.device, tree.n_tokens
+    n_heads = _heads(qkv, "qkv", n, D) - 2 * cache.n_kv_heads
+    cos = _need(rope_cos, "rope_cos", dev, torch.float32)
+    sin = _need(rope_sin, "rope_sin", dev, torch.float32, rope_cos.shape)
+    if rope_cos.dim() != 2 or rope_cos.shape[1] != D:
         raise ValueError(f"RoPE tables: need [positions, {D}]")
-    if q_out is not None:
-        _need(q_out, "q_out", cache.device, qkv.dtype, (tree.n_tokens, n_heads * D))
-    _call(cache.device, "eesd_kv_append", dt, cache.ref, layer, qkv.data_ptr(), _row_stride(qkv), n_heads,
-          tree.tok_pos.data_ptr(), tree.tok_slot.data_ptr(), tree.tok_row.data_ptr(), tree.n_tokens, rope_cos.data_ptr(),
-          rope_sin.data_ptr(), rope_cos.shape[0], lib.ptr(q_out), tree.status.data_ptr())
+    q = None if q_out is None else _need(q_out, "q_out", dev, qkv.dtype, (n, n_heads * D))
+    _call(dev, "eesd_kv_append", dt, cache.ref, layer, qkv.data_ptr(), _row_stride(qkv), n_heads, tree.ptr_pos, tree.ptr_slot,
+          tree.ptr_row, n, cos, sin, rope_cos.shape[0], q, tree.ptr_status)
+
+
+def _heads(t: torch.Tensor, what: str, n: int, D: int) -> int:
+    """Heads in the rows of ``t``: [n, heads D] with unit stride in a row."""
+    if t.dim() != 2 or t.shape[0] != n or t.stride(1) != 1 or t.shape[1] % D:
+        raise ValueError(f"{what}: need [{n}, heads x {D}] rows with unit stride, got {list(t.shape)}")
+    return t.shape[1] // D
 
 
 def _row_stride(t: torch.Tensor) -> int:
@@ -202,17 +219,13 @@ def kv_read(cache: KVCache, tok_row: torch.Tensor, tok_slot: torch.Tensor, k_out
     some = k_out if k_out is not None else v_out
     if some is None:
         raise ValueError("kv_read: both outputs are None")
-    dt = cache.model_dtype(some, "output")
-    n = tok_row.numel()
-    _need(tok_row, "tok_row", cache.device, torch.int32, (n,))
-    _need(tok_slot, "tok_slot", cache.device, torch.int32, (n,))
-    for t, what in ((k_out, "k_out"), (v_out, "v_out")):
-        if t is not None:
-            _need(t, what, cache.device, some.dtype, (n, cache.n_kv_heads, cache.head_dim))
-    if status is not None:
-        _need(status, "status", cache.device, torch.int32, (1,))
-    _call(cache.device, "eesd_kv_read", dt, cache.ref, layer, tok_slot.data_ptr(), tok_row.data_ptr(), n, lib.ptr(k_out),
-          lib.ptr(v_out), lib.ptr(status))
+    dt, dev, n = cache.model_dtype(some, "output"), cache.device, tok_row.numel()
+    shape = (n, cache.n_kv_heads, cache.head_dim)
+    row, slot = _need(tok_row, "tok_row", dev, torch.int32, (n,)), _need(tok_slot, "tok_slot", dev, torch.int32, (n,))
+    k = None if k_out is None else _need(k_out, "k_out", dev, some.dtype, shape)
+    v = None if v_out is None else _need(v_out, "v_out", dev, some.dtype, shape)
+    st = None if status is None else _need(status, "status", dev, torch.int32, (1,))
+    _call(dev, "eesd_kv_read", dt, cache.ref, layer, slot, row, n, k, v, st)
 
 
 def attention_workspace(tree: TreeBatch, cache: KVCache, n_heads: int, dtype: torch.dtype = torch.bfloat16,
@@ -231,20 +244,16 @@ def tree_attention(q: torch.Tensor, cache: KVCache, tree: TreeBatch, out: Option
     be strided, e.g. the q columns of a fused projection); the result is [n_tokens, Hq D] in q's dtype.  See
     ``eesd_attn_tree`` for what a node sees and for ``split_keys``."""
     dt = cache.model_dtype(q, "q")
-    D = cache.head_dim
-    if q.dim() != 2 or q.shape[0] != tree.n_tokens or q.stride(1) != 1 or q.shape[1] % D:
-        raise ValueError(f"q: need [{tree.n_tokens}, Hq D] rows with unit stride, got {list(q.shape)}")
-    n_heads = q.shape[1] // D
+    dev, n = cache.device, tree.n_tokens
+    n_heads = _heads(q, "q", n, cache.head_dim)
     if out is None:
-        out = torch.empty(tree.n_tokens, n_heads * D, dtype=q.dtype, device=q.device)
-    else:
-        _need(out, "out", cache.device, q.dtype, (tree.n_tokens, n_heads * D))
+        out = torch.empty(n, q.shape[1], dtype=q.dtype, device=dev)
+    o = _need(out, "out", dev, q.dtype, (n, q.shape[1]))
     if workspace is None:
         workspace = attention_workspace(tree, cache, n_heads, q.dtype, split_keys)
-    else:
-        _need(workspace, "workspace", cache.device, torch.uint8)
-    _call(cache.device, "eesd_attn_tree", dt, cache.ref, layer, tree.ref, q.data_ptr(), _row_stride(q), n_heads, out.data_ptr(),
-          split_keys, workspace.data_ptr(), workspace.numel(), tree.status.data_ptr())
+    ws = _need(workspace, "workspace", dev, torch.uint8)
+    _call(dev, "eesd_attn_tree", dt, cache.ref, layer, tree.ref, q.data_ptr(), _row_stride(q), n_heads, o, split_keys, ws,
+          workspace.numel(), tree.ptr_status)
     return out
 
 
@@ -252,17 +261,17 @@ def tree_accept(y: torch.Tensor, ids: torch.Tensor, tree: TreeBatch, path: torch
                 next_ids: torch.Tensor) -> None:
     """Greedy walk through every block's tree: ``ids`` [n_tokens] the nodes' tokens, ``y`` [n_tokens] the model's
     token after each node.  ``path`` [n_blocks, max_nodes] (-1 behind the end), ``n_acc`` and ``next_ids`` [n_blocks]."""
-    for t, what, shape in ((y, "y", (tree.n_tokens,)), (ids, "ids", (tree.n_tokens,)),
-                           (path, "path", (tree.n_blocks, tree.max_nodes)), (n_acc, "n_acc", (tree.n_blocks,)),
-                           (next_ids, "next_ids", (tree.n_blocks,))):
-        _need(t, what, tree.device, torch.int32, shape)
-    _call(tree.device, "eesd_tree_accept", y.data_ptr(), ids.data_ptr(), tree.ref, path.data_ptr(), n_acc.data_ptr(),
-          next_ids.data_ptr(), tree.status.data_ptr())
+    dev, i32, n, nb = tree.device, torch.int32, (tree.n_tokens,), (tree.n_blocks,)
+    _call(dev, "eesd_tree_accept", _need(y, "y", dev, i32, n), _need(ids, "ids", dev, i32, n), tree.ref,
+          _need(path, "path", dev, i32, (tree.n_blocks, tree.max_nodes)), _need(n_acc, "n_acc", dev, i32, nb),
+          _need(next_ids, "next_ids", dev, i32, nb), tree.ptr_status)
 
 
 def kv_compact(cache: KVCache, tree: TreeBatch, path: torch.Tensor, n_acc: torch.Tensor) -> None:
     """Move the accepted path's K and V of every layer to the slots behind ``ctx`` (blocks on different rows)."""
-    _need(path, "path", tree.device, torch.int32, (tree.n_blocks, tree.max_nodes))
-    _need(n_acc, "n_acc", tree.device, torch.int32, (tree.n_blocks,))
-    dt = lib.F32 if cache.format == "f32" else lib.BF16
-    _call(cache.device, "eesd_kv_compact", dt, cache.ref, tree.ref, path.data_ptr(), n_acc.data_ptr(), tree.status.data_ptr())
+    dev, i32 = tree.device, torch.int32
+    if cache.device != dev:
+        raise ValueError(f"kv_compact: a batch on {dev} and a cache on {cache.device}")
+    _call(dev, "eesd_kv_compact", lib.F32 if cache.format == "f32" else lib.BF16, cache.ref, tree.ref,
+          _need(path, "path", dev, i32, (tree.n_blocks, tree.max_nodes)), _need(n_acc, "n_acc", dev, i32, (tree.n_blocks,)),
+          tree.ptr_status)
