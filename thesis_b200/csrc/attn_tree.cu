@@ -187,10 +187,14 @@ __global__ void __launch_bounds__(128, MmaShape<D, FMT, MT>::CTAS)
   constexpr bool Q8 = FMT != EESD_KV_MODEL;
   constexpr int KG = P::KG, NS = P::NS, ROWS = P::ROWS, LDQ = P::LDQ, OLD = P::OLD, ND = D / 8, KK = D / 16;
   constexpr int HALF = 4096;                           // K bytes (then V bytes) of a stage
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&kmap);
+    tma_prefetch_desc(&vmap);
+  }
   pdl_trigger();
   pdl_wait();
   extern __shared__ uint8_t smem8[];
-  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem8) + 1023) & ~uintptr_t(1023));
+  uint8_t* sm = smem8 + (-smem_u32(smem8) & 1023);                      // an offset: the compiler still knows it as shared memory
   uint8_t* stages = sm;                                                 // [4 warps][NS][K | V]
   uint8_t* qs = sm + 4 * NS * P::STAGE;
   uint8_t* exps = qs + P::Q_BYTES;                                      // [4][NS][K bytes 64 | V bytes 64]
@@ -242,37 +246,56 @@ __global__ void __launch_bounds__(128, MmaShape<D, FMT, MT>::CTAS)
     for (int i = 0; i < NS && i < my_groups; ++i) issue(i);
   }
   if (threadIdx.x == 0) flags[0] = flags[1] = 0;
-  // q rows of the tile (zeros behind nrows) and their nodes' masks
-  for (int r = warp; r < ROWS; r += 4) {
-    const int R = r0 + r;
+  // q rows of the tile (zeros behind nrows) and their nodes' masks: TPR threads per row, all loads at once
+  {
+    constexpr int TPR = 128 / ROWS, V = D / 8 / TPR;                    // 16-byte chunks per thread, TPR apart
+    const int r = threadIdx.x / TPR, part = threadIdx.x % TPR, R = r0 + r;
     const bool in = r < nrows;
-    const bf16* src = q + (size_t)(bi.start + (in ? R / g.G : 0)) * g.ld_q + (kvh * g.G + (in ? R % g.G : 0)) * D;
-    if constexpr (!Q8) {
-      for (int e = lane * 2; e < D; e += 64)
-        *reinterpret_cast<uint32_t*>(qs + (r * LDQ + e) * 2) = in ? *reinterpret_cast<const uint32_t*>(src + e) : 0u;
-    } else {
-      uint32_t v[D / 64], amax = 0;
+    const int node = in ? R / g.G : 0;
+    const bf16* src = q + (size_t)(bi.start + node) * g.ld_q + (kvh * g.G + (in ? R - node * g.G : 0)) * D;
+    uint4 u[V];
 #pragma unroll
-      for (int j = 0; j < D / 64; ++j) {
-        v[j] = in ? *reinterpret_cast<const uint32_t*>(src + lane * 2 + 64 * j) : 0u;
-        amax = max(amax, max(v[j] << 16 & 0x7fff0000u, v[j] & 0x7fff0000u));
+    for (int i = 0; i < V; ++i) u[i] = in ? *reinterpret_cast<const uint4*>(src + (part + i * TPR) * 8) : make_uint4(0, 0, 0, 0);
+    uint64_t mk[4 / (TPR < 4 ? TPR : 4)];
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(mk) / 8); ++i) {
+      const int w = part + i * TPR;
+      mk[i] = g.mask && in && w < g.words ? g.mask[(size_t)(bi.start + node) * g.words + w] : 0ull;
+    }
+    if constexpr (!Q8) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) *reinterpret_cast<uint4*>(qs + (r * LDQ + (part + i * TPR) * 8) * 2) = u[i];
+    } else {
+      uint32_t amax = 0;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const uint32_t x[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+#pragma unroll
+        for (int y = 0; y < 4; ++y) amax = max(amax, max(x[y] << 16 & 0x7fff0000u, x[y] & 0x7fff0000u));
       }
-      amax = __reduce_max_sync(0xffffffffu, amax);
+#pragma unroll
+      for (int o = 1; o < TPR; o <<= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
       // take the largest element's power of two out (|q'| < 2): f16 keeps every bit of a bf16 down to 2^-14 of
       // the row's largest, and below that an absolute 2^-25 of it
       const int e = min(max((int)(amax >> 23), 27), 227);
       const float inv = __int_as_float((254 - e) << 23);
-      if (lane == 0) qscale[r] = __int_as_float(e << 23);
+      if (part == 0) qscale[r] = __int_as_float(e << 23);
 #pragma unroll
-      for (int j = 0; j < D / 64; ++j) {
-        const int d = lane * 2 + 64 * j;                                // dims d, d + 1 of the row, in fragment order
-        const int t = d / (D / 4), kk = d % (D / 4) / 4, pair = d % 4 / 2;
-        const uint32_t h = pack2<FMT>(__uint_as_float(v[j] << 16) * inv, __uint_as_float(v[j] & 0xffff0000u) * inv);
-        const int m = r >> 4, rr = r & 15;                              // a0: row g, pair 0; a1: row g + 8; a2, a3: pair 1
-        reinterpret_cast<uint32_t*>(qs)[((m * KK + kk) * 32 + (rr & 7) * 4 + t) * 4 + (rr >> 3) + 2 * pair] = h;
+      for (int i = 0; i < V; ++i) {
+        const uint32_t x[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const int d = (part + i * TPR) * 8 + 2 * y;                   // dims d, d + 1 of the row, in fragment order
+          const int t = d / (D / 4), kk = d % (D / 4) / 4, pair = d % 4 / 2;
+          const uint32_t h = pack2<FMT>(__uint_as_float(x[y] << 16) * inv, __uint_as_float(x[y] & 0xffff0000u) * inv);
+          const int m = r >> 4, rr = r & 15;                            // a0: row g, pair 0; a1: row g + 8; a2, a3: pair 1
+          reinterpret_cast<uint32_t*>(qs)[((m * KK + kk) * 32 + (rr & 7) * 4 + t) * 4 + (rr >> 3) + 2 * pair] = h;
+        }
       }
     }
-    if (lane < 4) masks[r * 4 + lane] = (g.mask && in && lane < g.words) ? g.mask[(size_t)(bi.start + R / g.G) * g.words + lane] : 0ull;
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(mk) / 8); ++i)
+      if (part + i * TPR < 4) masks[r * 4 + part + i * TPR] = mk[i];
   }
   __syncthreads();
 
@@ -732,7 +755,8 @@ cudaError_t launch_mma(const Plan& p, const TreeGeom& g, const CacheGeom& c, con
                        const void* q, void* out, cudaStream_t s) {
   using S = MmaShape<D, FMT, MT>;
   auto kernel = attn_tree_mma_kernel<D, FMT, MT>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::smem);
+  static SmemOnce once;
+  const cudaError_t e = once.set(reinterpret_cast<const void*>(kernel), S::smem);
   if (e != cudaSuccess) return e;
   return launch_pdl(kernel, dim3(p.splits, p.tiles * c.n_kv_heads, n_blocks), dim3(128), S::smem, s, km, vm, g, c,
                     static_cast<const bf16*>(q), static_cast<bf16*>(out));
@@ -747,7 +771,8 @@ template <typename T, int FMT, int D>
 cudaError_t launch_simt(const TreeGeom& g, const CacheGeom& c, int n_blocks, const void* q, void* out, cudaStream_t s) {
   const dim3 grid((g.max_nodes * g.G + 31) / 32, c.n_kv_heads, n_blocks);
   constexpr size_t smem = (32 * D + 32 * (D + 1) + 32 * D) * 4;
-  const cudaError_t e = cudaFuncSetAttribute(attn_tree_simt_kernel<T, FMT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static SmemOnce once;
+  const cudaError_t e = once.set(reinterpret_cast<const void*>(attn_tree_simt_kernel<T, FMT, D>), smem);
   if (e != cudaSuccess) return e;
   return launch_pdl(attn_tree_simt_kernel<T, FMT, D>, grid, dim3(128), smem, s, g, c, static_cast<const T*>(q), static_cast<T*>(out));
 }

@@ -1030,7 +1030,8 @@ cudaError_t launch(const TcSchedule& sc, const TreeGeom& g, const CacheGeom& c, 
                    const void* q, void* out, cudaStream_t s) {
   using S = TcShape<D, FMT>;
   auto kernel = attn_tree_tc_kernel<D, FMT>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::smem);
+  static SmemOnce once;
+  cudaError_t e = once.set(reinterpret_cast<const void*>(kernel), S::smem);
   if (e != cudaSuccess) return e;
   e = launch_pdl(kernel, dim3(sc.ctas), dim3(kThreads), S::smem, s, km, vm, g, c, sc, static_cast<const bf16*>(q), static_cast<bf16*>(out));
   if (e == cudaSuccess && !sc.chunk_tiles && sc.ctas > 1)
