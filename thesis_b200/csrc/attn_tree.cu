@@ -127,17 +127,23 @@ __global__ void __launch_bounds__(128) attn_tree_simt_kernel(TreeGeom g, CacheGe
 }
 
 // ---------------------------------------------------------------- small row tiles: mma.sync
-// One CTA per (row tile of 16 MT rows, KV head, key range of a block): a few query rows against a stream of
-// keys, bound by the bytes of K and V.  Its 4 warps are independent: warp w takes every fourth group of KG keys
-// (16 .. 64, 8 KB of K and V) through a TMA ring of its own, so nothing in the key loop waits for another warp;
-// the warps' running (max, sum, output) meet once at the end.
+// One CTA per (row tile of 8 NT rows, KV head, key range of a block): a few query rows against a stream of keys,
+// bound by the bytes of K and V.  Its 4 warps are independent: warp w takes every fourth group of KG keys (16 .. 64,
+// 8 KB of K and V) through a TMA ring of its own, so nothing in the key loop waits for another warp; the warps'
+// running (max, sum, output) meet once at the end.
 //
-// S = Q K^T and O = P V run on m16n8k16.  Both products may order their contraction index as they like, which
-// the 8-bit formats use: thread (g, t) = (lane / 4, lane % 4) takes the dims [t D/4, (t + 1) D/4) of key g as K
-// fragments and the dims [g D/8, (g + 1) D/8) of keys 2t, 2t + 1, 2t + 8, 2t + 9 as V fragments, so K and V come
-// from shared memory as 16-byte words and turn into f16 pairs in registers, without a transpose.  The values'
-// powers of two never touch the operands: K's scale multiplies the score, V's the weight (relative to the
-// largest one so far of the row, eref, as the running maximum does), a power of two of each q row its f16 form.
+// The products are the transposed ones, S^T = K Q^T and O^T = V^T P^T on m16n8k16: 16 keys (or dims) fill the M side,
+// and the query rows, 4 to 32 of them, are the N side in steps of 8, so few rows cost few products and few registers
+// (O^T is 32 registers per 8 rows of 128 dims).  A thread has S of two rows; a row's maximum would be a reduction over 8
+// lanes, so it is only taken when some score is 2^8 above the running reference.  P^T becomes an operand by
+// transposing its 8 x 8 blocks between lanes (movmatrix).
+//
+// Both products may order their contraction index, and O^T its rows, as they like, which the 8-bit formats use:
+// thread (g, t) = (lane / 4, lane % 4) takes the dims [t D/4, (t + 1) D/4) of keys g and g + 8 as K fragments and the
+// dims [g D/8, (g + 1) D/8) of keys 2t, 2t + 1, 2t + 8, 2t + 9 as V fragments, so K and V come from shared memory as
+// 16-byte words and turn into f16 pairs in registers, without a transpose.  The values' powers of two never touch the
+// operands: K's scale multiplies the score, V's the weight (relative to the largest one so far of the row, er, as the
+// running maximum does), a power of two of each q row its f16 form.
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -148,10 +154,10 @@ __device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t (&r)[4]) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr));
 }
-__device__ __forceinline__ uint2 lds64(uint32_t addr) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
-  return v;
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
 template <int FMT> __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if constexpr (FMT == EESD_KV_MODEL)
@@ -165,27 +171,27 @@ template <int FMT> __device__ __forceinline__ void mma16816(float (&c)[4], const
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-template <int D, int FMT, int MT> struct MmaShape {
+
+template <int D, int FMT, int NT> struct MmaShape {
   static constexpr int kEb = FMT == EESD_KV_MODEL ? 2 : 1;
   static constexpr int KG = 4096 / (D * kEb);          // keys per group: 4 KB of K, 4 KB of V
-  static constexpr int NS = MT == 1 ? 2 : 3;           // ring stages per warp
-  static constexpr int CTAS = MT == 1 ? 3 : 2;         // resident CTAs per SM
-  static constexpr int ROWS = 16 * MT;
+  static constexpr int CTAS = NT == 4 || (NT == 3 && D == 128 && kEb == 1) ? 2 : 3;   // resident CTAs per SM, by registers
+  static constexpr int NS = CTAS == 2 ? 3 : 2;         // ring stages per warp
+  static constexpr int ROWS = 8 * NT;
   static constexpr int STAGE = 8192;
-  static constexpr int LDQ = D + 8;                    // bf16: padded q row (elements), conflict-free ldmatrix
-  static constexpr int Q_BYTES = FMT == EESD_KV_MODEL ? ROWS * LDQ * 2 : MT * (D / 16) * 512;
+  static constexpr int Q_BYTES = ROWS * D * 2;         // fragment order: [n-tile][k-step][lane] pairs of words
   static constexpr int OLD = D + 4;
   static constexpr size_t smem = 1024 + 4 * NS * STAGE + Q_BYTES + 4 * NS * 128 + ROWS * 32 + ROWS * 4 + 4 * NS * 8 + 16;
   static_assert((4 * ROWS * OLD + 12 * ROWS) * 4 <= 4 * NS * STAGE, "the merge does not fit the stage memory");
 };
 
-template <int D, int FMT, int MT>
-__global__ void __launch_bounds__(128, MmaShape<D, FMT, MT>::CTAS)
+template <int D, int FMT, int NT>
+__global__ void __launch_bounds__(128, MmaShape<D, FMT, NT>::CTAS)
     attn_tree_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, TreeGeom g, CacheGeom c,
                          const bf16* __restrict__ q, bf16* __restrict__ out) {
-  using P = MmaShape<D, FMT, MT>;
+  using P = MmaShape<D, FMT, NT>;
   constexpr bool Q8 = FMT != EESD_KV_MODEL;
-  constexpr int KG = P::KG, NS = P::NS, ROWS = P::ROWS, LDQ = P::LDQ, OLD = P::OLD, ND = D / 8, KK = D / 16;
+  constexpr int KG = P::KG, NS = P::NS, ROWS = P::ROWS, OLD = P::OLD, MD = D / 16;   // 16-dim steps of both products
   constexpr int HALF = 4096;                           // K bytes (then V bytes) of a stage
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&kmap);
@@ -219,18 +225,18 @@ __global__ void __launch_bounds__(128, MmaShape<D, FMT, MT>::CTAS)
   const int slot0 = (int)cache_slot(c, bi.row, kvh, 0);                 // fits: the entry point bounds the layer's slots
 
   const uint32_t st0 = smem_u32(stages) + warp * NS * P::STAGE;
-  const uint32_t ex0 = smem_u32(exps) + warp * NS * 128;
   const uint32_t fb0 = smem_u32(full + warp * NS);
+  uint8_t* const ex0 = exps + warp * NS * 128;
   auto issue = [&](int i) {                                             // lane 0: this warp's i-th group
     const int s = i % NS, key = k_lo + (warp + 4 * i) * KG;
     const uint32_t fb = fb0 + s * 8, dst = st0 + s * P::STAGE;
     if constexpr (Q8) {
-      const uint32_t eb = min(KG, c.max_seq - key);                     // max_seq % 16 == 0 and key % 16 == 0
+      const uint32_t eb = min(KG, c.max_seq - key), ex = smem_u32(ex0 + s * 128);   // max_seq % 16 == 0 and key % 16 == 0
       mbar_arrive_expect_tx(fb, P::STAGE + 2 * eb);
       tma_load_2d(dst, &kmap, 0, slot0 + key, fb);
       tma_load_2d(dst + HALF, &vmap, 0, slot0 + key, fb);
-      bulk_g2s(ex0 + s * 128, c.ke + slot0 + key, eb, fb);
-      bulk_g2s(ex0 + s * 128 + 64, c.ve + slot0 + key, eb, fb);
+      bulk_g2s(ex, c.ke + slot0 + key, eb, fb);
+      bulk_g2s(ex + 64, c.ve + slot0 + key, eb, fb);
     } else {
       mbar_arrive_expect_tx(fb, P::STAGE);
 #pragma unroll
@@ -246,26 +252,19 @@ __global__ void __launch_bounds__(128, MmaShape<D, FMT, MT>::CTAS)
     for (int i = 0; i < NS && i < my_groups; ++i) issue(i);
   }
   if (threadIdx.x == 0) flags[0] = flags[1] = 0;
-  // q rows of the tile (zeros behind nrows) and their nodes' masks: TPR threads per row, all loads at once
+  // q rows of the tile (zeros behind nrows) and their nodes' masks, all loads at once: 4 threads per row
   {
-    constexpr int TPR = 128 / ROWS, V = D / 8 / TPR;                    // 16-byte chunks per thread, TPR apart
-    const int r = threadIdx.x / TPR, part = threadIdx.x % TPR, R = r0 + r;
+    constexpr int V = D / 32;                                           // 16-byte chunks per thread, 4 apart
+    const int r = threadIdx.x / 4, part = threadIdx.x % 4, R = r0 + r;
     const bool in = r < nrows;
     const int node = in ? R / g.G : 0;
     const bf16* src = q + (size_t)(bi.start + node) * g.ld_q + (kvh * g.G + (in ? R - node * g.G : 0)) * D;
     uint4 u[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) u[i] = in ? *reinterpret_cast<const uint4*>(src + (part + i * TPR) * 8) : make_uint4(0, 0, 0, 0);
-    uint64_t mk[4 / (TPR < 4 ? TPR : 4)];
-#pragma unroll
-    for (int i = 0; i < (int)(sizeof(mk) / 8); ++i) {
-      const int w = part + i * TPR;
-      mk[i] = g.mask && in && w < g.words ? g.mask[(size_t)(bi.start + node) * g.words + w] : 0ull;
-    }
-    if constexpr (!Q8) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) *reinterpret_cast<uint4*>(qs + (r * LDQ + (part + i * TPR) * 8) * 2) = u[i];
-    } else {
+    for (int i = 0; i < V; ++i) u[i] = in ? *reinterpret_cast<const uint4*>(src + (part + i * 4) * 8) : make_uint4(0, 0, 0, 0);
+    const uint64_t mk = g.mask && in && part < g.words ? g.mask[(size_t)(bi.start + node) * g.words + part] : 0ull;
+    float inv = 1.f;
+    if constexpr (Q8) {
       uint32_t amax = 0;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
@@ -273,241 +272,225 @@ __global__ void __launch_bounds__(128, MmaShape<D, FMT, MT>::CTAS)
 #pragma unroll
         for (int y = 0; y < 4; ++y) amax = max(amax, max(x[y] << 16 & 0x7fff0000u, x[y] & 0x7fff0000u));
       }
-#pragma unroll
-      for (int o = 1; o < TPR; o <<= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
       // take the largest element's power of two out (|q'| < 2): f16 keeps every bit of a bf16 down to 2^-14 of
       // the row's largest, and below that an absolute 2^-25 of it
       const int e = min(max((int)(amax >> 23), 27), 227);
-      const float inv = __int_as_float((254 - e) << 23);
-      if (part == 0) qscale[r] = __int_as_float(e << 23);
+      inv = __int_as_float((254 - e) << 23);
+      if (r < ROWS && part == 0) qscale[r] = __int_as_float(e << 23);
+    }
+    if (r < ROWS) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const uint32_t x[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
-          const int d = (part + i * TPR) * 8 + 2 * y;                   // dims d, d + 1 of the row, in fragment order
-          const int t = d / (D / 4), kk = d % (D / 4) / 4, pair = d % 4 / 2;
-          const uint32_t h = pack2<FMT>(__uint_as_float(x[y] << 16) * inv, __uint_as_float(x[y] & 0xffff0000u) * inv);
-          const int m = r >> 4, rr = r & 15;                            // a0: row g, pair 0; a1: row g + 8; a2, a3: pair 1
-          reinterpret_cast<uint32_t*>(qs)[((m * KK + kk) * 32 + (rr & 7) * 4 + t) * 4 + (rr >> 3) + 2 * pair] = h;
+          const int d = (part + i * 4) * 8 + 2 * y;                     // dims d, d + 1 of the row; word 0 or 1 of a B fragment
+          const int t = Q8 ? d / (D / 4) : d % 8 / 2, kk = Q8 ? d % (D / 4) / 4 : d / 16, w = Q8 ? d % 4 / 2 : d % 16 / 8;
+          const uint32_t h = Q8 ? pack2<FMT>(__uint_as_float(x[y] << 16) * inv, __uint_as_float(x[y] & 0xffff0000u) * inv) : x[y];
+          reinterpret_cast<uint32_t*>(qs)[(((r >> 3) * MD + kk) * 32 + (r & 7) * 4 + t) * 2 + w] = h;
         }
       }
+      masks[r * 4 + part] = mk;
     }
-#pragma unroll
-    for (int i = 0; i < (int)(sizeof(mk) / 8); ++i)
-      if (part + i * TPR < 4) masks[r * 4 + part + i * TPR] = mk[i];
   }
   __syncthreads();
 
-  float o[MT][ND][4], m[MT][2], l[MT][2], rf[MT][2];
-  int er[MT][2];                                                        // 8-bit: exponent byte of the largest V scale so far
+  // this thread's rows of n-tile n: 8 n + 2 tq, + 1
+  float o[NT][MD][4], m[NT][2], l[NT][2], rf[NT][2];
+  int er[NT][2];                                                        // 8-bit: exponent byte of the largest V scale so far
 #pragma unroll
-  for (int a = 0; a < MT; ++a)
+  for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      m[a][h] = -INFINITY;
-      l[a][h] = 0.f;
-      er[a][h] = 0;
-      rf[a][h] = g.scale * 1.4426950408889634f * (Q8 ? qscale[a * 16 + h * 8 + gq] * kHalfUnit<FMT> : 1.f);
+      m[n][h] = -INFINITY;
+      l[n][h] = 0.f;
+      er[n][h] = 1;
+      rf[n][h] = g.scale * 1.4426950408889634f * (Q8 ? qscale[8 * n + 2 * tq + h] * kHalfUnit<FMT> : 1.f);
 #pragma unroll
-      for (int n = 0; n < ND; ++n) o[a][n][2 * h] = o[a][n][2 * h + 1] = 0.f;
+      for (int d = 0; d < MD; ++d) o[n][d][h] = o[n][d][2 + h] = 0.f;
     }
+  const uint2* qf = reinterpret_cast<const uint2*>(qs) + lane;
   int done = 0;                                                         // groups waited for
-  bool ok = true;
+  bool ok = true, hit = false;
+#pragma unroll 1
   for (int i = 0; i < my_groups; ++i) {
     const int s = i % NS;
-    ok = mbar_wait(fb0 + s * 8, (i / NS) & 1, flags, g.spin);
-    if (!__all_sync(0xffffffffu, ok)) {
-      ok = false;
-      break;
-    }
+    ok = __all_sync(0xffffffffu, mbar_wait(fb0 + s * 8, (i / NS) & 1, flags, g.spin));
+    if (!ok) break;
     done = i + 1;
-    const uint32_t kt = st0 + s * P::STAGE, vt = kt + HALF, ex = ex0 + s * 128;
+    const uint32_t kt = st0 + s * P::STAGE, vt = kt + HALF;
+    const uint8_t* ks = stages + (warp * NS + s) * P::STAGE;
+    const uint8_t* vs = ks + HALF;
+    const uint8_t* ex = ex0 + s * 128;
     const int key0 = k_lo + (warp + 4 * i) * KG;
     const bool partial = key0 + KG > min(all_see, k_hi);                // some row does not see some key of the group
-    float sc[MT][KG / 8][4];
-#pragma unroll
-    for (int a = 0; a < MT; ++a)
-#pragma unroll
-      for (int n = 0; n < KG / 8; ++n) sc[a][n][0] = sc[a][n][1] = sc[a][n][2] = sc[a][n][3] = 0.f;
-    if constexpr (!Q8) {
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-        uint32_t a[MT][4];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-          ldsm_x4(smem_u32(qs) + ((mt * 16 + (lane & 15)) * LDQ + kk * 16 + (lane >> 4) * 8) * 2, a[mt]);
-        const int dim = kk * 16 + ((lane >> 3) & 1) * 8;
-#pragma unroll
-        for (int n2 = 0; n2 < KG / 16; ++n2) {
-          const int key = n2 * 16 + (lane & 7) + ((lane >> 4) << 3);
-          uint32_t b[4];
-          ldsm_x4(kt + (dim >> 6) * KG * 128 + key * 128 + ((((dim & 63) >> 3) ^ (key & 7)) << 4), b);
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            mma16816<FMT>(sc[mt][2 * n2], a[mt], b[0], b[1]);
-            mma16816<FMT>(sc[mt][2 * n2 + 1], a[mt], b[2], b[3]);
-          }
-        }
-      }
-    } else {
-#pragma unroll
-      for (int n = 0; n < KG / 8; ++n) {
-        const int key = n * 8 + gq;
-#pragma unroll
-        for (int u = 0; u < D / 64; ++u) {                              // 16 bytes: four k-steps
-          const int ch = tq * (D / 64) + u;
-          const uint32_t sw = D == 128 ? (ch ^ (key & 7)) << 4 : (ch ^ ((key >> 1) & 3)) << 4;
-          const uint4 w = lds128(kt + key * D + sw);
-          const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            uint32_t b0, b1;
-            unpack4<FMT>(ww[x], b0, b1);
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-              const uint4 av = lds128(smem_u32(qs) + ((mt * KK + u * 4 + x) * 32 + lane) * 16);
-              const uint32_t a[4] = {av.x, av.y, av.z, av.w};
-              mma16816<FMT>(sc[mt][n], a, b0, b1);
-            }
-          }
-        }
-      }
-    }
-    // per-key factors of the 8-bit formats: this thread's columns are keys 8 n + 2 tq, + 1
-    float fk[Q8 ? KG / 8 : 1][2], fv[Q8 ? KG / 8 : 1][2];
-    int evb[Q8 ? KG / 8 : 1][2];
-    if constexpr (Q8) {
-#pragma unroll
-      for (int n = 0; n < KG / 8; ++n) {
-        const uint32_t kb = lds_u16(ex + n * 8 + 2 * tq), vb = lds_u16(ex + 64 + n * 8 + 2 * tq);
-        fk[n][0] = exp_scale(kb & 255);
-        fk[n][1] = exp_scale(kb >> 8);
-        evb[n][0] = vb & 255;
-        evb[n][1] = vb >> 8;
-        fv[n][0] = exp_scale(evb[n][0]);
-        fv[n][1] = exp_scale(evb[n][1]);
-      }
-    }
-    int emax = 0;
-    if constexpr (Q8) {
-      if (!partial) {
-#pragma unroll
-        for (int n = 0; n < KG / 8; ++n)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) emax = max(emax, evb[n][e] == 255 ? 0 : evb[n][e]);
-        emax = __reduce_max_sync(0xffffffffu, emax);
-      }
-    }
-#pragma unroll
-    for (int a = 0; a < MT; ++a) {
-      float corr[2];
-      bool moved = false;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = a * 16 + h * 8 + gq;
-        uint32_t see[KG > 32 ? 2 : 1] = {};
-        int em = emax;
-        if (partial) {
-          em = 0;
-          const int node = (r0 + min(r, nrows - 1)) / g.G;
-#pragma unroll
-          for (int w = 0; w < (KG > 32 ? 2 : 1); ++w) {
-            const int kb = key0 + 32 * w;
-            see[w] = sees32(g.mask ? masks + r * 4 : nullptr, 4, node, kb - bi.ctx);
-            const int left = k_hi - kb;
-            if (left < 32) see[w] &= left <= 0 ? 0u : (1u << left) - 1;
-          }
-        }
-        float mx = -INFINITY;
-#pragma unroll
-        for (int n = 0; n < KG / 8; ++n)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float& x = sc[a][n][2 * h + e];
-            x *= Q8 ? rf[a][h] * fk[Q8 ? n : 0][e] : rf[a][h];
-            if (partial) {
-              const int bit = n * 8 + 2 * tq + e;
-              const bool sees = see[bit >> 5] >> (bit & 31) & 1;
-              if (!sees) x = -INFINITY;
-              if constexpr (Q8) em = max(em, sees && evb[n][e] != 255 ? evb[n][e] : 0);
-            }
-            mx = fmaxf(mx, x);
-          }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        if (Q8 && partial) {
-          em = max(em, __shfl_xor_sync(0xffffffffu, em, 1));
-          em = max(em, __shfl_xor_sync(0xffffffffu, em, 2));
-        }
-        const float mn = fmaxf(m[a][h], mx);
-        const float ms = mn == -INFINITY ? 0.f : mn;
-        corr[h] = fast_exp2(m[a][h] - ms);
-        moved = moved || mn != m[a][h];
-        m[a][h] = mn;
-        float rv = 0.f;
-        if constexpr (Q8) {
-          const int en = max(er[a][h], em);
-          rv = __int_as_float((254 - max(en, 1)) << 23);                // 2^-(en - 127)
-        }
-        float sum = 0.f;
-#pragma unroll
-        for (int n = 0; n < KG / 8; ++n)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float& x = sc[a][n][2 * h + e];
-            const float p = fast_exp2(x - ms);
-            sum += p;
-            if constexpr (Q8) x = p == 0.f ? 0.f : p * (fv[n][e] * rv);
-            else x = p;
-          }
-        l[a][h] = l[a][h] * corr[h] + sum;
-        if constexpr (Q8) {
-          const int en = max(er[a][h], em);
-          if (en != er[a][h]) {
-            corr[h] *= er[a][h] == 0 ? 0.f : fast_exp2((float)(er[a][h] - en));
-            moved = true;
-          }
-          er[a][h] = en;
-        }
-      }
-      if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-        for (int n = 0; n < ND; ++n) {
-          o[a][n][0] *= corr[0];
-          o[a][n][1] *= corr[0];
-          o[a][n][2] *= corr[1];
-          o[a][n][3] *= corr[1];
-        }
-      }
-    }
-    bool hit = false;
-#pragma unroll
+#pragma unroll 1
     for (int st = 0; st < KG / 16; ++st) {
-      uint32_t p[MT][4];
+      // ---- S^T of 16 keys: rows (keys) gq and gq + 8
+      float sc[NT][4];
 #pragma unroll
-      for (int a = 0; a < MT; ++a) {
-        p[a][0] = pack2<FMT>(sc[a][2 * st][0], sc[a][2 * st][1]);
-        p[a][1] = pack2<FMT>(sc[a][2 * st][2], sc[a][2 * st][3]);
-        p[a][2] = pack2<FMT>(sc[a][2 * st + 1][0], sc[a][2 * st + 1][1]);
-        p[a][3] = pack2<FMT>(sc[a][2 * st + 1][2], sc[a][2 * st + 1][3]);
-      }
+      for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
       if constexpr (!Q8) {
 #pragma unroll
-        for (int n2 = 0; n2 < ND; n2 += 2) {
-          const int key = st * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
-          const int dim = n2 * 8 + (lane >> 4) * 8;
-          uint32_t b[4];
-          ldsm_x4_t(vt + (dim >> 6) * KG * 128 + key * 128 + ((((dim & 63) >> 3) ^ (key & 7)) << 4), b);
+        for (int kk = 0; kk < MD; ++kk) {
+          const int key = st * 16 + (lane & 15), dim = kk * 16 + (lane >> 4) * 8;
+          uint32_t a[4];
+          ldsm_x4(kt + (dim >> 6) * KG * 128 + key * 128 + ((((dim & 63) >> 3) ^ (key & 7)) << 4), a);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const uint2 b = qf[(n * MD + kk) * 32];
+            mma16816<FMT>(sc[n], a, b.x, b.y);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < D / 64; ++u) {                              // 16 bytes of each key: four k-steps
+          const int ch = tq * (D / 64) + u;
+          uint4 w[2];
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const int key = st * 16 + gq + 8 * y;
+            w[y] = *reinterpret_cast<const uint4*>(ks + key * D + ((D == 128 ? ch ^ (key & 7) : ch ^ ((key >> 1) & 3)) << 4));
+          }
+          const uint32_t w0[4] = {w[0].x, w[0].y, w[0].z, w[0].w}, w1[4] = {w[1].x, w[1].y, w[1].z, w[1].w};
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            uint32_t a[4];
+            unpack4<FMT>(w0[y], a[0], a[2]);
+            unpack4<FMT>(w1[y], a[1], a[3]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              const uint2 b = qf[(n * MD + u * 4 + y) * 32];
+              mma16816<FMT>(sc[n], a, b.x, b.y);
+            }
+          }
+        }
+      }
+      // ---- scores in the log2 domain; masks
+      float fv[2] = {1.f, 1.f};
+      int em = 0, e8[2] = {0, 0};
+      if constexpr (Q8) {
+        const float fk0 = exp_scale(ex[st * 16 + gq]), fk1 = exp_scale(ex[st * 16 + gq + 8]);
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const int e = ex[64 + st * 16 + gq + 8 * y];
+          fv[y] = exp_scale(e);
+          e8[y] = e == 255 ? 0 : e;
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            sc[n][h] *= rf[n][h] * fk0;
+            sc[n][2 + h] *= rf[n][h] * fk1;
+          }
+        em = __reduce_max_sync(0xffffffffu, max(e8[0], e8[1]));
+      } else {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            sc[n][h] *= rf[n][h];
+            sc[n][2 + h] *= rf[n][h];
+          }
+      }
+      int em_row[NT][2];
+      bool seen[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        em_row[n][0] = em_row[n][1] = em;
+        seen[n][0] = seen[n][1] = seen[n][2] = seen[n][3] = true;
+      }
+      if (partial) {
+        const int left = k_hi - key0 - st * 16;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int r = 8 * n + 2 * tq + h;
+            uint32_t see = sees32(g.mask ? masks + r * 4 : nullptr, 4, (r0 + min(r, nrows - 1)) / g.G, key0 + st * 16 - bi.ctx);
+            if (left < 16) see &= left <= 0 ? 0u : (1u << left) - 1;
+            seen[n][h] = see >> gq & 1;
+            seen[n][2 + h] = see >> (gq + 8) & 1;
+            if (!seen[n][h]) sc[n][h] = -INFINITY;
+            if (!seen[n][2 + h]) sc[n][2 + h] = -INFINITY;
+            if constexpr (Q8) {                                         // V's largest exponent among the keys this row sees
+              int e = max(seen[n][h] ? e8[0] : 0, seen[n][2 + h] ? e8[1] : 0);
+#pragma unroll
+              for (int x = 4; x < 32; x <<= 1) e = max(e, __shfl_xor_sync(0xffffffffu, e, x));
+              em_row[n][h] = e;
+            }
+          }
+      }
+      // ---- a new reference where a score is more than 2^8 above it, or V's scale more than 2^4 (weights stay below 2^12,
+      // in range of f16); -inf - -inf compares false, as a row that has seen nothing should
+      bool need = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          need = need || fmaxf(sc[n][h], sc[n][2 + h]) - m[n][h] > 8.f || (Q8 && em_row[n][h] > er[n][h] + 4);
+      if (__any_sync(0xffffffffu, need)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float mx = fmaxf(sc[n][h], sc[n][2 + h]);
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+            const float mn = fmaxf(m[n][h], mx);
+            float f = m[n][h] == -INFINITY ? 0.f : fast_exp2(m[n][h] - mn);
+            m[n][h] = mn;
+            l[n][h] *= f;
+            if constexpr (Q8) {
+              const int en = max(er[n][h], em_row[n][h]);
+              f *= fast_exp2((float)(er[n][h] - en));
+              er[n][h] = en;
+            }
+#pragma unroll
+            for (int d = 0; d < MD; ++d) {
+              o[n][d][h] *= f;
+              o[n][d][2 + h] *= f;
+            }
+          }
+      }
+      // ---- weights, and P^T as an operand
+      uint32_t pb[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float w[4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float ms = m[n][h] == -INFINITY ? 0.f : m[n][h];
+          const float p0 = fast_exp2(sc[n][h] - ms), p1 = fast_exp2(sc[n][2 + h] - ms);
+          l[n][h] += p0 + p1;
+          if constexpr (Q8) {
+            const float rv = __int_as_float((254 - er[n][h]) << 23);    // 2^-(er - 127)
+            w[h] = seen[n][h] ? p0 * (fv[0] * rv) : 0.f;
+            w[2 + h] = seen[n][2 + h] ? p1 * (fv[1] * rv) : 0.f;
+          } else {
+            w[h] = p0;
+            w[2 + h] = p1;
+          }
+        }
+        pb[n][0] = transpose8(pack2<FMT>(w[0], w[1]));
+        pb[n][1] = transpose8(pack2<FMT>(w[2], w[3]));
+      }
+      // ---- O^T += V^T P^T
+      if constexpr (!Q8) {
+#pragma unroll
+        for (int d = 0; d < MD; ++d) {
+          const int key = st * 16 + (lane & 7) + (lane >> 4) * 8, dim = d * 16 + ((lane >> 3) & 1) * 8;
+          uint32_t a[4];
+          ldsm_x4_t(vt + (dim >> 6) * KG * 128 + key * 128 + ((((dim & 63) >> 3) ^ (key & 7)) << 4), a);
           if (partial) {                 // 0 x NaN would reach every row: drop it here, put it back at the end
 #pragma unroll
-            for (int x = 0; x < 4; ++x) b[x] = drop_nonfinite(b[x], hit);
+            for (int x = 0; x < 4; ++x) a[x] = drop_nonfinite(a[x], hit);
           }
 #pragma unroll
-          for (int a = 0; a < MT; ++a) {
-            mma16816<FMT>(o[a][n2], p[a], b[0], b[1]);
-            mma16816<FMT>(o[a][n2 + 1], p[a], b[2], b[3]);
-          }
+          for (int n = 0; n < NT; ++n) mma16816<FMT>(o[n][d], a, pb[n][0], pb[n][1]);
         }
       } else {
         // keys 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9 of this step, D / 8 bytes each
@@ -516,10 +499,10 @@ __global__ void __launch_bounds__(128, MmaShape<D, FMT, MT>::CTAS)
         for (int x = 0; x < 4; ++x) {
           const int key = st * 16 + 2 * tq + (x & 1) + (x >> 1) * 8;
           if constexpr (D == 128) {
-            const uint4 v = lds128(vt + key * D + ((gq ^ (key & 7)) << 4));
+            const uint4 v = *reinterpret_cast<const uint4*>(vs + key * D + ((gq ^ (key & 7)) << 4));
             w[x][0] = v.x, w[x][1] = v.y, w[x][2] = v.z, w[x][3] = v.w;
           } else {
-            const uint2 v = lds64(vt + key * D + ((((gq >> 1) ^ ((key >> 1) & 3)) << 4) | (gq & 1) << 3));
+            const uint2 v = *reinterpret_cast<const uint2*>(vs + key * D + ((((gq >> 1) ^ ((key >> 1) & 3)) << 4) | (gq & 1) << 3));
             w[x][0] = v.x, w[x][1] = v.y;
           }
           if constexpr (FMT == EESD_KV_INT8)
@@ -527,27 +510,26 @@ __global__ void __launch_bounds__(128, MmaShape<D, FMT, MT>::CTAS)
             for (int y = 0; y < D / 32; ++y) w[x][y] ^= 0x80808080u;
         }
 #pragma unroll
-        for (int n = 0; n < ND; ++n) {
-          const int y = n >> 2, z = n & 3;
-          uint32_t b0, b1;
-          if constexpr (FMT == EESD_KV_E4M3) {                          // bytes into the high halves of each lane
-            const uint32_t sel = (4 + z) << 12 | (z << 4);              // [., z of x, ., z of y]: low bytes are masked off
-            b0 = bytes_to_half2<FMT>(__byte_perm(w[0][y], w[1][y], sel));
-            b1 = bytes_to_half2<FMT>(__byte_perm(w[2][y], w[3][y], sel));
-          } else {
-            const uint32_t sel = (4 + z) << 4 | z;                      // [z of x, z of y, ., .], then 0x64 in between
-            b0 = bytes_to_half2<FMT>(__byte_perm(__byte_perm(w[0][y], w[1][y], sel), 0x64646464u, 0x4140));
-            b1 = bytes_to_half2<FMT>(__byte_perm(__byte_perm(w[2][y], w[3][y], sel), 0x64646464u, 0x4140));
+        for (int d = 0; d < MD; ++d) {
+          uint32_t a[4];                                                // dims gq D/8 + 2 d (a0, a2) and + 1 (a1, a3)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int b = 2 * d + (x & 1), y = b >> 2, z = b & 3, k = x >> 1;
+            if constexpr (FMT == EESD_KV_E4M3) {                        // bytes into the high halves of each lane
+              a[x] = bytes_to_half2<FMT>(__byte_perm(w[2 * k][y], w[2 * k + 1][y], (4 + z) << 12 | z << 4));
+            } else {
+              a[x] = bytes_to_half2<FMT>(__byte_perm(__byte_perm(w[2 * k][y], w[2 * k + 1][y], (4 + z) << 4 | z), 0x64646464u, 0x4140));
+            }
           }
 #pragma unroll
-          for (int a = 0; a < MT; ++a) mma16816<FMT>(o[a][n], p[a], b0, b1);
+          for (int n = 0; n < NT; ++n) mma16816<FMT>(o[n][d], a, pb[n][0], pb[n][1]);
         }
       }
     }
-    if (!Q8 && hit) flags[1] = 1;
     __syncwarp();                                                       // every lane is done with the stage
     if (lane == 0 && i + NS < my_groups) issue(i + NS);
   }
+  if (!Q8 && hit) flags[1] = 1;
   if (!ok) {
     if (lane == 0) {
       set_status(g.status, kStatusTimeoutMma);
@@ -566,30 +548,36 @@ __global__ void __launch_bounds__(128, MmaShape<D, FMT, MT>::CTAS)
   float* Lw = Mw + 4 * ROWS;
   float* Ew = Lw + 4 * ROWS;
 #pragma unroll
-  for (int a = 0; a < MT; ++a)
+  for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int r = a * 16 + h * 8 + gq;
-      float s = l[a][h];
-      s += __shfl_xor_sync(0xffffffffu, s, 1);
-      s += __shfl_xor_sync(0xffffffffu, s, 2);
-      if (tq == 0) {
-        Mw[warp * ROWS + r] = m[a][h];
+      const int r = 8 * n + 2 * tq + h;
+      float s = l[n][h];
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+      if (gq == 0) {
+        Mw[warp * ROWS + r] = m[n][h];
         Lw[warp * ROWS + r] = s;
-        Ew[warp * ROWS + r] = (float)er[a][h];
+        Ew[warp * ROWS + r] = (float)er[n][h];
       }
       float* dst = Ow + (warp * ROWS + r) * OLD;
 #pragma unroll
-      for (int n = 0; n < ND; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) dst[Q8 ? (2 * tq + e) * ND + n : n * 8 + 2 * tq + e] = o[a][n][2 * h + e];
+      for (int d = 0; d < MD; ++d) {
+        if constexpr (Q8) {
+          *reinterpret_cast<float2*>(dst + gq * (D / 8) + 2 * d) = make_float2(o[n][d][h], o[n][d][2 + h]);
+        } else {
+          dst[d * 16 + gq] = o[n][d][h];
+          dst[d * 16 + gq + 8] = o[n][d][2 + h];
+        }
+      }
     }
   __syncthreads();
   const bool whole = n_keys <= g.chunk;
   constexpr int LPR = D / 4;                                            // threads per row, 4 dims each
+#pragma unroll 2
   for (int r = threadIdx.x / LPR; r < nrows; r += 128 / LPR) {
     const int d = threadIdx.x % LPR * 4;
-    float M = -INFINITY, E = 0.f;
+    float M = -INFINITY, E = 1.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       M = fmaxf(M, Mw[w * ROWS + r]);
@@ -606,12 +594,13 @@ __global__ void __launch_bounds__(128, MmaShape<D, FMT, MT>::CTAS)
       acc[0] += fo * v.x, acc[1] += fo * v.y, acc[2] += fo * v.z, acc[3] += fo * v.w;
     }
     float inv = L == 0.f ? 0.f : 1.f / L;                               // a row that sees nothing: zeros
-    if constexpr (Q8) inv *= kHalfUnit<FMT> * __int_as_float((int)fmaxf(E, 1.f) << 23);
+    if constexpr (Q8) inv *= kHalfUnit<FMT> * __int_as_float((int)E << 23);
     const int R = r0 + r, node = R / g.G;
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[e] *= inv;
     if (!Q8 && flags[1]) {                                              // the dropped elements of keys this row sees
       const uint64_t* mk = g.mask ? masks + r * 4 : nullptr;
+#pragma unroll 1
       for (int key = max(k_lo, min(all_see, k_hi)); key < k_hi; ++key)
         if (sees32(mk, 4, node, key - bi.ctx) & 1) {
           const bf16* v = static_cast<const bf16*>(c.v) + ((size_t)slot0 + key) * D + d;
@@ -622,7 +611,7 @@ __global__ void __launch_bounds__(128, MmaShape<D, FMT, MT>::CTAS)
           }
         }
     }
-    const size_t at = (size_t)(bi.start + node) * g.n_heads + kvh * g.G + R % g.G;
+    const size_t at = (size_t)(bi.start + node) * g.n_heads + kvh * g.G + R - node * g.G;
     if (whole) {
       *reinterpret_cast<uint2*>(out + at * D + d) = make_uint2(pack2<EESD_KV_MODEL>(acc[0], acc[1]), pack2<EESD_KV_MODEL>(acc[2], acc[3]));
     } else {
@@ -704,7 +693,7 @@ int encode_cache_map(CUtensorMap* map, const void* base, const EesdKvCache* c, i
 
 struct Plan {
   bool tc;              // tcgen05 kernel (attn_tree_tc.cu), else mma.sync
-  int mt;               // mma.sync: 16-row m-tiles per CTA
+  int nt;               // mma.sync: 8-row tiles per CTA
   int rows, tiles;      // rows per tile, row tiles of the largest block
   int chunk, splits;    // keys per CTA, key ranges of the longest row
   int ctas;             // tcgen05: persistent CTAs
@@ -724,8 +713,8 @@ Plan plan_for(const EesdKvCache* c, const EesdTree* t, int n_heads, int split_ke
   Plan p{};
   const int G = n_heads / c->n_kv_heads, rows = t->max_nodes * G;
   p.tc = rows > 32;
-  p.mt = rows <= 16 ? 1 : 2;
-  p.rows = p.tc ? (rows <= 128 ? 128 : 256) : 16 * p.mt;
+  p.nt = std::min(4, (rows + 7) / 8);
+  p.rows = p.tc ? (rows <= 128 ? 128 : 256) : 8 * p.nt;
   p.tiles = (rows + p.rows - 1) / p.rows;
   const long long units = (long long)t->n_blocks * c->n_kv_heads * p.tiles;
   p.chunk = split_keys;
@@ -736,7 +725,7 @@ Plan plan_for(const EesdKvCache* c, const EesdTree* t, int n_heads, int split_ke
     p.ctas = (int)std::max(1LL, std::min<long long>(sm_count(), (most + 7) / 8));
     if (!p.chunk) parts = (size_t)p.ctas * 2 * p.rows;
   } else if (!p.chunk) {
-    const int slots = sm_count() * (p.mt == 1 ? 3 : 2);
+    const int slots = sm_count() * (p.nt == 4 || (p.nt == 3 && c->head_dim == 128 && c->format != EESD_KV_MODEL) ? 2 : 3);
     const int want = (int)std::max(1LL, slots / std::max(1LL, units));
     const int per = (t->max_ctx + want - 1) / want;
     p.chunk = (per + 255) / 256 * 256;
@@ -750,11 +739,11 @@ Plan plan_for(const EesdKvCache* c, const EesdTree* t, int n_heads, int split_ke
   return p;
 }
 
-template <int D, int FMT, int MT>
+template <int D, int FMT, int NT>
 cudaError_t launch_mma(const Plan& p, const TreeGeom& g, const CacheGeom& c, const CUtensorMap& km, const CUtensorMap& vm, int n_blocks,
                        const void* q, void* out, cudaStream_t s) {
-  using S = MmaShape<D, FMT, MT>;
-  auto kernel = attn_tree_mma_kernel<D, FMT, MT>;
+  using S = MmaShape<D, FMT, NT>;
+  auto kernel = attn_tree_mma_kernel<D, FMT, NT>;
   static SmemOnce once;
   const cudaError_t e = once.set(reinterpret_cast<const void*>(kernel), S::smem);
   if (e != cudaSuccess) return e;
@@ -762,9 +751,14 @@ cudaError_t launch_mma(const Plan& p, const TreeGeom& g, const CacheGeom& c, con
                     static_cast<const bf16*>(q), static_cast<bf16*>(out));
 }
 template <int D, int FMT>
-cudaError_t launch_mt(const Plan& p, const TreeGeom& g, const CacheGeom& c, const CUtensorMap& km, const CUtensorMap& vm, int nb,
+cudaError_t launch_nt(const Plan& p, const TreeGeom& g, const CacheGeom& c, const CUtensorMap& km, const CUtensorMap& vm, int nb,
                       const void* q, void* out, cudaStream_t s) {
-  return p.mt == 1 ? launch_mma<D, FMT, 1>(p, g, c, km, vm, nb, q, out, s) : launch_mma<D, FMT, 2>(p, g, c, km, vm, nb, q, out, s);
+  switch (p.nt) {
+    case 1: return launch_mma<D, FMT, 1>(p, g, c, km, vm, nb, q, out, s);
+    case 2: return launch_mma<D, FMT, 2>(p, g, c, km, vm, nb, q, out, s);
+    case 3: return launch_mma<D, FMT, 3>(p, g, c, km, vm, nb, q, out, s);
+    default: return launch_mma<D, FMT, 4>(p, g, c, km, vm, nb, q, out, s);
+  }
 }
 
 template <typename T, int FMT, int D>
@@ -789,12 +783,12 @@ cudaError_t launch_f32(int fmt, int D, const TreeGeom& g, const CacheGeom& c, in
 cudaError_t launch_bf16(int fmt, int D, const Plan& p, const TreeGeom& g, const CacheGeom& c, const CUtensorMap& km, const CUtensorMap& vm,
                         int nb, const void* q, void* out, cudaStream_t s) {
   switch (fmt * 2 + (D == 128)) {
-    case 0: return launch_mt<64, EESD_KV_MODEL>(p, g, c, km, vm, nb, q, out, s);
-    case 1: return launch_mt<128, EESD_KV_MODEL>(p, g, c, km, vm, nb, q, out, s);
-    case 2: return launch_mt<64, EESD_KV_E4M3>(p, g, c, km, vm, nb, q, out, s);
-    case 3: return launch_mt<128, EESD_KV_E4M3>(p, g, c, km, vm, nb, q, out, s);
-    case 4: return launch_mt<64, EESD_KV_INT8>(p, g, c, km, vm, nb, q, out, s);
-    default: return launch_mt<128, EESD_KV_INT8>(p, g, c, km, vm, nb, q, out, s);
+    case 0: return launch_nt<64, EESD_KV_MODEL>(p, g, c, km, vm, nb, q, out, s);
+    case 1: return launch_nt<128, EESD_KV_MODEL>(p, g, c, km, vm, nb, q, out, s);
+    case 2: return launch_nt<64, EESD_KV_E4M3>(p, g, c, km, vm, nb, q, out, s);
+    case 3: return launch_nt<128, EESD_KV_E4M3>(p, g, c, km, vm, nb, q, out, s);
+    case 4: return launch_nt<64, EESD_KV_INT8>(p, g, c, km, vm, nb, q, out, s);
+    default: return launch_nt<128, EESD_KV_INT8>(p, g, c, km, vm, nb, q, out, s);
   }
 }
 
