@@ -96,27 +96,9 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// mbar_wait that suspends the thread for up to 2 us per poll: most of the 20 warps wait most of the time, and polling
-// would take the issue slots of those that do not.
-__device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t limit) {
-#pragma unroll 1
-  for (uint32_t i = 0; i < limit; ++i) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred P;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2, %3;\n\t"
-        "selp.b32 %0, 1, 0, P;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity), "r"(2000u)
-        : "memory");
-    if (ok) return true;
-    if ((i & 255u) == 255u && *abort_flag) return false;
-  }
-  return false;
-}
 // The whole warp waits and goes on together (what follows are warp-wide instructions).
 __device__ __forceinline__ bool warp_wait(const void* bar, uint32_t parity, volatile int* abort_flag, uint32_t limit) {
-  return __all_sync(0xffffffffu, wait_on(smem_u32(bar), parity, abort_flag, limit));
+  return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, abort_flag, limit));
 }
 template <int N> __device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -261,7 +243,7 @@ template <int D, int FMT> struct TcShape {
   static constexpr int RS = Q8 ? 6 : 0;                // raw stages
   static constexpr int FR = 8;                         // factor ring: six tiles can be between conversion and softmax
   [[maybe_unused]] static constexpr int kUp = FMT == EESD_KV_E4M3 ? 14 : 5;   // a tile's largest 8-bit elements in f16: 28672, 4064
-  static constexpr int QB = 128 * D * 2;               // Q of stream 1 (more than 128 rows)
+  static constexpr int QB = 128 * D * 2 + 128 * 128;   // Q of stream 1 (more than 128 rows), half rows on their way to TMEM
   static constexpr size_t ctl = 16384;
   static constexpr size_t smem = 1024 + (size_t)2 * NS * TILE + (size_t)RS * RAW + QB + ctl;
 };
@@ -272,14 +254,14 @@ struct TcControl {
   uint64_t piece_full[kPieces], piece_empty[kPieces];
   Piece piece[kPieces];                    // tiles == 0: there are no more
   uint64_t s_full[2], s_free[2], p_ready[2], pv_done[2], q_ready, o_done, ml_ready, epi_done, drain[2];
-  // 8-bit, per tile: 2^ek and 2^(ev - ref) of its keys where some row does not wholly see it (0 for NaN and slots past
-  // the end), else one factor for K, kt; ref is the exponent byte that V is relative to
+  // 8-bit, per tile: 2^ek of its keys, or one factor kt; 2^(ev - ref) of its keys where some row does not wholly see it
+  // (0 for NaN and slots past the end); ref is the exponent byte that V is relative to
   alignas(16) float fk[8][KT];
   alignas(16) float fv[8][KT];
   float kt[8];
   alignas(16) uint8_t ev[8][KT];           // V's exponent bytes, 0 likewise
   alignas(16) uint8_t exps[6][2 * KT];     // raw exponent bytes, K then V
-  int ref[8];
+  int ref[8], k_keyed[8];
   uint32_t nan[8][2];                      // keys whose V is NaN
   float ml[2][2][3][128];                  // one row tile: max, sum and eref of the streams (by piece parity)
   long long lo, hi, base;
@@ -301,7 +283,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_wait();
   extern __shared__ uint8_t smem8[];
   uint8_t* sm = smem8 + (-smem_u32(smem8) & 1023);     // an offset, so that the compiler still knows it as shared memory
-  const uint32_t kbuf = smem_u32(sm), vbuf = kbuf + NS * S::TILE, raw = vbuf + NS * S::TILE, qbuf = raw + S::RS * S::RAW;
+  const uint32_t kbuf = smem_u32(sm), vbuf = kbuf + NS * S::TILE, raw = vbuf + NS * S::TILE, qbuf = raw + S::RS * S::RAW,
+                 qstage = qbuf + 128 * D * 2;
   TcControl& ct = *reinterpret_cast<TcControl*>(sm + 2 * NS * S::TILE + S::RS * S::RAW + S::QB);
   volatile int* abort_flag = &ct.abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -395,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
   }
   // Every role reads its pieces, in order, from the ring that warp 2 fills.
-  auto piece_wait = [&](int k) { return wait_on(smem_u32(&ct.piece_full[k % kPieces]), k / kPieces & 1, abort_flag, g.spin); };
+  auto piece_wait = [&](int k) { return mbar_wait(smem_u32(&ct.piece_full[k % kPieces]), k / kPieces & 1, abort_flag, g.spin); };
   auto piece_free = [&](int k) { mbar_arrive(smem_u32(&ct.piece_empty[k % kPieces])); };
   const uint32_t tmem = ct.tmem;
 
@@ -416,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int t = p.t0; t < p.t1; ++t, ++cnt) {
           if constexpr (Q8) {
             const int s = cnt % RS;
-            if (!(ok = wait_on(smem_u32(&ct.raw_empty[s]), (cnt / RS & 1) ^ 1, abort_flag, g.spin))) break;
+            if (!(ok = mbar_wait(smem_u32(&ct.raw_empty[s]), (cnt / RS & 1) ^ 1, abort_flag, g.spin))) break;
             const uint32_t fb = smem_u32(&ct.raw_full[s]), dst = raw + s * S::RAW, ex = smem_u32(ct.exps[s]);
             const uint32_t eb = min(KT, c.max_seq - t * KT);          // max_seq % 16 == 0
             mbar_arrive_expect_tx(fb, S::RAW + 2 * eb);
@@ -428,12 +411,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           } else {
             const int s = cnt % NS;
             const uint32_t ph = (cnt / NS & 1) ^ 1;
-            if (!(ok = wait_on(smem_u32(&ct.kempty[s]), ph, abort_flag, g.spin))) break;
+            if (!(ok = mbar_wait(smem_u32(&ct.kempty[s]), ph, abort_flag, g.spin))) break;
             const uint32_t kb = smem_u32(&ct.kfull[s]), vb = smem_u32(&ct.vfull[s]);
             mbar_arrive_expect_tx(kb, S::TILE);
             for (int h = 0; h < HALVES; ++h) tma_load_2d(kbuf + s * S::TILE + h * KT * 128, &kmap, h * 64, slot0 + t * KT, kb);
             k_issued = cnt + 1;
-            if (!(ok = wait_on(smem_u32(&ct.vempty[s]), ph, abort_flag, g.spin))) break;
+            if (!(ok = mbar_wait(smem_u32(&ct.vempty[s]), ph, abort_flag, g.spin))) break;
             mbar_arrive_expect_tx(vb, S::TILE);
             for (int h = 0; h < HALVES; ++h) tma_load_2d(vbuf + s * S::TILE + h * KT * 128, &vmap, h * 64, slot0 + t * KT, vb);
             v_issued = cnt + 1;
@@ -474,16 +457,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_commit(smem_u32(bar));
           if (!two) tc_commit(smem_u32(bar));
         };
-        if (!(ok = wait_on(smem_u32(&ct.q_ready), piece & 1, abort_flag, g.spin))) break;
+        if (!(ok = mbar_wait(smem_u32(&ct.q_ready), piece & 1, abort_flag, g.spin))) break;
         // S of the stream's next tile as soon as the last one is in registers, then O of the last one when its softmax ends
 #pragma unroll 1
         for (int i = t0 - step; i < nt; i += step) {
           const int j = i + step;
           if (j < nt) {
             const int cnt = cnt0 + j, st = cnt % NS;
-            if (n_q && !(ok = wait_on(smem_u32(&ct.s_free[x]), (n_q - 1) & 1, abort_flag, g.spin))) break;
+            if (n_q && !(ok = mbar_wait(smem_u32(&ct.s_free[x]), (n_q - 1) & 1, abort_flag, g.spin))) break;
             ++n_q;
-            if (!(ok = wait_on(smem_u32(&ct.kfull[st]), cnt / NS & 1, abort_flag, g.spin))) break;
+            if (!(ok = mbar_wait(smem_u32(&ct.kfull[st]), cnt / NS & 1, abort_flag, g.spin))) break;
             tc_fence_after();
             issued = true;
             const uint64_t kd = sw128_kmajor_desc(kbuf + st * S::TILE);
@@ -502,8 +485,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (i >= 0) {
             const int cnt = cnt0 + i, st = cnt % NS;
-            if (!(ok = wait_on(smem_u32(Q8 ? &ct.vfull[st] : &ct.vclean[st]), cnt / NS & 1, abort_flag, g.spin))) break;
-            if (!(ok = wait_on(smem_u32(&ct.p_ready[x]), n_p++ & 1, abort_flag, g.spin))) break;
+            if (!(ok = mbar_wait(smem_u32(Q8 ? &ct.vfull[st] : &ct.vclean[st]), cnt / NS & 1, abort_flag, g.spin))) break;
+            if (!(ok = mbar_wait(smem_u32(&ct.p_ready[x]), n_p++ & 1, abort_flag, g.spin))) break;
             tc_fence_after();
             const uint64_t vd = sw128_mnmajor_desc(vbuf + st * S::TILE, KT * 128);
 #pragma unroll
@@ -535,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       Piece p;
 #pragma unroll 1
       for (int k = 0;; ++k) {
-        if (!(ok = wait_on(smem_u32(&ct.piece_empty[k % kPieces]), (k / kPieces & 1) ^ 1, abort_flag, g.spin))) break;
+        if (!(ok = mbar_wait(smem_u32(&ct.piece_empty[k % kPieces]), (k / kPieces & 1) ^ 1, abort_flag, g.spin))) break;
         const bool more = it.next(g, c, sc, p);
         if (!more) p.tiles = 0;
         ct.piece[k % kPieces] = p;
@@ -553,18 +536,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int ti = tid & 127;
     const bool is_v = warp >= 16;
     // The raw tile's bytes as f16, row r times 2^(e_r - top) (none below 2^-24; byte 255, a NaN, comes out as one);
-    // top = 0: all rows times 2^flat.  A thread has one 16-byte chunk of every 16th (D = 64: 32nd) row; the 8 lanes of a
+    // top = 0: all rows times 2^flat; zeros from row `left` on.  A thread has one 16-byte chunk of every 16th (D = 64: 32nd) row; the 8 lanes of a
     // phase are on 8 rows and one chunk, conflict-free in both swizzles.
     constexpr int kChunks = D / 16, kRowStep = 128 / kChunks;
     const uint32_t ch = (uint32_t)ti / 8 % kChunks, row0 = (uint32_t)ti / (8 * kChunks) * 8 + (ti & 7);
     const uint32_t from = row0 * D + ((D == 128 ? ch ^ (row0 & 7) : ch ^ (row0 >> 1 & 3)) << 4);
     const uint32_t to0 = (ch >> 2) * (KT * 128) + row0 * 128 + ((2 * ch & 7 ^ (row0 & 7)) << 4), to1 = to0 ^ 16;
-    [[maybe_unused]] auto convert = [&](const uint8_t* src, uint8_t* dst, const uint8_t* e, int top, int flat) {
+    [[maybe_unused]] auto convert = [&](const uint8_t* src, uint8_t* dst, const uint8_t* e, int top, int flat, int left) {
 #pragma unroll
       for (int i = 0; i < KT / kRowStep; ++i) {
         const uint4 w = *reinterpret_cast<const uint4*>(src + from + i * (kRowStep * D));
         const int er = e[row0 + i * kRowStep], x = top ? er - top : flat;
-        const uint32_t h = top && er == 255 ? 0x7fffu : x >= -14 ? (uint32_t)(x + 15) << 10 : x >= -24 ? 1u << (x + 24) : 0u;
+        const uint32_t h = (int)row0 + i * kRowStep >= left ? 0u : top && er == 255 ? 0x7fffu : x >= -14 ? (uint32_t)(x + 15) << 10 : x >= -24 ? 1u << (x + 24) : 0u;
         const uint32_t m = __byte_perm(h, 0, 0x1010);
         const Scaler<FMT> sc8(m);
         uint4 a, b;
@@ -595,18 +578,24 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint8_t* ex = ct.exps[rs] + (is_v ? KT : 0);
           const uint32_t v = *reinterpret_cast<const uint16_t*>(ex + 2 * lane);
           const int a0 = v & 255, a1 = v >> 8;
-          const int em = __reduce_max_sync(0xffffffffu, max(2 * lane < left && a0 != 255 ? a0 : 0, 2 * lane + 1 < left && a1 != 255 ? a1 : 0));
-          const int top = partial ? 0 : max(em, 27) - S::kUp;
-          // V's factors in a tile that some row does not wholly see are relative to 2^60 below the largest, so that they
-          // last for rows whose own largest is far smaller
-          const int ref = partial ? em - 60 : em;
+          const bool in0 = 2 * lane < left, in1 = 2 * lane + 1 < left;
+          const int em = __reduce_max_sync(0xffffffffu, max(in0 && a0 != 255 ? a0 : 0, in1 && a1 != 255 ? a1 : 0));
+          // In a tile that some row does not wholly see, V's scales stay with the weights: they decide a row's precision.
+          // K's are folded where that is exact (within 2^16 of each other).
+          bool keyed = partial && is_v;
+          if (partial && !is_v) keyed = __any_sync(0xffffffffu, (in0 && a0 < em - 16) || (in1 && a1 < em - 16));
+          const int top = keyed ? 0 : max(em, 27) - S::kUp;
+          // V's factors in a keyed tile are relative to 2^60 below the largest, so that they last for rows whose own
+          // largest is far smaller
+          const int ref = keyed ? em - 60 : em;
           if (!(ok = warp_wait(is_v ? &ct.vempty[st] : &ct.kempty[st], (cnt / NS & 1) ^ 1, abort_flag, g.spin))) break;
           // (the factor ring's last reader is behind the products that freed this stage)
           if (ti == 0) {
             if (is_v) ct.ref[f] = ref;
             else ct.kt[f] = __int_as_float(max(top, 1) << 23);
+            if (!is_v) ct.k_keyed[f] = keyed;
           }
-          if (partial && ti < KT) {
+          if (keyed && ti < KT) {
             const int e = ex[ti], d = e - ref + 127;
             if (!is_v) {
               ct.fk[f][ti] = exp_scale(e);
@@ -619,7 +608,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           warp_arrive(&ct.ffull[f]);
-          convert(sm + 2 * NS * S::TILE + rs * S::RAW + (is_v ? S::RAW / 2 : 0), sm + ((is_v ? NS : 0) + st) * S::TILE, ex, top, is_v ? S::kUp : 0);
+          convert(sm + 2 * NS * S::TILE + rs * S::RAW + (is_v ? S::RAW / 2 : 0), sm + ((is_v ? NS : 0) + st) * S::TILE, ex, top, is_v ? S::kUp : 0, left);
           warp_arrive(is_v ? &ct.vfull[st] : &ct.kfull[st]);
           warp_arrive(&ct.raw_empty[rs]);
         } else {
@@ -659,7 +648,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int x = (warp >> 2) - 1, r = tid & 127;
     const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);         // TMEM lane quadrant of the warp
     const uint32_t tS = lanes + kColS + x * kSP, tP = lanes + kColP + x * kSP, tO = lanes + kColO + x * 128;
-    int cnt0 = 0, n_s = 0, piece = 0, n_ml = 0;
+    int cnt0 = 0, n_s = 0, n_ml = 0;
     bool ok = true;
     struct Row {
       bool two, in;
@@ -676,43 +665,67 @@ __global__ void __launch_bounds__(kThreads, 1)
       return w;
     };
     const float scale_l2 = g.scale * 1.4426950408889634f;
-    // The q row of a piece to where the products read it: bf16 as it is, or f16 with the largest element's power of two
-    // taken out (returned with the softmax scale).  32 words at a time: the whole row in registers would spill the softmax.
+    // The q rows of a piece to where the products read them: bf16 as it is, or f16 with the largest element's power of two
+    // taken out (a row's softmax scale with it is returned).  A warp reads its 32 rows in 256-byte runs (D = 128) and
+    // turns them, half a row at a time, through shared memory: into the operand tile of stream 1, or into the lanes'
+    // rows in TMEM.
     auto put_q = [&](const Piece& p) {
-      const Row w = row_of(p);
-      const uint4* src = reinterpret_cast<const uint4*>(q + (size_t)(p.bi.start + w.node) * g.ld_q + (size_t)w.head * D);
-      float rf = scale_l2, inv = 1.f;
-      if constexpr (Q8) {
-        uint32_t amax = 0;
+      const bool two = p.nrows > 128;
+      constexpr int C = D / 8, RPI = 32 / C, N = 32 / RPI;              // chunks per row, rows per load, loads
+      const int row0 = (two ? x * 128 : 0) + (warp & 3) * 32 + lane / C, chunk = lane % C;
+      uint4 u[N];
+      int node = (p.r0 + row0) / g.G, head = p.r0 + row0 - node * g.G;  // of the row, and its head of the group
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          const uint4 u = w.in ? src[i] : make_uint4(0, 0, 0, 0);
-          const uint32_t hi = max(max(u.x & 0x7fff0000u, u.y & 0x7fff0000u), max(u.z & 0x7fff0000u, u.w & 0x7fff0000u));
-          const uint32_t lo = max(max(u.x << 16 & 0x7fff0000u, u.y << 16 & 0x7fff0000u), max(u.z << 16 & 0x7fff0000u, u.w << 16 & 0x7fff0000u));
-          amax = max(amax, max(hi, lo));
-        }
-        const int e = min(max((int)(amax >> 23), 27), 227);
-        inv = __int_as_float((254 - e) << 23);
-        rf *= __int_as_float(e << 23) * kHalfUnit<FMT>;
+      for (int i = 0; i < N; ++i) {
+        const bf16* src = q + (size_t)(p.bi.start + node) * g.ld_q + (size_t)(p.h * g.G + head) * D;
+        u[i] = row0 + i * RPI < p.nrows ? reinterpret_cast<const uint4*>(src)[chunk] : make_uint4(0, 0, 0, 0);
+        head += RPI;
+#pragma unroll
+        for (int y = 0; y < RPI; ++y)
+          if (head >= g.G) head -= g.G, ++node;
       }
-#pragma unroll 1
-      for (int b = 0; b < D / 64; ++b) {
-        uint32_t v[32];
+      float rf = scale_l2;
+      if constexpr (Q8) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint4 u = w.in ? src[8 * b + i] : make_uint4(0, 0, 0, 0);
-          v[4 * i] = u.x, v[4 * i + 1] = u.y, v[4 * i + 2] = u.z, v[4 * i + 3] = u.w;
+        for (int i = 0; i < N; ++i) {
+          uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w}, amax = 0;
+#pragma unroll
+          for (int y = 0; y < 4; ++y) amax = max(amax, max(w[y] << 16 & 0x7fff0000u, w[y] & 0x7fff0000u));
+#pragma unroll
+          for (int o = 1; o < C; o <<= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+          const int e = min(max((int)(amax >> 23), 27), 227);
+          const float inv = __int_as_float((254 - e) << 23);
+          // the lane whose row this is
+#pragma unroll
+          for (int y = 0; y < RPI; ++y) {
+            const float f = __shfl_sync(0xffffffffu, __int_as_float(e << 23), y * C);
+            if (lane == i * RPI + y) rf *= f * kHalfUnit<FMT>;
+          }
+#pragma unroll
+          for (int y = 0; y < 4; ++y) w[y] = pack2<FMT>(__uint_as_float(w[y] << 16) * inv, __uint_as_float(w[y] & 0xffff0000u) * inv);
+          u[i] = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        if constexpr (Q8) {
+      }
+      const uint32_t stage = x == 0 ? qstage : qbuf;                    // [128 rows][128 B], swizzled as the operand tile is
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = pack2<FMT>(__uint_as_float(v[i] << 16) * inv, __uint_as_float(v[i] & 0xffff0000u) * inv);
+      for (int b = 0; b < D / 64; ++b) {
+        if (x == 0 || two) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            const int rr = (warp & 3) * 32 + i * RPI + lane / C;
+            if (chunk / 8 == b) sts128(stage + (x == 0 ? 0 : b * (128 * 128)) + rr * 128 + (((chunk & 7) ^ (rr & 7)) << 4), u[i]);
+          }
         }
         if (x == 0) {
-          tmem_st32(lanes + kColQ + 32 * b, v);
-        } else if (w.two) {
+          __syncwarp();
+          uint32_t v[32];
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            sts128(qbuf + b * (128 * 128) + r * 128 + ((i ^ (r & 7)) << 4), make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]));
+          for (int i = 0; i < 8; ++i) {
+            const uint4 t = lds128(stage + r * 128 + ((i ^ (r & 7)) << 4));
+            v[4 * i] = t.x, v[4 * i + 1] = t.y, v[4 * i + 2] = t.z, v[4 * i + 3] = t.w;
+          }
+          tmem_st32(lanes + kColQ + 32 * b, v);
+          __syncwarp();
         }
       }
       if (x == 0) tmem_wait_st();
@@ -721,20 +734,109 @@ __global__ void __launch_bounds__(kThreads, 1)
       warp_arrive(&ct.q_ready);
       return rf;
     };
-    float rf = 0.f;
-    bool more = false;
-    if ((ok = __all_sync(0xffffffffu, piece_wait(0))) && ct.piece[0].tiles) {
-      rf = put_q(ct.piece[0]);
-      more = true;
-    }
+    float rf = 0.f, m = -INFINITY, l = 0.f;
+    int er = 0, nt = 0;                                                 // er: 8-bit: exponent byte that O and l are relative to
+    bool begun = false, two = false;
+    // One turn: the next piece's Q goes out, then the last piece's output (its products are done, and the next one's first
+    // S runs meanwhile), then the next piece's tiles.
 #pragma unroll 1
-    while (more) {
-      const Piece& cur = ct.piece[piece % kPieces];
-      const int nt = cur.t1 - cur.t0;
-      const bool two = cur.nrows > 128;
-      float m = -INFINITY, l = 0.f;
-      int er = 0;                                                       // 8-bit: exponent byte that O and l are relative to
-      bool begun = false;
+    for (int piece = -1;;) {
+      if (!(ok = __all_sync(0xffffffffu, piece_wait(piece + 1)))) break;
+      const Piece& nxt = ct.piece[(piece + 1) % kPieces];
+      const bool more = nxt.tiles != 0;
+      float(&ml)[2][3][128] = ct.ml[piece & 1];
+      if (piece >= 0 && !two) {
+        ml[x][0][r] = m;
+        ml[x][1][r] = l;
+        ml[x][2][r] = begun ? (float)er : -1.f;                         // -1: the stream had no tile, its O is not there
+        warp_arrive(&ct.ml_ready);
+        if (!(ok = warp_wait(&ct.ml_ready, n_ml++ & 1, abort_flag, g.spin))) break;
+      }
+      float rf_next = 0.f;
+      if (more) rf_next = put_q(nxt);
+      if (piece >= 0) {
+        if (!(ok = warp_wait(&ct.o_done, piece & 1, abort_flag, g.spin))) break;
+        const Piece& cur = ct.piece[piece % kPieces];
+        tc_fence_after();
+        float f0 = 1.f, f1 = 0.f, M = m, L = l, E = (float)er;
+        if (!two) {
+          const float m0 = ml[0][0][r], m1 = ml[1][0][r], e0 = ml[0][2][r], e1 = ml[1][2][r];
+          M = fmaxf(m0, m1);
+          const float ms = M == -INFINITY ? 0.f : M;
+          E = fmaxf(fmaxf(e0, e1), 0.f);
+          const float w0 = fast_exp2(m0 - ms), w1 = e1 < 0.f ? 0.f : fast_exp2(m1 - ms);
+          L = w0 * ml[0][1][r] + (e1 < 0.f ? 0.f : w1 * ml[1][1][r]);
+          f0 = Q8 ? w0 * fast_exp2(e0 - E) : w0;
+          f1 = e1 < 0.f ? 0.f : Q8 ? w1 * fast_exp2(e1 - E) : w1;
+        }
+        float inv = L == 0.f ? 0.f : 1.f / L;                             // a row that sees nothing: zeros
+        if constexpr (Q8) inv *= kHalfUnit<FMT> / (1 << S::kUp) * __int_as_float((int)fmaxf(E, 1.f) << 23);
+        const Row cw = row_of(cur);
+        const bool join = !two && nt > 1;
+        const size_t at = (size_t)(cur.bi.start + cw.node) * g.n_heads + cw.head;
+        const bool to_out = sc.chunk_tiles ? cur.tiles <= sc.chunk_tiles : cur.whole();
+        const size_t part = sc.chunk_tiles ? at * g.splits + cur.t0 / sc.chunk_tiles
+                                           : ((size_t)blockIdx.x * 2 + (cur.index ? 1 : 0)) * sc.rows + cw.row;
+        // one row tile: each stream's threads write half of the columns
+        const int d0 = two ? 0 : x * (D / 2), d1 = two ? D : d0 + D / 2;
+#pragma unroll 1
+        for (int d = d0; d < d1; d += 16) {
+          uint32_t o[16], o1[16];
+          tmem_ld_16(two ? tO + d : lanes + kColO + d, o);
+          if (join) tmem_ld_16(lanes + kColO + 128 + d, o1);
+          tmem_wait_ld();
+          float z[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) z[j] = __uint_as_float(o[j]) * (f0 * inv);
+          if (join) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) z[j] = fmaf(__uint_as_float(o1[j]), f1 * inv, z[j]);
+          }
+          if (!Q8 && cw.in && *reinterpret_cast<volatile int*>(&ct.dropped)) {   // the dropped elements of keys this row sees
+            const uint64_t* mk = g.mask ? g.mask + (size_t)(cur.bi.start + cw.node) * g.words : nullptr;
+#pragma unroll 1
+            for (int key = max(cur.t0 * KT, cur.all_see); key < min(cur.t1 * KT, cur.n_keys); ++key)
+              if (sees32(mk, g.words, cw.node, key - cur.bi.ctx) & 1) {
+                const bf16* vp = static_cast<const bf16*>(c.v) + (cache_slot(c, cur.bi.row, cur.h, key)) * D + d;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                  const float y = __bfloat162float(vp[j]);
+                  if (!(fabsf(y) < INFINITY)) z[j] += y;
+                }
+              }
+          }
+          if (cw.in && to_out) {
+#pragma unroll
+            for (int j = 0; j < 16; j += 8)
+              *reinterpret_cast<uint4*>(out + at * D + d + j) =
+                  make_uint4(pack2<EESD_KV_MODEL>(z[j], z[j + 1]), pack2<EESD_KV_MODEL>(z[j + 2], z[j + 3]),
+                             pack2<EESD_KV_MODEL>(z[j + 4], z[j + 5]), pack2<EESD_KV_MODEL>(z[j + 6], z[j + 7]));
+          } else if (cw.in) {
+#pragma unroll
+            for (int j = 0; j < 16; j += 4)
+              *reinterpret_cast<float4*>(g.part_o + part * D + d + j) = make_float4(z[j], z[j + 1], z[j + 2], z[j + 3]);
+          }
+          __syncwarp();
+        }
+        tc_fence_before();
+        warp_arrive(&ct.epi_done);
+        if (cw.in && !to_out && (two || x == 0)) g.part_ml[part] = make_float2(M, L);
+        if (tid == 128 && !sc.chunk_tiles && cur.t0 == 0 && cur.t1 < cur.tiles)
+          sc.cuts[blockIdx.x] = TcCut{cur.u0, cur.e, cur.h, cur.index ? 1 : 0, cur.tiles};
+        cnt0 += nt;
+        __syncwarp();
+        if (lane == 0) piece_free(piece);
+      }
+      if (!more) break;
+      ++piece;
+      const Piece& cur = nxt;
+      nt = cur.t1 - cur.t0;
+      two = cur.nrows > 128;
+      rf = rf_next;
+      m = -INFINITY;
+      l = 0.f;
+      er = 0;
+      begun = false;
 #pragma unroll 1
       for (int i = two ? 0 : x; i < nt; i += two ? 1 : 2) {
         const int t = cur.t0 + i, cnt = cnt0 + i, f = cnt % FR;
@@ -766,85 +868,97 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           return begun && __any_sync(0xffffffffu, need);
         };
-        const float rt = Q8 && !partial ? rf * ct.kt[f] : rf;
-        bool rescale = false, slow = partial;
-        if (__builtin_expect(!partial, 1)) {
-          float mx0 = -INFINITY, mx1 = -INFINITY;
+        // Every choice below is made so that what a row does not see does not change a bit of its result: the forms of the
+        // exponent differ between rows only by the row's own scores.
+        const bool k_keyed = Q8 && ct.k_keyed[f], v_keyed = Q8 && partial;
+        const float rt = Q8 && !k_keyed ? rf * ct.kt[f] : rf;
+        if (__builtin_expect(k_keyed, 0)) {
 #pragma unroll
-          for (int j = 0; j < KT; j += 4) {
-            mx0 = fmaxf(mx0, fmaxf(__uint_as_float(a[j]), __uint_as_float(a[j + 1])));
-            mx1 = fmaxf(mx1, fmaxf(__uint_as_float(a[j + 2]), __uint_as_float(a[j + 3])));
-          }
-          rescale = move_to(fmaxf(mx0, mx1) * rt);
-          // One FMA per score leaves 2^-24 |m| of it in the exponent: nothing at ordinary sizes, but at very large ones
-          // the largest score has to come out as exactly 0.  V's scale relative to er goes into the exponent, so l
-          // collects the same units and is brought back by the exact power of two; below 2^-40 that is not f16 any more.
-          slow = __any_sync(0xffffffffu, !(fabsf(m) <= 65536.f) || (Q8 && em - er < -40));
+          for (int j = 0; j < KT; ++j) a[j] = __float_as_uint(__uint_as_float(a[j]) * ct.fk[f][j]);
         }
-        uint32_t w[KT / 2];
-        if (__builtin_expect(!slow, 1)) {
-          const float nbs = (Q8 ? (float)(ref - er) : 0.f) - m;
-          const f32x2 nb = pack_f2(nbs, nbs), rt2 = pack_f2(rt, rt);
-          f32x2 sum0 = pack_f2(0.f, 0.f), sum1 = pack_f2(0.f, 0.f);
+        float vc = 0.f;                                                 // 2^(ref - er): V's factors relative to the row
+        if (__builtin_expect(partial, 0)) {                             // which keys the row sees
+          const int node = row_of(cur).node, left = cur.n_keys - t * KT;
+          const uint64_t* mk = g.mask ? g.mask + (size_t)(cur.bi.start + node) * g.words : nullptr;
+          uint32_t s0 = sees32(mk, g.words, node, t * KT - cur.bi.ctx), s1 = sees32(mk, g.words, node, t * KT + 32 - cur.bi.ctx);
+          if (left < 32) s0 &= (1u << left) - 1;
+          if (left < 64) s1 &= left <= 32 ? 0u : (1u << (left - 32)) - 1;
 #pragma unroll
-          for (int j = 0; j < KT; j += 4) {
-            const float2 y0 = unpack_f2(fma2(pack_f2(__uint_as_float(a[j]), __uint_as_float(a[j + 1])), rt2, nb));
-            const float2 y1 = unpack_f2(fma2(pack_f2(__uint_as_float(a[j + 2]), __uint_as_float(a[j + 3])), rt2, nb));
-            const float e0 = fast_exp2(y0.x), e1 = fast_exp2(y0.y), e2 = fast_exp2(y1.x), e3 = fast_exp2(y1.y);
-            sum0 = add2(sum0, pack_f2(e0, e1));
-            sum1 = add2(sum1, pack_f2(e2, e3));
-            w[j / 2] = pack2<FMT>(e0, e1);
-            w[j / 2 + 1] = pack2<FMT>(e2, e3);
-          }
-          const float2 sv = unpack_f2(add2(sum0, sum1));
-          l = Q8 ? fmaf(sv.x + sv.y, __int_as_float((127 - (ref - er)) << 23), l) : l + sv.x + sv.y;
-        } else {
-          // scores, one by one with what is particular to a key: its scale and whether the row sees it
-          uint32_t s0 = ~0u, s1 = ~0u;
-          const bool keyed = Q8 && partial;
-          if (partial) {
-            const int node = row_of(cur).node, left = cur.n_keys - t * KT;
-            const uint64_t* mk = g.mask ? g.mask + (size_t)(cur.bi.start + node) * g.words : nullptr;
-            s0 = sees32(mk, g.words, node, t * KT - cur.bi.ctx);
-            s1 = sees32(mk, g.words, node, t * KT + 32 - cur.bi.ctx);
-            if (left < 32) s0 &= (1u << left) - 1;
-            if (left < 64) s1 &= left <= 32 ? 0u : (1u << (left - 32)) - 1;
-            if constexpr (Q8) {                                         // V's largest exponent among the keys this row sees
-              uint32_t top = 0;
+          for (int j = 0; j < KT; ++j) a[j] = (j < 32 ? s0 : s1) >> (j & 31) & 1 ? a[j] : 0xff800000u;
+          if constexpr (Q8) {                                           // V's largest exponent among them
+            uint32_t top = 0;
 #pragma unroll 2
-              for (int j = 0; j < KT / 4; ++j) {
-                const uint32_t bits = (j < 8 ? s0 >> 4 * j : s1 >> (4 * j - 32)) & 15;
-                top = __vmaxu4(top, reinterpret_cast<const uint32_t*>(ct.ev[f])[j] & ((bits * 0x204081u & 0x1010101u) * 255u));
-              }
-              em = max(max(top & 255, top >> 8 & 255), max(top >> 16 & 255, top >> 24));
-              if ((ct.nan[f][0] & s0) | (ct.nan[f][1] & s1)) l = __int_as_float(0x7fffffff);   // the row sees a V that is NaN
+            for (int j = 0; j < KT / 4; ++j) {
+              const uint32_t bits = (j < 8 ? s0 >> 4 * j : s1 >> (4 * j - 32)) & 15;
+              top = __vmaxu4(top, reinterpret_cast<const uint32_t*>(ct.ev[f])[j] & ((bits * 0x204081u & 0x1010101u) * 255u));
+            }
+            em = max(max(top & 255, top >> 8 & 255), max(top >> 16 & 255, top >> 24));
+            if ((ct.nan[f][0] & s0) | (ct.nan[f][1] & s1)) l = __int_as_float(0x7fffffff);   // the row sees a V that is NaN
+          }
+        }
+        float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < KT; j += 4) {
+          mx0 = fmaxf(mx0, fmaxf(__uint_as_float(a[j]), __uint_as_float(a[j + 1])));
+          mx1 = fmaxf(mx1, fmaxf(__uint_as_float(a[j + 2]), __uint_as_float(a[j + 3])));
+        }
+        const bool rescale = move_to(fmaxf(mx0, mx1) * rt);
+        if (v_keyed) vc = __int_as_float(min(max(ref - er + 127, 1), 254) << 23);
+        // One FMA per score leaves 2^-24 |m| of it in the exponent: nothing at ordinary sizes, but at very large ones the
+        // largest score has to come out as exactly 0.  V's common scale relative to er goes into the exponent, so l
+        // collects the same units and is brought back by the exact power of two; below 2^-40 that is not f16 any more.
+        const bool huge = !(fabsf(m) <= 65536.f || m == -INFINITY), gone = Q8 && !partial && em - er < -40;
+        const int dd = Q8 && !partial && !gone ? ref - er : 0;
+        const float ms = m == -INFINITY ? 0.f : m, nbs = (float)dd - ms;
+        uint32_t w[KT / 2];
+        f32x2 sum0 = pack_f2(0.f, 0.f), sum1 = pack_f2(0.f, 0.f);
+        if (__builtin_expect(!__any_sync(0xffffffffu, huge || gone), 1)) {
+          const f32x2 nb = pack_f2(nbs, nbs), rt2 = pack_f2(rt, rt);
+          if (__builtin_expect(!v_keyed, 1)) {
+#pragma unroll
+            for (int j = 0; j < KT; j += 4) {
+              const float2 y0 = unpack_f2(fma2(pack_f2(__uint_as_float(a[j]), __uint_as_float(a[j + 1])), rt2, nb));
+              const float2 y1 = unpack_f2(fma2(pack_f2(__uint_as_float(a[j + 2]), __uint_as_float(a[j + 3])), rt2, nb));
+              const float e0 = fast_exp2(y0.x), e1 = fast_exp2(y0.y), e2 = fast_exp2(y1.x), e3 = fast_exp2(y1.y);
+              sum0 = add2(sum0, pack_f2(e0, e1));
+              sum1 = add2(sum1, pack_f2(e2, e3));
+              w[j / 2] = pack2<FMT>(e0, e1);
+              w[j / 2 + 1] = pack2<FMT>(e2, e3);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < KT; j += 4) {
+              const float2 y0 = unpack_f2(fma2(pack_f2(__uint_as_float(a[j]), __uint_as_float(a[j + 1])), rt2, nb));
+              const float2 y1 = unpack_f2(fma2(pack_f2(__uint_as_float(a[j + 2]), __uint_as_float(a[j + 3])), rt2, nb));
+              const float e0 = fast_exp2(y0.x), e1 = fast_exp2(y0.y), e2 = fast_exp2(y1.x), e3 = fast_exp2(y1.y);
+              const float4 v = reinterpret_cast<const float4*>(ct.fv[f])[j / 4];
+              sum0 = add2(sum0, pack_f2(e0, e1));
+              sum1 = add2(sum1, pack_f2(e2, e3));
+              // an unseen key's factor may be out of range, its weight is 0
+              w[j / 2] = pack2<FMT>(e0 == 0.f ? 0.f : e0 * (v.x * vc), e1 == 0.f ? 0.f : e1 * (v.y * vc));
+              w[j / 2 + 1] = pack2<FMT>(e2 == 0.f ? 0.f : e2 * (v.z * vc), e3 == 0.f ? 0.f : e3 * (v.w * vc));
             }
           }
-          float mx = -INFINITY;
-#pragma unroll
-          for (int j = 0; j < KT; ++j) {
-            const float y = __fmul_rn(__uint_as_float(a[j]), keyed ? __fmul_rn(rt, ct.fk[f][j]) : rt);
-            a[j] = (j < 32 ? s0 : s1) >> (j & 31) & 1 ? __float_as_uint(y) : 0xff800000u;
-            mx = fmaxf(mx, __uint_as_float(a[j]));
-          }
-          if (partial) rescale = move_to(mx);
-          const bool gone = Q8 && em - er < -40;
-          const int dd = Q8 && !gone ? min(ref - er, 100) : 0;
-          const float ms = m == -INFINITY ? 0.f : m;
-          float sum = 0.f;
+        } else {                                                        // the same, row by row in its own form
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int j = 0; j < KT; j += 2) {
             float e[2];
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
-              e[b] = fast_exp2(__fadd_rn(__fadd_rn(__uint_as_float(a[j + b]), -ms), (float)dd));
-              sum += e[b];
-              if (Q8) e[b] = gone ? 0.f : keyed ? e[b] * ct.fv[f][j + b] : e[b];
+              const float y = __uint_as_float(a[j + b]);
+              e[b] = fast_exp2(huge ? __fadd_rn(__fadd_rn(__fmul_rn(y, rt), -ms), (float)dd) : fmaf(y, rt, nbs));
+              sum[(j + b) & 3] += e[b];
+              if (v_keyed) e[b] = e[b] == 0.f ? 0.f : e[b] * (ct.fv[f][j + b] * vc);
+              if (gone) e[b] = 0.f;
             }
             w[j / 2] = pack2<FMT>(e[0], e[1]);
           }
-          l = Q8 ? fmaf(sum, __int_as_float((127 - dd) << 23), l) : l + sum;
+          sum0 = pack_f2(sum[0], sum[1]);
+          sum1 = pack_f2(sum[2], sum[3]);
         }
+        const float2 sv = unpack_f2(add2(sum0, sum1));
+        l = Q8 ? fmaf(sv.x + sv.y, __int_as_float((127 - dd) << 23), l) : l + (sv.x + sv.y);
         // ---- P, once the product that read the last one is done (O is at rest then)
         if (n_s && !(ok = warp_wait(&ct.pv_done[x], (n_s - 1) & 1, abort_flag, g.spin))) break;
         ++n_s;
@@ -869,90 +983,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         warp_arrive(&ct.p_ready[x]);
       }
       if (!ok) break;
-      // ---- the next piece's Q goes out before this one's output: its first S runs under it
-      if (!(ok = __all_sync(0xffffffffu, piece_wait(piece + 1)))) break;
-      const Piece& nxt = ct.piece[(piece + 1) % kPieces];
-      more = nxt.tiles != 0;
-      float(&ml)[2][3][128] = ct.ml[piece & 1];
-      if (!two) {
-        ml[x][0][r] = m;
-        ml[x][1][r] = l;
-        ml[x][2][r] = begun ? (float)er : -1.f;                         // -1: the stream had no tile, its O is not there
-        warp_arrive(&ct.ml_ready);
-        if (!(ok = warp_wait(&ct.ml_ready, n_ml++ & 1, abort_flag, g.spin))) break;
-      }
-      if (more) rf = put_q(nxt);
-      if (!(ok = warp_wait(&ct.o_done, piece & 1, abort_flag, g.spin))) break;
-      tc_fence_after();
-      float f0 = 1.f, f1 = 0.f, M = m, L = l, E = (float)er;
-      if (!two) {
-        const float m0 = ml[0][0][r], m1 = ml[1][0][r], e0 = ml[0][2][r], e1 = ml[1][2][r];
-        M = fmaxf(m0, m1);
-        const float ms = M == -INFINITY ? 0.f : M;
-        E = fmaxf(fmaxf(e0, e1), 0.f);
-        const float w0 = fast_exp2(m0 - ms), w1 = e1 < 0.f ? 0.f : fast_exp2(m1 - ms);
-        L = w0 * ml[0][1][r] + (e1 < 0.f ? 0.f : w1 * ml[1][1][r]);
-        f0 = Q8 ? w0 * fast_exp2(e0 - E) : w0;
-        f1 = e1 < 0.f ? 0.f : Q8 ? w1 * fast_exp2(e1 - E) : w1;
-      }
-      float inv = L == 0.f ? 0.f : 1.f / L;                             // a row that sees nothing: zeros
-      if constexpr (Q8) inv *= kHalfUnit<FMT> / (1 << S::kUp) * __int_as_float((int)fmaxf(E, 1.f) << 23);
-      const Row cw = row_of(cur);
-      const bool join = !two && nt > 1;
-      const size_t at = (size_t)(cur.bi.start + cw.node) * g.n_heads + cw.head;
-      const bool to_out = sc.chunk_tiles ? cur.tiles <= sc.chunk_tiles : cur.whole();
-      const size_t part = sc.chunk_tiles ? at * g.splits + cur.t0 / sc.chunk_tiles
-                                         : ((size_t)blockIdx.x * 2 + (cur.index ? 1 : 0)) * sc.rows + cw.row;
-      // one row tile: each stream's threads write half of the columns
-      const int d0 = two ? 0 : x * (D / 2), d1 = two ? D : d0 + D / 2;
-#pragma unroll 1
-      for (int d = d0; d < d1; d += 16) {
-        uint32_t o[16], o1[16];
-        tmem_ld_16(two ? tO + d : lanes + kColO + d, o);
-        if (join) tmem_ld_16(lanes + kColO + 128 + d, o1);
-        tmem_wait_ld();
-        float z[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) z[j] = __uint_as_float(o[j]) * (f0 * inv);
-        if (join) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) z[j] = fmaf(__uint_as_float(o1[j]), f1 * inv, z[j]);
-        }
-        if (!Q8 && cw.in && *reinterpret_cast<volatile int*>(&ct.dropped)) {   // the dropped elements of keys this row sees
-          const uint64_t* mk = g.mask ? g.mask + (size_t)(cur.bi.start + cw.node) * g.words : nullptr;
-#pragma unroll 1
-          for (int key = max(cur.t0 * KT, cur.all_see); key < min(cur.t1 * KT, cur.n_keys); ++key)
-            if (sees32(mk, g.words, cw.node, key - cur.bi.ctx) & 1) {
-              const bf16* vp = static_cast<const bf16*>(c.v) + (cache_slot(c, cur.bi.row, cur.h, key)) * D + d;
-#pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                const float y = __bfloat162float(vp[j]);
-                if (!(fabsf(y) < INFINITY)) z[j] += y;
-              }
-            }
-        }
-        if (cw.in && to_out) {
-#pragma unroll
-          for (int j = 0; j < 16; j += 8)
-            *reinterpret_cast<uint4*>(out + at * D + d + j) =
-                make_uint4(pack2<EESD_KV_MODEL>(z[j], z[j + 1]), pack2<EESD_KV_MODEL>(z[j + 2], z[j + 3]),
-                           pack2<EESD_KV_MODEL>(z[j + 4], z[j + 5]), pack2<EESD_KV_MODEL>(z[j + 6], z[j + 7]));
-        } else if (cw.in) {
-#pragma unroll
-          for (int j = 0; j < 16; j += 4)
-            *reinterpret_cast<float4*>(g.part_o + part * D + d + j) = make_float4(z[j], z[j + 1], z[j + 2], z[j + 3]);
-        }
-        __syncwarp();
-      }
-      tc_fence_before();
-      warp_arrive(&ct.epi_done);
-      if (cw.in && !to_out && (two || x == 0)) g.part_ml[part] = make_float2(M, L);
-      if (tid == 128 && !sc.chunk_tiles && cur.t0 == 0 && cur.t1 < cur.tiles)
-        sc.cuts[blockIdx.x] = TcCut{cur.u0, cur.e, cur.h, cur.index ? 1 : 0, cur.tiles};
-      cnt0 += nt;
-      __syncwarp();
-      if (lane == 0) piece_free(piece);
-      ++piece;
     }
     if (!ok) {
       set_status(g.status, kStatusTimeoutEpilogue);
