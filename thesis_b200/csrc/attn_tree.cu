@@ -735,7 +735,7 @@ Plan plan_for(const EesdKvCache* c, const EesdTree* t, int n_heads, int split_ke
   const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
   p.ml_off = up(parts * c->head_dim * 4);
   p.cuts_off = p.ml_off + up(parts * 8);
-  p.bytes = std::max<size_t>(p.cuts_off + (p.tc ? up(((size_t)p.ctas + 1) * sizeof(TcCut)) : 0), 256);
+  p.bytes = std::max<size_t>(p.cuts_off + (p.tc ? up((size_t)p.ctas * sizeof(TcCut)) : 0), 256);
   return p;
 }
 

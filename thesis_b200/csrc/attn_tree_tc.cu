@@ -48,6 +48,9 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void bulk_prefetch_l2(const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
+}
 // One lane of a converged warp.  The branch on it keeps the warp's scalar registers usable, which a branch on the
 // lane number does not: a product then issues every 42 clocks (N = 64) instead of every 118.
 __device__ __forceinline__ bool elect_one() {
@@ -162,7 +165,7 @@ __device__ __forceinline__ Entry entry_of(const TreeGeom& g, const CacheGeom& c,
   return x;
 }
 struct Piece : Entry {
-  int e, h, t0, t1, index;  // entry, KV head, key tiles [t0, t1), number of the piece in its CTA
+  int h, t0, t1, index;     // KV head, key tiles [t0, t1), number of the piece in its CTA
   long long u0;             // flat position of the unit
   __device__ bool whole() const { return t0 == 0 && t1 == tiles; }
 };
@@ -177,7 +180,7 @@ struct PieceIter {
       if (loaded != e) {
         bool bad;
         static_cast<Entry&>(p) = entry_of(g, c, sc, e, bad);
-        p.e = loaded = e;
+        loaded = e;
       }
       const int len = p.length();
       const long long span = (long long)len * c.n_kv_heads;
@@ -235,6 +238,7 @@ template <int FMT> struct Scaler {
   }
 };
 
+template <int FMT> constexpr int kUp = FMT == EESD_KV_E4M3 ? 14 : 5;   // a tile's largest 8-bit elements in f16: 28672, 4064
 template <int D, int FMT> struct TcShape {
   static constexpr bool Q8 = FMT != EESD_KV_MODEL;
   static constexpr int TILE = KT * D * 2;              // bytes of one 16-bit K (or V) tile
@@ -242,7 +246,6 @@ template <int D, int FMT> struct TcShape {
   static constexpr int NS = Q8 ? 2 : 5;                // 16-bit K / V stages
   static constexpr int RS = Q8 ? 6 : 0;                // raw stages
   static constexpr int FR = 8;                         // factor ring: six tiles can be between conversion and softmax
-  [[maybe_unused]] static constexpr int kUp = FMT == EESD_KV_E4M3 ? 14 : 5;   // a tile's largest 8-bit elements in f16: 28672, 4064
   static constexpr int QB = 128 * D * 2 + 128 * 128;   // Q of stream 1 (more than 128 rows), half rows on their way to TMEM
   static constexpr size_t ctl = 16384;
   static constexpr size_t smem = 1024 + (size_t)2 * NS * TILE + (size_t)RS * RAW + QB + ctl;
@@ -264,7 +267,7 @@ struct TcControl {
   int ref[8], k_keyed[8];
   uint32_t nan[8][2];                      // keys whose V is NaN
   float ml[2][2][3][128];                  // one row tile: max, sum and eref of the streams (by piece parity)
-  long long lo, hi, base;
+  long long lo, hi, base, run;
   long long wsum[20];
   uint32_t tmem;
   int e0;
@@ -355,12 +358,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     const int Hkv = c.n_kv_heads;
     const long long W = total * Hkv, n = gridDim.x;
-    const long long lo = blockIdx.x * W / n, hi = (blockIdx.x + 1) * W / n;
+    const long long run = max(1LL, (W + n - 1) / n), lo = min(W, blockIdx.x * run), hi = min(W, lo + run);
     if (tid == 0) {
       ct.lo = lo;
       ct.hi = hi;
-      sc.cuts[blockIdx.x].e = -1;                                       // no unit of this run goes on in the next one
-      if (blockIdx.x == 0) sc.cuts[gridDim.x].u0 = W;
+      ct.run = run;
+      sc.cuts[blockIdx.x].nrows = 0;                                    // no unit of this run goes on in the next one
     }
     if (lo >= before * Hkv && lo < (before + sum) * Hkv) {
       long long base = before * Hkv;
@@ -524,6 +527,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         ct.piece[k % kPieces] = p;
         mbar_arrive(smem_u32(&ct.piece_full[k % kPieces]));
         if (!more) break;
+        // its rows of q on their way to L2: a token's heads of the group lie together
+        for (int node = p.r0 / g.G; node <= (p.r0 + p.nrows - 1) / g.G; ++node)
+          bulk_prefetch_l2(q + (size_t)(p.bi.start + node) * g.ld_q + (size_t)p.h * g.G * D, g.G * D * 2);
       }
       if (!ok) {
         set_status(g.status, kStatusTimeoutProducer);
@@ -543,12 +549,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t from = row0 * D + ((D == 128 ? ch ^ (row0 & 7) : ch ^ (row0 >> 1 & 3)) << 4);
     const uint32_t to0 = (ch >> 2) * (KT * 128) + row0 * 128 + ((2 * ch & 7 ^ (row0 & 7)) << 4), to1 = to0 ^ 16;
     [[maybe_unused]] auto convert = [&](const uint8_t* src, uint8_t* dst, const uint8_t* e, int top, int flat, int left) {
+      // the warp's 32 rows' factors, one per lane
+      static_assert(KT / kRowStep * 8 <= 32, "a warp's rows");
+      const int mine = row0 + lane / 8 % (KT / kRowStep) * kRowStep, er = e[mine], x = top ? er - top : flat;
+      const uint32_t h = mine >= left ? 0u : top && er == 255 ? 0x7fffu : x >= -14 ? (uint32_t)(x + 15) << 10 : x >= -24 ? 1u << (x + 24) : 0u;
 #pragma unroll
       for (int i = 0; i < KT / kRowStep; ++i) {
         const uint4 w = *reinterpret_cast<const uint4*>(src + from + i * (kRowStep * D));
-        const int er = e[row0 + i * kRowStep], x = top ? er - top : flat;
-        const uint32_t h = (int)row0 + i * kRowStep >= left ? 0u : top && er == 255 ? 0x7fffu : x >= -14 ? (uint32_t)(x + 15) << 10 : x >= -24 ? 1u << (x + 24) : 0u;
-        const uint32_t m = __byte_perm(h, 0, 0x1010);
+        const uint32_t m = __byte_perm(__shfl_sync(0xffffffffu, h, lane % 8 + 8 * i), 0, 0x1010);
         const Scaler<FMT> sc8(m);
         uint4 a, b;
         sc8(w.x, a.x, a.y);
@@ -584,7 +592,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           // K's are folded where that is exact (within 2^16 of each other).
           bool keyed = partial && is_v;
           if (partial && !is_v) keyed = __any_sync(0xffffffffu, (in0 && a0 < em - 16) || (in1 && a1 < em - 16));
-          const int top = keyed ? 0 : max(em, 27) - S::kUp;
+          const int top = keyed ? 0 : max(em, 27) - kUp<FMT>;
           // V's factors in a keyed tile are relative to 2^60 below the largest, so that they last for rows whose own
           // largest is far smaller
           const int ref = keyed ? em - 60 : em;
@@ -608,7 +616,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           warp_arrive(&ct.ffull[f]);
-          convert(sm + 2 * NS * S::TILE + rs * S::RAW + (is_v ? S::RAW / 2 : 0), sm + ((is_v ? NS : 0) + st) * S::TILE, ex, top, is_v ? S::kUp : 0, left);
+          convert(sm + 2 * NS * S::TILE + rs * S::RAW + (is_v ? S::RAW / 2 : 0), sm + ((is_v ? NS : 0) + st) * S::TILE, ex, top, is_v ? kUp<FMT> : 0, left);
           warp_arrive(is_v ? &ct.vfull[st] : &ct.kfull[st]);
           warp_arrive(&ct.raw_empty[rs]);
         } else {
@@ -686,21 +694,33 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       float rf = scale_l2;
       if constexpr (Q8) {
+        // The rows' largest elements: each step halves the lanes that hold one row and the rows that a lane holds, so
+        // lane c of a row's C lanes ends with row c's.
+        static_assert(N == C, "as many loads as lanes on a row");
+        uint32_t amax[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w}, amax = 0;
+          const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+          amax[i] = 0;
 #pragma unroll
-          for (int y = 0; y < 4; ++y) amax = max(amax, max(w[y] << 16 & 0x7fff0000u, w[y] & 0x7fff0000u));
+          for (int y = 0; y < 4; ++y) amax[i] = max(amax[i], max(w[y] << 16 & 0x7fff0000u, w[y] & 0x7fff0000u));
+        }
 #pragma unroll
-          for (int o = 1; o < C; o <<= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-          const int e = min(max((int)(amax >> 23), 27), 227);
-          const float inv = __int_as_float((254 - e) << 23);
-          // the lane whose row this is
+        for (int o = C / 2; o > 0; o >>= 1) {
+          const bool up = lane & o;
 #pragma unroll
-          for (int y = 0; y < RPI; ++y) {
-            const float f = __shfl_sync(0xffffffffu, __int_as_float(e << 23), y * C);
-            if (lane == i * RPI + y) rf *= f * kHalfUnit<FMT>;
+          for (int i = 0; i < o; ++i) {
+            const uint32_t send = up ? amax[i] : amax[i + o], keep = up ? amax[i + o] : amax[i];
+            amax[i] = max(keep, __shfl_xor_sync(0xffffffffu, send, o));
           }
+        }
+        const int e = min(max((int)(amax[0] >> 23), 27), 227);
+        const int own = __shfl_sync(0xffffffffu, e, lane % RPI * C + lane / RPI);   // of the row whose thread this is
+        rf *= __int_as_float(own << 23) * kHalfUnit<FMT>;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float inv = __int_as_float((254 - __shfl_sync(0xffffffffu, e, (lane & ~(C - 1)) | i)) << 23);
+          uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
 #pragma unroll
           for (int y = 0; y < 4; ++y) w[y] = pack2<FMT>(__uint_as_float(w[y] << 16) * inv, __uint_as_float(w[y] & 0xffff0000u) * inv);
           u[i] = make_uint4(w[0], w[1], w[2], w[3]);
@@ -770,13 +790,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           f1 = e1 < 0.f ? 0.f : Q8 ? w1 * fast_exp2(e1 - E) : w1;
         }
         float inv = L == 0.f ? 0.f : 1.f / L;                             // a row that sees nothing: zeros
-        if constexpr (Q8) inv *= kHalfUnit<FMT> / (1 << S::kUp) * __int_as_float((int)fmaxf(E, 1.f) << 23);
+        if constexpr (Q8) inv *= kHalfUnit<FMT> / (1 << kUp<FMT>) * __int_as_float((int)fmaxf(E, 1.f) << 23);
         const Row cw = row_of(cur);
         const bool join = !two && nt > 1;
         const size_t at = (size_t)(cur.bi.start + cw.node) * g.n_heads + cw.head;
         const bool to_out = sc.chunk_tiles ? cur.tiles <= sc.chunk_tiles : cur.whole();
-        const size_t part = sc.chunk_tiles ? at * g.splits + cur.t0 / sc.chunk_tiles
-                                           : ((size_t)blockIdx.x * 2 + (cur.index ? 1 : 0)) * sc.rows + cw.row;
+        const size_t slot = (size_t)blockIdx.x * 2 + (cur.index ? 1 : 0);
+        const size_t part = sc.chunk_tiles ? at * g.splits + cur.t0 / sc.chunk_tiles : slot * sc.rows + cw.row;
+        // partial outputs: row by row for the fixed split's join; else four columns of all rows, then the next four, so
+        // that a warp's store is one run of 512 bytes (row by row its 32 lines took 4 k clocks of a piece)
+        float4* const po = reinterpret_cast<float4*>(g.part_o) + (sc.chunk_tiles ? part * (D / 4) : slot * (D / 4) * sc.rows + cw.row);
+        const int po_step = sc.chunk_tiles ? 1 : sc.rows;
         // one row tile: each stream's threads write half of the columns
         const int d0 = two ? 0 : x * (D / 2), d1 = two ? D : d0 + D / 2;
 #pragma unroll 1
@@ -814,7 +838,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           } else if (cw.in) {
 #pragma unroll
             for (int j = 0; j < 16; j += 4)
-              *reinterpret_cast<float4*>(g.part_o + part * D + d + j) = make_float4(z[j], z[j + 1], z[j + 2], z[j + 3]);
+              po[(size_t)((d + j) / 4) * po_step] = make_float4(z[j], z[j + 1], z[j + 2], z[j + 3]);
           }
           __syncwarp();
         }
@@ -822,7 +846,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         warp_arrive(&ct.epi_done);
         if (cw.in && !to_out && (two || x == 0)) g.part_ml[part] = make_float2(M, L);
         if (tid == 128 && !sc.chunk_tiles && cur.t0 == 0 && cur.t1 < cur.tiles)
-          sc.cuts[blockIdx.x] = TcCut{cur.u0, cur.e, cur.h, cur.index ? 1 : 0, cur.tiles};
+          sc.cuts[blockIdx.x] = TcCut{cur.bi.start, cur.r0, cur.nrows, cur.h, cur.index ? 1 : 0,
+                                      (int)((cur.u0 + kUnitCost + cur.tiles - 1) / ct.run)};
         cnt0 += nt;
         __syncwarp();
         if (lane == 0) piece_free(piece);
@@ -995,64 +1020,45 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 1) tmem_dealloc(tmem, 512);
 }
 
-// Joins the pieces of the unit that goes from run blockIdx.x on into the next ones, in run order.  One warp per row.
+// Joins the pieces of the unit that goes from run blockIdx.x on into the next ones, in run order.  A block has 32 rows, a
+// lane one of them and a warp 16 columns; all of a step's loads are in flight at once.
 template <int D>
-__global__ void __launch_bounds__(256) attn_tree_tc_join_kernel(TreeGeom g, CacheGeom c, TcSchedule sc, bf16* __restrict__ out) {
+__global__ void __launch_bounds__(D * 2) attn_tree_tc_join_kernel(TreeGeom g, TcSchedule sc, bf16* __restrict__ out) {
   pdl_trigger();
   pdl_wait();
-  const int c0 = blockIdx.x, lane = threadIdx.x & 31;
+  const int c0 = blockIdx.x, row = blockIdx.y * 32 + (threadIdx.x & 31), d = (threadIdx.x >> 5) * 16;
   const TcCut cut = sc.cuts[c0];
-  if (cut.e < 0) return;
-  const long long W = sc.cuts[sc.ctas].u0, n = sc.ctas;
-  bool bad;
-  const Entry x = entry_of(g, c, sc, cut.e, bad);
-  // run k is [k W / n, (k + 1) W / n): the run that holds position u is the last one that starts at or before it
-  const int c1 = (int)(((cut.u0 + kUnitCost + cut.tiles) * n - 1) / W);
-  auto slot = [&](int k, int row) { return ((size_t)k * 2 + (k == c0 ? cut.second : 0)) * sc.rows + row; };
-  auto empty = [&](int k) { return k * W / n == (k + 1) * W / n; };     // a run of no position writes nothing
-  const int row = blockIdx.y * 8 + (threadIdx.x >> 5);
-  if (row >= x.nrows) return;
-  const int R = x.r0 + row, node = R / g.G;
-  float M = -INFINITY;
-  for (int k = c0 + lane; k <= c1; k += 32)
-    if (!empty(k)) M = fmaxf(M, g.part_ml[slot(k, row)].x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  if (row >= cut.nrows) return;
+  auto slot = [&](int k) { return (size_t)k * 2 + (k == c0 ? cut.second : 0); };
+  float M = -INFINITY, L = 0.f, acc[16];
+#pragma unroll 4
+  for (int k = c0; k <= cut.last; ++k) M = fmaxf(M, g.part_ml[slot(k) * sc.rows + row].x);
   const float ms = M == -INFINITY ? 0.f : M;
-  constexpr int E = D / 32;
-  float L = 0.f, acc[E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  for (int k0 = c0; k0 <= c1; k0 += 32) {
-    float w = 0.f;
-    if (k0 + lane <= c1 && !empty(k0 + lane)) {
-      const float2 v = g.part_ml[slot(k0 + lane, row)];
-      w = v.y * fast_exp2(v.x - ms);
-    }
-    const int cnt = min(32, c1 - k0 + 1);
-    for (int kb = 0; kb < cnt; kb += 8) {                               // eight loads in flight
-      float v[8][E];
+  for (int j = 0; j < 16; ++j) acc[j] = 0.f;
+#pragma unroll 4
+  for (int k = c0; k <= cut.last; ++k) {
+    const float2 ml = g.part_ml[slot(k) * sc.rows + row];
+    const float4* src = reinterpret_cast<const float4*>(g.part_o) + (slot(k) * (D / 4) + d / 4) * sc.rows + row;
+    const float w = ml.y * fast_exp2(ml.x - ms);
+    L += w;
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const float* src = g.part_o + slot(min(k0 + kb + u, c1), row) * D + lane * E;
-#pragma unroll
-        for (int e = 0; e < E; ++e) v[u][e] = src[e];
-      }
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const float wk = kb + u < 32 ? __shfl_sync(0xffffffffu, w, (kb + u) & 31) : 0.f;
-        if (kb + u < cnt && wk != 0.f) {                                // what an empty run left there is not read
-          L += wk;
-#pragma unroll
-          for (int e = 0; e < E; ++e) acc[e] = fmaf(wk, v[u][e], acc[e]);
-        }
-      }
+    for (int j = 0; j < 4; ++j) {
+      const float4 v = src[(size_t)j * sc.rows];
+      acc[4 * j] = fmaf(w, v.x, acc[4 * j]);
+      acc[4 * j + 1] = fmaf(w, v.y, acc[4 * j + 1]);
+      acc[4 * j + 2] = fmaf(w, v.z, acc[4 * j + 2]);
+      acc[4 * j + 3] = fmaf(w, v.w, acc[4 * j + 3]);
     }
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
-  bf16* dst = out + ((size_t)(x.bi.start + node) * g.n_heads + cut.h * g.G + R % g.G) * D + lane * E;
+  const int R = cut.r0 + row, node = R / g.G;
+  bf16* dst = out + ((size_t)(cut.start + node) * g.n_heads + cut.h * g.G + R - node * g.G) * D + d;
+  uint32_t w[8];
 #pragma unroll
-  for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack2<EESD_KV_MODEL>(acc[e] * inv, acc[e + 1] * inv);
+  for (int j = 0; j < 8; ++j) w[j] = pack2<EESD_KV_MODEL>(acc[2 * j] * inv, acc[2 * j + 1] * inv);
+  *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+  *reinterpret_cast<uint4*>(dst + 8) = make_uint4(w[4], w[5], w[6], w[7]);
 }
 
 template <int D, int FMT>
@@ -1065,7 +1071,7 @@ cudaError_t launch(const TcSchedule& sc, const TreeGeom& g, const CacheGeom& c, 
   if (e != cudaSuccess) return e;
   e = launch_pdl(kernel, dim3(sc.ctas), dim3(kThreads), S::smem, s, km, vm, g, c, sc, static_cast<const bf16*>(q), static_cast<bf16*>(out));
   if (e == cudaSuccess && !sc.chunk_tiles && sc.ctas > 1)
-    e = launch_pdl(attn_tree_tc_join_kernel<D>, dim3(sc.ctas, (std::min(sc.rows, g.max_nodes * g.G) + 7) / 8), dim3(256), 0, s, g, c, sc,
+    e = launch_pdl(attn_tree_tc_join_kernel<D>, dim3(sc.ctas, (std::min(sc.rows, g.max_nodes * g.G) + 31) / 32), dim3(D * 2), 0, s, g, sc,
                    static_cast<bf16*>(out));
   return e;
 }

@@ -10,10 +10,10 @@ namespace eesd {
 struct TreeGeom;
 struct CacheGeom;
 
-// The unit that a run's last piece begins and the next runs go on with (e < 0: none).
+// The unit that a run's last piece begins and the next runs go on with (nrows = 0: none).
 struct TcCut {
-  long long u0;               // flat position of the unit (behind the last run: the length of the flat axis)
-  int e, h, second, tiles;    // entry, KV head, whether the piece is not the run's first, key tiles
+  int start, r0, nrows, h;    // its block's first token, first row of the row tile, rows, KV head
+  int second, last;           // whether the piece is not the run's first; the last run with a piece of the unit
 };
 
 struct TcSchedule {
@@ -22,7 +22,7 @@ struct TcSchedule {
   int tiles_max;        // row tiles of the largest block
   int entries;          // n_blocks * tiles_max
   int chunk_tiles;      // 0: equal runs; else key tiles per piece, cut at multiples of it
-  TcCut* cuts;          // [ctas + 1]
+  TcCut* cuts;          // [ctas]
 };
 
 cudaError_t launch_attn_tree_tc(int fmt, int D, const TcSchedule& sc, const TreeGeom& g, const CacheGeom& c, const CUtensorMap& km,
