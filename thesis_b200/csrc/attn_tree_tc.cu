@@ -101,6 +101,7 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 
 // The whole warp waits and goes on together (what follows are warp-wide instructions).
 __device__ __forceinline__ bool warp_wait(const void* bar, uint32_t parity, volatile int* abort_flag, uint32_t limit) {
+  if (__builtin_expect(__all_sync(0xffffffffu, mbar_try_wait(smem_u32(bar), parity)), 1)) return true;
   return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, abort_flag, limit));
 }
 template <int N> __device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -253,7 +254,7 @@ template <int D, int FMT> struct TcShape {
 constexpr int kPieces = 4;                 // pieces between the schedule warp and the slowest role
 constexpr int kReaders = 19;               // warps that read them: TMA, 2 MMA, 8 softmax, 8 conversion
 struct TcControl {
-  uint64_t kfull[5], kempty[5], vfull[5], vempty[5], vclean[5], raw_full[6], raw_empty[6], ffull[8];
+  uint64_t kfull[5], kempty[5], vfull[5], vempty[5], vclean[5], raw_full[6], raw_empty[6];
   uint64_t piece_full[kPieces], piece_empty[kPieces];
   Piece piece[kPieces];                    // tiles == 0: there are no more
   uint64_t s_full[2], s_free[2], p_ready[2], pv_done[2], q_ready, o_done, ml_ready, epi_done, drain[2];
@@ -324,7 +325,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(smem_u32(&ct.raw_full[i]), 1);
         mbar_init(smem_u32(&ct.raw_empty[i]), 8);
       }
-      for (int i = 0; i < FR; ++i) mbar_init(smem_u32(&ct.ffull[i]), 8);
       for (int i = 0; i < 2; ++i) {
         mbar_init(smem_u32(&ct.s_full[i]), 1);
         mbar_init(smem_u32(&ct.s_free[i]), 4);
@@ -582,41 +582,44 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!(ok = warp_wait(&ct.raw_full[rs], cnt / RS & 1, abort_flag, g.spin))) break;
           const bool partial = (t + 1) * KT > min(p.all_see, p.n_keys);
           const int left = p.n_keys - t * KT;
-          // the tile's largest exponent (of slots before its end, NaN apart)
-          const uint8_t* ex = ct.exps[rs] + (is_v ? KT : 0);
-          const uint32_t v = *reinterpret_cast<const uint16_t*>(ex + 2 * lane);
-          const int a0 = v & 255, a1 = v >> 8;
+          // the largest exponents (of slots before the tile's end, NaN apart)
           const bool in0 = 2 * lane < left, in1 = 2 * lane + 1 < left;
-          const int em = __reduce_max_sync(0xffffffffu, max(in0 && a0 != 255 ? a0 : 0, in1 && a1 != 255 ? a1 : 0));
+          auto largest = [&](const uint8_t* e, int& a0, int& a1) {
+            const uint32_t v = *reinterpret_cast<const uint16_t*>(e + 2 * lane);
+            a0 = v & 255, a1 = v >> 8;
+            return __reduce_max_sync(0xffffffffu, max(in0 && a0 != 255 ? a0 : 0, in1 && a1 != 255 ? a1 : 0));
+          };
+          int a0, a1;
+          const uint8_t *ek = ct.exps[rs], *ev = ek + KT;
+          const int em = largest(is_v ? ev : ek, a0, a1);
           // In a tile that some row does not wholly see, V's scales stay with the weights: they decide a row's precision.
           // K's are folded where that is exact (within 2^16 of each other).
           bool keyed = partial && is_v;
           if (partial && !is_v) keyed = __any_sync(0xffffffffu, (in0 && a0 < em - 16) || (in1 && a1 < em - 16));
           const int top = keyed ? 0 : max(em, 27) - kUp<FMT>;
-          // V's factors in a keyed tile are relative to 2^60 below the largest, so that they last for rows whose own
-          // largest is far smaller
-          const int ref = keyed ? em - 60 : em;
           if (!(ok = warp_wait(is_v ? &ct.vempty[st] : &ct.kempty[st], (cnt / NS & 1) ^ 1, abort_flag, g.spin))) break;
-          // (the factor ring's last reader is behind the products that freed this stage)
-          if (ti == 0) {
-            if (is_v) ct.ref[f] = ref;
-            else ct.kt[f] = __int_as_float(max(top, 1) << 23);
-            if (!is_v) ct.k_keyed[f] = keyed;
-          }
-          if (keyed && ti < KT) {
-            const int e = ex[ti], d = e - ref + 127;
-            if (!is_v) {
-              ct.fk[f][ti] = exp_scale(e);
-            } else {
+          if (!is_v) {
+            // What the softmax needs to know of the tile: it is there once S is.  The ring's last reader is behind the
+            // products that freed this stage.
+            // V's factors in a keyed tile are relative to 2^60 below the largest, so that they last for rows whose own
+            // largest is far smaller.
+            const int em_v = largest(ev, a0, a1), ref = partial ? em_v - 60 : em_v;
+            if (ti == 0) {
+              ct.ref[f] = ref;
+              ct.kt[f] = keyed ? 1.f : __int_as_float(max(top, 1) << 23);
+              ct.k_keyed[f] = keyed;
+            }
+            if (partial && ti < KT) {
+              const int e = ev[ti], d = e - ref + 127;
               const bool nan = e == 255, in = ti < left;
+              if (keyed) ct.fk[f][ti] = exp_scale(ek[ti]);
               ct.ev[f][ti] = nan || !in ? 0 : (uint8_t)e;
               ct.fv[f][ti] = nan || !in || d <= 0 ? 0.f : __int_as_float(d << 23);
               const uint32_t nans = __ballot_sync(0xffffffffu, nan && in);
               if (lane == 0) ct.nan[f][ti >> 5] = nans;
             }
           }
-          warp_arrive(&ct.ffull[f]);
-          convert(sm + 2 * NS * S::TILE + rs * S::RAW + (is_v ? S::RAW / 2 : 0), sm + ((is_v ? NS : 0) + st) * S::TILE, ex, top, is_v ? kUp<FMT> : 0, left);
+          convert(sm + 2 * NS * S::TILE + rs * S::RAW + (is_v ? S::RAW / 2 : 0), sm + ((is_v ? NS : 0) + st) * S::TILE, is_v ? ev : ek, top, is_v ? kUp<FMT> : 0, left);
           warp_arrive(is_v ? &ct.vfull[st] : &ct.kfull[st]);
           warp_arrive(&ct.raw_empty[rs]);
         } else {
@@ -862,47 +865,31 @@ __global__ void __launch_bounds__(kThreads, 1)
       l = 0.f;
       er = 0;
       begun = false;
+      const int whole_to = min(cur.all_see, cur.n_keys);
 #pragma unroll 1
       for (int i = two ? 0 : x; i < nt; i += two ? 1 : 2) {
         const int t = cur.t0 + i, cnt = cnt0 + i, f = cnt % FR;
         if (!(ok = warp_wait(&ct.s_full[x], n_s & 1, abort_flag, g.spin))) break;
         tc_fence_after();
-        if (Q8 && !(ok = warp_wait(&ct.ffull[f], cnt / FR & 1, abort_flag, g.spin))) break;
         uint32_t a[KT];
         tmem_ld32(tS, a);
         tmem_ld32(tS + 32, a + 32);
+        const int ref = Q8 ? ct.ref[f] : 0;
+        const float rt = Q8 ? rf * ct.kt[f] : rf;
         tmem_wait_ld();
         tc_fence_before();
         warp_arrive(&ct.s_free[x]);
-        const bool partial = (t + 1) * KT > min(cur.all_see, cur.n_keys);   // some row does not see some key of the tile
-        const int ref = Q8 ? ct.ref[f] : 0;
-        int em = ref;
-        // O, l and m move to a new reference only when the old one is too small by 2^8 (2^4 for V's scale): the weights
-        // stay below 2^12, in range of f16.  O is then to be scaled by cf.
-        float cf = 1.f;
-        auto move_to = [&](float mx) {
-          const float mn = fmaxf(m, mx);
-          const bool need = !begun || mn > m + 8.f || (Q8 && em > er + 4);
-          if (need) {
-            const int en = max(er, em);
-            cf = m == -INFINITY ? 0.f : fast_exp2(m - mn);
-            l *= cf;
-            if (Q8) cf *= er == 0 ? 0.f : fast_exp2((float)(er - en));
-            m = mn;
-            er = en;
-          }
-          return begun && __any_sync(0xffffffffu, need);
-        };
+        // the product that read the last P is done by now, most often: asked here, looked at when P is ready
+        const bool pv_was_done = n_s == 0 || mbar_try_wait(smem_u32(&ct.pv_done[x]), (n_s - 1) & 1);
+        const bool partial = (t + 1) * KT > whole_to;                   // some row does not see some key of the tile
         // Every choice below is made so that what a row does not see does not change a bit of its result: the forms of the
         // exponent differ between rows only by the row's own scores.
-        const bool k_keyed = Q8 && ct.k_keyed[f], v_keyed = Q8 && partial;
-        const float rt = Q8 && !k_keyed ? rf * ct.kt[f] : rf;
-        if (__builtin_expect(k_keyed, 0)) {
-#pragma unroll
-          for (int j = 0; j < KT; ++j) a[j] = __float_as_uint(__uint_as_float(a[j]) * ct.fk[f][j]);
-        }
-        float vc = 0.f;                                                 // 2^(ref - er): V's factors relative to the row
+        int em = ref;
         if (__builtin_expect(partial, 0)) {                             // which keys the row sees
+          if (Q8 && ct.k_keyed[f]) {
+#pragma unroll
+            for (int j = 0; j < KT; ++j) a[j] = __float_as_uint(__uint_as_float(a[j]) * ct.fk[f][j]);
+          }
           const int node = row_of(cur).node, left = cur.n_keys - t * KT;
           const uint64_t* mk = g.mask ? g.mask + (size_t)(cur.bi.start + node) * g.words : nullptr;
           uint32_t s0 = sees32(mk, g.words, node, t * KT - cur.bi.ctx), s1 = sees32(mk, g.words, node, t * KT + 32 - cur.bi.ctx);
@@ -927,19 +914,38 @@ __global__ void __launch_bounds__(kThreads, 1)
           mx0 = fmaxf(mx0, fmaxf(__uint_as_float(a[j]), __uint_as_float(a[j + 1])));
           mx1 = fmaxf(mx1, fmaxf(__uint_as_float(a[j + 2]), __uint_as_float(a[j + 3])));
         }
-        const bool rescale = move_to(fmaxf(mx0, mx1) * rt);
-        if (v_keyed) vc = __int_as_float(min(max(ref - er + 127, 1), 254) << 23);
+        // O, l and m move to a new reference only when the old one is too small by 2^8 (2^4 for V's scale): the weights
+        // stay below 2^12, in range of f16.  O is then to be scaled by cf.
         // One FMA per score leaves 2^-24 |m| of it in the exponent: nothing at ordinary sizes, but at very large ones the
         // largest score has to come out as exactly 0.  V's common scale relative to er goes into the exponent, so l
         // collects the same units and is brought back by the exact power of two; below 2^-40 that is not f16 any more.
-        const bool huge = !(fabsf(m) <= 65536.f || m == -INFINITY), gone = Q8 && !partial && em - er < -40;
+        const float mn = fmaxf(m, fmaxf(mx0, mx1) * rt);
+        const bool need = !begun || mn > m + 8.f || (Q8 && em > er + 4);
+        auto is_huge = [&] { return !(fabsf(m) <= 65536.f || m == -INFINITY); };
+        auto is_gone = [&] { return Q8 && !partial && em - er < -40; };
+        float cf = 1.f;
+        bool rescale = false, huge = false, gone = false, odd = false;
+        if (__builtin_expect(__any_sync(0xffffffffu, need || is_huge() || is_gone()), 0)) {
+          if (need) {
+            const int en = max(er, em);
+            cf = m == -INFINITY ? 0.f : fast_exp2(m - mn);
+            l *= cf;
+            if (Q8) cf *= er == 0 ? 0.f : fast_exp2((float)(er - en));
+            m = mn;
+            er = en;
+          }
+          rescale = begun && __any_sync(0xffffffffu, need);
+          huge = is_huge(), gone = is_gone();
+          odd = __any_sync(0xffffffffu, huge || gone);
+        }
         const int dd = Q8 && !partial && !gone ? ref - er : 0;
         const float ms = m == -INFINITY ? 0.f : m, nbs = (float)dd - ms;
+        const float vc = Q8 ? __int_as_float(min(max(ref - er + 127, 1), 254) << 23) : 0.f;   // V's factors relative to the row
         uint32_t w[KT / 2];
         f32x2 sum0 = pack_f2(0.f, 0.f), sum1 = pack_f2(0.f, 0.f);
-        if (__builtin_expect(!__any_sync(0xffffffffu, huge || gone), 1)) {
+        if (__builtin_expect(!odd, 1)) {
           const f32x2 nb = pack_f2(nbs, nbs), rt2 = pack_f2(rt, rt);
-          if (__builtin_expect(!v_keyed, 1)) {
+          if (__builtin_expect(!(Q8 && partial), 1)) {
 #pragma unroll
             for (int j = 0; j < KT; j += 4) {
               const float2 y0 = unpack_f2(fma2(pack_f2(__uint_as_float(a[j]), __uint_as_float(a[j + 1])), rt2, nb));
@@ -974,7 +980,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               const float y = __uint_as_float(a[j + b]);
               e[b] = fast_exp2(huge ? __fadd_rn(__fadd_rn(__fmul_rn(y, rt), -ms), (float)dd) : fmaf(y, rt, nbs));
               sum[(j + b) & 3] += e[b];
-              if (v_keyed) e[b] = e[b] == 0.f ? 0.f : e[b] * (ct.fv[f][j + b] * vc);
+              if (Q8 && partial) e[b] = e[b] == 0.f ? 0.f : e[b] * (ct.fv[f][j + b] * vc);
               if (gone) e[b] = 0.f;
             }
             w[j / 2] = pack2<FMT>(e[0], e[1]);
@@ -985,7 +991,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float2 sv = unpack_f2(add2(sum0, sum1));
         l = Q8 ? fmaf(sv.x + sv.y, __int_as_float((127 - dd) << 23), l) : l + (sv.x + sv.y);
         // ---- P, once the product that read the last one is done (O is at rest then)
-        if (n_s && !(ok = warp_wait(&ct.pv_done[x], (n_s - 1) & 1, abort_flag, g.spin))) break;
+        if (!__all_sync(0xffffffffu, pv_was_done) && !(ok = warp_wait(&ct.pv_done[x], (n_s - 1) & 1, abort_flag, g.spin))) break;
         ++n_s;
         tc_fence_after();
         if (__builtin_expect(rescale, 0)) {
