@@ -99,6 +99,15 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Whether the phase is complete, now (try_wait may stay for a while)
+__device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred P;\n\tmbarrier.test_wait.parity.shared::cta.b64 P, [%1], %2;\n\tselp.b32 %0, 1, 0, P;\n\t}"
+               : "=r"(ok)
+               : "r"(bar), "r"(parity)
+               : "memory");
+  return ok != 0;
+}
 // The whole warp waits and goes on together (what follows are warp-wide instructions).
 __device__ __forceinline__ bool warp_wait(const void* bar, uint32_t parity, volatile int* abort_flag, uint32_t limit) {
   if (__builtin_expect(__all_sync(0xffffffffu, mbar_try_wait(smem_u32(bar), parity)), 1)) return true;
@@ -880,7 +889,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
         warp_arrive(&ct.s_free[x]);
         // the product that read the last P is done by now, most often: asked here, looked at when P is ready
-        const bool pv_was_done = n_s == 0 || mbar_try_wait(smem_u32(&ct.pv_done[x]), (n_s - 1) & 1);
+        const bool pv_was_done = n_s == 0 || mbar_test_wait(smem_u32(&ct.pv_done[x]), (n_s - 1) & 1);
         const bool partial = (t + 1) * KT > whole_to;                   // some row does not see some key of the tile
         // Every choice below is made so that what a row does not see does not change a bit of its result: the forms of the
         // exponent differ between rows only by the row's own scores.
