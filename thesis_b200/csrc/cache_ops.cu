@@ -158,11 +158,28 @@ template <> __device__ __forceinline__ void store4<bf16>(bf16* p, const float (&
   *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
 }
 
+// 8 elements, written once and read by others: past the caches
+template <typename T> __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    __stcs(reinterpret_cast<float4*>(p), make_float4(x[0], x[1], x[2], x[3]));
+    __stcs(reinterpret_cast<float4*>(p) + 1, make_float4(x[4], x[5], x[6], x[7]));
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 a = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&a);
+    }
+    __stcs(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
+  }
+}
+
 // A group of D / 8 lanes owns one head of one token: lane l holds elements 4 l .. 4 l + 3 of both halves,
 // that is four rotation pairs, so the rotation needs no exchange and the largest |x| of the vector is a
-// shuffle over the group.  Bound by the bytes of qkv, q_out and the cache.
+// shuffle over the group.  Bound by the bytes of qkv, q_out and the cache, at few tokens by the chain of loads: a thread's
+// kBatch heads are asked for before the token's position, on which the tables and the slot hang, is there.
 template <typename T, int FMT, int D>
-__global__ void __launch_bounds__(128) kv_append_kernel(const T* __restrict__ qkv, int ld_qkv, T* __restrict__ q_out, int ld_qo,
+__global__ void __launch_bounds__(256) kv_append_kernel(const T* qkv, int ld_qkv, T* q_out, int ld_qo,
                                                         int n_heads, const int32_t* __restrict__ tok_pos,
                                                         const int32_t* __restrict__ tok_slot,
                                                         const int32_t* __restrict__ tok_row, CacheGeom c,
@@ -170,15 +187,26 @@ __global__ void __launch_bounds__(128) kv_append_kernel(const T* __restrict__ qk
                                                         int rope_len, int* status) {
   pdl_trigger();
   pdl_wait();
-  constexpr int L = D / 8, GROUPS = 128 / L, H2 = D / 2;
-  const int t = blockIdx.x;
+  constexpr int L = D / 8, GROUPS = 256 / L, H2 = D / 2, kBatch = 3;
+  const int t = blockIdx.x, l = threadIdx.x % L, first = threadIdx.x / L;
+  const T* base = qkv + (size_t)t * ld_qkv + 4 * l;
+  const int heads = n_heads + 2 * c.n_kv_heads;
+  float x[kBatch][2][4];
+  // every lane of a warp takes part in the shuffles: head numbers past the end repeat the last head, unstored
+  auto load = [&](int h0) {
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int h = min(h0 + b * GROUPS, heads - 1);
+      load4<T>(base + (size_t)h * D, x[b][0]);
+      load4<T>(base + (size_t)h * D + H2, x[b][1]);
+    }
+  };
+  load(first);
   const int pos = tok_pos[t], row = tok_row[t], slot = tok_slot[t];
   if (pos < 0 || pos >= rope_len || row < 0 || row >= c.max_batch || slot < 0 || slot >= c.max_seq) {
     if (threadIdx.x == 0) set_status(status, kStatusBadIndex);
     return;
   }
-  const int l = threadIdx.x % L;
-  const T* base = qkv + (size_t)t * ld_qkv + 4 * l;
   float c1[4], c2[4], s1[4], s2[4];
   load4<float>(cosb + (size_t)pos * D + 4 * l, c1);
   load4<float>(cosb + (size_t)pos * D + H2 + 4 * l, c2);
@@ -191,103 +219,121 @@ __global__ void __launch_bounds__(128) kv_append_kernel(const T* __restrict__ qk
     s1[i] = rnd<T>(s1[i]);
     s2[i] = rnd<T>(s2[i]);
   }
-  const int heads = n_heads + 2 * c.n_kv_heads;
-  // every lane of a warp takes part in the shuffles: head numbers past the end repeat the last head, unstored
-  for (int h0 = 0; h0 < heads; h0 += GROUPS) {
-    const int hh = h0 + threadIdx.x / L;
-    const bool in = hh < heads;
-    const int h = in ? hh : heads - 1;
-    float x1[4], x2[4];
-    load4<T>(base + (size_t)h * D, x1);
-    load4<T>(base + (size_t)h * D + H2, x2);
-    if (h < n_heads + c.n_kv_heads) {
+  for (int h0 = first;; load(h0)) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // the roundings of the reference's apply_rope in the model dtype, no contraction to FMA
-        const float a = __fadd_rn(rnd<T>(__fmul_rn(x1[i], c1[i])), rnd<T>(__fmul_rn(-x2[i], s1[i])));
-        const float b = __fadd_rn(rnd<T>(__fmul_rn(x2[i], c2[i])), rnd<T>(__fmul_rn(x1[i], s2[i])));
-        x1[i] = rnd<T>(a);
-        x2[i] = rnd<T>(b);
+    for (int b = 0; b < kBatch; ++b) {
+      const int hh = h0 + b * GROUPS;
+      const bool in = hh < heads;
+      const int h = in ? hh : heads - 1;
+      float(&x1)[4] = x[b][0];
+      float(&x2)[4] = x[b][1];
+      if (h < n_heads + c.n_kv_heads) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          // the roundings of the reference's apply_rope in the model dtype, no contraction to FMA
+          const float a = __fadd_rn(rnd<T>(__fmul_rn(x1[i], c1[i])), rnd<T>(__fmul_rn(-x2[i], s1[i])));
+          const float b = __fadd_rn(rnd<T>(__fmul_rn(x2[i], c2[i])), rnd<T>(__fmul_rn(x1[i], s2[i])));
+          x1[i] = rnd<T>(a);
+          x2[i] = rnd<T>(b);
+        }
+      }
+      if (h < n_heads) {
+        if (in) {
+          T* q = q_out + (size_t)t * ld_qo + (size_t)h * D + 4 * l;
+          store4<T>(q, x1);
+          store4<T>(q + H2, x2);
+        }
+        if constexpr (FMT == EESD_KV_MODEL) continue;
+      }
+      const bool isk = h < n_heads + c.n_kv_heads;
+      const size_t at = cache_slot(c, row, isk ? h - n_heads : h - n_heads - c.n_kv_heads, slot);
+      if constexpr (FMT == EESD_KV_MODEL) {
+        if (in) {
+          T* d = static_cast<T*>(const_cast<void*>(isk ? c.k : c.v)) + at * D + 4 * l;
+          store4<T>(d, x1);
+          store4<T>(d + H2, x2);
+        }
+      } else {
+        uint32_t amax = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) amax = max(amax, max(__float_as_uint(x1[i]) & 0x7fffffffu, __float_as_uint(x2[i]) & 0x7fffffffu));
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        if (!in || h < n_heads) continue;
+        const int eb = exp_byte<FMT>(amax);
+        const float inv = exp_inv_scale(eb);
+        uint32_t w1 = 0, w2 = 0;
+        if (eb != 255) {
+          w1 = quant2<FMT>(x1[0] * inv, x1[1] * inv) | quant2<FMT>(x1[2] * inv, x1[3] * inv) << 16;
+          w2 = quant2<FMT>(x2[0] * inv, x2[1] * inv) | quant2<FMT>(x2[2] * inv, x2[3] * inv) << 16;
+        }
+        uint8_t* d = static_cast<uint8_t*>(const_cast<void*>(isk ? c.k : c.v)) + at * D + 4 * l;
+        *reinterpret_cast<uint32_t*>(d) = w1;
+        *reinterpret_cast<uint32_t*>(d + H2) = w2;
+        if (l == 0) const_cast<uint8_t*>(isk ? c.ke : c.ve)[at] = (uint8_t)eb;
       }
     }
-    if (h < n_heads) {
-      if (in) {
-        T* q = q_out + (size_t)t * ld_qo + (size_t)h * D + 4 * l;
-        store4<T>(q, x1);
-        store4<T>(q + H2, x2);
-      }
-      if constexpr (FMT == EESD_KV_MODEL) continue;
-    }
-    const bool isk = h < n_heads + c.n_kv_heads;
-    const size_t at = cache_slot(c, row, isk ? h - n_heads : h - n_heads - c.n_kv_heads, slot);
-    if constexpr (FMT == EESD_KV_MODEL) {
-      if (in) {
-        T* d = static_cast<T*>(const_cast<void*>(isk ? c.k : c.v)) + at * D + 4 * l;
-        store4<T>(d, x1);
-        store4<T>(d + H2, x2);
-      }
-    } else {
-      uint32_t amax = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) amax = max(amax, max(__float_as_uint(x1[i]) & 0x7fffffffu, __float_as_uint(x2[i]) & 0x7fffffffu));
-#pragma unroll
-      for (int o = L / 2; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-      if (!in || h < n_heads) continue;
-      const int eb = exp_byte<FMT>(amax);
-      const float inv = exp_inv_scale(eb);
-      uint32_t w1 = 0, w2 = 0;
-      if (eb != 255) {
-        w1 = quant2<FMT>(x1[0] * inv, x1[1] * inv) | quant2<FMT>(x1[2] * inv, x1[3] * inv) << 16;
-        w2 = quant2<FMT>(x2[0] * inv, x2[1] * inv) | quant2<FMT>(x2[2] * inv, x2[3] * inv) << 16;
-      }
-      uint8_t* d = static_cast<uint8_t*>(const_cast<void*>(isk ? c.k : c.v)) + at * D + 4 * l;
-      *reinterpret_cast<uint32_t*>(d) = w1;
-      *reinterpret_cast<uint32_t*>(d + H2) = w2;
-      if (l == 0) const_cast<uint8_t*>(isk ? c.ke : c.ve)[at] = (uint8_t)eb;
-    }
+    h0 += kBatch * GROUPS;
+    if (h0 - first >= heads) break;
   }
 }
 
 // ---------------------------------------------------------------- read-back
-// One thread per 8 elements: an 8-byte (8-bit formats) load and 16-byte stores, neighbouring threads on
-// neighbouring chunks of a head, then heads, then tokens.  Bound by the bytes of the output.
+// A warp per token, neighbouring lanes on neighbouring 8-element chunks of a head (an 8-byte load in the 8-bit formats,
+// 16-byte stores), four loads of different heads in flight.  Bound by the bytes of the output.
 template <typename T, int FMT, int D>
 __global__ void __launch_bounds__(256) kv_read_kernel(CacheGeom c, const int32_t* __restrict__ tok_slot,
                                                       const int32_t* __restrict__ tok_row, int n_tok, T* __restrict__ k_out,
                                                       T* __restrict__ v_out, int* status) {
   pdl_trigger();
   pdl_wait();
-  constexpr int C = D / 8;
-  const size_t per = (size_t)c.n_kv_heads * C;
+  constexpr int C = D / 8, STEP = 32 / C, U = 4;
   const bool isk = blockIdx.y == 0 && k_out;
   T* out = isk ? k_out : v_out;
-  const size_t n = (size_t)n_tok * per;
-  for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x) {
-    const int t = (int)(i / per), r = (int)(i - (size_t)t * per), h = r / C, ch = r % C;
+  const void* src = isk ? c.k : c.v;
+  const uint8_t* exps = isk ? c.ke : c.ve;
+  const int lane = threadIdx.x & 31, ch = lane % C;
+  for (long long t = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); t < n_tok; t += (long long)gridDim.x * 8) {
     const int row = tok_row[t], slot = tok_slot[t];
     if (row < 0 || row >= c.max_batch || slot < 0 || slot >= c.max_seq) {
       set_status(status, kStatusBadIndex);
       continue;
     }
-    const size_t at = cache_slot(c, row, h, slot);
-    T* o = out + ((size_t)t * c.n_kv_heads + h) * D + ch * 8;
-    const void* src = isk ? c.k : c.v;
-    float x[4], y[4];
-    if constexpr (FMT == EESD_KV_MODEL) {
-      load4<T>(static_cast<const T*>(src) + at * D + ch * 8, x);
-      load4<T>(static_cast<const T*>(src) + at * D + ch * 8 + 4, y);
-    } else {
-      const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(src) + at * D + ch * 8);
-      const float s = exp_scale((isk ? c.ke : c.ve)[at]) * kHalfUnit<FMT>;
-      uint32_t a, b, e, f;
-      unpack4<FMT>(w.x, a, b);
-      unpack4<FMT>(w.y, e, f);
-      const float2 fa = half2_to_float2(a), fb = half2_to_float2(b), fe = half2_to_float2(e), ff = half2_to_float2(f);
-      x[0] = fa.x * s, x[1] = fa.y * s, x[2] = fb.x * s, x[3] = fb.y * s;
-      y[0] = fe.x * s, y[1] = fe.y * s, y[2] = ff.x * s, y[3] = ff.y * s;
+    for (int h0 = lane / C; h0 < c.n_kv_heads; h0 += U * STEP) {
+      float x[U][8];
+      uint2 w[U];
+      int e[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int h = h0 + u * STEP;
+        if (h >= c.n_kv_heads) break;
+        const size_t at = cache_slot(c, row, h, slot);
+        if constexpr (FMT == EESD_KV_MODEL) {
+          load4<T>(static_cast<const T*>(src) + at * D + ch * 8, *reinterpret_cast<float(*)[4]>(x[u]));
+          load4<T>(static_cast<const T*>(src) + at * D + ch * 8 + 4, *reinterpret_cast<float(*)[4]>(x[u] + 4));
+        } else {
+          w[u] = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(src) + at * D + ch * 8);
+          e[u] = exps[at];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int h = h0 + u * STEP;
+        if (h >= c.n_kv_heads) break;
+        if constexpr (FMT != EESD_KV_MODEL) {
+          const float s = exp_scale(e[u]) * kHalfUnit<FMT>;
+          uint32_t p[4];
+          unpack4<FMT>(w[u].x, p[0], p[1]);
+          unpack4<FMT>(w[u].y, p[2], p[3]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = half2_to_float2(p[i]);
+            x[u][2 * i] = f.x * s, x[u][2 * i + 1] = f.y * s;
+          }
+        }
+        store8<T>(out + ((size_t)t * c.n_kv_heads + h) * D + ch * 8, x[u]);
+      }
     }
-    store4<T>(o, x);
-    store4<T>(o + 4, y);
   }
 }
 
@@ -401,8 +447,8 @@ template <typename T, int FMT>
 cudaError_t append_d(int D, int n_tok, cudaStream_t s, const T* qkv, int ld, T* q_out, int ldo, int H, const int32_t* pos,
                      const int32_t* slot, const int32_t* row, const CacheGeom& g, const float* cs, const float* sn, int rl, int* st) {
   if (D == 64)
-    return launch_pdl(kv_append_kernel<T, FMT, 64>, dim3(n_tok), dim3(128), 0, s, qkv, ld, q_out, ldo, H, pos, slot, row, g, cs, sn, rl, st);
-  return launch_pdl(kv_append_kernel<T, FMT, 128>, dim3(n_tok), dim3(128), 0, s, qkv, ld, q_out, ldo, H, pos, slot, row, g, cs, sn, rl, st);
+    return launch_pdl(kv_append_kernel<T, FMT, 64>, dim3(n_tok), dim3(256), 0, s, qkv, ld, q_out, ldo, H, pos, slot, row, g, cs, sn, rl, st);
+  return launch_pdl(kv_append_kernel<T, FMT, 128>, dim3(n_tok), dim3(256), 0, s, qkv, ld, q_out, ldo, H, pos, slot, row, g, cs, sn, rl, st);
 }
 template <typename T>
 cudaError_t append_t(int fmt, int D, int n_tok, cudaStream_t s, void* qkv, int ld, void* q_out, int ldo, int H, const int32_t* pos,
@@ -491,8 +537,7 @@ int eesd_kv_read(int dtype, const EesdKvCache* c, int layer, const int32_t* tok_
     return fail_arg(EESD_ERR_ARG, "kv_read: outputs must be 16-byte aligned");
   if ((rc = check_stream("kv_read", stream))) return rc;
   const CacheGeom g = cache_layer(c, dtype, layer);
-  const size_t n = (size_t)n_tok * c->n_kv_heads * (c->head_dim / 8);
-  const size_t ctas = (n + 255) / 256;
+  const int ctas = n_tok / 8 + (n_tok % 8 != 0);                         // 8 warps each, a token per warp
   const dim3 grid((unsigned)(ctas < 148 * 16 ? ctas : 148 * 16), (k_out && v_out) ? 2 : 1);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e = dtype == EESD_BF16 ? read_t<bf16>(c->format, c->head_dim, grid, s, g, tok_slot, tok_row, n_tok, k_out, v_out, status)
