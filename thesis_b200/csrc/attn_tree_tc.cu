@@ -360,14 +360,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc_fence_after();
     long long before = inc - sum, total = 0;
-#pragma unroll 1
+#pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) {
-      if (w < warp) before += ct.wsum[w];
-      total += ct.wsum[w];
+      const long long v = ct.wsum[w];
+      if (w < warp) before += v;
+      total += v;
     }
     const int Hkv = c.n_kv_heads;
     const long long W = total * Hkv, n = gridDim.x;
-    const long long run = max(1LL, (W + n - 1) / n), lo = min(W, blockIdx.x * run), hi = min(W, lo + run);
+    const long long run = max(1LL, W < (1LL << 31) - n ? (long long)((uint32_t)(W + n - 1) / (uint32_t)n) : (W + n - 1) / n), lo = min(W, blockIdx.x * run), hi = min(W, lo + run);
     if (tid == 0) {
       ct.lo = lo;
       ct.hi = hi;
@@ -562,9 +563,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       static_assert(KT / kRowStep * 8 <= 32, "a warp's rows");
       const int mine = row0 + lane / 8 % (KT / kRowStep) * kRowStep, er = e[mine], x = top ? er - top : flat;
       const uint32_t h = mine >= left ? 0u : top && er == 255 ? 0x7fffu : x >= -14 ? (uint32_t)(x + 15) << 10 : x >= -24 ? 1u << (x + 24) : 0u;
+      uint4 raw4[KT / kRowStep];                                        // all loads before the first store
+#pragma unroll
+      for (int i = 0; i < KT / kRowStep; ++i) raw4[i] = *reinterpret_cast<const uint4*>(src + from + i * (kRowStep * D));
 #pragma unroll
       for (int i = 0; i < KT / kRowStep; ++i) {
-        const uint4 w = *reinterpret_cast<const uint4*>(src + from + i * (kRowStep * D));
+        const uint4 w = raw4[i];
         const uint32_t m = __byte_perm(__shfl_sync(0xffffffffu, h, lane % 8 + 8 * i), 0, 0x1010);
         const Scaler<FMT> sc8(m);
         uint4 a, b;
@@ -607,7 +611,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (partial && !is_v) keyed = __any_sync(0xffffffffu, (in0 && a0 < em - 16) || (in1 && a1 < em - 16));
           const int top = keyed ? 0 : max(em, 27) - kUp<FMT>;
           if (!(ok = warp_wait(is_v ? &ct.vempty[st] : &ct.kempty[st], (cnt / NS & 1) ^ 1, abort_flag, g.spin))) break;
-          if (!is_v) {
+          if (!is_v && (partial || warp == 12)) {
             // What the softmax needs to know of the tile: it is there once S is.  The ring's last reader is behind the
             // products that freed this stage.
             // V's factors in a keyed tile are relative to 2^60 below the largest, so that they last for rows whose own
@@ -629,8 +633,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           convert(sm + 2 * NS * S::TILE + rs * S::RAW + (is_v ? S::RAW / 2 : 0), sm + ((is_v ? NS : 0) + st) * S::TILE, is_v ? ev : ek, top, is_v ? kUp<FMT> : 0, left);
-          warp_arrive(is_v ? &ct.vfull[st] : &ct.kfull[st]);
-          warp_arrive(&ct.raw_empty[rs]);
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(smem_u32(is_v ? &ct.vfull[st] : &ct.kfull[st]));
+            mbar_arrive(smem_u32(&ct.raw_empty[rs]));
+          }
         } else {
           if (!(ok = warp_wait(&ct.vfull[st], cnt / NS & 1, abort_flag, g.spin))) break;
           if ((t + 1) * KT > min(p.all_see, p.n_keys)) {
