@@ -600,6 +600,97 @@ def test_attention_matches_the_chain_attention(cuda_dev):
     assert (err <= 2 * (2.0 ** -8 * A * 2) * 1.02).all()               # each side: weights and output rounded
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("H,Hkv,D,T", [(5, 1, 64, 256), (2, 2, 128, 256), (48, 1, 128, 1), (40, 1, 64, 3), (33, 1, 128, 9)])
+def test_attention_widest_trees_and_groups(cuda_dev, fmt, H, Hkv, D, T):
+    """The most nodes that a mask has, groups of more heads than a small tile has rows, and row counts that end in
+    every part of the larger tiles."""
+    rng = np.random.default_rng(T)
+    cache = make_cache(cuda_dev, fmt, 3, Hkv, 576, D, seed=D)
+    blocks = [(0, 190, random_tree(T, rng)), (2, 0, random_tree(max(1, T - 100), rng)), (1, 320, random_tree(T, rng))]
+    t = tr.TreeBatch(blocks, cache)
+    q = queries(cuda_dev, t.n_tokens, H * D, seed=H)
+    out = tr.tree_attention(q, cache, t)
+    t.check()
+    check_attention(out, q, cache, blocks, sees_of(blocks), H)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int8"])
+@pytest.mark.parametrize("n", [1, 3, 60])
+def test_attention_many_small_units(cuda_dev, fmt, n):
+    """Ragged short contexts: runs that hold many units, or less than one, and CTAs that are left without a run."""
+    H, Hkv, D = 16, 1, 64
+    rng = np.random.default_rng(n)
+    cache = make_cache(cuda_dev, fmt, 3, Hkv, 1088, D)
+    for _ in range(4):
+        blocks = [(int(rng.integers(3)), int(rng.choice([0, 1, 63, 64, 447, 449, 511, 513, 1000])), int(rng.integers(3, 25)))
+                  for _ in range(n)]
+        t = tr.TreeBatch(blocks, cache)
+        q = queries(cuda_dev, t.n_tokens, H * D)
+        out = tr.tree_attention(q, cache, t)
+        t.check()
+        check_attention(out, q, cache, blocks, sees_of(blocks), H)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("T", [3, 40])
+def test_attention_reports_a_wait_that_runs_out(cuda_dev, fmt, T):
+    """With a poll limit of 0 every pipeline wait gives up: the status word says so and the next call is right."""
+    cache = make_cache(cuda_dev, fmt, 2, 2, 640, 128)
+    rng = np.random.default_rng(T)
+    blocks = [(0, 500, random_tree(T, rng)), (1, 64, random_tree(2, rng))]
+    t = tr.TreeBatch(blocks, cache)
+    q = queries(cuda_dev, t.n_tokens, 8 * 128)
+    good = tr.tree_attention(q, cache, t)
+    t.check()
+    lib.call("eesd_set_option", lib.OPT_SPIN_LIMIT, 0)
+    try:
+        tr.tree_attention(q, cache, t)
+        torch.cuda.synchronize()
+    finally:
+        lib.call("eesd_set_option", lib.OPT_SPIN_LIMIT, -1)
+    with pytest.raises(lib.EesdError):
+        t.check()
+    assert torch.equal(tr.tree_attention(q, cache, t), good)
+    t.check()
+
+
+def test_attention_calls_at_once(cuda_dev):
+    """Calls on two streams, each with its own workspace, while a third launches its round: the bits of calls one by one."""
+    H, Hkv, D = 8, 2, 128
+    rng = np.random.default_rng(5)
+    caches = [make_cache(cuda_dev, f, 2, Hkv, 4352, D, seed=i) for i, f in enumerate(("e4m3", "bf16", "int8"))]
+    trees = [tr.TreeBatch([(0, 4100, random_tree(T, rng)), (1, 700, random_tree(5, rng))], c) for T, c in zip((40, 60, 5), caches)]
+    qs = [queries(cuda_dev, t.n_tokens, H * D, seed=i) for i, t in enumerate(trees)]
+    want = [tr.tree_attention(q, c, t) for q, c, t in zip(qs, caches, trees)]
+    ws = [tr.attention_workspace(t, c, H) for t, c in zip(trees, caches)]
+    outs = [[torch.zeros_like(w) for _ in range(6)] for w in want]
+    streams = [torch.cuda.Stream() for _ in trees]
+    torch.cuda.synchronize()
+    for k in range(6):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                tr.tree_attention(qs[i], caches[i], trees[i], outs[i][k], workspace=ws[i])
+    torch.cuda.synchronize()
+    for w, o, t in zip(want, outs, trees):
+        t.check()
+        assert all(torch.equal(w, x) for x in o)
+
+
+def test_batch_and_cache_on_different_devices_are_refused(cuda_dev):
+    cache = make_cache(cuda_dev, "e4m3", 1, 1, 64, 64)
+    t = tr.TreeBatch([(0, 8, 2)], cache)
+    cos, sin = tables(cuda_dev, 64, 64)
+    q = queries(cuda_dev, 2, 64)
+    t.device = torch.device("cuda", 7)
+    with pytest.raises(ValueError):
+        tr.tree_attention(q, cache, t)
+    with pytest.raises(ValueError):
+        tr.kv_append(queries(cuda_dev, 2, 3 * 64), cache, t, cos, sin)
+    with pytest.raises(ValueError):
+        tr.kv_compact(cache, t, torch.zeros(1, 2, dtype=torch.int32, device=cuda_dev), torch.ones(1, dtype=torch.int32, device=cuda_dev))
+
+
 # ----------------------------------------------------------------- acceptance and compaction
 def walk(y, ids, parents):
     path = [0]

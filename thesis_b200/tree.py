@@ -171,6 +171,12 @@ class TreeBatch:
         self.ptr_status = self.status.data_ptr()
         self.update()
 
+    def on(self, cache: "KVCache") -> "TreeBatch":
+        """The batch itself, if it is on the cache's device."""
+        if self.device != cache.device:
+            raise ValueError(f"a batch on {self.device} and a cache on {cache.device}")
+        return self
+
     def update(self) -> None:
         """Positions, slots, rows and the mask from ``blk`` and ``parent`` (one launch)."""
         _call(self.device, "eesd_tree_meta", self.ref, self._cache.max_batch, self._cache.max_seq, self.ptr_status)
@@ -190,7 +196,7 @@ def kv_append(qkv: torch.Tensor, cache: KVCache, tree: TreeBatch, rope_cos: torc
     """RoPE of q and k of ``qkv`` [n_tokens, (Hq + 2 Hkv) D] (rows may be strided) and the (quantising) append of k
     and v.  The rotated q goes to ``q_out`` [n_tokens, Hq D], or back into ``qkv``."""
     dt = cache.model_dtype(qkv, "qkv")
-    D, dev, n = cache.head_dim, cache.device, tree.n_tokens
+    D, dev, n = cache.head_dim, cache.device, tree.on(cache).n_tokens
     n_heads = _heads(qkv, "qkv", n, D) - 2 * cache.n_kv_heads
     cos = _need(rope_cos, "rope_cos", dev, torch.float32)
     sin = _need(rope_sin, "rope_sin", dev, torch.float32, rope_cos.shape)
@@ -244,7 +250,7 @@ def tree_attention(q: torch.Tensor, cache: KVCache, tree: TreeBatch, out: Option
     be strided, e.g. the q columns of a fused projection); the result is [n_tokens, Hq D] in q's dtype.  See
     ``eesd_attn_tree`` for what a node sees and for ``split_keys``."""
     dt = cache.model_dtype(q, "q")
-    dev, n = cache.device, tree.n_tokens
+    dev, n = cache.device, tree.on(cache).n_tokens
     n_heads = _heads(q, "q", n, cache.head_dim)
     if out is None:
         out = torch.empty(n, q.shape[1], dtype=q.dtype, device=dev)
@@ -269,9 +275,7 @@ def tree_accept(y: torch.Tensor, ids: torch.Tensor, tree: TreeBatch, path: torch
 
 def kv_compact(cache: KVCache, tree: TreeBatch, path: torch.Tensor, n_acc: torch.Tensor) -> None:
     """Move the accepted path's K and V of every layer to the slots behind ``ctx`` (blocks on different rows)."""
-    dev, i32 = tree.device, torch.int32
-    if cache.device != dev:
-        raise ValueError(f"kv_compact: a batch on {dev} and a cache on {cache.device}")
+    dev, i32 = tree.on(cache).device, torch.int32
     _call(dev, "eesd_kv_compact", lib.F32 if cache.format == "f32" else lib.BF16, cache.ref, tree.ref,
           _need(path, "path", dev, i32, (tree.n_blocks, tree.max_nodes)), _need(n_acc, "n_acc", dev, i32, (tree.n_blocks,)),
           tree.ptr_status)
