@@ -301,7 +301,7 @@ typedef struct EesdTree {
   int32_t max_ctx;               /* host: largest ctx + T, at least (<= max_seq) */
   int32_t words;                 /* 64-bit words per mask row: (max_nodes + 63) / 64, at most 4; 0 without a mask */
   int32_t reserved;              /* 0 */
-  const int32_t* blk;            /* [n_blocks, 4] = (start, T, row, ctx); the blocks tile the tokens */
+  const int32_t* blk;            /* [n_blocks, 4] = (start, T, row, ctx), 16-byte aligned; the blocks tile the tokens */
   const int32_t* parent;         /* [n_tokens], NULL: every block is a chain */
   int32_t* tok_pos;              /* [n_tokens] RoPE position: ctx + depth */
   int32_t* tok_slot;             /* [n_tokens] cache slot: ctx + i */
@@ -339,9 +339,10 @@ int eesd_kv_read(int dtype, const EesdKvCache* cache, int layer, const int32_t* 
  * infinities among them, do not reach it.  q: rotated queries, tokens ld_q elements apart (ld_q % 8 == 0,
  * 16-byte aligned), Hq D used; out [n_tokens, Hq D].  split_keys: 0 lets the library split long key ranges
  * over CTAs as the launch needs; a multiple of 256 fixes the split, so that a block's result does not
- * depend on the other blocks of the launch (at the same max_nodes, which decides the kernel).  workspace: eesd_attn_tree_workspace_bytes() bytes, 256-byte aligned,
- * not initialised, not shared by calls that may overlap.  A block that does not fit the tree's maxima or
- * the cache sets a bit in *status and is skipped. */
+ * depend on the other blocks of the launch (at the same max_nodes, which decides the kernel).  workspace:
+ * eesd_attn_tree_workspace_bytes() bytes, 256-byte aligned, not initialised, not shared by calls that may
+ * overlap.  A block that does not fit the tree's maxima or the cache sets a bit in *status and is skipped.
+ * The same call gives the same bits again; what a node does not see does not change a bit of its row. */
 size_t eesd_attn_tree_workspace_bytes(int dtype, const EesdKvCache* cache, const EesdTree* tree, int n_heads, int split_keys);
 int eesd_attn_tree(int dtype, const EesdKvCache* cache, int layer, const EesdTree* tree, const void* q, int ld_q,
                    int n_heads, void* out, int split_keys, void* workspace, size_t workspace_bytes, int32_t* status,

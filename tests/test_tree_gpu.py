@@ -833,6 +833,27 @@ def test_round_of_tree_drafts(cuda_dev, fmt):
                     assert torch.equal(x.contiguous().view(torch.uint8), w.contiguous().view(torch.uint8))
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "f32"])
+def test_wrapped_tensors_are_the_cache(cuda_dev, fmt):
+    """A cache over existing tensors, as a model's: written and read in place, the same bits as a cache of its own."""
+    L, B, H, Hkv, D, S = 2, 2, 4, 2, 64, 128
+    dt = torch.bfloat16 if fmt == "bf16" else torch.float32
+    own = tr.KVCache(L, B, Hkv, S, D, fmt, cuda_dev)
+    k, v = torch.zeros(L, B, Hkv, S, D, dtype=dt, device=cuda_dev), torch.zeros(L, B, Hkv, S, D, dtype=dt, device=cuda_dev)
+    over = tr.KVCache.wrap(k, v)
+    cos, sin = tables(cuda_dev, S, D)
+    blocks = [(1, 0, 30), (0, 0, [-1, 0, 0, 2])]
+    outs = []
+    for cache in (own, over):
+        t = tr.TreeBatch(blocks, cache)
+        qkv = queries(cuda_dev, t.n_tokens, (H + 2 * Hkv) * D, dtype=dt)
+        tr.kv_append(qkv, cache, t, cos, sin, layer=1)
+        outs.append(tr.tree_attention(qkv[:, :H * D], cache, t, layer=1))
+        t.check()
+    assert torch.equal(*outs) and torch.equal(k, own.k) and torch.equal(v, own.v)
+    assert k[1, 1, :, :30].abs().sum() > 0 and (k[0] == 0).all()
+
+
 def test_round_is_capturable(cuda_dev):
     """A whole round as one graph, replayed with other contents: the eager results."""
     L, B, H, Hkv, D, S = 2, 2, 4, 2, 64, 192

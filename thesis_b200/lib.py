@@ -124,7 +124,7 @@ def check(rc: int, what: str = "") -> None:
         raise EesdError(f"{what or 'eesd call'} failed with status {rc}: {msg}")
 
 
-# entry points that launch exactly one kernel (counted for the bench's launch total)
+# entry points that launch one kernel (counted for the bench's launch total; eesd_attn_tree may launch a second that joins)
 KERNEL_CALLS = {"eesd_pack_weight", "eesd_copy_rows", "eesd_gather_ids", "eesd_scatter_ids", "eesd_greedy_accept",
                 "eesd_round_meta", "eesd_round_advance", "eesd_rmsnorm",
                 "eesd_gemm", "eesd_attn_varlen_gqa", "eesd_rope_kv_append", "eesd_tree_meta", "eesd_kv_append",
