@@ -720,9 +720,9 @@ Plan plan_for(const EesdKvCache* c, const EesdTree* t, int n_heads, int split_ke
   p.chunk = split_keys;
   size_t parts = 0;     // partial rows
   if (p.tc) {
-    // a run of less than 8 tiles is not worth a CTA of its own
+    // a CTA for every unit, and more where runs of 8 tiles and more remain
     const long long most = units * ((t->max_ctx + 63) / 64);
-    p.ctas = (int)std::max(1LL, std::min<long long>(sm_count(), (most + 7) / 8));
+    p.ctas = (int)std::max(1LL, std::min<long long>(sm_count(), std::max(units, (most + 7) / 8)));
     if (!p.chunk) parts = (size_t)p.ctas * 2 * p.rows;
   } else if (!p.chunk) {
     const int slots = sm_count() * (p.nt == 4 || (p.nt == 3 && c->head_dim == 128 && c->format != EESD_KV_MODEL) ? 2 : 3);

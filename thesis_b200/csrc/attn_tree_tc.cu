@@ -1042,45 +1042,65 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 1) tmem_dealloc(tmem, 512);
 }
 
-// Joins the pieces of the unit that goes from run blockIdx.x on into the next ones, in run order.  A block has 32 rows, a
-// lane one of them and a warp 16 columns; all of a step's loads are in flight at once.
+// Joins the pieces of the unit that goes from run blockIdx.x on into the next ones, in run order.  A block has 32 rows and
+// 64 columns, a lane one row and a warp 16 columns.  Bound by the latency of its loads where a unit is in many pieces (a
+// long context of one KV head: all of them), so the warps share the search for the largest reference and four pieces'
+// loads are in flight.
 template <int D>
-__global__ void __launch_bounds__(D * 2) attn_tree_tc_join_kernel(TreeGeom g, TcSchedule sc, bf16* __restrict__ out) {
+__global__ void __launch_bounds__(128) attn_tree_tc_join_kernel(TreeGeom g, TcSchedule sc, bf16* __restrict__ out) {
   pdl_trigger();
   pdl_wait();
-  const int c0 = blockIdx.x, row = blockIdx.y * 32 + (threadIdx.x & 31), d = (threadIdx.x >> 5) * 16;
+  constexpr int W = 4, U = 4, N = 16;
+  __shared__ float top[W][32];
+  const int c0 = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = (blockIdx.z * W + warp) * N;
   const TcCut cut = sc.cuts[c0];
-  if (row >= cut.nrows) return;
+  if ((int)blockIdx.y * 32 >= cut.nrows) return;
+  const int row = blockIdx.y * 32 + lane, at = min(row, cut.nrows - 1);
   auto slot = [&](int k) { return (size_t)k * 2 + (k == c0 ? cut.second : 0); };
-  float M = -INFINITY, L = 0.f, acc[16];
+  float M = -INFINITY, L = 0.f, acc[N];
 #pragma unroll 4
-  for (int k = c0; k <= cut.last; ++k) M = fmaxf(M, g.part_ml[slot(k) * sc.rows + row].x);
+  for (int k = c0 + warp; k <= cut.last; k += W) M = fmaxf(M, g.part_ml[slot(k) * sc.rows + at].x);
+  top[warp][lane] = M;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < W; ++w) M = fmaxf(M, top[w][lane]);
   const float ms = M == -INFINITY ? 0.f : M;
 #pragma unroll
-  for (int j = 0; j < 16; ++j) acc[j] = 0.f;
-#pragma unroll 4
-  for (int k = c0; k <= cut.last; ++k) {
-    const float2 ml = g.part_ml[slot(k) * sc.rows + row];
-    const float4* src = reinterpret_cast<const float4*>(g.part_o) + (slot(k) * (D / 4) + d / 4) * sc.rows + row;
-    const float w = ml.y * fast_exp2(ml.x - ms);
-    L += w;
+  for (int j = 0; j < N; ++j) acc[j] = 0.f;
+  for (int k0 = c0; k0 <= cut.last; k0 += U) {
+    float2 ml[U];
+    float4 v[U][N / 4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float4 v = src[(size_t)j * sc.rows];
-      acc[4 * j] = fmaf(w, v.x, acc[4 * j]);
-      acc[4 * j + 1] = fmaf(w, v.y, acc[4 * j + 1]);
-      acc[4 * j + 2] = fmaf(w, v.z, acc[4 * j + 2]);
-      acc[4 * j + 3] = fmaf(w, v.w, acc[4 * j + 3]);
+    for (int u = 0; u < U; ++u) {
+      if (k0 + u > cut.last) break;
+      ml[u] = g.part_ml[slot(k0 + u) * sc.rows + at];
+      const float4* src = reinterpret_cast<const float4*>(g.part_o) + (slot(k0 + u) * (D / 4) + d / 4) * sc.rows + at;
+#pragma unroll
+      for (int j = 0; j < N / 4; ++j) v[u][j] = src[(size_t)j * sc.rows];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (k0 + u > cut.last) break;
+      const float w = ml[u].y * fast_exp2(ml[u].x - ms);
+      L += w;
+#pragma unroll
+      for (int j = 0; j < N / 4; ++j) {
+        acc[4 * j] = fmaf(w, v[u][j].x, acc[4 * j]);
+        acc[4 * j + 1] = fmaf(w, v[u][j].y, acc[4 * j + 1]);
+        acc[4 * j + 2] = fmaf(w, v[u][j].z, acc[4 * j + 2]);
+        acc[4 * j + 3] = fmaf(w, v[u][j].w, acc[4 * j + 3]);
+      }
     }
   }
+  if (row >= cut.nrows) return;
   const float inv = L == 0.f ? 0.f : 1.f / L;
   const int R = cut.r0 + row, node = R / g.G;
   bf16* dst = out + ((size_t)(cut.start + node) * g.n_heads + cut.h * g.G + R - node * g.G) * D + d;
-  uint32_t w[8];
+  uint32_t w[N / 2];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) w[j] = pack2<EESD_KV_MODEL>(acc[2 * j] * inv, acc[2 * j + 1] * inv);
-  *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-  *reinterpret_cast<uint4*>(dst + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+  for (int j = 0; j < N / 2; ++j) w[j] = pack2<EESD_KV_MODEL>(acc[2 * j] * inv, acc[2 * j + 1] * inv);
+#pragma unroll
+  for (int j = 0; j < N / 2; j += 4) *reinterpret_cast<uint4*>(dst + 2 * j) = make_uint4(w[j], w[j + 1], w[j + 2], w[j + 3]);
 }
 
 template <int D, int FMT>
@@ -1093,7 +1113,7 @@ cudaError_t launch(const TcSchedule& sc, const TreeGeom& g, const CacheGeom& c, 
   if (e != cudaSuccess) return e;
   e = launch_pdl(kernel, dim3(sc.ctas), dim3(kThreads), S::smem, s, km, vm, g, c, sc, static_cast<const bf16*>(q), static_cast<bf16*>(out));
   if (e == cudaSuccess && !sc.chunk_tiles && sc.ctas > 1)
-    e = launch_pdl(attn_tree_tc_join_kernel<D>, dim3(sc.ctas, (std::min(sc.rows, g.max_nodes * g.G) + 31) / 32), dim3(D * 2), 0, s, g, sc,
+    e = launch_pdl(attn_tree_tc_join_kernel<D>, dim3(sc.ctas, (std::min(sc.rows, g.max_nodes * g.G) + 31) / 32, D / 64), dim3(128), 0, s, g, sc,
                    static_cast<bf16*>(out));
   return e;
 }
