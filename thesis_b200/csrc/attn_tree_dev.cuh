@@ -15,6 +15,7 @@ struct TreeGeom {
   int* status;
   uint32_t spin;       // poll limit of the pipeline waits
   int chunk, splits;   // keys per CTA; key ranges of the longest row
+  bool sort;           // long blocks first
   float* part_o;       // [n_tokens, Hq, splits, D] normalised partial outputs
   float2* part_ml;     // [n_tokens, Hq, splits] (max in the log2 domain, sum)
 };
