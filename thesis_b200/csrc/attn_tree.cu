@@ -643,15 +643,21 @@ __global__ void __launch_bounds__(128, MmaShape<D, FMT, NT>::CTAS)
   }
 }
 
-// Joins the key ranges of a row in range order (no atomics: the same bits every time): partial outputs are
-// normalised, range c weighs L_c 2^(M_c - M).  One warp per row.
-template <int D>
+// Joins the key ranges of a row: partial outputs are normalised, range c weighs L_c 2^(M_c - M).  Ranges go round four
+// classes (eight with D = 64, two to a warp) that are summed apart and then in order, without atomics: the same bits every time
+// and with WPR = 1 or 4 warps per row.  Bound by the latency of its loads: 16 are in flight (a tree of 5
+// nodes at 32 k slots over bf16, 42 ranges: 44 us in all, with four warps per row instead of one 2 us less; with the loads
+// in one chain it was 52).
+template <int D, int WPR>
 __global__ void __launch_bounds__(128) attn_tree_join_kernel(TreeGeom g, CacheGeom c, int rows_per_tile, bf16* __restrict__ out) {
   pdl_trigger();
   pdl_wait();
+  constexpr int GR = 128 / D, U = 4, CLS = 4 / WPR;                     // ranges of a warp's load, loads of a class in flight, classes of a warp
+  __shared__ float4 part[4][33];                                        // WPR = 4: acc of the warps' lanes, and L
   BlockInfo bi;
   if (!load_block(g, c, blockIdx.z, bi)) return;
-  const int R = blockIdx.x * 4 + (threadIdx.x >> 5), kvh = blockIdx.y, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, grp = lane / (D / 4), kvh = blockIdx.y;
+  const int R = WPR == 4 ? blockIdx.x : blockIdx.x * 4 + warp, cls0 = WPR == 4 ? warp : 0;
   if (R >= bi.T * g.G) return;
   const int node = R / g.G;
   // the key count of the row tile that R was in
@@ -661,36 +667,68 @@ __global__ void __launch_bounds__(128) attn_tree_join_kernel(TreeGeom g, CacheGe
   const int n = (n_keys + g.chunk - 1) / g.chunk;
   const size_t at = (size_t)(bi.start + node) * g.n_heads + kvh * g.G + R % g.G;
   const float2* ml = g.part_ml + at * g.splits;
-  const float* po = g.part_o + at * g.splits * D;
+  const float4* po = reinterpret_cast<const float4*>(g.part_o + at * g.splits * D) + lane % (D / 4);
   float M = -INFINITY;
   for (int s = lane; s < n; s += 32) M = fmaxf(M, ml[s].x);
   M = warp_max(M);
   const float ms = M == -INFINITY ? 0.f : M;
-  float L = 0.f;
-  constexpr int E = D / 32;
-  float acc[E];
+  float L[CLS];
+  float4 acc[CLS];
 #pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  for (int s0 = 0; s0 < n; s0 += 32) {
-    float w = 0.f;
-    if (s0 + lane < n) {
-      const float2 v = ml[s0 + lane];
-      w = v.y * fast_exp2(v.x - ms);
-    }
-    const int cnt = min(32, n - s0);
-#pragma unroll 4
-    for (int s = 0; s < cnt; ++s) {
-      const float ws = __shfl_sync(0xffffffffu, w, s);
-      L += ws;
-      const float* src = po + (size_t)(s0 + s) * D + lane * E;
+  for (int k = 0; k < CLS; ++k) L[k] = 0.f, acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s0 = 0; s0 < n; s0 += 4 * GR * U) {
+    float4 v[U][CLS];
+    float2 m[U][CLS];
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = ws == 0.f ? acc[e] : fmaf(ws, src[e], acc[e]);
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int k = 0; k < CLS; ++k) {
+        const int s = min(s0 + (u * 4 + cls0 + k) * GR + grp, n - 1);
+        m[u][k] = ml[s];
+        v[u][k] = po[(size_t)s * (D / 4)];
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int k = 0; k < CLS; ++k) {
+        const float w = s0 + (u * 4 + cls0 + k) * GR + grp < n ? m[u][k].y * fast_exp2(m[u][k].x - ms) : 0.f;
+        if (w == 0.f) continue;
+        L[k] += w;
+        acc[k].x = fmaf(w, v[u][k].x, acc[k].x);
+        acc[k].y = fmaf(w, v[u][k].y, acc[k].y);
+        acc[k].z = fmaf(w, v[u][k].z, acc[k].z);
+        acc[k].w = fmaf(w, v[u][k].w, acc[k].w);
+      }
+  }
+  auto add = [](float4& a, const float4& b) { a.x += b.x, a.y += b.y, a.z += b.z, a.w += b.w; };
+  if constexpr (GR == 2) {
+#pragma unroll
+    for (int k = 0; k < CLS; ++k) {
+      L[k] += __shfl_xor_sync(0xffffffffu, L[k], 16);
+      add(acc[k], make_float4(__shfl_xor_sync(0xffffffffu, acc[k].x, 16), __shfl_xor_sync(0xffffffffu, acc[k].y, 16),
+                              __shfl_xor_sync(0xffffffffu, acc[k].z, 16), __shfl_xor_sync(0xffffffffu, acc[k].w, 16)));
     }
   }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-  bf16* dst = out + at * D + lane * E;
+  if constexpr (WPR == 4) {
+    part[warp][lane] = acc[0];
+    if (lane == 0) part[warp][32].x = L[0];
+    __syncthreads();
+    if (warp) return;
+    for (int k = 1; k < 4; ++k) {
+      add(acc[0], part[k][lane]);
+      L[0] += part[k][32].x;
+    }
+  } else {
 #pragma unroll
-  for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack2<EESD_KV_MODEL>(acc[e] * inv, acc[e + 1] * inv);
+    for (int k = 1; k < CLS; ++k) {
+      add(acc[0], acc[k]);
+      L[0] += L[k];
+    }
+  }
+  const float inv = L[0] == 0.f ? 0.f : 1.f / L[0];
+  if (grp == 0)
+    *reinterpret_cast<uint2*>(out + at * D + lane * 4) = make_uint2(pack2<EESD_KV_MODEL>(acc[0].x * inv, acc[0].y * inv),
+                                                                    pack2<EESD_KV_MODEL>(acc[0].z * inv, acc[0].w * inv));
 }
 
 // ---------------------------------------------------------------- plan and launch
@@ -712,6 +750,7 @@ int encode_cache_map(CUtensorMap* map, const void* base, const EesdKvCache* c, i
   return r == CUDA_SUCCESS ? EESD_OK : fail_arg(EESD_ERR_CUDA, "attn_tree: cache tensor map (%d)", (int)r);
 }
 
+constexpr int kWide = 8;   // from 9 key ranges on the join has four warps per row (42 ranges 46 -> 44 us; at 3 it would cost 50 -> 52)
 struct Plan {
   bool tc;              // tcgen05 kernel (attn_tree_tc.cu), else mma.sync
   int nt;               // mma.sync: 8-row tiles per CTA
@@ -876,9 +915,13 @@ int eesd_attn_tree(int dtype, const EesdKvCache* c, int layer, const EesdTree* t
       e = launch_bf16(c->format, c->head_dim, p, g, cg, km, vm, t->n_blocks, q, out, s);
     }
     if (e == cudaSuccess && p.splits > 1) {
-      const dim3 grid((t->max_nodes * g.G + 3) / 4, c->n_kv_heads, t->n_blocks);
-      e = c->head_dim == 64 ? launch_pdl(attn_tree_join_kernel<64>, grid, dim3(128), 0, s, g, cg, p.rows, static_cast<bf16*>(out))
-                            : launch_pdl(attn_tree_join_kernel<128>, grid, dim3(128), 0, s, g, cg, p.rows, static_cast<bf16*>(out));
+      // four warps per row where a row may be in many ranges
+      const bool wide = p.splits > kWide;
+      const int rows = t->max_nodes * g.G;
+      const dim3 grid(wide ? rows : (rows + 3) / 4, c->n_kv_heads, t->n_blocks);
+      auto kernel = c->head_dim == 64 ? (wide ? attn_tree_join_kernel<64, 4> : attn_tree_join_kernel<64, 1>)
+                                      : (wide ? attn_tree_join_kernel<128, 4> : attn_tree_join_kernel<128, 1>);
+      e = launch_pdl(kernel, grid, dim3(128), 0, s, g, cg, p.rows, static_cast<bf16*>(out));
     }
   }
   return e == cudaSuccess ? EESD_OK : fail_arg(EESD_ERR_CUDA, "attn_tree: launch: %s", cudaGetErrorString(e));
