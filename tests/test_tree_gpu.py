@@ -633,6 +633,32 @@ def test_attention_many_small_units(cuda_dev, fmt, n):
 
 
 @pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("n", [30, 128, 129])
+def test_attention_many_blocks(cuda_dev, fmt, n):
+    """More CTAs than SMs with few rows each: the long blocks run first, every block once, equal lengths among them; one
+    block does not fit and is skipped wherever it stands in that order."""
+    H, Hkv, D = 12, 6, 64
+    rng = np.random.default_rng(n)
+    cache = make_cache(cuda_dev, fmt, 4, Hkv, 320, D)
+    blocks = [(int(rng.integers(4)), int(rng.choice([0, 5, 5, 64, 200, 300])), int(rng.integers(1, 4))) for _ in range(n)]
+    t = tr.TreeBatch(blocks, cache)
+    q = queries(cuda_dev, t.n_tokens, H * D)
+    out = tr.tree_attention(q, cache, t)
+    t.check()
+    check_attention(out, q, cache, blocks, sees_of(blocks), H)
+    t = tr.TreeBatch(blocks, cache)
+    t.blk[n // 2, 3] = 2 ** 31 - 2                                     # T + ctx wraps
+    start, T = int(t.blk[n // 2, 0]), int(t.blk[n // 2, 1])
+    again = torch.full_like(out, 3.0)
+    tr.tree_attention(q, cache, t, again)
+    with pytest.raises(lib.EesdError):
+        t.check()
+    assert (again[start:start + T] == 3).all()
+    again[start:start + T] = out[start:start + T]
+    assert torch.equal(again, out)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
 @pytest.mark.parametrize("T", [3, 40])
 def test_attention_reports_a_wait_that_runs_out(cuda_dev, fmt, T):
     """With a poll limit of 0 every pipeline wait gives up: the status word says so and the next call is right."""

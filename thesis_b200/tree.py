@@ -236,8 +236,8 @@ def kv_read(cache: KVCache, tok_row: torch.Tensor, tok_slot: torch.Tensor, k_out
 
 def attention_workspace(tree: TreeBatch, cache: KVCache, n_heads: int, dtype: torch.dtype = torch.bfloat16,
                         split_keys: int = 0) -> torch.Tensor:
-    """A workspace for ``tree_attention`` calls of this batch (or of smaller ones).  Calls that may overlap on
-    the GPU need one each."""
+    """A workspace for ``tree_attention`` calls of this batch (another batch may need more: a call with too little is
+    refused).  Calls that may overlap on the GPU need one each."""
     n = lib.load().eesd_attn_tree_workspace_bytes(DTYPES[dtype], cache.ref, tree.ref, n_heads, split_keys)
     if n == 0:
         raise lib.EesdError(f"attention workspace: {lib.load().eesd_last_error().decode(errors='replace')}")
