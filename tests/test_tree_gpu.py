@@ -289,6 +289,26 @@ def test_append_matches_the_unquantised_append(cuda_dev):
     assert torch.equal(qkv, old) and torch.equal(a.k, b.k) and torch.equal(a.v, b.v)
 
 
+def test_append_rotates_every_bf16_as_the_unquantised_append(cuda_dev):
+    """The same with random bit patterns: subnormals, the largest values, infinities (NaN compared as NaN)."""
+    H, Hkv, D, S = 8, 2, 64, 256
+    a, b = (tr.KVCache(1, 1, Hkv, S, D, "bf16", cuda_dev) for _ in range(2))
+    t = tr.TreeBatch([(0, 0, 256)], a)
+    rng = np.random.default_rng(3)
+    bits = rng.integers(0, 1 << 16, (256, (H + 2 * Hkv) * D)).astype(np.uint16)
+    bits[64:128] &= 0x83ff                                              # at most 2^-119, half of them subnormal in products
+    bits[128:192] = bits[128:192] & 0x80ff | 0x7e80                     # at least 2^126: sums that overflow
+    qkv = torch.from_numpy(bits.view(np.int16)).to(cuda_dev).view(torch.bfloat16)
+    cos, sin = tables(cuda_dev, S, D)
+    old = qkv.clone()
+    lib.call("eesd_rope_kv_append", lib.BF16, old.data_ptr(), t.tok_pos.data_ptr(), t.tok_row.data_ptr(), t.n_tokens, H, Hkv, D,
+             cos.data_ptr(), sin.data_ptr(), b.k.data_ptr(), b.v.data_ptr(), 1, S, None, lib.stream_ptr())
+    tr.kv_append(qkv, a, t, cos, sin)
+    for x, w in ((qkv, old), (a.k, b.k), (a.v, b.v)):
+        same = (x.contiguous().view(torch.int16) == w.contiguous().view(torch.int16)) | (x.isnan() & w.isnan())
+        assert same.all(), int((~same).sum())
+
+
 @pytest.mark.parametrize("fmt", ["e4m3", "int8"])
 def test_exponent_borders(cuda_dev, fmt):
     """Largest values on both sides of every border Q 2^e, halfway values, the clamp at 2^-100."""

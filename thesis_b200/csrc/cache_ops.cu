@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(128) tree_meta_kernel(EesdTree t, int max_batc
 }
 
 // ---------------------------------------------------------------- append
-// 4 consecutive elements as floats, and back
+// 4 consecutive elements as floats
 template <typename T> __device__ __forceinline__ void load4(const T* p, float (&x)[4]);
 template <> __device__ __forceinline__ void load4<float>(const float* p, float (&x)[4]) {
   const float4 v = *reinterpret_cast<const float4*>(p);
@@ -149,15 +149,6 @@ template <> __device__ __forceinline__ void load4<bf16>(const bf16* p, float (&x
   x[0] = __uint_as_float(v.x << 16), x[1] = __uint_as_float(v.x & 0xffff0000u);
   x[2] = __uint_as_float(v.y << 16), x[3] = __uint_as_float(v.y & 0xffff0000u);
 }
-template <typename T> __device__ __forceinline__ void store4(T* p, const float (&x)[4]);
-template <> __device__ __forceinline__ void store4<float>(float* p, const float (&x)[4]) {
-  *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
-}
-template <> __device__ __forceinline__ void store4<bf16>(bf16* p, const float (&x)[4]) {
-  __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
-  *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
-}
-
 // 8 elements, written once and read by others: past the caches
 template <typename T> __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
   if constexpr (sizeof(T) == 4) {
@@ -174,12 +165,74 @@ template <typename T> __device__ __forceinline__ void store8(T* p, const float (
   }
 }
 
+// Four consecutive elements of each half of a head, that is four rotation pairs, and the tables' entries for them.  The
+// roundings are those of the reference's apply_rope in the model dtype: every product and every sum rounded, no contraction.
+template <typename T> struct Rope;
+template <> struct Rope<float> {
+  using Quad = float4;
+  float4 c1, c2, s1, s2;
+  __device__ void load(const float* cosb, const float* sinb, int half) {
+    c1 = *reinterpret_cast<const float4*>(cosb), c2 = *reinterpret_cast<const float4*>(cosb + half);
+    s1 = *reinterpret_cast<const float4*>(sinb), s2 = *reinterpret_cast<const float4*>(sinb + half);
+  }
+  static __device__ void turn(float& x, float& y, float c1, float c2, float s1, float s2) {
+    const float a = __fadd_rn(__fmul_rn(x, c1), __fmul_rn(-y, s1)), b = __fadd_rn(__fmul_rn(y, c2), __fmul_rn(x, s2));
+    x = a, y = b;
+  }
+  __device__ void rotate(float4& x, float4& y) const {
+    turn(x.x, y.x, c1.x, c2.x, s1.x, s2.x);
+    turn(x.y, y.y, c1.y, c2.y, s1.y, s2.y);
+    turn(x.z, y.z, c1.z, c2.z, s1.z, s2.z);
+    turn(x.w, y.w, c1.w, c2.w, s1.w, s2.w);
+  }
+  static __device__ uint32_t amax(const float4& x, const float4& y) {   // bits of the largest |element| as fp32
+    auto m = [](const float4& v) {
+      return max(max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu),
+                 max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu));
+    };
+    return max(m(x), m(y));
+  }
+  static __device__ float4 floats(const float4& x) { return x; }
+};
+// bf16: two elements an instruction.  A product of two bf16 is exact in fp32, and so is a sum of two as far as bf16 can
+// tell, so rounding once to bf16 is what rounding the fp32 result is.
+template <> struct Rope<bf16> {
+  using Quad = uint2;
+  uint2 c1, c2, s1, s2;
+  static __device__ uint2 rounded(const float* p) {
+    const float4 v = *reinterpret_cast<const float4*>(p);
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+    return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+  }
+  __device__ void load(const float* cosb, const float* sinb, int half) {
+    c1 = rounded(cosb), c2 = rounded(cosb + half), s1 = rounded(sinb), s2 = rounded(sinb + half);
+  }
+  static __device__ void turn(uint32_t& x, uint32_t& y, uint32_t c1, uint32_t c2, uint32_t s1, uint32_t s2) {
+    auto v = [](const uint32_t& u) { return *reinterpret_cast<const __nv_bfloat162*>(&u); };
+    const __nv_bfloat162 a = __hsub2_rn(__hmul2_rn(v(x), v(c1)), __hmul2_rn(v(y), v(s1)));
+    const __nv_bfloat162 b = __hadd2_rn(__hmul2_rn(v(y), v(c2)), __hmul2_rn(v(x), v(s2)));
+    x = *reinterpret_cast<const uint32_t*>(&a), y = *reinterpret_cast<const uint32_t*>(&b);
+  }
+  __device__ void rotate(uint2& x, uint2& y) const {
+    turn(x.x, y.x, c1.x, c2.x, s1.x, s2.x);
+    turn(x.y, y.y, c1.y, c2.y, s1.y, s2.y);
+  }
+  static __device__ uint32_t amax(const uint2& x, const uint2& y) {
+    const uint32_t m = __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), __vmaxu2(y.x & 0x7fff7fffu, y.y & 0x7fff7fffu));
+    return max(m << 16, m & 0xffff0000u);
+  }
+  static __device__ float4 floats(const uint2& x) {
+    return make_float4(__uint_as_float(x.x << 16), __uint_as_float(x.x & 0xffff0000u), __uint_as_float(x.y << 16),
+                       __uint_as_float(x.y & 0xffff0000u));
+  }
+};
+
 // A group of D / 8 lanes owns one head of one token: lane l holds elements 4 l .. 4 l + 3 of both halves,
 // that is four rotation pairs, so the rotation needs no exchange and the largest |x| of the vector is a
 // shuffle over the group.  Bound by the bytes of qkv, q_out and the cache, at few tokens by the chain of loads: a thread's
 // kBatch heads are asked for before the token's position, on which the tables and the slot hang, is there.  Metadata, append
 // and read-back of 320 tokens (32 query and 8 KV heads of 128, e4m3) take 6.4 us of device time (9.6 with one head after the other),
-// of 2048 tokens over int8 19 us, 3.1 TB/s.
+// of 2048 tokens over int8 15.5 us, 3.8 TB/s (19 with the rotation of bf16 in fp32).
 template <typename T, int FMT, int D>
 __global__ void __launch_bounds__(256) kv_append_kernel(const T* qkv, int ld_qkv, T* q_out, int ld_qo,
                                                         int n_heads, const int32_t* __restrict__ tok_pos,
@@ -193,14 +246,15 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const T* qkv, int ld_qkv
   const int t = blockIdx.x, l = threadIdx.x % L, first = threadIdx.x / L;
   const T* base = qkv + (size_t)t * ld_qkv + 4 * l;
   const int heads = n_heads + 2 * c.n_kv_heads;
-  float x[kBatch][2][4];
+  using R = Rope<T>;
+  typename R::Quad x[kBatch][2];
   // every lane of a warp takes part in the shuffles: head numbers past the end repeat the last head, unstored
   auto load = [&](int h0) {
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       const int h = min(h0 + b * GROUPS, heads - 1);
-      load4<T>(base + (size_t)h * D, x[b][0]);
-      load4<T>(base + (size_t)h * D + H2, x[b][1]);
+      x[b][0] = *reinterpret_cast<const typename R::Quad*>(base + (size_t)h * D);
+      x[b][1] = *reinterpret_cast<const typename R::Quad*>(base + (size_t)h * D + H2);
     }
   };
   load(first);
@@ -209,41 +263,21 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const T* qkv, int ld_qkv
     if (threadIdx.x == 0) set_status(status, kStatusBadIndex);
     return;
   }
-  float c1[4], c2[4], s1[4], s2[4];
-  load4<float>(cosb + (size_t)pos * D + 4 * l, c1);
-  load4<float>(cosb + (size_t)pos * D + H2 + 4 * l, c2);
-  load4<float>(sinb + (size_t)pos * D + 4 * l, s1);
-  load4<float>(sinb + (size_t)pos * D + H2 + 4 * l, s2);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    c1[i] = rnd<T>(c1[i]);
-    c2[i] = rnd<T>(c2[i]);
-    s1[i] = rnd<T>(s1[i]);
-    s2[i] = rnd<T>(s2[i]);
-  }
+  R rope;
+  rope.load(cosb + (size_t)pos * D + 4 * l, sinb + (size_t)pos * D + 4 * l, H2);
   for (int h0 = first;; load(h0)) {
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       const int hh = h0 + b * GROUPS;
       const bool in = hh < heads;
       const int h = in ? hh : heads - 1;
-      float(&x1)[4] = x[b][0];
-      float(&x2)[4] = x[b][1];
-      if (h < n_heads + c.n_kv_heads) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          // the roundings of the reference's apply_rope in the model dtype, no contraction to FMA
-          const float a = __fadd_rn(rnd<T>(__fmul_rn(x1[i], c1[i])), rnd<T>(__fmul_rn(-x2[i], s1[i])));
-          const float b = __fadd_rn(rnd<T>(__fmul_rn(x2[i], c2[i])), rnd<T>(__fmul_rn(x1[i], s2[i])));
-          x1[i] = rnd<T>(a);
-          x2[i] = rnd<T>(b);
-        }
-      }
+      typename R::Quad &x1 = x[b][0], &x2 = x[b][1];
+      if (h < n_heads + c.n_kv_heads) rope.rotate(x1, x2);
       if (h < n_heads) {
         if (in) {
           T* q = q_out + (size_t)t * ld_qo + (size_t)h * D + 4 * l;
-          store4<T>(q, x1);
-          store4<T>(q + H2, x2);
+          *reinterpret_cast<typename R::Quad*>(q) = x1;
+          *reinterpret_cast<typename R::Quad*>(q + H2) = x2;
         }
         if constexpr (FMT == EESD_KV_MODEL) continue;
       }
@@ -252,13 +286,11 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const T* qkv, int ld_qkv
       if constexpr (FMT == EESD_KV_MODEL) {
         if (in) {
           T* d = static_cast<T*>(const_cast<void*>(isk ? c.k : c.v)) + at * D + 4 * l;
-          store4<T>(d, x1);
-          store4<T>(d + H2, x2);
+          *reinterpret_cast<typename R::Quad*>(d) = x1;
+          *reinterpret_cast<typename R::Quad*>(d + H2) = x2;
         }
       } else {
-        uint32_t amax = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) amax = max(amax, max(__float_as_uint(x1[i]) & 0x7fffffffu, __float_as_uint(x2[i]) & 0x7fffffffu));
+        uint32_t amax = R::amax(x1, x2);
 #pragma unroll
         for (int o = L / 2; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
         if (!in || h < n_heads) continue;
@@ -266,8 +298,9 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const T* qkv, int ld_qkv
         const float inv = exp_inv_scale(eb);
         uint32_t w1 = 0, w2 = 0;
         if (eb != 255) {
-          w1 = quant2<FMT>(x1[0] * inv, x1[1] * inv) | quant2<FMT>(x1[2] * inv, x1[3] * inv) << 16;
-          w2 = quant2<FMT>(x2[0] * inv, x2[1] * inv) | quant2<FMT>(x2[2] * inv, x2[3] * inv) << 16;
+          const float4 y1 = R::floats(x1), y2 = R::floats(x2);
+          w1 = quant2<FMT>(y1.x * inv, y1.y * inv) | quant2<FMT>(y1.z * inv, y1.w * inv) << 16;
+          w2 = quant2<FMT>(y2.x * inv, y2.y * inv) | quant2<FMT>(y2.z * inv, y2.w * inv) << 16;
         }
         uint8_t* d = static_cast<uint8_t*>(const_cast<void*>(isk ? c.k : c.v)) + at * D + 4 * l;
         *reinterpret_cast<uint32_t*>(d) = w1;
