@@ -195,19 +195,28 @@ template <int D, int FMT, int NT> struct MmaShape {
 // short ones fill the SMs that are done: 64 single tokens at 129 to 1023 slots over int8 25 us instead of 28, 5-node trees
 // over bf16 36 instead of 41.  It costs up to 2 us, so only grids that leave SMs two CTAs and more do it; beyond kSorted
 // blocks the order given evens out by itself.
-constexpr int kSorted = 128;
+constexpr int kSorted = 128;                                             // a CTA's threads
 __device__ __forceinline__ int longest_first(const TreeGeom& g) {
-  __shared__ int len[kSorted], pick;
+  __shared__ alignas(16) unsigned long long key[kSorted];
+  __shared__ int pick;
   const int n = gridDim.z, t = threadIdx.x;                             // one thread per block of the batch
   if (!g.sort) return blockIdx.z;
-  int mine = 0, rank = 0;
+  unsigned long long mine = 0;                                          // T + ctx, and the earlier block first among equals
   if (t < n) {
     const int4 v = *reinterpret_cast<const int4*>(g.blk + 4 * t);
-    len[t] = mine = (int)((unsigned)v.y + (unsigned)v.w);               // T + ctx
+    mine = (unsigned long long)((unsigned)v.y + (unsigned)v.w) << 8 | (unsigned)(255 - t);
   }
+  key[t] = mine;
   __syncthreads();
-  for (int j = 0; j < n; ++j) rank += len[j] > mine || (len[j] == mine && j < t);
-  if (t < n && rank == (int)blockIdx.z) pick = t;
+  if (t < n) {
+    int rank = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; j += 2) {
+      const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(key + j);
+      rank += (v.x > mine) + (v.y > mine);
+    }
+    if (rank == (int)blockIdx.z) pick = t;
+  }
   __syncthreads();
   return pick;
 }
