@@ -900,6 +900,38 @@ def test_wrapped_tensors_are_the_cache(cuda_dev, fmt):
     assert k[1, 1, :, :30].abs().sum() > 0 and (k[0] == 0).all()
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("T", [5, 40])
+def test_cache_beyond_32_bit_offsets(cuda_dev, fmt, T):
+    """The last row of a layer with more than 2^31 elements: the bits of the same round in a small cache."""
+    H, Hkv, D, S, ctx = 4, 1, 128, 256, 200
+    cos, sin = tables(cuda_dev, S, D)
+    rng = np.random.default_rng(T)
+    p = random_tree(T, rng)
+    results = []
+    for B in (2, 70000):
+        cache = tr.KVCache(1, B, Hkv, S, D, fmt, cuda_dev)
+        assert B == 2 or cache.k.numel() > 2 ** 31
+        first = tr.TreeBatch([(B - 1, 0, ctx)], cache)
+        tr.kv_append(queries(cuda_dev, ctx, (H + 2 * Hkv) * D, seed=1), cache, first, cos, sin)
+        t = tr.TreeBatch([(B - 1, ctx, p)], cache)
+        qkv = queries(cuda_dev, T, (H + 2 * Hkv) * D, seed=2)
+        tr.kv_append(qkv, cache, t, cos, sin)
+        out = tr.tree_attention(qkv[:, :H * D], cache, t)
+        path = torch.tensor([[0, 2, 4] + [-1] * (T - 3)], dtype=torch.int32, device=cuda_dev)
+        tr.kv_compact(cache, t, path, torch.tensor([2], dtype=torch.int32, device=cuda_dev))
+        rows = torch.full((ctx + 3,), B - 1, dtype=torch.int32, device=cuda_dev)
+        slots = torch.arange(ctx + 3, dtype=torch.int32, device=cuda_dev)
+        k, v = (torch.zeros(ctx + 3, Hkv, D, dtype=torch.bfloat16, device=cuda_dev) for _ in range(2))
+        tr.kv_read(cache, rows, slots, k, v)
+        first.check()
+        t.check()
+        results.append((out, k, v))
+        del cache, first, t
+        torch.cuda.empty_cache()
+    assert all(torch.equal(a, b) for a, b in zip(*results)) and results[0][1][-1].abs().sum() > 0
+
+
 def test_round_is_capturable(cuda_dev):
     """A whole round as one graph, replayed with other contents: the eager results."""
     L, B, H, Hkv, D, S = 2, 2, 4, 2, 64, 192
