@@ -273,7 +273,7 @@ int eesd_head_argmax_static(const void* x, int x_rows, const int32_t* rows, int 
  * that positions ctx .. ctx + n_acc of every row hold the path; rollback stays a length reset). */
 
 #define EESD_KV_MODEL 0        /* elements of the model dtype (EESD_BF16 or EESD_F32) */
-#define EESD_KV_E4M3 1         /* 8-bit floats (4 exponent, 3 mantissa bits, no infinities), max 448 */
+#define EESD_KV_E4M3 1         /* 8-bit floats (4 exponent, 3 mantissa bits), max 448; the NaN pattern is never stored */
 #define EESD_KV_INT8 2         /* 8-bit integers -127 .. 127 */
 
 /* 8-bit formats: K and V each have one power-of-two scale 2^e per (row, KV head, slot), stored as the

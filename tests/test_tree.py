@@ -88,6 +88,13 @@ def test_other_refusals(L):
     assert L.eesd_tree_meta(C.byref(tree(tok_slot=None)), 4, 512, None, None) == lib.ERR_ARG
 
 
+@pytest.mark.parametrize("n_blocks,max_nodes", [(2, 1 << 30), (2, (1 << 23) + 1), (65535, 1 << 21)])
+def test_row_counts_past_32_bits_are_refused(L, n_blocks, max_nodes):
+    t = tree(n_blocks=n_blocks, max_nodes=max_nodes, words=0, mask=None, parent=None)
+    assert attn(L, t=t) == lib.ERR_ARG and b"rows" in L.eesd_last_error()
+    assert L.eesd_attn_tree_workspace_bytes(lib.BF16, C.byref(cache()), C.byref(t), 4, 0) == 0
+
+
 def test_empty_calls_do_nothing(L):
     c, none = C.byref(cache()), tree(n_tokens=0, n_blocks=0, blk=None)
     assert attn(L, t=none, q=None, out=None) == lib.OK

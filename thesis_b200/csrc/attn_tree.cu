@@ -876,6 +876,10 @@ int check_attn(int dtype, const EesdKvCache* c, int layer, const EesdTree* t, in
   if (rc) return rc;
   if (n_heads <= 0 || n_heads % c->n_kv_heads) return fail_arg(EESD_ERR_ARG, "attn_tree: heads %d / %d", n_heads, c->n_kv_heads);
   if (split_keys < 0 || split_keys % 256) return fail_arg(EESD_ERR_ARG, "attn_tree: split_keys %d (0 or a multiple of 256)", split_keys);
+  const long long rows = (long long)t->max_nodes * (n_heads / c->n_kv_heads);   // the grids and the schedule count them in 32 bits
+  if (rows > 1 << 24 || rows * t->n_blocks >= 1LL << 37)
+    return fail_arg(EESD_ERR_ARG, "attn_tree: %d blocks of max_nodes %d x %d heads are too many rows", t->n_blocks, t->max_nodes,
+                    n_heads / c->n_kv_heads);
   if (t->n_tokens && t->n_blocks && t->max_ctx > c->max_seq)
     return fail_arg(EESD_ERR_ARG, "attn_tree: max_ctx %d > max_seq %d", t->max_ctx, c->max_seq);
   return EESD_OK;
