@@ -806,7 +806,9 @@ Plan plan_for(const EesdKvCache* c, const EesdTree* t, int n_heads, int split_ke
     const int slots = sm_count() * (p.nt == 4 || (p.nt == 3 && c->head_dim == 128 && c->format != EESD_KV_MODEL) ? 2 : 3);
     const int want = (int)std::max(1LL, slots / std::max(1LL, units));
     const int per = (t->max_ctx + want - 1) / want;
-    p.chunk = (per + 255) / 256 * 256;
+    // up to 512 slots the join costs more than a second range saves (one token at 300 slots 8.3 us whole, 10.5 in two; 8 at
+    // 500: 14 and 17); at 1000 it no longer does (in two 17, in four 15)
+    p.chunk = t->max_ctx <= 512 ? 512 : (per + 255) / 256 * 256;
   }
   p.splits = p.chunk ? (t->max_ctx + p.chunk - 1) / p.chunk : 1;
   if (p.splits > 1) parts = (size_t)t->n_tokens * n_heads * p.splits;
