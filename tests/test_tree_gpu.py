@@ -986,3 +986,24 @@ def test_round_is_capturable(cuda_dev):
         for a, b in zip(result(), want):
             assert torch.equal(a, b)
     t.check()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_one_row_tile_at_every_ring_position(cuda_dev, fmt, D):
+    """33 to 128 query rows per KV head: two streams share the key tiles, at every number of tiles from 1 to 11 and one after
+    another, so that a stage is reused at every distance and by either stream."""
+    H, Hkv = 12, 1
+    rng = np.random.default_rng(D)
+    cache = make_cache(cuda_dev, fmt, 3, Hkv, 768, D, seed=D)
+    for n in (4, 33):
+        blocks = [(int(rng.integers(3)), 64 * int(rng.integers(11)) + int(rng.integers(50)), random_tree(int(rng.integers(3, 11)), rng))
+                  for _ in range(n)]
+        t = tr.TreeBatch(blocks, cache)
+        q = queries(cuda_dev, t.n_tokens, H * D, seed=n)
+        out = tr.tree_attention(q, cache, t)
+        t.check()
+        check_attention(out, q, cache, blocks, sees_of(blocks), H)
+        fixed = tr.tree_attention(q, cache, t, split_keys=256)
+        t.check()
+        check_attention(fixed, q, cache, blocks, sees_of(blocks), H)

@@ -261,7 +261,10 @@ template <int D, int FMT> struct TcShape {
   static constexpr bool Q8 = FMT != EESD_KV_MODEL;
   static constexpr int TILE = KT * D * 2;              // bytes of one 16-bit K (or V) tile
   static constexpr int RAW = KT * D * 2;               // 8-bit: K and V bytes of one tile
-  static constexpr int NS = Q8 ? 2 : 5;                // 16-bit K / V stages
+  // 16-bit K / V stages.  Even: with one row tile each stream waits for every other tile only, and a stage that both used in turn
+  // would have it wait for a phase whose predecessor, the other stream's tile, may not have landed: a parity wait then returns at once.
+  static constexpr int NS = Q8 ? 2 : 4;
+  static_assert(NS % 2 == 0, "a stage belongs to one stream");
   static constexpr int RS = Q8 ? 6 : 0;                // raw stages
   static constexpr int FR = 8;                         // factor ring: six tiles can be between conversion and softmax
   static constexpr int QB = 128 * D * 2 + 128 * 128;   // Q of stream 1 (more than 128 rows), half rows on their way to TMEM
@@ -271,7 +274,7 @@ template <int D, int FMT> struct TcShape {
 constexpr int kPieces = 4;                 // pieces between the schedule warp and the slowest role
 constexpr int kReaders = 19;               // warps that read them: TMA, 2 MMA, 8 softmax, 8 conversion
 struct TcControl {
-  uint64_t kfull[5], kempty[5], vfull[5], vempty[5], vclean[5], raw_full[6], raw_empty[6];
+  uint64_t kfull[4], kempty[4], vfull[4], vempty[4], vclean[4], raw_full[6], raw_empty[6];
   uint64_t piece_full[kPieces], piece_empty[kPieces];
   Piece piece[kPieces];                    // tiles == 0: there are no more
   uint64_t s_full[2], s_free[2], p_ready[2], pv_done[2], q_ready, o_done, ml_ready, epi_done, drain[2];
