@@ -140,3 +140,13 @@ def fault(pieces, NS, q8, weights_first, ml_issuer):
 @pytest.mark.parametrize("pieces", [[(6, False)], [(3, False), (2, False)], [(1, False), (3, False)], [(2, True), (3, False)]], ids=str)
 def test_k_stages_hold_the_tile_that_a_product_reads(pieces):
     assert fault(pieces, stages(False), False, True, 1) is None
+
+
+def first_weights_before_v():
+    return re.search(r"if \(i == t0 && !\(ok = mbar_wait\(smem_u32\(&ct\.p_ready", SOURCE) is not None
+
+
+# The two stages of the 8-bit tiles change hands between pieces: after an odd one a stream's first V stage was the other's.
+@pytest.mark.parametrize("pieces", [[(3, False), (3, False)], [(1, False), (2, False), (2, False)], [(3, False), (2, True)]], ids=str)
+def test_first_v_of_a_piece_is_waited_for_in_its_own_phase(pieces):
+    assert fault(pieces, stages(True), True, first_weights_before_v(), 1) is None

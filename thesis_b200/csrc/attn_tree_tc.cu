@@ -509,8 +509,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (i >= 0) {
             const int cnt = cnt0 + i, st = cnt % NS;
+            // The weights of a piece's first tile come after the last piece's output, so every earlier V has landed then.  Without
+            // that a wait for V may be about the other stream's tile that the stage held before, and return at once; later
+            // tiles' stages were this stream's own, and their V is asked for first, while the softmax works.
+            if (i == t0 && !(ok = mbar_wait(smem_u32(&ct.p_ready[x]), n_p & 1, abort_flag, g.spin))) break;
             if (!(ok = mbar_wait(smem_u32(Q8 ? &ct.vfull[st] : &ct.vclean[st]), cnt / NS & 1, abort_flag, g.spin))) break;
-            if (!(ok = mbar_wait(smem_u32(&ct.p_ready[x]), n_p++ & 1, abort_flag, g.spin))) break;
+            if (i != t0 && !(ok = mbar_wait(smem_u32(&ct.p_ready[x]), n_p & 1, abort_flag, g.spin))) break;
+            ++n_p;
             tc_fence_after();
             const uint64_t vd = sw128_mnmajor_desc(vbuf + st * S::TILE, KT * 128);
 #pragma unroll
