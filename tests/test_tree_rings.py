@@ -150,3 +150,14 @@ def first_weights_before_v():
 @pytest.mark.parametrize("pieces", [[(3, False), (3, False)], [(1, False), (2, False), (2, False)], [(3, False), (2, True)]], ids=str)
 def test_first_v_of_a_piece_is_waited_for_in_its_own_phase(pieces):
     assert fault(pieces, stages(True), True, first_weights_before_v(), 1) is None
+
+
+def issuer_arrivals_on_ml():
+    """How many arrivals beside the eight softmax warps' complete ml_ready."""
+    return int(re.search(r"mbar_init\(smem_u32\(&ct\.ml_ready\), (\d+)\)", SOURCE).group(1)) - 8
+
+
+# A piece of one key tile leaves stream 1 without a product: its issuing thread must not fall a phase of q_ready behind.
+@pytest.mark.parametrize("pieces", [[(1, False)] * 3, [(1, False), (1, True), (1, False)], [(2, False), (1, False), (1, False)]], ids=str)
+def test_pieces_of_one_tile_do_not_run_ahead_of_stream_1(pieces):
+    assert fault(pieces, stages(True), True, first_weights_before_v(), issuer_arrivals_on_ml()) is None

@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(smem_u32(&ct.piece_empty[i]), kReaders);
       }
       mbar_init(smem_u32(&ct.q_ready), 8);
-      mbar_init(smem_u32(&ct.ml_ready), 8);
+      mbar_init(smem_u32(&ct.ml_ready), 9);                            // the softmax warps, and stream 1's issuing thread
       mbar_init(smem_u32(&ct.epi_done), 8);
       mbar_init(smem_u32(&ct.o_done), 2);
       mbar_init(smem_u32(&ct.drain[0]), 1);
@@ -482,6 +482,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!two) tc_commit(smem_u32(bar));
         };
         if (!(ok = mbar_wait(smem_u32(&ct.q_ready), piece & 1, abort_flag, g.spin))) break;
+        // With one key tile stream 1 has no product that the softmax would wait for: it says that it has seen this Q, or the next
+        // one's phase could end before it looks, and it would wait for good.
+        if (!two && x == 1) mbar_arrive(smem_u32(&ct.ml_ready));
         // S of the stream's next tile as soon as the last one is in registers, then O of the last one when its softmax ends
 #pragma unroll 1
         for (int i = t0 - step; i < nt; i += step) {
