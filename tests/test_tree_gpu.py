@@ -1007,3 +1007,37 @@ def test_attention_one_row_tile_at_every_ring_position(cuda_dev, fmt, D):
         fixed = tr.tree_attention(q, cache, t, split_keys=256)
         t.check()
         check_attention(fixed, q, cache, blocks, sees_of(blocks), H)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("T", [3, 20, 60])
+def test_attention_waits_that_run_out_part_of_the_way(cuda_dev, fmt, T):
+    """Poll limits at which some roles give up while others have loads in flight: a call either reports it or is right, and
+    what runs on the same SMs right behind it is right."""
+    cache = make_cache(cuda_dev, fmt, 2, 2, 4224, 128)
+    rng = np.random.default_rng(T)
+    t = tr.TreeBatch([(0, 4100, random_tree(T, rng)), (1, 64, random_tree(2, rng))], cache)
+    q = queries(cuda_dev, t.n_tokens, 8 * 128)
+    ws, ws2 = (tr.attention_workspace(t, cache, 8) for _ in range(2))
+    good = tr.tree_attention(q, cache, t, workspace=ws)
+    t.check()
+    outs = [torch.empty_like(good) for _ in range(2)]
+    reported = 0
+    try:
+        for limit in (0, 1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 64, 128):
+            for _ in range(3):
+                lib.call("eesd_set_option", lib.OPT_SPIN_LIMIT, limit)
+                tr.tree_attention(q, cache, t, outs[0], workspace=ws)
+                lib.call("eesd_set_option", lib.OPT_SPIN_LIMIT, -1)
+                tr.tree_attention(q, cache, t, outs[1], workspace=ws2)
+                torch.cuda.synchronize()
+                assert torch.equal(outs[1], good), limit
+                try:
+                    t.check()
+                except lib.EesdError:
+                    reported += 1
+                else:
+                    assert torch.equal(outs[0], good), limit
+    finally:
+        lib.call("eesd_set_option", lib.OPT_SPIN_LIMIT, -1)
+    assert reported > 0
