@@ -1041,3 +1041,40 @@ def test_attention_waits_that_run_out_part_of_the_way(cuda_dev, fmt, T):
     finally:
         lib.call("eesd_set_option", lib.OPT_SPIN_LIMIT, -1)
     assert reported > 0
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("ctx,p,H", [(9, 1, 8), (300, 1, 8), (63, 1, 8), (100, [-1, 0, 0, 1, 3], 8), (77, 20, 8), (100, "tree40", 8), (1000, 3, 8),
+                                     (300, 1, 80), (64, 33, 80), (4400, 2, 8), (4400, 40, 8)], ids=str)
+def test_attention_nonfinite_values_of_seen_slots(cuda_dev, D, ctx, p, H):
+    """bf16 cache, K finite: NaN or an infinity in one element of V, in committed slots on both sides of every tile and
+    group border and in the nodes' own: all nodes that see the slot get it, in that element alone; the others nothing."""
+    Hkv = 2
+    p = random_tree(40, np.random.default_rng(1)) if p == "tree40" else p
+    T = p if isinstance(p, int) else len(p)
+    see = sees_of([(0, ctx, p)])[0]
+    cache = make_cache(cuda_dev, "bf16", 1, Hkv, 4480, D, seed=T)
+    t = tr.TreeBatch([(0, ctx, p)], cache)
+    q = queries(cuda_dev, T, H * D) * 0.25                              # no weight of a seen slot vanishes
+    clean = {split: tr.tree_attention(q, cache, t, split_keys=split).view(T, H, D) for split in (0, 256)}
+    slots = sorted({0, ctx - 1, ctx, ctx + T - 1, ctx // 16 * 16, ctx // 32 * 32, ctx // 64 * 64, max(0, ctx // 64 * 64 - 1)})
+    for n, slot in enumerate(slots):
+        value = (math.nan, math.inf, -math.inf)[n % 3]
+        keep = cache.v[0, 0, :, slot, 5].clone()
+        cache.v[0, 0, :, slot, 5] = value
+        for split, want in clean.items():
+            out = tr.tree_attention(q, cache, t, split_keys=split).view(T, H, D)
+            t.check()
+            for i in range(T):
+                sees = slot < ctx or bool(see[i, slot - ctx])
+                rest = torch.ones(D, dtype=torch.bool, device=cuda_dev)
+                rest[5] = False
+                assert torch.equal(out[i][:, rest], want[i][:, rest])
+                got = out[i][:, 5]
+                if not sees:
+                    assert torch.equal(got, want[i][:, 5]), (slot, i)
+                elif math.isnan(value):
+                    assert got.isnan().all(), (slot, i)
+                else:
+                    assert (got == value).all(), (slot, i, got)
+        cache.v[0, 0, :, slot, 5] = keep

@@ -637,7 +637,7 @@ __global__ void __launch_bounds__(128, MmaShape<D, FMT, NT>::CTAS)
     if (!Q8 && flags[1]) {                                              // the dropped elements of keys this row sees
       const uint64_t* mk = g.mask ? masks + r * 4 : nullptr;
 #pragma unroll 1
-      for (int key = max(k_lo, min(all_see, k_hi)); key < k_hi; ++key)
+      for (int key = max(k_lo, min(all_see, k_hi) / KG * KG); key < k_hi; ++key)   // from the first partial group on
         if (sees32(mk, 4, node, key - bi.ctx) & 1) {
           const bf16* v = static_cast<const bf16*>(c.v) + ((size_t)slot0 + key) * D + d;
 #pragma unroll

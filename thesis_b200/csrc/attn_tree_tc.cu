@@ -850,10 +850,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int j = 0; j < 16; ++j) z[j] = fmaf(__uint_as_float(o1[j]), f1 * inv, z[j]);
           }
-          if (!Q8 && cw.in && *reinterpret_cast<volatile int*>(&ct.dropped)) {   // the dropped elements of keys this row sees
+          if (!Q8 && cw.in && *reinterpret_cast<volatile int*>(&ct.dropped)) {   // the dropped elements of keys this row sees,
             const uint64_t* mk = g.mask ? g.mask + (size_t)(cur.bi.start + cw.node) * g.words : nullptr;
 #pragma unroll 1
-            for (int key = max(cur.t0 * KT, cur.all_see); key < min(cur.t1 * KT, cur.n_keys); ++key)
+            for (int key = max(cur.t0 * KT, min(cur.all_see, cur.n_keys) / KT * KT); key < min(cur.t1 * KT, cur.n_keys); ++key)   // in partial tiles
               if (sees32(mk, g.words, cw.node, key - cur.bi.ctx) & 1) {
                 const bf16* vp = static_cast<const bf16*>(c.v) + (cache_slot(c, cur.bi.row, cur.h, key)) * D + d;
 #pragma unroll
