@@ -1078,3 +1078,26 @@ def test_attention_nonfinite_values_of_seen_slots(cuda_dev, D, ctx, p, H):
                 else:
                     assert (got == value).all(), (slot, i, got)
         cache.v[0, 0, :, slot, 5] = keep
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("T", [1, 40])
+def test_attention_nan_in_a_range_of_vanishing_weight(cuda_dev, fmt, T):
+    """A NaN of V in a slot whose weight is far below fp32, in another key range than the largest score: it is seen all the
+    same (0 x NaN), whichever way the keys are split."""
+    H, Hkv, D, ctx = 4, 1, 64, 1000
+    cache = make_cache(cuda_dev, fmt, 1, Hkv, 1088, D)
+    t = tr.TreeBatch([(0, ctx, T)], cache)
+    q = queries(cuda_dev, T, H * D)
+    q[:] = 1.0
+    cache.k[0, 0, :, :ctx] = torch.zeros(1, device=cuda_dev).to(cache.k.dtype)
+    cache.k[0, 0, :, 900] = torch.full((1,), 64.0, device=cuda_dev).to(cache.k.dtype)   # the score of 900: 512 2^e, all others' 0 or small
+    if cache.quantised:
+        cache.k_exp[0, 0, :, 900] = 127
+        cache.v_exp[0, 0, :, 10] = 255
+    else:
+        cache.v[0, 0, :, 10] = math.nan
+    for split in (0, 256, 512):
+        out = tr.tree_attention(q, cache, t, split_keys=split)
+        t.check()
+        assert out.isnan().all(), split

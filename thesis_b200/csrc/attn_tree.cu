@@ -706,8 +706,9 @@ __global__ void __launch_bounds__(128) attn_tree_join_kernel(TreeGeom g, CacheGe
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int k = 0; k < CLS; ++k) {
-        const float w = s0 + (u * 4 + cls0 + k) * GR + grp < n ? m[u][k].y * fast_exp2(m[u][k].x - ms) : 0.f;
-        if (w == 0.f) continue;
+        // a range that the row sees counts even where its weight vanishes: 0 x NaN is a NaN, as within a range
+        if (s0 + (u * 4 + cls0 + k) * GR + grp >= n || m[u][k].y == 0.f) continue;
+        const float w = m[u][k].y * fast_exp2(m[u][k].x - ms);
         L[k] += w;
         acc[k].x = fmaf(w, v[u][k].x, acc[k].x);
         acc[k].y = fmaf(w, v[u][k].y, acc[k].y);
