@@ -1101,3 +1101,33 @@ def test_attention_nan_in_a_range_of_vanishing_weight(cuda_dev, fmt, T):
         out = tr.tree_attention(q, cache, t, split_keys=split)
         t.check()
         assert out.isnan().all(), split
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("T,H,Hkv,D", [(6, 8, 2, 64), (6, 8, 2, 128), (3, 2, 2, 128), (16, 4, 2, 64), (40, 8, 2, 128), (100, 4, 2, 64)])
+def test_attention_large_keys_and_values_that_others_see(cuda_dev, fmt, T, H, Hkv, D):
+    """Finite keys with scores far above the rest, and values of a far larger scale, in a slot that only some nodes see: not
+    a bit of the others' rows changes."""
+    ctx = 75
+    rng = np.random.default_rng(T)
+    p = random_tree(T, rng)
+    see = ancestors(p)
+    cache = make_cache(cuda_dev, fmt, 1, Hkv, 256, D, seed=T)
+    t = tr.TreeBatch([(0, ctx, p)], cache)
+    q = queries(cuda_dev, T, H * D)
+    clean = tr.tree_attention(q, cache, t)
+    for node in sorted({1, T // 2, T - 1}):
+        blind = torch.from_numpy(~see[:, node])
+        for part in ("k", "v"):
+            x, e = getattr(cache, part), getattr(cache, part + "_exp")
+            keep = (x if e is None else e)[0, 0, :, ctx + node].clone()
+            for up in (3, 6, 40):
+                if e is None:
+                    x[0, 0, :, ctx + node] = keep * 2.0 ** up
+                else:
+                    e[0, 0, :, ctx + node] = keep + up
+                out = tr.tree_attention(q, cache, t)
+                t.check()
+                assert torch.equal(out[blind], clean[blind]), (node, part, up)
+                assert part == "k" and up == 3 or not torch.equal(out[~blind], clean[~blind])
+            (x if e is None else e)[0, 0, :, ctx + node] = keep

@@ -476,12 +476,14 @@ __global__ void __launch_bounds__(128, MmaShape<D, FMT, NT>::CTAS)
             float mx = fmaxf(sc[n][h], sc[n][2 + h]);
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-            const float mn = fmaxf(m[n][h], mx);
+            // a row moves by what it sees itself, whatever its neighbours in the tile see: the condition again, of the whole row
+            const bool own = mx - m[n][h] > 8.f || (Q8 && em_row[n][h] > er[n][h] + 4);
+            const float mn = own ? fmaxf(m[n][h], mx) : m[n][h];
             float f = m[n][h] == -INFINITY ? 0.f : fast_exp2(m[n][h] - mn);
             m[n][h] = mn;
             l[n][h] *= f;
             if constexpr (Q8) {
-              const int en = max(er[n][h], em_row[n][h]);
+              const int en = own ? max(er[n][h], em_row[n][h]) : er[n][h];
               f *= fast_exp2((float)(er[n][h] - en));
               er[n][h] = en;
             }
