@@ -1131,3 +1131,29 @@ def test_attention_large_keys_and_values_that_others_see(cuda_dev, fmt, T, H, Hk
                 assert torch.equal(out[blind], clean[blind]), (node, part, up)
                 assert part == "k" and up == 3 or not torch.equal(out[~blind], clean[~blind])
             (x if e is None else e)[0, 0, :, ctx + node] = keep
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("T", [6, 40, 100])
+def test_attention_largest_exponent_that_others_see(cuda_dev, fmt, T):
+    """Values near the smallest scale, and one of the largest scale that a bf16 vector can have in a slot that only some
+    nodes see: the others' rows keep every bit."""
+    H, Hkv, D, ctx = 8, 2, 64, 75
+    rng = np.random.default_rng(T)
+    p = random_tree(T, rng)
+    see = ancestors(p)
+    cache = make_cache(cuda_dev, fmt, 1, Hkv, 256, D, seed=T)
+    for down in (60, 90):
+        cache.v_exp[:] = torch.clamp(cache.v_exp.int() - down, min=27).to(torch.uint8)
+        t = tr.TreeBatch([(0, ctx, p)], cache)
+        q = queries(cuda_dev, T, H * D)
+        clean = tr.tree_attention(q, cache, t)
+        check_attention(clean, q, cache, [(0, ctx, p)], [see], H)
+        for node in (1, T - 1):
+            keep = cache.v_exp[0, 0, :, ctx + node].clone()
+            cache.v_exp[0, 0, :, ctx + node] = 247 if fmt == "int8" else 245
+            out = tr.tree_attention(q, cache, t)
+            t.check()
+            blind = torch.from_numpy(~see[:, node])
+            assert torch.equal(out[blind], clean[blind]), (down, node)
+            cache.v_exp[0, 0, :, ctx + node] = keep

@@ -278,7 +278,7 @@ struct TcControl {
   uint64_t piece_full[kPieces], piece_empty[kPieces];
   Piece piece[kPieces];                    // tiles == 0: there are no more
   uint64_t s_full[2], s_free[2], p_ready[2], pv_done[2], q_ready, o_done, ml_ready, epi_done, drain[2];
-  // 8-bit, per tile: 2^ek of its keys, or one factor kt; 2^(ev - ref) of its keys where some row does not wholly see it
+  // 8-bit, per tile: 2^ek of its keys, or one factor kt; 2^ev of its keys where some row does not wholly see it
   // (0 for NaN and slots past the end); ref is the exponent byte that V is relative to
   alignas(16) float fk[8][KT];
   alignas(16) float fv[8][KT];
@@ -629,20 +629,20 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!is_v && (partial || warp == 12)) {
             // What the softmax needs to know of the tile: it is there once S is.  The ring's last reader is behind the
             // products that freed this stage.
-            // V's factors in a keyed tile are relative to 2^60 below the largest, so that they last for rows whose own
-            // largest is far smaller.
-            const int em_v = largest(ev, a0, a1), ref = partial ? em_v - 60 : em_v;
+            // V's factors in a keyed tile are the bare powers of two: a row's own reference makes them relative, so that
+            // they last whatever the largest of a slot that it does not see.
+            const int em_v = largest(ev, a0, a1), ref = partial ? 127 : em_v;
             if (ti == 0) {
               ct.ref[f] = ref;
               ct.kt[f] = keyed ? 1.f : __int_as_float(max(top, 1) << 23);
               ct.k_keyed[f] = keyed;
             }
             if (partial && ti < KT) {
-              const int e = ev[ti], d = e - ref + 127;
+              const int e = ev[ti];
               const bool nan = e == 255, in = ti < left;
               if (keyed) ct.fk[f][ti] = exp_scale(ek[ti]);
               ct.ev[f][ti] = nan || !in ? 0 : (uint8_t)e;
-              ct.fv[f][ti] = nan || !in || d <= 0 ? 0.f : __int_as_float(d << 23);
+              ct.fv[f][ti] = nan || !in ? 0.f : exp_scale(e);
               const uint32_t nans = __ballot_sync(0xffffffffu, nan && in);
               if (lane == 0) ct.nan[f][ti >> 5] = nans;
             }
