@@ -293,7 +293,6 @@ struct TcControl {
   uint32_t tmem;
   int e0;
   int abort, dropped;
-  int issued[2];                           // loads that the TMA warp began: raw or K tiles, V tiles
 };
 static_assert(sizeof(TcControl) <= 16384 && alignof(TcControl) <= 16, "control block");
 
@@ -333,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (lane == 31) ct.wsum[warp] = inc;
     if (tid == 0) {
-      ct.abort = ct.dropped = ct.issued[0] = ct.issued[1] = 0;
+      ct.abort = ct.dropped = 0;
       ct.e0 = E;
       for (int i = 0; i < NS; ++i) {
         mbar_init(smem_u32(&ct.kfull[i]), Q8 ? 4 : 1);
@@ -454,8 +453,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         set_status(g.status, kStatusTimeoutProducer);
         *abort_flag = 1;
       }
-      ct.issued[0] = k_issued;
-      ct.issued[1] = v_issued;
+      // Nothing may be in flight when the CTA exits, and after an abort, perhaps one that is still to come, nobody else waits
+      // for what has been issued: the last load of every stage is waited for here.
+      for (int i = max(0, k_issued - (Q8 ? RS : NS)); i < k_issued; ++i)
+        mbar_drain(Q8 ? smem_u32(&ct.raw_full[i % RS]) : smem_u32(&ct.kfull[i % NS]), (i / (Q8 ? RS : NS)) & 1);
+      for (int i = max(0, v_issued - NS); i < v_issued; ++i) mbar_drain(smem_u32(&ct.vfull[i % NS]), (i / NS) & 1);
     }
   } else if (warp == 1 || warp == 3) {
     // ------------------------------------------------------------ MMA issue of stream x
@@ -1054,13 +1056,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  // No copy may be in flight when the CTA exits.  After a clean run every load has been waited for; where some role gave up, and
-  // all have ended by now, the last load of every stage is waited for here.
-  if (tid == 0 && *abort_flag) {
-    const int ring = Q8 ? RS : NS, k_issued = ct.issued[0], v_issued = ct.issued[1];
-    for (int i = max(0, k_issued - ring); i < k_issued; ++i) mbar_drain(smem_u32(Q8 ? &ct.raw_full[i % ring] : &ct.kfull[i % ring]), i / ring & 1);
-    for (int i = max(0, v_issued - NS); i < v_issued; ++i) mbar_drain(smem_u32(&ct.vfull[i % NS]), i / NS & 1);
-  }
   if (warp == 1) tmem_dealloc(tmem, 512);
 }
 
