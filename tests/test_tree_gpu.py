@@ -1157,3 +1157,49 @@ def test_attention_largest_exponent_that_others_see(cuda_dev, fmt, T):
             blind = torch.from_numpy(~see[:, node])
             assert torch.equal(out[blind], clean[blind]), (down, node)
             cache.v_exp[0, 0, :, ctx + node] = keep
+
+
+def check_weighted(out, q, cache, ctx, p, H, above, exact_keys=()):
+    """As check_attention, for one block, with the f16 weights' subnormal step counted against what matters: their reference lies at
+    most 2^above over the largest p_j max|v_j| of the row (not over the largest |v_j|), so a key loses at most
+    2^-25 2^above of that.  ``exact_keys``: slots whose score has no rounding error."""
+    K, V = values64(cache)
+    T, D, G, see = len(p), cache.head_dim, H // cache.n_kv_heads, ancestors(p)
+    got = out.view(T, H, D).double()
+    for i in range(T):
+        use = torch.tensor([True] * ctx + [bool(x) for x in see[i]], device=q.device)
+        rough = use.clone()
+        rough[list(exact_keys)] = False
+        for h in range(H):
+            k, v = K[0, h // G, :ctx + T], V[0, h // G, :ctx + T]
+            qq = q[i, h * D:(h + 1) * D].double()
+            w = torch.softmax(torch.where(use, k @ qq / math.sqrt(D), -math.inf), 0)
+            ref, A = w @ v, w @ v.abs()
+            es = 2.0 ** -24 * (D + 8) * (k[rough].abs() @ qq.abs()).max() / math.sqrt(D)
+            sub = int(use.sum()) * 2.0 ** (above - 25) * (w * v.abs().amax(1)).max()
+            tol = 2.0 ** -8 * ref.abs() * (1 + 2.0 ** -7) + A * (2.0 ** -11 * (1 + 2.0 ** -7) + 2 * es + 2.0 ** -20) + sub + 1e-30
+            err = (got[i, h] - ref).abs()
+            assert (err <= tol).all(), (i, h, float((err / tol).max()))
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T", [1, 6])
+def test_attention_large_values_of_small_weight(cuda_dev, fmt, D, T):
+    """8-bit caches: a seen slot whose values are 2^20 to 2^70 times the others' and whose weight is far smaller still, or about
+    the inverse of that: what the others contribute stays."""
+    H, Hkv, ctx = 8, 2, 333
+    p = random_tree(T, np.random.default_rng(T))
+    q = 1.5 + 0.1 * queries(cuda_dev, T, H * D).float()
+    q = q.bfloat16()
+    for slot in (0, 50, ctx - 1):
+        cache = make_cache(cuda_dev, fmt, 1, Hkv, 384, D, seed=D)
+        cache.k[0, 0, :, slot] = torch.full((1,), -QMAX[fmt], device=cuda_dev).to(cache.k.dtype)
+        cache.k_exp[0, 0, :, slot] = 127 + (-7 if fmt == "e4m3" else -5)     # -3.5, -4 each: scores of -42 to -68, weights of 2^-60 to 2^-98
+        v0 = cache.v_exp[0, 0, :, slot].clone()
+        for up in (20, 30, 50, 70):
+            cache.v_exp[0, 0, :, slot] = v0 + up
+            t = tr.TreeBatch([(0, ctx, p)], cache)
+            out = tr.tree_attention(q, cache, t)
+            t.check()
+            check_weighted(out, q, cache, ctx, p, H, 1)

@@ -142,8 +142,8 @@ __global__ void __launch_bounds__(128) attn_tree_simt_kernel(TreeGeom g, CacheGe
 // thread (g, t) = (lane / 4, lane % 4) takes the dims [t D/4, (t + 1) D/4) of keys g and g + 8 as K fragments and the
 // dims [g D/8, (g + 1) D/8) of keys 2t, 2t + 1, 2t + 8, 2t + 9 as V fragments, so K and V come from shared memory as
 // 16-byte words and turn into f16 pairs in registers, without a transpose.  The values' powers of two never touch the
-// operands: K's scale multiplies the score, V's the weight (relative to the largest one so far of the row, er, as the
-// running maximum does), a power of two of each q row its f16 form.  Weights are rounded to f16 (2^-11; a bf16 cache:
+// operands: K's scale multiplies the score, V's the weight (relative to the row's largest weight x scale so far, er, as
+// the score is to the running maximum), a power of two of each q row its f16 form.  Weights are rounded to f16 (2^-11; a bf16 cache:
 // to bf16, 2^-8, the type of V), sums and outputs are fp32.
 //
 // Measured (32 query and 8 KV heads of 128): 64 trees of 5 nodes at 129 to 1023 slots over bf16 36 us, 4.4 TB/s, 67 % of the
@@ -220,6 +220,8 @@ __device__ __forceinline__ int longest_first(const TreeGeom& g) {
   __syncthreads();
   return pick;
 }
+
+constexpr float kNone = -3.402823466e38f;                                // the maximum of no scores: finite, so that -inf minus it is no NaN
 
 template <int D, int FMT, int NT>
 __global__ void __launch_bounds__(128, MmaShape<D, FMT, NT>::CTAS)
@@ -335,14 +337,16 @@ __global__ void __launch_bounds__(128, MmaShape<D, FMT, NT>::CTAS)
 
   // this thread's rows of n-tile n: 8 n + 2 tq, + 1
   float o[NT][MD][4], m[NT][2], l[NT][2], rf[NT][2];
-  int er[NT][2];                                                        // 8-bit: exponent byte of the largest V scale so far
+  int er[NT][2];                                                        // 8-bit: exponent byte that the weights are relative to
+  float top[NT][2];                                                     // and er + 12: beyond it a weight's exponent asks for another
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      m[n][h] = -INFINITY;
+      m[n][h] = kNone;
       l[n][h] = 0.f;
       er[n][h] = 1;
+      top[n][h] = 13.f;
       rf[n][h] = g.scale * 1.4426950408889634f * (Q8 ? qscale[8 * n + 2 * tq + h] * kHalfUnit<FMT> : 1.f);
 #pragma unroll
       for (int d = 0; d < MD; ++d) o[n][d][h] = o[n][d][2 + h] = 0.f;
@@ -405,15 +409,14 @@ __global__ void __launch_bounds__(128, MmaShape<D, FMT, NT>::CTAS)
         }
       }
       // ---- scores in the log2 domain; masks
-      float fv[2] = {1.f, 1.f};
-      int em = 0, e8[2] = {0, 0};
+      float fv[2] = {1.f, 1.f}, ev[2] = {0.f, 0.f};                       // V's scale and its exponent byte (a NaN's counts as none)
       if constexpr (Q8) {
         const float fk0 = exp_scale(ex[st * 16 + gq]), fk1 = exp_scale(ex[st * 16 + gq + 8]);
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
           const int e = ex[64 + st * 16 + gq + 8 * y];
           fv[y] = exp_scale(e);
-          e8[y] = e == 255 ? 0 : e;
+          ev[y] = e == 255 ? -INFINITY : (float)e;
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -422,7 +425,6 @@ __global__ void __launch_bounds__(128, MmaShape<D, FMT, NT>::CTAS)
             sc[n][h] *= rf[n][h] * fk0;
             sc[n][2 + h] *= rf[n][h] * fk1;
           }
-        em = __reduce_max_sync(0xffffffffu, max(e8[0], e8[1]));
       } else {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -432,13 +434,9 @@ __global__ void __launch_bounds__(128, MmaShape<D, FMT, NT>::CTAS)
             sc[n][2 + h] *= rf[n][h];
           }
       }
-      int em_row[NT][2];
       bool seen[NT][4];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        em_row[n][0] = em_row[n][1] = em;
-        seen[n][0] = seen[n][1] = seen[n][2] = seen[n][3] = true;
-      }
+      for (int n = 0; n < NT; ++n) seen[n][0] = seen[n][1] = seen[n][2] = seen[n][3] = true;
       if (partial) {
         const int left = k_hi - key0 - st * 16;
 #pragma unroll
@@ -452,41 +450,52 @@ __global__ void __launch_bounds__(128, MmaShape<D, FMT, NT>::CTAS)
             seen[n][2 + h] = see >> (gq + 8) & 1;
             if (!seen[n][h]) sc[n][h] = -INFINITY;
             if (!seen[n][2 + h]) sc[n][2 + h] = -INFINITY;
-            if constexpr (Q8) {                                         // V's largest exponent among the keys this row sees
-              int e = max(seen[n][h] ? e8[0] : 0, seen[n][2 + h] ? e8[1] : 0);
-#pragma unroll
-              for (int x = 4; x < 32; x <<= 1) e = max(e, __shfl_xor_sync(0xffffffffu, e, x));
-              em_row[n][h] = e;
-            }
           }
       }
-      // ---- a new reference where a score is more than 2^8 above it, or V's scale more than 2^4 (weights stay below 2^12,
-      // in range of f16); -inf - -inf compares false, as a row that has seen nothing should
+      // ---- a new reference where a score is more than 2^8 above it, or a weight with V's scale would pass 2^12 (in range of
+      // f16).  A weight's exponent is the difference first: scores may be too large to hold V's exponent beside them.
+      float x[NT][4];
       bool need = false;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          need = need || fmaxf(sc[n][h], sc[n][2 + h]) - m[n][h] > 8.f || (Q8 && em_row[n][h] > er[n][h] + 4);
+        for (int h = 0; h < 2; ++h) {
+          x[n][h] = sc[n][h] - m[n][h];
+          x[n][2 + h] = sc[n][2 + h] - m[n][h];
+          need = need || fmaxf(x[n][h], x[n][2 + h]) > 8.f || (Q8 && fmaxf(x[n][h] + ev[0], x[n][2 + h] + ev[1]) > top[n][h]);
+        }
       if (__any_sync(0xffffffffu, need)) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            float mx = fmaxf(sc[n][h], sc[n][2 + h]);
+            auto row_max = [](float v) {
 #pragma unroll
-            for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+              for (int y = 4; y < 32; y <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, y));
+              return v;
+            };
+            // (every lane takes part in every reduction: none of them behind a condition)
+            const float mx = row_max(fmaxf(sc[n][h], sc[n][2 + h]));
+            float tx = -INFINITY;
+            if constexpr (Q8) tx = row_max(fmaxf(x[n][h] + ev[0], x[n][2 + h] + ev[1]));
             // a row moves by what it sees itself, whatever its neighbours in the tile see: the condition again, of the whole row
-            const bool own = mx - m[n][h] > 8.f || (Q8 && em_row[n][h] > er[n][h] + 4);
+            const bool own = mx - m[n][h] > 8.f || (Q8 && tx > top[n][h]);
             const float mn = own ? fmaxf(m[n][h], mx) : m[n][h];
-            float f = m[n][h] == -INFINITY ? 0.f : fast_exp2(m[n][h] - mn);
-            m[n][h] = mn;
+            const float df = m[n][h] - mn;
+            float f = fast_exp2(df);
             l[n][h] *= f;
+            x[n][h] = sc[n][h] - mn;
+            x[n][2 + h] = sc[n][2 + h] - mn;
             if constexpr (Q8) {
-              const int en = own ? max(er[n][h], em_row[n][h]) : er[n][h];
-              f *= fast_exp2((float)(er[n][h] - en));
+              // relative to the largest weight x scale, which a V of a large scale and no weight does not raise.  Rounded down, so
+              // that it does not creep up with every move of m; 1 .. 253 keep 2^(127 - er) a normal float.
+              tx = row_max(fmaxf(x[n][h] + ev[0], x[n][2 + h] + ev[1]));
+              const int en = own ? min(max((int)floorf(fmaxf(tx, df + (float)er[n][h])), 1), 253) : er[n][h];
+              f = fast_exp2(df + (float)(er[n][h] - en));
               er[n][h] = en;
+              top[n][h] = (float)(en + 12);
             }
+            m[n][h] = mn;
 #pragma unroll
             for (int d = 0; d < MD; ++d) {
               o[n][d][h] *= f;
@@ -501,13 +510,12 @@ __global__ void __launch_bounds__(128, MmaShape<D, FMT, NT>::CTAS)
         float w[4];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float ms = m[n][h] == -INFINITY ? 0.f : m[n][h];
-          const float p0 = fast_exp2(sc[n][h] - ms), p1 = fast_exp2(sc[n][2 + h] - ms);
+          const float p0 = fast_exp2(x[n][h]), p1 = fast_exp2(x[n][2 + h]);
           l[n][h] += p0 + p1;
           if constexpr (Q8) {
             const float rv = __int_as_float((254 - er[n][h]) << 23);    // 2^-(er - 127)
-            w[h] = seen[n][h] ? p0 * (fv[0] * rv) : 0.f;
-            w[2 + h] = seen[n][2 + h] ? p1 * (fv[1] * rv) : 0.f;
+            w[h] = seen[n][h] ? p0 * fv[0] * rv : 0.f;
+            w[2 + h] = seen[n][2 + h] ? p1 * fv[1] * rv : 0.f;
           } else {
             w[h] = p0;
             w[2 + h] = p1;
@@ -615,27 +623,33 @@ __global__ void __launch_bounds__(128, MmaShape<D, FMT, NT>::CTAS)
 #pragma unroll 2
   for (int r = threadIdx.x / LPR; r < nrows; r += 128 / LPR) {
     const int d = threadIdx.x % LPR * 4;
-    float M = -INFINITY, E = 1.f;
+    float M = kNone, top = -INFINITY;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       M = fmaxf(M, Mw[w * ROWS + r]);
-      E = fmaxf(E, Ew[w * ROWS + r]);
     }
-    const float ms = M == -INFINITY ? 0.f : M;
+    if constexpr (Q8) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) top = fmaxf(top, Mw[w * ROWS + r] - M + Ew[w * ROWS + r]);
+    }
+    const float E = fminf(fmaxf(floorf(top), 1.f), 253.f);
     float L = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float f = fast_exp2(Mw[w * ROWS + r] - ms);
-      const float fo = Q8 ? f * fast_exp2(Ew[w * ROWS + r] - E) : f;
+      const float f = fast_exp2(Mw[w * ROWS + r] - M);
+      const float fo = Q8 ? fast_exp2(Mw[w * ROWS + r] - M + (Ew[w * ROWS + r] - E)) : f;
       L += f * Lw[w * ROWS + r];
       const float4 v = *reinterpret_cast<const float4*>(Ow + (w * ROWS + r) * OLD + d);
       acc[0] += fo * v.x, acc[1] += fo * v.y, acc[2] += fo * v.z, acc[3] += fo * v.w;
     }
     float inv = L == 0.f ? 0.f : 1.f / L;                               // a row that sees nothing: zeros
-    if constexpr (Q8) inv *= kHalfUnit<FMT> * __int_as_float((int)E << 23);
     const int R = r0 + r, node = R / g.G;
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[e] *= inv;
+    if constexpr (Q8) {                                                 // (the product of the three may pass fp32)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] = acc[e] * kHalfUnit<FMT> * __int_as_float((int)E << 23);
+    }
     if (!Q8 && flags[1]) {                                              // the dropped elements of keys this row sees
       const uint64_t* mk = g.mask ? masks + r * 4 : nullptr;
 #pragma unroll 1
