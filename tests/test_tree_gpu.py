@@ -1184,7 +1184,7 @@ def check_weighted(out, q, cache, ctx, p, H, above, exact_keys=()):
 
 @pytest.mark.parametrize("fmt", ["e4m3", "int8"])
 @pytest.mark.parametrize("D", [64, 128])
-@pytest.mark.parametrize("T", [1, 6])
+@pytest.mark.parametrize("T", [1, 6, 40, 100])
 def test_attention_large_values_of_small_weight(cuda_dev, fmt, D, T):
     """8-bit caches: a seen slot whose values are 2^20 to 2^70 times the others' and whose weight is far smaller still, or about
     the inverse of that: what the others contribute stays."""
@@ -1193,7 +1193,7 @@ def test_attention_large_values_of_small_weight(cuda_dev, fmt, D, T):
     q = 1.5 + 0.1 * queries(cuda_dev, T, H * D).float()
     q = q.bfloat16()
     for slot in (0, 50, ctx - 1):
-        cache = make_cache(cuda_dev, fmt, 1, Hkv, 384, D, seed=D)
+        cache = make_cache(cuda_dev, fmt, 1, Hkv, 448, D, seed=D)
         cache.k[0, 0, :, slot] = torch.full((1,), -QMAX[fmt], device=cuda_dev).to(cache.k.dtype)
         cache.k_exp[0, 0, :, slot] = 127 + (-7 if fmt == "e4m3" else -5)     # -3.5, -4 each: scores of -42 to -68, weights of 2^-60 to 2^-98
         v0 = cache.v_exp[0, 0, :, slot].clone()
@@ -1202,4 +1202,24 @@ def test_attention_large_values_of_small_weight(cuda_dev, fmt, D, T):
             t = tr.TreeBatch([(0, ctx, p)], cache)
             out = tr.tree_attention(q, cache, t)
             t.check()
-            check_weighted(out, q, cache, ctx, p, H, 1)
+            check_weighted(out, q, cache, ctx, p, H, 1 if T * H // Hkv <= 32 else 9)   # tcgen05: a tile's largest scale stands for all of its keys within 2^8
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T", [1, 6, 40, 100])
+def test_attention_keys_of_scales_far_apart(cuda_dev, fmt, D, T):
+    """8-bit caches: a key 2^10 to 2^60 times the others that q is orthogonal to: its score is 0, and the others' keep their bits."""
+    H, Hkv, ctx = 8, 2, 333
+    p = random_tree(T, np.random.default_rng(T))
+    q = torch.ones(T, H * D, dtype=torch.bfloat16, device=cuda_dev)
+    for slot in (0, 50, 200, ctx - 1):
+        cache = make_cache(cuda_dev, fmt, 1, Hkv, 448, D, seed=D)
+        sign = torch.where(torch.arange(D, device=cuda_dev) % 2 == 0, 1.0, -1.0)
+        cache.k[0, 0, :, slot] = (sign * QMAX[fmt]).to(cache.k.dtype)
+        for up in (10, 20, 30, 60):
+            cache.k_exp[0, 0, :, slot] = 120 + up
+            t = tr.TreeBatch([(0, ctx, p)], cache)
+            out = tr.tree_attention(q, cache, t)
+            t.check()
+            check_weighted(out, q, cache, ctx, p, H, 1 if T * H // Hkv <= 32 else 9, exact_keys=[slot])

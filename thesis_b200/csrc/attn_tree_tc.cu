@@ -13,10 +13,9 @@
 // over all key tiles; with fewer, both share the rows and take every other key tile, and meet at the end.
 //
 // 8-bit caches: a warpgroup turns the TMA-loaded bytes into the f16 tiles that the products read, each key's power of
-// two relative to the tile's largest multiplied in (exact, as f16 goes, while they are within 2^21, e4m3, or 2^29, int8,
-// and zero from 2^38 or 2^29 on), so the softmax sees one scale per tile.  In tiles that some row
-// does not wholly see a key's scale stays out of the operands and multiplies scores and weights instead: what
-// a row does not see must not decide its precision.
+// two relative to the tile's largest multiplied in (exact: K's within 2^16, V's within 2^8 of each other), so the softmax sees
+// one scale per tile.  Scales that lie further apart stay out of the operands and multiply scores and weights instead, and so
+// do V's in tiles that some row does not wholly see: what a row does not see must not decide its precision.
 //
 // Roles of the 20 warps: 0 TMA, 1 and 3 MMA issue of stream 0 and 1 (a satisfied barrier wait costs some 150 clocks,
 // and each tile takes four of them), 2 the schedule, 4-7 and 8-11 softmax of stream 0 and 1 (a thread is a row),
@@ -273,19 +272,21 @@ template <int D, int FMT> struct TcShape {
 };
 constexpr int kPieces = 4;                 // pieces between the schedule warp and the slowest role
 constexpr int kReaders = 19;               // warps that read them: TMA, 2 MMA, 8 softmax, 8 conversion
+enum : int { kHowK = 1 << 8, kHowV = 1 << 9, kHowWide = 1 << 10 };
 struct TcControl {
   uint64_t kfull[4], kempty[4], vfull[4], vempty[4], vclean[4], raw_full[6], raw_empty[6];
   uint64_t piece_full[kPieces], piece_empty[kPieces];
   Piece piece[kPieces];                    // tiles == 0: there are no more
   uint64_t s_full[2], s_free[2], p_ready[2], pv_done[2], q_ready, o_done, ml_ready, epi_done, drain[2];
-  // 8-bit, per tile: 2^ek of its keys, or one factor kt; 2^ev of its keys where some row does not wholly see it
-  // (0 for NaN and slots past the end); ref is the exponent byte that V is relative to
+  // 8-bit, per tile: ref is V's largest exponent byte, kt the one factor of its keys, and how (kHow*, above ref's byte) what is not in
+  // the operands.  Keyed K: 2^ek of the keys multiplies the scores.  Keyed V: 2^ev of the keys multiplies the weights, ev is the exponent
+  // byte (0 for NaN and slots past the end); wide: they lie so far apart that the largest does not stand for the others.
   alignas(16) float fk[8][KT];
   alignas(16) float fv[8][KT];
   float kt[8];
-  alignas(16) uint8_t ev[8][KT];           // V's exponent bytes, 0 likewise
+  alignas(16) uint8_t ev[8][KT];
   alignas(16) uint8_t exps[6][2 * KT];     // raw exponent bytes, K then V
-  int ref[8], k_keyed[8];
+  int ref[8];
   uint32_t nan[8][2];                      // keys whose V is NaN
   float ml[2][2][3][128];                  // one row tile: max, sum and eref of the streams (by piece parity)
   long long lo, hi, base, run;
@@ -619,34 +620,43 @@ __global__ void __launch_bounds__(kThreads, 1)
             a0 = v & 255, a1 = v >> 8;
             return __reduce_max_sync(0xffffffffu, max(in0 && a0 != 255 ? a0 : 0, in1 && a1 != 255 ? a1 : 0));
           };
+          // whether some scale lies more than 2^d below the largest (vectors at the smallest scale, zeros most often, apart)
+          auto spread = [&](int em, int d, int a0, int a1) {
+            return __any_sync(0xffffffffu, (in0 && a0 > 27 && a0 < em - d) || (in1 && a1 > 27 && a1 < em - d));
+          };
           int a0, a1;
           const uint8_t *ek = ct.exps[rs], *ev = ek + KT;
           const int em = largest(is_v ? ev : ek, a0, a1);
-          // In a tile that some row does not wholly see, V's scales stay with the weights: they decide a row's precision.
-          // K's are folded where that is exact (within 2^16 of each other).
-          bool keyed = partial && is_v;
-          if (partial && !is_v) keyed = __any_sync(0xffffffffu, (in0 && a0 < em - 16) || (in1 && a1 < em - 16));
+          // Scales far apart stay out of the operand: K's where f16 would round (beyond 2^16), V's where what is small beside the
+          // largest could matter all the same (beyond 2^8).  So do V's in a tile that some row does not wholly see: a slot that a row
+          // does not see must not decide its precision.
+          const bool keyed = spread(em, is_v ? 8 : 16, a0, a1) || (is_v && partial);
           const int top = keyed ? 0 : max(em, 27) - kUp<FMT>;
+          int ref = 0;
+          if (!is_v && warp == 12) {
+            ref = largest(ev, a0, a1);
+            const bool wide = spread(ref, 8, a0, a1);
+            ref |= (keyed ? kHowK : 0) | (wide || partial ? kHowV : 0) | (wide ? kHowWide : 0);
+          }
           if (!(ok = warp_wait(is_v ? &ct.vempty[st] : &ct.kempty[st], (cnt / NS & 1) ^ 1, abort_flag, g.spin))) break;
-          if (!is_v && (partial || warp == 12)) {
+          if (!is_v && warp == 12) {
             // What the softmax needs to know of the tile: it is there once S is.  The ring's last reader is behind the
             // products that freed this stage.
-            // V's factors in a keyed tile are the bare powers of two: a row's own reference makes them relative, so that
-            // they last whatever the largest of a slot that it does not see.
-            const int em_v = largest(ev, a0, a1), ref = partial ? 127 : em_v;
-            if (ti == 0) {
+            if (lane == 0) {
               ct.ref[f] = ref;
               ct.kt[f] = keyed ? 1.f : __int_as_float(max(top, 1) << 23);
-              ct.k_keyed[f] = keyed;
             }
-            if (partial && ti < KT) {
-              const int e = ev[ti];
-              const bool nan = e == 255, in = ti < left;
-              if (keyed) ct.fk[f][ti] = exp_scale(ek[ti]);
-              ct.ev[f][ti] = nan || !in ? 0 : (uint8_t)e;
-              ct.fv[f][ti] = nan || !in ? 0.f : exp_scale(e);
-              const uint32_t nans = __ballot_sync(0xffffffffu, nan && in);
-              if (lane == 0) ct.nan[f][ti >> 5] = nans;
+            if (ref > 255) {
+#pragma unroll
+              for (int y = 0; y < KT; y += 32) {
+                const int j = lane + y, e = ev[j];
+                const bool nan = e == 255, in = j < left;
+                ct.fk[f][j] = exp_scale(ek[j]);
+                ct.ev[f][j] = nan || !in ? 0 : (uint8_t)e;
+                ct.fv[f][j] = nan || !in ? 0.f : exp_scale(e);
+                const uint32_t nans = __ballot_sync(0xffffffffu, nan && in);
+                if (lane == 0) ct.nan[f][y >> 5] = nans;
+              }
             }
           }
           convert(sm + 2 * NS * S::TILE + rs * S::RAW + (is_v ? S::RAW / 2 : 0), sm + ((is_v ? NS : 0) + st) * S::TILE, is_v ? ev : ek, top, is_v ? kUp<FMT> : 0, left);
@@ -791,7 +801,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       return rf;
     };
     float rf = 0.f, m = -INFINITY, l = 0.f;
-    int er = 0, nt = 0;                                                 // er: 8-bit: exponent byte that O and l are relative to
+    int er = 1, nt = 0;                                                 // er: 8-bit: exponent byte that the weights and O are relative to
     bool begun = false, two = false;
     // One turn: the next piece's Q goes out, then the last piece's output (its products are done, and the next one's first
     // S runs meanwhile), then the next piece's tiles.
@@ -814,19 +824,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!(ok = warp_wait(&ct.o_done, piece & 1, abort_flag, g.spin))) break;
         const Piece& cur = ct.piece[piece % kPieces];
         tc_fence_after();
-        float f0 = 1.f, f1 = 0.f, M = m, L = l, E = (float)er;
+        float f0 = 1.f, f1 = 0.f, M = m, L = l;
+        int E = er;
         if (!two) {
           const float m0 = ml[0][0][r], m1 = ml[1][0][r], e0 = ml[0][2][r], e1 = ml[1][2][r];
           M = fmaxf(m0, m1);
           const float ms = M == -INFINITY ? 0.f : M;
-          E = fmaxf(fmaxf(e0, e1), 0.f);
-          const float w0 = fast_exp2(m0 - ms), w1 = e1 < 0.f ? 0.f : fast_exp2(m1 - ms);
-          L = w0 * ml[0][1][r] + (e1 < 0.f ? 0.f : w1 * ml[1][1][r]);
-          f0 = Q8 ? w0 * fast_exp2(e0 - E) : w0;
-          f1 = e1 < 0.f ? 0.f : Q8 ? w1 * fast_exp2(e1 - E) : w1;
+          f0 = fast_exp2(m0 - ms), f1 = e1 < 0.f ? 0.f : fast_exp2(m1 - ms);
+          L = f0 * ml[0][1][r] + (e1 < 0.f ? 0.f : f1 * ml[1][1][r]);
+          if constexpr (Q8) {                                             // both relative to the larger weight x scale
+            E = min(max((int)floorf(fmaxf(m0 - ms + e0, e1 < 0.f ? -INFINITY : m1 - ms + e1)), 1), 253);
+            f0 = fast_exp2(m0 - ms + (e0 - (float)E));
+            f1 = e1 < 0.f ? 0.f : fast_exp2(m1 - ms + (e1 - (float)E));
+          }
         }
         float inv = L == 0.f ? 0.f : 1.f / L;                             // a row that sees nothing: zeros
-        if constexpr (Q8) inv *= kHalfUnit<FMT> / (1 << kUp<FMT>) * __int_as_float((int)fmaxf(E, 1.f) << 23);
+        if constexpr (Q8) inv *= kHalfUnit<FMT> / (1 << kUp<FMT>) * __int_as_float(E << 23);
         const Row cw = row_of(cur);
         const bool join = !two && nt > 1;
         const size_t at = (size_t)(cur.bi.start + cw.node) * g.n_heads + cw.head;
@@ -896,7 +909,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       rf = rf_next;
       m = -INFINITY;
       l = 0.f;
-      er = 0;
+      er = 1;
       begun = false;
       const int whole_to = min(cur.all_see, cur.n_keys);
 #pragma unroll 1
@@ -907,7 +920,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t a[KT];
         tmem_ld32(tS, a);
         tmem_ld32(tS + 32, a + 32);
-        const int ref = Q8 ? ct.ref[f] : 0;
+        const int how = Q8 ? ct.ref[f] : 0;
         const float rt = Q8 ? rf * ct.kt[f] : rf;
         tmem_wait_ld();
         tc_fence_before();
@@ -917,9 +930,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool partial = (t + 1) * KT > whole_to;                   // some row does not see some key of the tile
         // Every choice below is made so that what a row does not see does not change a bit of its result: the forms of the
         // exponent differ between rows only by the row's own scores.
-        int em = ref;
-        if (__builtin_expect(partial, 0)) {                             // which keys the row sees
-          if (Q8 && ct.k_keyed[f]) {
+        int em = how & 255;                                             // V's largest exponent among the keys that the row sees
+        if (__builtin_expect(partial || how > 255, 0)) {                // which keys those are
+          if (how & kHowK) {
 #pragma unroll
             for (int j = 0; j < KT; ++j) a[j] = __float_as_uint(__uint_as_float(a[j]) * ct.fk[f][j]);
           }
@@ -930,7 +943,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (left < 64) s1 &= left <= 32 ? 0u : (1u << (left - 32)) - 1;
 #pragma unroll
           for (int j = 0; j < KT; ++j) a[j] = (j < 32 ? s0 : s1) >> (j & 31) & 1 ? a[j] : 0xff800000u;
-          if constexpr (Q8) {                                           // V's largest exponent among them
+          if (how & kHowV) {
             uint32_t top = 0;
 #pragma unroll 2
             for (int j = 0; j < KT / 4; ++j) {
@@ -938,6 +951,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               top = __vmaxu4(top, reinterpret_cast<const uint32_t*>(ct.ev[f])[j] & ((bits * 0x204081u & 0x1010101u) * 255u));
             }
             em = max(max(top & 255, top >> 8 & 255), max(top >> 16 & 255, top >> 24));
+            if (em == 0) em = er;                                       // none: nothing that would ask for another reference
             if ((ct.nan[f][0] & s0) | (ct.nan[f][1] & s1)) l = __int_as_float(0x7fffffff);   // the row sees a V that is NaN
           }
         }
@@ -947,38 +961,52 @@ __global__ void __launch_bounds__(kThreads, 1)
           mx0 = fmaxf(mx0, fmaxf(__uint_as_float(a[j]), __uint_as_float(a[j + 1])));
           mx1 = fmaxf(mx1, fmaxf(__uint_as_float(a[j + 2]), __uint_as_float(a[j + 3])));
         }
-        // O, l and m move to a new reference only when the old one is too small by 2^8 (2^4 for V's scale): the weights
-        // stay below 2^12, in range of f16.  O is then to be scaled by cf.
+        // O, l and m move to a new reference only when the old one is too small by 2^8, or the weights with V's scale, relative
+        // to 2^er, would pass 2^12 (in range of f16).  O is then to be scaled by cf.
         // One FMA per score leaves 2^-24 |m| of it in the exponent: nothing at ordinary sizes, but at very large ones the
         // largest score has to come out as exactly 0.  V's common scale relative to er goes into the exponent, so l
-        // collects the same units and is brought back by the exact power of two; below 2^-40 that is not f16 any more.
-        const float mn = fmaxf(m, fmaxf(mx0, mx1) * rt);
-        const bool need = !begun || mn > m + 8.f || (Q8 && em > er + 4);
+        // collects the same units and is brought back by the exact power of two; beyond 2^40 weights and l go apart.
+        const float mx = fmaxf(mx0, mx1) * rt, mn = fmaxf(m, mx);
+        const int de = em - er;
+        const bool rises = !begun || mn > m + 8.f;
         auto is_huge = [&] { return !(fabsf(m) <= 65536.f || m == -INFINITY); };
-        auto is_gone = [&] { return Q8 && !partial && em - er < -40; };
+        auto is_far = [&] { return Q8 && !(how & kHowV) && abs(em - er) > 40; };
         float cf = 1.f;
-        bool rescale = false, huge = false, gone = false, odd = false;
-        if (__builtin_expect(__any_sync(0xffffffffu, need || is_huge() || is_gone()), 0)) {
+        bool rescale = false, huge = false, far = false, odd = false;
+        // (unless m rises or em is more than 2^3 above er, no weight passes 2^12)
+        if (__builtin_expect(__any_sync(0xffffffffu, rises || is_huge() || (Q8 && (unsigned)(de + 40) > 43u)), 0)) {
+          const float up = mn - m;
+          float heavy = mx - mn + (float)de;                            // 8-bit: the largest weight x scale, or what it is at most: log2, over mn and 2^er
+          if (__builtin_expect(how & kHowWide, 0)) {
+            heavy = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < KT; ++j)                                // (rounded as mx is)
+              if (const int e = ct.ev[f][j]) heavy = fmaxf(heavy, __fadd_rn(__fmul_rn(__uint_as_float(a[j]), rt), -mn) + (float)(e - er));
+          }
+          const bool need = rises || (Q8 && heavy + up > 12.f);
           if (need) {
-            const int en = max(er, em);
-            cf = m == -INFINITY ? 0.f : fast_exp2(m - mn);
+            cf = m == -INFINITY ? 0.f : fast_exp2(-up);
             l *= cf;
-            if (Q8) cf *= er == 0 ? 0.f : fast_exp2((float)(er - en));
+            if constexpr (Q8) {
+              // rounded down, so that it does not creep up with every move of m; 1 .. 253 keep 2^(127 - er) a normal float
+              const int en = min(max(er + (int)floorf(fmaxf(heavy, -up)), 1), 253);
+              cf = m == -INFINITY ? 0.f : fast_exp2((float)(er - en) - up);
+              er = en;
+            }
             m = mn;
-            er = en;
           }
           rescale = begun && __any_sync(0xffffffffu, need);
-          huge = is_huge(), gone = is_gone();
-          odd = __any_sync(0xffffffffu, huge || gone);
+          huge = is_huge(), far = is_far();
+          odd = __any_sync(0xffffffffu, huge || far);
         }
-        const int dd = Q8 && !partial && !gone ? ref - er : 0;
+        const int dd = Q8 && !(how & kHowV) && !far ? em - er : 0;
         const float ms = m == -INFINITY ? 0.f : m, nbs = (float)dd - ms;
-        const float vc = Q8 ? __int_as_float(min(max(ref - er + 127, 1), 254) << 23) : 0.f;   // V's factors relative to the row
+        const float vc = Q8 ? __int_as_float((254 - er) << 23) : 0.f;   // 2^(127 - er)
         uint32_t w[KT / 2];
         f32x2 sum0 = pack_f2(0.f, 0.f), sum1 = pack_f2(0.f, 0.f);
         if (__builtin_expect(!odd, 1)) {
           const f32x2 nb = pack_f2(nbs, nbs), rt2 = pack_f2(rt, rt);
-          if (__builtin_expect(!(Q8 && partial), 1)) {
+          if (__builtin_expect(!(how & kHowV), 1)) {
 #pragma unroll
             for (int j = 0; j < KT; j += 4) {
               const float2 y0 = unpack_f2(fma2(pack_f2(__uint_as_float(a[j]), __uint_as_float(a[j + 1])), rt2, nb));
@@ -999,8 +1027,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               sum0 = add2(sum0, pack_f2(e0, e1));
               sum1 = add2(sum1, pack_f2(e2, e3));
               // an unseen key's factor may be out of range, its weight is 0
-              w[j / 2] = pack2<FMT>(e0 == 0.f ? 0.f : e0 * (v.x * vc), e1 == 0.f ? 0.f : e1 * (v.y * vc));
-              w[j / 2 + 1] = pack2<FMT>(e2 == 0.f ? 0.f : e2 * (v.z * vc), e3 == 0.f ? 0.f : e3 * (v.w * vc));
+              w[j / 2] = pack2<FMT>(e0 == 0.f ? 0.f : e0 * v.x * vc, e1 == 0.f ? 0.f : e1 * v.y * vc);
+              w[j / 2 + 1] = pack2<FMT>(e2 == 0.f ? 0.f : e2 * v.z * vc, e3 == 0.f ? 0.f : e3 * v.w * vc);
             }
           }
         } else {                                                        // the same, row by row in its own form
@@ -1011,10 +1039,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
               const float y = __uint_as_float(a[j + b]);
-              e[b] = fast_exp2(huge ? __fadd_rn(__fadd_rn(__fmul_rn(y, rt), -ms), (float)dd) : fmaf(y, rt, nbs));
+              const float z = huge ? __fadd_rn(__fadd_rn(__fmul_rn(y, rt), -ms), (float)dd) : fmaf(y, rt, nbs);
+              e[b] = fast_exp2(z);
               sum[(j + b) & 3] += e[b];
-              if (Q8 && partial) e[b] = e[b] == 0.f ? 0.f : e[b] * (ct.fv[f][j + b] * vc);
-              if (gone) e[b] = 0.f;
+              if (how & kHowV) e[b] = e[b] == 0.f ? 0.f : e[b] * ct.fv[f][j + b] * vc;
+              if (far) e[b] = fast_exp2(z + (float)(em - er));
             }
             w[j / 2] = pack2<FMT>(e[0], e[1]);
           }
