@@ -301,7 +301,8 @@ typedef struct EesdTree {
   int32_t max_ctx;               /* host: largest ctx + T, at least (<= max_seq) */
   int32_t words;                 /* 64-bit words per mask row: (max_nodes + 63) / 64, at most 4; 0 without a mask */
   int32_t reserved;              /* 0 */
-  const int32_t* blk;            /* [n_blocks, 4] = (start, T, row, ctx), 16-byte aligned; the blocks tile the tokens */
+  const int32_t* blk;            /* [n_blocks, 4] = (start, T, row, ctx), 16-byte aligned; no two blocks
+                                    share a token, tokens of no block are padding */
   const int32_t* parent;         /* [n_tokens], NULL: every block is a chain */
   int32_t* tok_pos;              /* [n_tokens] RoPE position: ctx + depth */
   int32_t* tok_slot;             /* [n_tokens] cache slot: ctx + i */
@@ -313,7 +314,8 @@ typedef struct EesdTree {
 /* tok_pos, tok_slot, tok_row and (unless NULL) mask from blk and parent, on the device: a node sees its
  * ancestors and itself.  A block outside the tokens or the cache, or a parent that does not come before
  * its node, sets a bit in *status (device int32, nullable); the tokens of a bad block get slot -1, which
- * eesd_kv_append and eesd_kv_read skip, and a bad parent counts as -1. */
+ * eesd_kv_append and eesd_kv_read skip, and a bad parent counts as -1.  Tokens that no block covers (a block that
+ * the program has cut short) are padding: position, slot and row -1, skipped without a status bit. */
 int eesd_tree_meta(const EesdTree* tree, int max_batch, int max_seq, int32_t* status, void* stream);
 
 /* RoPE of q and k and the KV append of n_tok packed tokens into layer `layer`, quantising where the
@@ -321,14 +323,14 @@ int eesd_tree_meta(const EesdTree* tree, int max_batch, int max_seq, int32_t* st
  * element is the quantised model-dtype element.  qkv [n_tok, (Hq + 2 Hkv) D], tokens ld_qkv elements apart
  * (ld_qkv % 8 == 0); q_out [n_tok, Hq D] receives the rotated q (NULL: in place in qkv).  tok_pos indexes the
  * RoPE tables [rope_len, D], tok_slot (NULL: tok_pos) the cache.  A token whose position, row or slot is
- * out of range sets a bit in *status and is skipped.  Two tokens with the same row and slot: the slot
+ * out of range sets a bit in *status and is skipped (all three -1, padding: skipped without).  Two tokens with the same row and slot: the slot
  * holds neither reliably. */
 int eesd_kv_append(int dtype, const EesdKvCache* cache, int layer, void* qkv, int ld_qkv, int n_heads,
                    const int32_t* tok_pos, const int32_t* tok_slot, const int32_t* tok_row, int n_tok,
                    const float* rope_cos, const float* rope_sin, int rope_len, void* q_out, int32_t* status, void* stream);
 
 /* k_out / v_out [n_tok, Hkv, D] (each nullable, 16-byte aligned) = the values of layer `layer` at
- * (tok_row[t], tok_slot[t]), in dtype.  A token out of range sets a bit in *status; its outputs are left. */
+ * (tok_row[t], tok_slot[t]), in dtype.  A token out of range sets a bit in *status (row and slot -1, padding: none); its outputs are left. */
 int eesd_kv_read(int dtype, const EesdKvCache* cache, int layer, const int32_t* tok_slot, const int32_t* tok_row, int n_tok,
                  void* k_out, void* v_out, int32_t* status, void* stream);
 

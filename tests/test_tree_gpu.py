@@ -1223,3 +1223,63 @@ def test_attention_keys_of_scales_far_apart(cuda_dev, fmt, D, T):
             out = tr.tree_attention(q, cache, t)
             t.check()
             check_weighted(out, q, cache, ctx, p, H, 1 if T * H // Hkv <= 32 else 9, exact_keys=[slot])
+
+
+@pytest.mark.parametrize("chains", [True, False])
+def test_blocks_cut_short_leave_padding(cuda_dev, chains):
+    """Blocks shortened or moved on the device: tokens that no block covers any more are no tokens.  They get slot -1, are
+    neither written to the cache nor reported, and their rows of the outputs stay as they were."""
+    H, Hkv, D, S = 4, 2, 64, 256
+    cos, sin = tables(cuda_dev, S, D)
+    rng = np.random.default_rng(4)
+    sizes = [5, 4, 7, 3]
+    blocks = [(b, 10 * b + 3, n if chains else random_tree(n, rng)) for b, n in enumerate(sizes)]
+    first = [0, 5, 9, 16]
+    cache = make_cache(cuda_dev, "int8", 4, Hkv, S, D)
+    for edits, gone in (([(0, 1, 3)], [3, 4]), ([(3, 1, 1)], [17, 18]), ([(0, 0, 2), (0, 1, 3)], [0, 1]), ([(1, 1, 1), (2, 1, 2)], [6, 7, 8] + list(range(11, 16))),
+                        ([(0, 1, 1), (1, 1, 1), (2, 1, 1), (3, 1, 1)], [i for i in range(19) if i not in first])):
+        if not chains and edits[0][1] == 0:
+            continue                                                    # a tree that starts elsewhere needs other parents
+        t = tr.TreeBatch(blocks, cache, max_ctx=S)
+        t.check()
+        for b, col, v in edits:
+            t.blk[b, col] = v
+        t.blk[:, 3] += 2                                               # stale slots would lie under the new tokens
+        t.update()
+        t.check()
+        live = torch.tensor([i not in gone for i in range(19)], device=cuda_dev)
+        for x in (t.tok_slot, t.tok_row, t.tok_pos):
+            assert (x[~live] == -1).all() and (x[live] >= 0).all()
+        before = [x.view(torch.uint8).clone() for x in (cache.k, cache.v, cache.k_exp, cache.v_exp)]
+        qkv = queries(cuda_dev, 19, (H + 2 * Hkv) * D)
+        q = torch.full((19, H * D), 7.0, dtype=torch.bfloat16, device=cuda_dev)
+        tr.kv_append(qkv, cache, t, cos, sin, q_out=q)
+        k, out = torch.full((19, Hkv, D), 7.0, dtype=torch.bfloat16, device=cuda_dev), torch.full_like(q, 7.0)
+        tr.kv_read(cache, t.tok_row, t.tok_slot, k, None, status=t.status)
+        tr.tree_attention(q, cache, t, out)
+        t.check()
+        for x in (q, k, out):
+            assert (x[~live] == 7).all() and (x[live] != 7).any()
+        row, slot = t.tok_row[live].long(), t.tok_slot[live].long()
+        for x, b in zip((cache.k, cache.v, cache.k_exp, cache.v_exp), before):
+            x = x.view(torch.uint8).clone()
+            x[0, row, :, slot] = b[0, row, :, slot]
+            assert torch.equal(x, b)
+
+
+def test_tokens_of_a_block_out_of_range_get_no_slot(cuda_dev):
+    """A block whose place does not fit is reported, and the tokens that it leaves behind are not written."""
+    cache = make_cache(cuda_dev, "int8", 3, 1, 128, 64)
+    for col, bad in ((0, -1), (0, 50), (1, 0), (1, -3), (1, 50)):
+        t = tr.TreeBatch([(0, 3, 2), (1, 7, 3), (2, 9, 4)], cache)
+        t.check()
+        t.blk[1, col] = bad
+        t.update()
+        with pytest.raises(lib.EesdError):
+            t.check()
+        assert t.tok_slot.tolist() == [3, 4, -1, -1, -1, 9, 10, 11, 12], (col, bad)
+        t.blk[0, col], t.blk[2, col] = bad, bad
+        t.update()
+        with pytest.raises(lib.EesdError):
+            t.check()
+        assert t.tok_slot.tolist() == [-1] * 9

@@ -80,16 +80,34 @@ namespace {
 // ---------------------------------------------------------------- metadata
 // One CTA per block.  Each thread walks up from its nodes through the parents in shared memory (at most
 // depth steps), counting the depth and setting the ancestors' bits.  Latency-bound: 2 to 3 us for 64 trees of 5 nodes.
+// Tokens that no block covers get -1, or they would keep what an earlier round left there and be written to its slots.  A block
+// followed by the next one, as usual, has nothing to do for that; else its CTA looks for the block that comes next.
 __global__ void __launch_bounds__(128) tree_meta_kernel(EesdTree t, int max_batch, int max_seq, int* status) {
   pdl_trigger();
   pdl_wait();
   __shared__ int16_t par[EESD_TREE_MAX_NODES];
   const int b = blockIdx.x;
   const int start = t.blk[4 * b], T = t.blk[4 * b + 1], row = t.blk[4 * b + 2], ctx = t.blk[4 * b + 3];
-  if (start < 0 || T <= 0 || start > t.n_tokens - T) {
+  auto fits = [&](int s, int n) { return s >= 0 && n > 0 && s <= t.n_tokens - n; };
+  __shared__ int next;
+  auto uncovered = [&](int from) {                                      // tokens from `from` up to the next block
+    __syncthreads();
+    if (threadIdx.x == 0) next = t.n_tokens;
+    __syncthreads();
+    for (int j = threadIdx.x; j < t.n_blocks; j += blockDim.x) {
+      const int s = t.blk[4 * j], n = t.blk[4 * j + 1];
+      if (fits(s, n) && s + n > from) atomicMin(&next, max(s, from));
+    }
+    __syncthreads();
+    for (int i = from + threadIdx.x; i < next; i += blockDim.x) t.tok_pos[i] = t.tok_slot[i] = t.tok_row[i] = -1;
+  };
+  if (b == 0 && !(start == 0 && fits(start, T))) uncovered(0);
+  if (!fits(start, T)) {
     if (threadIdx.x == 0) set_status(status, kStatusBadIndex);
     return;
   }
+  const int end = start + T;
+  if (end < t.n_tokens && !(b + 1 < t.n_blocks && t.blk[4 * b + 4] == end && fits(end, t.blk[4 * b + 5]))) uncovered(end);
   const bool ok = row >= 0 && row < max_batch && ctx >= 0 && T <= t.max_nodes && ctx <= max_seq - T;
   if (!ok && threadIdx.x == 0) set_status(status, kStatusBadIndex);
   const bool tree = t.parent && T <= EESD_TREE_MAX_NODES;   // the entry point refuses parents with larger max_nodes
@@ -260,7 +278,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const T* qkv, int ld_qkv
   load(first);
   const int pos = tok_pos[t], row = tok_row[t], slot = tok_slot[t];
   if (pos < 0 || pos >= rope_len || row < 0 || row >= c.max_batch || slot < 0 || slot >= c.max_seq) {
-    if (threadIdx.x == 0) set_status(status, kStatusBadIndex);
+    if (threadIdx.x == 0 && (pos != -1 || row != -1 || slot != -1)) set_status(status, kStatusBadIndex);   // all -1: padding
     return;
   }
   R rope;
@@ -332,7 +350,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(CacheGeom c, const int32_t
   for (long long t = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); t < n_tok; t += (long long)gridDim.x * 8) {
     const int row = tok_row[t], slot = tok_slot[t];
     if (row < 0 || row >= c.max_batch || slot < 0 || slot >= c.max_seq) {
-      set_status(status, kStatusBadIndex);
+      if (row != -1 || slot != -1) set_status(status, kStatusBadIndex);   // both -1: padding
       continue;
     }
     for (int h0 = lane / C; h0 < c.n_kv_heads; h0 += U * STEP) {

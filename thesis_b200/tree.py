@@ -128,7 +128,8 @@ class TreeBatch:
     ``blk`` [n_blocks, 4] = (start, T, row, ctx), ``parent``, ``tok_pos``, ``tok_slot``, ``tok_row`` [n_tokens]
     int32 and ``mask`` [n_tokens, words] int64 are device tensors.  A program that advances ``ctx`` on the device
     edits ``blk`` and calls ``update``; ``max_ctx`` (default: the largest ``ctx + T`` given) has to bound ``ctx + T``
-    from then on too, as ``max_nodes`` does T."""
+    from then on too, as ``max_nodes`` does T.  A block may become shorter: tokens of no block are padding, with -1 for
+    position, slot and row, neither written nor read."""
 
     def __init__(self, blocks: Sequence[tuple], cache: KVCache, max_ctx: Optional[int] = None, max_nodes: Optional[int] = None):
         blk, par, chains, start = [], [], True, 0
