@@ -360,8 +360,8 @@ int eesd_tree_accept(const int32_t* y, const int32_t* ids, const EesdTree* tree,
 
 /* In all layers: slot ctx + j of every block's row = slot ctx + path[b, j], j = 1 .. n_acc[b] (K, V and
  * exponents).  path [n_blocks, max_nodes] must rise (eesd_tree_accept's does); a block whose path does not,
- * or that does not fit, sets a bit in *status and is left as it is.  Blocks of one call are on different
- * rows. */
+ * or that does not fit, sets a bit in *status and is left as it is, and so are blocks of one row whose slots
+ * (ctx .. ctx + T - 1) overlap. */
 int eesd_kv_compact(int dtype, const EesdKvCache* cache, const EesdTree* tree, const int32_t* path, const int32_t* n_acc,
                     int32_t* status, void* stream);
 

@@ -1283,3 +1283,54 @@ def test_tokens_of_a_block_out_of_range_get_no_slot(cuda_dev):
         with pytest.raises(lib.EesdError):
             t.check()
         assert t.tok_slot.tolist() == [-1] * 9
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int8"])
+def test_compact_refuses_blocks_that_share_slots(cuda_dev, fmt):
+    """Two blocks of one row: where their slots overlap both are reported and left, as are no others; apart they are moved."""
+    cache = make_cache(cuda_dev, fmt, 3, 2, 128, 64, layers=2)
+    state = [x.view(torch.uint8).clone() for x in (cache.k, cache.v, cache.k_exp, cache.v_exp) if x is not None]
+    raw = [x.view(torch.uint8) for x in (cache.k, cache.v, cache.k_exp, cache.v_exp) if x is not None]
+    for second, shared in ((4, True), (7, True), (0, True), (8, False), (60, False)):
+        for x, s in zip(raw, state):
+            x.copy_(s)
+        blocks = [(1, 4, 4), (1, second, 4 if second else 5), (2, 4, 4)]
+        t = tr.TreeBatch(blocks, cache)
+        t.check()
+        path = torch.full((3, t.max_nodes), -1, dtype=torch.int32, device=cuda_dev)
+        path[:, :3] = torch.tensor([0, 2, 3], device=cuda_dev)
+        n_acc = torch.full((3,), 2, dtype=torch.int32, device=cuda_dev)
+        tr.kv_compact(cache, t, path, n_acc)
+        if shared:
+            with pytest.raises(lib.EesdError):
+                t.check()
+        else:
+            t.check()
+        want = [s.clone() for s in state]
+        for b, (row, ctx, _) in enumerate(blocks):
+            if b == 2 or not shared:
+                for w, s in zip(want, state):
+                    w[:, row, :, ctx + 1:ctx + 3] = s[:, row, :, ctx + 2:ctx + 4]
+        for x, w in zip(raw, want):
+            assert torch.equal(x, w), second
+
+
+def test_compact_over_many_blocks(cuda_dev):
+    """More blocks than a CTA has threads, every one looked at for shared slots."""
+    n = 600
+    cache = make_cache(cuda_dev, "int8", n, 1, 64, 64)
+    k = cache.k.clone()
+    t = tr.TreeBatch([((7 * b) % n, 3 + b % 5, 4) for b in range(n)], cache)
+    path = torch.tensor([[0, 2, 3, -1]] * n, dtype=torch.int32, device=cuda_dev)
+    n_acc = torch.full((n,), 2, dtype=torch.int32, device=cuda_dev)
+    tr.kv_compact(cache, t, path, n_acc)
+    t.check()
+    for b in (0, 255, 256, 511, 599):
+        row, ctx = (7 * b) % n, 3 + b % 5
+        assert torch.equal(cache.k[0, row, 0, ctx + 1:ctx + 3], k[0, row, 0, ctx + 2:ctx + 4])
+    t.blk[590, 2], t.blk[590, 3] = t.blk[3, 2], t.blk[3, 3] + 3          # meets block 3
+    cache.k.copy_(k)
+    tr.kv_compact(cache, t, path, n_acc)
+    with pytest.raises(lib.EesdError):
+        t.check()
+    assert torch.equal(cache.k[0, 21], k[0, 21]) and not torch.equal(cache.k[0, 28], k[0, 28])

@@ -457,6 +457,11 @@ __global__ void __launch_bounds__(256) kv_compact_kernel(uint8_t* __restrict__ k
             acc >= 0 && acc < T;
   if (threadIdx.x == 0) first = acc + 1;
   __syncthreads();
+  // another block on slots of this one would read what this one moves: neither is touched
+  for (int j = threadIdx.x; ok && j < t.n_blocks; j += blockDim.x) {
+    const long long c = t.blk[4 * j + 3], n = t.blk[4 * j + 1];
+    if (j != b && n > 0 && t.blk[4 * j + 2] == row && c < ctx + T && ctx < c + n) ok = false;
+  }
   if (ok)
     for (int j = threadIdx.x; j <= acc; j += blockDim.x) {
       const int p = path[(size_t)b * t.max_nodes + j], before = j ? path[(size_t)b * t.max_nodes + j - 1] : -1;

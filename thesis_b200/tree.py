@@ -275,7 +275,8 @@ def tree_accept(y: torch.Tensor, ids: torch.Tensor, tree: TreeBatch, path: torch
 
 
 def kv_compact(cache: KVCache, tree: TreeBatch, path: torch.Tensor, n_acc: torch.Tensor) -> None:
-    """Move the accepted path's K and V of every layer to the slots behind ``ctx`` (blocks on different rows)."""
+    """Move the accepted path's K and V of every layer to the slots behind ``ctx``.  Blocks of one row whose slots
+    overlap are left as they are and reported."""
     dev, i32 = tree.on(cache).device, torch.int32
     _call(dev, "eesd_kv_compact", lib.F32 if cache.format == "f32" else lib.BF16, cache.ref, tree.ref,
           _need(path, "path", dev, i32, (tree.n_blocks, tree.max_nodes)), _need(n_acc, "n_acc", dev, i32, (tree.n_blocks,)),
