@@ -116,3 +116,15 @@ def test_the_python_face_refuses_host_tensors_and_formats():
         tr.KVCache.wrap(torch.zeros(1, 1, 1, 64, 64), torch.zeros(1, 1, 1, 64, 64))
     with pytest.raises(ValueError):
         tr.KVCache(1, 1, 1, 64, 64, "fp4")
+
+
+def test_row_strides_that_the_library_cannot_take():
+    """Rows 2^31 elements apart do not fit the C interface (they would be cut to 32 bits); one row has no stride."""
+    from thesis_b200 import tree as tr
+
+    far = torch.empty_strided((2, 128), (2 ** 31, 1), device="meta")
+    with pytest.raises(ValueError):
+        tr._row_stride(far)
+    assert tr._row_stride(torch.empty_strided((2, 128), (2 ** 31 - 8, 1), device="meta")) == 2 ** 31 - 8
+    for s in (1, 7, 132, 2 ** 40):
+        assert tr._row_stride(torch.empty_strided((1, 128), (s, 1), device="meta")) == 128

@@ -216,7 +216,11 @@ def _heads(t: torch.Tensor, what: str, n: int, D: int) -> int:
 
 
 def _row_stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    if t.shape[0] == 1:
+        return t.shape[1]
+    if t.stride(0) >= 2 ** 31:                           # ctypes would cut it to 32 bits
+        raise ValueError(f"rows {t.stride(0)} elements apart: at most 2^31 - 1")
+    return t.stride(0)
 
 
 def kv_read(cache: KVCache, tok_row: torch.Tensor, tok_slot: torch.Tensor, k_out: Optional[torch.Tensor],
