@@ -146,9 +146,9 @@ __global__ void __launch_bounds__(128) attn_tree_simt_kernel(TreeGeom g, CacheGe
 // the score is to the running maximum), a power of two of each q row its f16 form.  Weights are rounded to f16 (2^-11; a bf16 cache:
 // to bf16, 2^-8, the type of V), sums and outputs are fp32.
 //
-// Measured (32 query and 8 KV heads of 128): 64 trees of 5 nodes at 129 to 1023 slots over bf16 36 us, 4.4 TB/s, 67 % of the
+// Measured (32 query and 8 KV heads of 128): 64 trees of 5 nodes at 129 to 1023 slots over bf16 36 us, 4.4 TB/s, 68 % of the
 // copy rate; 64 single tokens over int8 25 us, 3.1 TB/s (the conversion of the bytes and a unit's start and end take the
-// issue slots); 8 trees of 17 nodes at 501 to 2013 slots, 32 KV heads over bf16, 51 us, 3.3 TB/s.
+// issue slots); 8 trees of 17 nodes at 501 to 2013 slots, 32 KV heads over bf16, 50 us, 3.4 TB/s.
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -805,8 +805,8 @@ Plan plan_for(const EesdKvCache* c, const EesdTree* t, int n_heads, int split_ke
   Plan p{};
   const int G = n_heads / c->n_kv_heads, rows = t->max_nodes * G;
   // Up to 32 rows the mma.sync kernel, whose cost grows with the rows in steps of 8; beyond, the tcgen05 kernel, whose tiles
-  // have 128 rows whatever is in them.  With 32 rows (mma.sync / tcgen05): 64 blocks at 129 to 1023 slots over bf16 57 / 69 us,
-  // over int8 68 / 85; 16 blocks at 300 to 4000 slots 58 / 52 and 67 / 58.  With 36 rows: 80 / 69, 98 / 89, 84 / 54, 98 / 58.
+  // have 128 rows whatever is in them.  With 32 rows (mma.sync / tcgen05): 64 blocks at 129 to 1023 slots over bf16 41 / 59 us,
+  // over int8 50 / 87; 16 blocks at 300 to 4000 slots 53 / 42 and 66 / 52.  With 36 rows: 68 / 60, 86 / 89, 81 / 42, 103 / 52.
   p.tc = rows > 32;
   p.nt = std::min(4, (rows + 7) / 8);
   p.rows = p.tc ? (rows <= 128 ? 128 : 256) : 8 * p.nt;
