@@ -341,7 +341,8 @@ int eesd_kv_read(int dtype, const EesdKvCache* cache, int layer, const int32_t* 
  * infinities among them, do not reach it.  q: rotated queries, tokens ld_q elements apart (ld_q % 8 == 0,
  * 16-byte aligned), Hq D used; out [n_tokens, Hq D].  split_keys: 0 lets the library split long key ranges
  * over CTAs as the launch needs; a multiple of 256 fixes the split, so that a block's result does not
- * depend on the other blocks of the launch (at the same max_nodes, which decides the kernel).  workspace:
+ * depend on the other blocks of the launch (at the same max_nodes, which decides the kernel, and over 8 bits
+ * with a mask in both launches or in neither).  workspace:
  * eesd_attn_tree_workspace_bytes() bytes, 256-byte aligned, not initialised, not shared by calls that may
  * overlap.  A block that does not fit the tree's maxima or the cache sets a bit in *status and is skipped.
  * The same call gives the same bits again; what a node does not see does not change a bit of its row. */

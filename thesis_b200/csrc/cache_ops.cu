@@ -79,7 +79,7 @@ namespace {
 
 // ---------------------------------------------------------------- metadata
 // One CTA per block.  Each thread walks up from its nodes through the parents in shared memory (at most
-// depth steps), counting the depth and setting the ancestors' bits.  Latency-bound: 2 to 3 us for 64 trees of 5 nodes.
+// depth steps), counting the depth and setting the ancestors' bits.  Latency-bound: 4 to 5 us for 64 trees of 5 nodes (profiled).
 // Tokens that no block covers get -1, or they would keep what an earlier round left there and be written to its slots.  A block
 // followed by the next one, as usual, has nothing to do for that; else its CTA looks for the block that comes next.
 __global__ void __launch_bounds__(128) tree_meta_kernel(EesdTree t, int max_batch, int max_seq, int* status) {
@@ -248,9 +248,9 @@ template <> struct Rope<bf16> {
 // A group of D / 8 lanes owns one head of one token: lane l holds elements 4 l .. 4 l + 3 of both halves,
 // that is four rotation pairs, so the rotation needs no exchange and the largest |x| of the vector is a
 // shuffle over the group.  Bound by the bytes of qkv, q_out and the cache, at few tokens by the chain of loads: a thread's
-// kBatch heads are asked for before the token's position, on which the tables and the slot hang, is there.  Metadata, append
-// and read-back of 320 tokens (32 query and 8 KV heads of 128, e4m3) take 6.4 us of device time (9.6 with one head after the other),
-// of 2048 tokens over int8 15.5 us, 3.8 TB/s (19 with the rotation of bf16 in fp32).
+// kBatch heads are asked for before the token's position, on which the tables and the slot hang, is there.  Append and
+// read-back of 320 tokens (32 query and 8 KV heads of 128, e4m3) take 6.1 us of device time, of 2048 tokens over int8 15.5 us,
+// 3.8 TB/s (19 with the rotation of bf16 in fp32).
 template <typename T, int FMT, int D>
 __global__ void __launch_bounds__(256) kv_append_kernel(const T* qkv, int ld_qkv, T* q_out, int ld_qo,
                                                         int n_heads, const int32_t* __restrict__ tok_pos,
@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(CacheGeom c, const int32_t
 
 // ---------------------------------------------------------------- acceptance
 // One warp per block: the walk is serial, each step one vote over the nodes behind the current one.  With the
-// compaction 4.6 us of device time for 4 trees of 15 nodes, 7.8 us for 32.
+// compaction 5.0 us of device time for 4 trees of 15 nodes, 8.8 us for 32 of 31.
 __global__ void __launch_bounds__(32) tree_accept_kernel(EesdTree t, const int32_t* __restrict__ y,
                                                          const int32_t* __restrict__ ids, int32_t* __restrict__ path,
                                                          int32_t* __restrict__ n_acc, int32_t* __restrict__ next, int* status) {
