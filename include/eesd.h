@@ -347,7 +347,7 @@ int eesd_kv_read(int dtype, const EesdKvCache* cache, int layer, const int32_t* 
  * overlap.  A block that does not fit the tree's maxima or the cache sets a bit in *status and is skipped.
  * The same call gives the same bits again; what a node does not see does not change a bit of its row.
  * Range: sums of unnormalised weights (up to 2^8 each) and values are held in fp32, and over 8-bit caches q in
- * f16 beside its row's power of two: |q| and, over EESD_KV_MODEL, |V| up to 2^100 stay in range whatever the scores.
+ * f16 beside its row's power of two: |q| and, over EESD_KV_MODEL, |V| up to 2^100 stay in range (scores beyond fp32 do not).
  * The weights' roundings, over 8 bits to f16, are relative to the row's largest weight x scale of V. */
 size_t eesd_attn_tree_workspace_bytes(int dtype, const EesdKvCache* cache, const EesdTree* tree, int n_heads, int split_keys);
 int eesd_attn_tree(int dtype, const EesdKvCache* cache, int layer, const EesdTree* tree, const void* q, int ld_q,

@@ -1334,3 +1334,40 @@ def test_compact_over_many_blocks(cuda_dev):
     with pytest.raises(lib.EesdError):
         t.check()
     assert torch.equal(cache.k[0, 21], k[0, 21]) and not torch.equal(cache.k[0, 28], k[0, 28])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("T", [1, 40])
+def test_attention_range(cuda_dev, fmt, T):
+    """|q| up to 2^100: the rows come out as the value of their largest score (the next one is far below); over a bf16 cache |V| up
+    to 2^100 as well, within the usual tolerance."""
+    H, Hkv, D, ctx = 4, 1, 64, 400
+    p = random_tree(T, np.random.default_rng(T))
+    cache = make_cache(cuda_dev, fmt, 1, Hkv, 512, D, seed=T)
+    t = tr.TreeBatch([(0, ctx, p)], cache)
+    q = queries(cuda_dev, T, H * D)
+    big = (q.float() * (2.0 ** 100 / float(q.float().abs().max()))).bfloat16()
+    out = tr.tree_attention(big, cache, t).view(T, H, D).double()
+    t.check()
+    K, V = values64(cache)
+    see = ancestors(p)
+    checked = 0
+    for i in range(T):
+        use = torch.tensor([True] * ctx + [bool(x) for x in see[i]], device=cuda_dev)
+        k, v = K[0, 0, :ctx + T][use], V[0, 0, :ctx + T][use]
+        for h in range(H):
+            qq = big[i, h * D:(h + 1) * D].double()
+            s = k @ qq / math.sqrt(D)
+            top = s.sort(descending=True)
+            off = 2 * 2.0 ** -24 * (D + 8) * float((k.abs() @ qq.abs()).max()) / math.sqrt(D)   # of two scores, as they are summed
+            assert out[i, h].isfinite().all()
+            if top.values[0] - top.values[1] > off + 200:
+                want = v[top.indices[0]]
+                assert ((out[i, h] - want).abs() <= want.abs() * (2.0 ** -8 + 2.0 ** -20)).all(), (i, h)
+                checked += 1
+    assert checked > T * H // 2
+    if fmt == "bf16":
+        cache.v *= 2.0 ** 100 / float(cache.v.float().abs().max())
+        out = tr.tree_attention(q, cache, t)
+        t.check()
+        check_attention(out, q, cache, [(0, ctx, p)], [see], H)

@@ -33,9 +33,9 @@ def programs(pieces, NS, q8, weights_first, ml_issuer):
     for x in (0, 1):
         count.update({("s_full", x): 1, ("s_free", x): 1, ("p_ready", x): 1, ("pv_done", x): 1})
     count.update({("q_ready",): 2, ("o_done",): 2, ("epi",): 2})
-    prog = {"K": [], "V": []}
+    prog = {"K": [], "V": []} if q8 else {"K": []}                      # over 16 bits one thread asks for K and V in turn
     for c in range(sum(n for n, _ in pieces)):
-        for role, kind in (("K", "k"), ("V", "v")):
+        for role, kind in (("K", "k"), ("V" if q8 else "K", "v")):
             if c >= NS:
                 prog[role].append(("w", (kind + "empty", c % NS), c // NS - 1))
             prog[role].append(("load", kind, c))
