@@ -1371,3 +1371,30 @@ def test_attention_range(cuda_dev, fmt, T):
         out = tr.tree_attention(q, cache, t)
         t.check()
         check_attention(out, q, cache, [(0, ctx, p)], [see], H)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("T", [6, 40, 100])
+def test_attention_scales_that_others_see_leave_small_weights(cuda_dev, fmt, T):
+    """8-bit caches: a row whose largest score has a value of small scale, zero in half of the dims, so that those dims are the sum of
+    weights at the end of f16; values of a large scale that only other nodes see must not change how they are rounded."""
+    H, Hkv, D, ctx = 8, 2, 64, 75
+    p = random_tree(T, np.random.default_rng(T))
+    see = ancestors(p)
+    cache = make_cache(cuda_dev, fmt, 1, Hkv, 256, D, seed=T)
+    cache.k[0, 0, :, 70] = torch.full((1,), QMAX[fmt], device=cuda_dev).to(cache.k.dtype)
+    cache.k_exp[0, 0, :, 70] = 127 + (-9 if fmt == "e4m3" else -7)       # 0.88, 0.99 each: scores of about 11, 12
+    cache.v_exp[0, 0, :, 70] -= 5
+    cache.v.view(torch.uint8)[0, 0, :, 70, ::2] = 0
+    t = tr.TreeBatch([(0, ctx, p)], cache)
+    q = (1.5 + 0.1 * queries(cuda_dev, T, H * D).float()).bfloat16()
+    clean = tr.tree_attention(q, cache, t)
+    check_weighted(clean, q, cache, ctx, p, H, 1 if T * H // Hkv <= 32 else 9)
+    for node in sorted({1, T // 2, T - 1}):
+        keep = cache.v_exp[0, 0, :, ctx + node].clone()
+        cache.v_exp[0, 0, :, ctx + node] = keep + 20
+        out = tr.tree_attention(q, cache, t)
+        t.check()
+        blind = torch.from_numpy(~see[:, node])
+        assert torch.equal(out[blind], clean[blind]), node
+        cache.v_exp[0, 0, :, ctx + node] = keep

@@ -275,7 +275,7 @@ template <int D, int FMT> struct TcShape {
 };
 constexpr int kPieces = 4;                 // pieces between the schedule warp and the slowest role
 constexpr int kReaders = 19;               // warps that read them: TMA, 2 MMA, 8 softmax, 8 conversion
-enum : int { kHowK = 1 << 8, kHowV = 1 << 9, kHowWide = 1 << 10 };
+enum : int { kHowK = 1 << 8, kHowV = 1 << 9 };
 struct TcControl {
   uint64_t kfull[4], kempty[4], vfull[4], vempty[4], vclean[4], raw_full[6], raw_empty[6];
   uint64_t piece_full[kPieces], piece_empty[kPieces];
@@ -283,7 +283,7 @@ struct TcControl {
   uint64_t s_full[2], s_free[2], p_ready[2], pv_done[2], q_ready, o_done, ml_ready, epi_done, drain[2];
   // 8-bit, per tile: ref is V's largest exponent byte, kt the one factor of its keys, and how (kHow*, above ref's byte) what is not in
   // the operands.  Keyed K: 2^ek of the keys multiplies the scores.  Keyed V: 2^ev of the keys multiplies the weights, ev is the exponent
-  // byte (0 for NaN and slots past the end); wide: they lie so far apart that the largest does not stand for the others.
+  // byte (0 for NaN and slots past the end).
   alignas(16) float fk[8][KT];
   alignas(16) float fv[8][KT];
   float kt[8];
@@ -638,8 +638,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           int ref = 0;
           if (!is_v && warp == 12) {
             ref = largest(ev, a0, a1);
-            const bool wide = spread(ref, 8, a0, a1);
-            ref |= (keyed ? kHowK : 0) | (wide || partial ? kHowV : 0) | (wide ? kHowWide : 0);
+            ref |= (keyed ? kHowK : 0) | (spread(ref, 8, a0, a1) || partial ? kHowV : 0);
           }
           if (!(ok = warp_wait(is_v ? &ct.vempty[st] : &ct.kempty[st], (cnt / NS & 1) ^ 1, abort_flag, g.spin))) break;
           if (!is_v && warp == 12) {
@@ -980,8 +979,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (__builtin_expect(__any_sync(0xffffffffu, rises || is_huge() || (Q8 && (unsigned)(de + 40) > 43u)), 0)) {
           const float up = mn - m;
           float heavy = mx - mn + (float)de;                            // 8-bit: the largest weight x scale, or what it is at most: log2, over mn and 2^er
-          if (__builtin_expect(how & kHowWide, 0)) {
-            heavy = -INFINITY;
+          if (__builtin_expect(how & kHowV, 0)) {                       // key by key: em may stand for a slot of no weight, and what
+            heavy = -INFINITY;                                          // others see must not choose between the two forms
 #pragma unroll
             for (int j = 0; j < KT; ++j)                                // (rounded as mx is)
               if (const int e = ct.ev[f][j]) heavy = fmaxf(heavy, __fadd_rn(__fmul_rn(__uint_as_float(a[j]), rt), -mn) + (float)(e - er));
