@@ -21,9 +21,9 @@
 // and each tile takes four of them), 2 the schedule, 4-7 and 8-11 softmax of stream 0 and 1 (a thread is a row),
 // 12-15 and 16-19 conversion of K and of V (8-bit), or 12-15 the check of V tiles that some row does not wholly see (bf16).
 //
-// Measured (32 query and 8 KV heads of 128): 48 nodes at 131 k slots over int8 191 us, 540 TFLOP/s, 1.42 TB/s; four 512-token
-// chunks at up to 3.6 k slots over e4m3 133 us, 518 TFLOP/s, over bf16 110 us, 627 TFLOP/s; 16 trees of 31 nodes at 1 k to 4 k slots
-// over e4m3 65 us, over bf16 52 us.  By the clock, in a copy that recorded it, a pair
+// Measured (32 query and 8 KV heads of 128): 48 nodes at 131 k slots over int8 192 us, 536 TFLOP/s, 1.41 TB/s; four 512-token
+// chunks at up to 3.6 k slots over e4m3 136 us, 507 TFLOP/s, over bf16 110 us, 624 TFLOP/s; 16 trees of 31 nodes at 1 k to 4 k slots
+// over e4m3 66 us, over bf16 53 us.  By the clock, in a copy that recorded it, a pair
 // of 128-row tiles takes some 2800 clocks per 64 keys, of which the products are 1000 and the exponentials 1024: what
 // bounds it is the chain wait, load, maximum, exponentials, store of the one softmax warp that a stream has per scheduler.
 // One row tile is bound by the conversion (1900 clocks a tile) and by the units' starts and ends, 7 k clocks each.  Tried and
@@ -161,8 +161,8 @@ template <int FMT> __device__ __forceinline__ uint32_t idesc_f32(int n, bool b_m
 // ------------------------------------------------------------------ the flat schedule
 // Entry e = (block, row tile); its unit of each KV head takes `tiles` key tiles.  On the flat axis a unit is kUnitCost
 // positions (what starting a unit costs, in tiles) and then its tiles; entries follow one another, their heads inside.
-// Measured with 4, 6, 8, 10 (us): four 512-token chunks over e4m3 162, 136, 133, 134, over bf16 113, 112, 110, 112; 16 trees of 31
-// nodes over e4m3 67.7, 65.0, 64.9, 66.5, over bf16 53.4, 52.3, 52.1, 52.5; nine 235-token chunks over int8 74, 72, 72, 70; 48 nodes at
+// Measured with 4, 6, 8, 10 (us): four 512-token chunks over e4m3 174, 141, 136, 137, over bf16 114, 112, 110, 112; 16 trees of 31
+// nodes over e4m3 68.8, 66.6, 65.8, 67.1, over bf16 53.8, 52.7, 52.5, 52.7; nine 235-token chunks over int8 78, 76, 75, 73; 48 nodes at
 // 131 k slots and 16 trees of 48 at 400 the same with all.
 constexpr int kUnitCost = 8;
 struct Entry {
